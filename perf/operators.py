@@ -245,7 +245,8 @@ def _plain_rotary(s):
 
 
 def _codes(x):
-    scale = (x.abs().amax(-1, keepdim=True) / 127).clamp(min=FLT_MIN)
+    top = x.abs().amax(-1, keepdim=True)
+    scale = (top / torch.full_like(top, 127)).clamp(min=FLT_MIN)  # (by a number torch multiplies with its reciprocal)
     t = (x / scale).clamp(-127, 127).double()  # adding a half in 32 bits would round up what is just below it
     return (torch.sign(t) * torch.floor(t.abs() + 0.5)).to(torch.int8), scale
 
