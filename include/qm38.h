@@ -350,6 +350,135 @@ qm_status qm_attn_prefill(qm_runtime* rt, qm_kv* seq, const uint16_t* q,
                           uint32_t H, uint32_t M, uint16_t* o);
 
 /* ------------------------------------------------------------------ */
+/* Rotary positions                                                    */
+/* ------------------------------------------------------------------ */
+/* No counterpart in the reference, whose only rotation is the half layout
+ * inside qm_attn_prepare. */
+#define QM_ROTARY_HALF 0        /* pairs (i, i + rotary_dim / 2) */
+#define QM_ROTARY_INTERLEAVED 1 /* pairs (2 i, 2 i + 1) */
+#define QM_ROTARY_PLAIN 0       /* f_i = theta^(-2 i / rotary_dim) radians per position */
+#define QM_ROTARY_LINEAR 1      /* f_i / factor */
+#define QM_ROTARY_YARN 2        /* f_i where a frequency turns more than beta_fast times within
+                                   original_positions, f_i / factor where it turns less than
+                                   beta_slow times, a linear ramp over i between the two */
+typedef struct qm_rotary_config {
+  uint32_t rotary_dim;         /* rotated elements of a head: even, 2..256 */
+  uint32_t layout;             /* QM_ROTARY_HALF or _INTERLEAVED */
+  float theta;                 /* > 1 */
+  uint32_t scaling;            /* QM_ROTARY_PLAIN, _LINEAR or _YARN */
+  float factor;                /* LINEAR, YARN: >= 1 */
+  uint32_t original_positions; /* YARN: positions the model was trained on, > 0 */
+  float beta_fast, beta_slow;  /* YARN: beta_fast > beta_slow > 0 (usually 32 and 1) */
+  float attention_factor;      /* of sine and cosine; 0: 0.1 ln(factor) + 1 with YARN, else 1 */
+} qm_rotary_config;
+
+/* bf16 rows of `heads` heads of `head_dim` elements; elements offset ..
+ * offset + rotary_dim - 1 of each head are rotated, the others copied.  Strides
+ * are the elements between rows (0: heads * head_dim); what lies between the
+ * rows is neither read nor written.  out == in with equal strides rotates in
+ * place. */
+typedef struct qm_rotary_tensor {
+  const uint16_t* in;
+  uint16_t* out;
+  uint32_t heads;
+  uint32_t head_dim;
+  uint32_t offset;
+  uint64_t in_stride, out_stride;
+} qm_rotary_tensor;
+
+/* Rotates M rows of 1..4 tensors (queries and keys of one step) in one launch:
+ * a pair (a, b) becomes (a cos - b sin, b cos + a sin) with the angle
+ * position * f_i, formed in fp64.  positions: device uint32 [M], or NULL for
+ * position_base + row (at most 2^32 - 1).  An output may overlap no tensor's
+ * memory but its own input's, and that only in place (QM_ERR_INVALID_ARGUMENT).
+ * Device pointers, asynchronous, no workspace (a captured call may be
+ * replayed); 2-byte alignment is enough, rows, heads and parts on 16 bytes are
+ * faster. */
+qm_status qm_rotary(qm_runtime* rt, const qm_rotary_config* cfg, const qm_rotary_tensor* tensors, uint32_t n_tensors,
+                    uint32_t M, const uint32_t* positions, uint32_t position_base);
+
+/* ------------------------------------------------------------------ */
+/* Latent attention                                                    */
+/* ------------------------------------------------------------------ */
+/* Attention whose keys and values come, for all heads, from one latent vector
+ * c_t and one rotated key k_t a token (no counterpart in the reference):
+ *   score(i, t, h) = softmax_scale (q_nope[i, h] . W_uk[h] c_t + q_rope[i, h] . k_t)
+ *   o[i, h]        = W_uv[h] sum_t softmax_t(score) c_t
+ * A layer's step: project, qm_rotary on the queries' and the key's rotated
+ * parts, then qm_latent_decode or qm_latent_prefill, which append the new
+ * tokens themselves. */
+
+/* The cache: per token rank + rope_dim int8 and two fp32 scales (the latent's
+ * and the key's), quantised as the Q8 KV cache does: s = max(absmax / 127,
+ * FLT_MIN), code = round half away(clamp(x / s, -127, 127)); a latent or key
+ * that holds a NaN or an infinity stands for NaN (its scale).  Token-major:
+ * codes [capacity][rank_pad + 64], rank_pad the next multiple of 128 (padding
+ * holds zero).  Capacity starts at 64 tokens and grows on demand as qm_kv's
+ * does; max_tokens = 0 means no limit, else appends past it fail with
+ * QM_ERR_CAPACITY_EXCEEDED.  rank 8..512 and rope_dim 8..64, multiples of 8,
+ * else QM_ERR_INVALID_ATTENTION_SHAPE. */
+typedef struct qm_latent_kv qm_latent_kv;
+qm_status qm_latent_kv_create(qm_runtime* rt, uint32_t rank, uint32_t rope_dim, uint32_t max_tokens,
+                              qm_latent_kv** out);
+void qm_latent_kv_destroy(qm_latent_kv* kv);
+uint32_t qm_latent_kv_length(const qm_latent_kv* kv);
+uint32_t qm_latent_kv_capacity(const qm_latent_kv* kv); /* tokens held without growing */
+qm_status qm_latent_kv_reserve(qm_latent_kv* kv, uint32_t additional);
+qm_status qm_latent_kv_truncate(qm_latent_kv* kv, uint32_t length);
+qm_status qm_latent_kv_clone(const qm_latent_kv* src, qm_latent_kv** out);
+/* Host copies of the active tokens: codes int8 [len][rank + rope_dim], scales
+ * fp32 [len][2].  Synchronous; either pointer may be NULL. */
+qm_status qm_latent_kv_read(const qm_latent_kv* kv, int8_t* codes, float* scales);
+
+/* Quantises M rows kv bf16 [M][rank + rope_dim] (latent, then rotated key) behind
+ * the cached tokens.  norm fp32 [rank] or NULL: the latent is RMS-normalised
+ * on its way (x / sqrt(mean x^2 + epsilon) * norm, in fp32).  kv must be
+ * 16-byte aligned.  This and the calls below refuse a stream that is being
+ * captured and the per-thread default stream (QM_ERR_INVALID_ARGUMENT): a call
+ * advances the host-side length when it is made. */
+qm_status qm_latent_append(qm_runtime* rt, qm_latent_kv* kv, const uint16_t* rows, const float* norm, float epsilon,
+                           uint32_t M);
+/* Reads tokens first .. first + count - 1 back: bf16 [count][rank + rope_dim],
+ * code * scale rounded to bf16.  Past the length: QM_ERR_INVALID_SEQUENCE_LENGTH.
+ * out must be 16-byte aligned. */
+qm_status qm_latent_load(qm_runtime* rt, const qm_latent_kv* kv, uint32_t first, uint32_t count, uint16_t* out);
+
+/* heads 1..1024; nope_dim and v_dim 8..128, rank and rope_dim as above, all
+ * multiples of 8, else QM_ERR_INVALID_ATTENTION_SHAPE.  softmax_scale is finite
+ * and > 0 (usually (nope_dim + rope_dim)^-1/2, times the square of a scaled
+ * rotation's attention factor where that is not in the rotation). */
+typedef struct qm_latent_config {
+  uint32_t heads, rank, nope_dim, rope_dim, v_dim;
+  float softmax_scale;
+} qm_latent_config;
+typedef struct qm_latent_weights qm_latent_weights;
+/* Lays out the projection kv_b [heads][nope_dim + v_dim][rank] (W_uk's rows, then
+ * W_uv's, of each head), bf16 in device memory or an affine-Q4 job of heads *
+ * (nope_dim + v_dim) rows (rank a multiple of 64; its values are rounded to
+ * bf16).  Synchronous; the source is not kept. */
+qm_status qm_latent_weights_create(qm_runtime* rt, const qm_latent_config* cfg, const uint16_t* kv_b,
+                                   qm_latent_weights** out);
+qm_status qm_latent_weights_create_q4(qm_runtime* rt, const qm_latent_config* cfg, const qm_q4_job* kv_b,
+                                      qm_latent_weights** out);
+void qm_latent_weights_destroy(qm_latent_weights* w);
+
+/* One new token for each of B <= 64 sequences (a ragged batch): appends it
+ * (qm_latent_append) and attends over the whole cache including it.
+ *   q  bf16 [B][heads][nope_dim + rope_dim], the last rope_dim rotated
+ *   kv bf16 [B][rank + rope_dim];  norm, epsilon as in qm_latent_append
+ *   o  bf16 [B][heads][v_dim]
+ * The absorbed form: queries through W_uk into the latent space, attention over
+ * the 8-bit cache (split over its length and joined), sums out through W_uv.
+ * q and kv must be 16-byte aligned.  All sequences must fit the weights' rank
+ * and rope_dim; none may appear twice. */
+qm_status qm_latent_decode(qm_runtime* rt, const qm_latent_weights* w, qm_latent_kv* const* seqs, uint32_t B,
+                           const uint16_t* q, const uint16_t* kv, const float* norm, float epsilon, uint16_t* o);
+/* M new rows of one sequence, row i attending over the cached tokens and the
+ * new rows up to itself.  Layouts as above with M in the place of B. */
+qm_status qm_latent_prefill(qm_runtime* rt, const qm_latent_weights* w, qm_latent_kv* seq, const uint16_t* q,
+                            const uint16_t* kv, const float* norm, float epsilon, uint32_t M, uint16_t* o);
+
+/* ------------------------------------------------------------------ */
 /* Gated DeltaNet                                                      */
 /* ------------------------------------------------------------------ */
 /* DeltaNetConfig (metal_runtime.rs:487-494). */

@@ -1,0 +1,89 @@
+// Launch interface of the latent cache and latent attention kernels
+// (latent_cache.hip, latent_absorbed.hip, latent_expanded.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace qm {
+
+constexpr uint32_t kLatentMaxRank = 512, kLatentMaxNope = 128, kLatentMaxV = 128;
+constexpr uint32_t kLatentRope = 64;   // stored width of the shared key (the extra elements hold zero)
+constexpr uint32_t kLatentTile = 32;   // tokens of a tile; a cache's capacity is a multiple
+constexpr uint32_t kLatentCols = 32;   // (row, head) columns of an absorbed-attention workgroup
+constexpr uint32_t kMaxLatentSeqs = 64;
+
+// Stored widths: a latent's (128 .. 512) and an expanded key's or value's (64, 128).
+inline uint32_t latent_rank_pad(uint32_t rank) { return (rank + 127) / 128 * 128; }
+inline uint32_t latent_head_pad(uint32_t d) { return d <= 64 ? 64 : 128; }
+
+// Where a sequence's tokens are: codes int8 [capacity][rank_pad + 64], scales
+// fp32 [capacity][2] (the latent's, the shared key's).
+struct LatentRows {
+  int8_t* codes;
+  float* scales;
+};
+
+struct LatentAppendArgs {
+  const uint16_t* kv;  // bf16 [items][rank + rope]
+  const float* norm;   // fp32 [rank] or null: stored as given
+  float eps;
+  uint32_t rank, rope, rank_pad;
+  uint32_t items;
+  // Item i becomes token pos[i] of seqs[i] (decode), or token pos[0] + i of seqs[0].
+  uint32_t decode;
+  LatentRows seqs[kMaxLatentSeqs];
+  uint32_t pos[kMaxLatentSeqs];
+};
+hipError_t launch_latent_append(const LatentAppendArgs& a, hipStream_t st);
+
+// bf16 [count][rank + rope] of tokens first .. first + count - 1.
+hipError_t launch_latent_load(const LatentRows& rows, uint32_t rank, uint32_t rope, uint32_t rank_pad, uint32_t first,
+                              uint32_t count, uint16_t* out, hipStream_t st);
+
+// Weights as the kernels read them, from kv_b [H][nope + v][rank]:
+//   down bf16 [H][rank_pad][nope_pad]          W_uk transposed: queries into the latent space
+//   up   bf16 [H][nope_pad + v_pad][rank_pad]  W_uk, then W_uv: out of it
+// zero in the padding.
+struct LatentDims {
+  uint32_t heads, rank, nope, rope, v;
+  uint32_t rank_pad, nope_pad, v_pad;
+};
+hipError_t launch_latent_weights(const LatentDims& d, const uint16_t* kv_b, uint16_t* down, uint16_t* up,
+                                 hipStream_t st);
+// The same from an affine-Q4 matrix [H * (nope + v)][rank] (rank a multiple of 64).
+hipError_t launch_latent_weights_q4(const LatentDims& d, const uint32_t* w, const uint16_t* s, const uint16_t* b,
+                                    uint16_t* down, uint16_t* up, hipStream_t st);
+
+// Absorbed attention.  Column c = row * H + head of a sequence; 32 columns
+// make a block.  Decode: one row for each sequence, H columns each.  Prefill:
+// one sequence of `rows` rows.
+struct LatentSeq {
+  LatentRows rows;
+  uint32_t start;        // position of the sequence's first new row
+  uint32_t unit_begin;   // first workgroup
+  uint32_t block_begin;  // first column block
+  uint32_t splits;       // workgroups sharing a column block's tiles
+};
+struct LatentAttnArgs {
+  const uint16_t* q;      // bf16 [rows][H][nope + rope]
+  uint16_t* o;            // bf16 [rows][H][v]
+  const uint16_t* down;
+  const uint16_t* up;
+  uint8_t* digits;        // queries in operand order, [block][rank_pad / 32 + 2][64 lanes][32 bytes]
+  float* qscale;          // [block][32][2]
+  float* partials;        // O [unit][32][rank_pad], then (max, sum) [unit][32][2]
+  uint16_t* mixed;        // bf16 [rows][H][rank_pad]: the joined sums of latents
+  LatentDims d;
+  float scale;            // of the scores
+  uint32_t rows;          // query rows of the call (decode: sequences)
+  uint32_t n_seqs;
+  uint32_t decode;
+  uint32_t blocks;        // column blocks of the call
+  uint32_t units;         // workgroups of the attention launch
+  uint32_t tiles_per_split;
+  LatentSeq seqs[kMaxLatentSeqs];
+};
+constexpr uint64_t latent_digit_bytes(uint32_t rank_pad) { return (uint64_t)(rank_pad / 32 + 2) * 64 * 32; }
+hipError_t launch_latent_absorbed(const LatentAttnArgs& a, hipStream_t st);
+
+}  // namespace qm

@@ -1,0 +1,466 @@
+// Latent attention, absorbed form: the queries go into the latent space
+// (q_nope W_uk), attend over the 8-bit cache as over one shared key and value
+// per token, and the sums of latents come out through W_uv.  For decode and
+// for few rows: a token costs 584 bytes (rank 512) whatever the heads.
+//
+// Four launches: latent_query_kernel, latent_attn_kernel (split over the
+// cache's length), latent_join_kernel, latent_up_kernel.
+#include <float.h>
+
+#include "latent.h"
+#include "latent_device.h"
+
+namespace qm {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoMax = -1e30f;  // running maximum before the first visible token
+
+// ---------------------------------------------------------------------------
+// Queries into the latent space, as two 8-bit digits
+// ---------------------------------------------------------------------------
+// qa[h][r] = sum_d q_nope[h][d] W_uk[h][d][r], then the row (and apart from it
+// the rotated part) as 16-bit integers: q = qs * (256 hi + lo), qs = absmax /
+// 32512, hi in -127..127, lo in -128..127.  The scores are then whole-number
+// products with the cache's codes on the i8 matrix cores, exact but for this
+// rounding (2^-17 of the row's largest element, where rounding qa to bf16 would
+// be 2^-9 of each), and the cache's bytes need no conversion.  A row with a NaN
+// or an infinity gets a NaN scale, which its scores keep.
+//
+// Workgroup = (16 rows, head); a wave takes a quarter of the latent.
+template <int RP>
+__global__ __launch_bounds__(256) void latent_query_kernel(LatentAttnArgs a) {
+  constexpr int kTiles = RP / 64;    // 16-wide tiles of a wave
+  constexpr int kStride = RP + 4;    // floats of a row in LDS
+  __shared__ float buf[16 * kStride];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t h = blockIdx.y, m0 = blockIdx.x * 16;
+  const uint32_t H = a.d.heads, nope = a.d.nope, qw = nope + a.d.rope, np = a.d.nope_pad;
+  const uint32_t n = lane & 15, kq = lane >> 4;
+  const uint16_t* down = a.down + (size_t)h * RP * np;
+  const uint16_t* qrow = a.q + ((size_t)min(m0 + n, a.rows - 1) * H + h) * qw;
+  u32x4 qa[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const uint32_t k = 32 * s + 8 * kq;
+    qa[s] = k < nope && m0 + n < a.rows ? *(const u32x4*)(qrow + k) : u32x4{0, 0, 0, 0};
+  }
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+    const uint32_t r = wave * (RP / 4) + 16 * t;
+    floatx4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      if (32u * s < np) acc = mfma16x16x32(qa[s], *(const u32x4*)(down + (size_t)(r + n) * np + 32 * s + 8 * kq), acc);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) buf[(4 * kq + i) * kStride + r + n] = acc[i];
+  }
+  __syncthreads();
+  // 16 threads a row.
+  const uint32_t row = threadIdx.x >> 4, t = threadIdx.x & 15, m = m0 + row;
+  const float* x = buf + row * kStride;
+  uint32_t top = 0, top_key = 0;  // largest absolute value, as bits: NaN and infinity come out on top
+#pragma unroll
+  for (int i = 0; i < RP / 16; ++i) top = max(top, __float_as_uint(x[t + 16 * i]) & 0x7FFFFFFFu);
+  const uint16_t* key = a.q + ((size_t)min(m, a.rows - 1) * H + h) * qw + nope;
+  float k[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    k[i] = 4 * t + i < a.d.rope ? bf16_to_f32(key[4 * t + i]) : 0.0f;
+    top_key = max(top_key, __float_as_uint(k[i]) & 0x7FFFFFFFu);
+  }
+#pragma unroll
+  for (int s = 1; s < 16; s *= 2) {
+    top = max(top, (uint32_t)__shfl_xor((int)top, s));
+    top_key = max(top_key, (uint32_t)__shfl_xor((int)top_key, s));
+  }
+  if (m >= a.rows) return;
+  const float qs = fmaxf(__uint_as_float(top) / 32512.0f, FLT_MIN);
+  const float ks = fmaxf(__uint_as_float(top_key) / 32512.0f, FLT_MIN);
+  const bool bad = top >= 0x7F800000u, bad_key = top_key >= 0x7F800000u;
+  const uint32_t c = a.decode ? h : m * H + h;
+  const size_t block = a.seqs[a.decode ? m : 0].block_begin + c / kLatentCols;
+  const uint32_t col = c % kLatentCols;
+  uint8_t* to = a.digits + block * latent_digit_bytes(RP);
+  auto digits = [](float v, float s, bool skip, uint32_t* hi, uint32_t* lo) __attribute__((always_inline)) {
+    const int q = skip ? 0 : (int)rintf(fminf(fmaxf(v / s, -32512.0f), 32512.0f));
+    const int h8 = (q + 128) >> 8;
+    *hi = (uint32_t)h8 & 255u;
+    *lo = (uint32_t)(q - 256 * h8) & 255u;
+  };
+#pragma unroll
+  for (int i = 0; i < RP / 256 + 1; ++i) {
+    const uint32_t chunk = t + 16 * i;  // 16 elements
+    if (chunk >= RP / 16) break;
+    uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      uint32_t h8, l8;
+      digits(x[16 * chunk + j], qs, bad, &h8, &l8);
+      hi[j / 4] |= h8 << (8 * (j % 4));
+      lo[j / 4] |= l8 << (8 * (j % 4));
+    }
+    uint8_t* at = to + ((size_t)(chunk / 2) * 64 + (chunk % 2) * 32 + col) * 32;
+    *(u32x4*)at = u32x4{hi[0], hi[1], hi[2], hi[3]};
+    *(u32x4*)(at + 16) = u32x4{lo[0], lo[1], lo[2], lo[3]};
+  }
+  {
+    uint32_t hi = 0, lo = 0;  // the key part: 4 elements a thread
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t h8, l8;
+      digits(k[j], ks, bad_key, &h8, &l8);
+      hi |= h8 << (8 * j);
+      lo |= l8 << (8 * j);
+    }
+    const uint32_t chunk = t / 4;
+    uint8_t* at = to + ((size_t)(RP / 32 + chunk / 2) * 64 + (chunk % 2) * 32 + col) * 32 + 4 * (t % 4);
+    *(uint32_t*)at = hi;
+    *(uint32_t*)(at + 16) = lo;
+  }
+  if (t == 0) {
+    const float nan = __uint_as_float(0x7FC00000u);
+    *(float2*)(a.qscale + (block * kLatentCols + col) * 2) = float2{bad ? nan : qs, bad_key ? nan : ks};
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Attention over the cache
+// ---------------------------------------------------------------------------
+// A wave takes 32 columns (heads of a row, or of several rows) and every fourth
+// 32-token tile of its workgroup's share of the cache, alone: it streams the
+// tiles' bytes into its own LDS ring by buffer->LDS DMA and never waits for the
+// other waves before the end.
+//   S^T[token][column] = codes . (hi, lo) on v_mfma_i32_32x32x32_i8, the token's
+//     and the column's scales applied in fp32;
+//   online softmax in fp32 (exp2 domain), the sums rescaled only when a column's
+//     maximum rises by more than 8 (p stays below 2^8);
+//   O^T[latent element][column] += codes^T P'^T on v_mfma_f32_32x32x16_bf16:
+//     P' = p * token scale rounded to bf16 (2^-9 of each term), the codes exact.
+//     S^T leaves a lane the P' of its own column in the order that the second
+//     product wants once the tokens of its operand are taken in the same order,
+//     so P' stays in registers; the codes' operand comes by transposing reads.
+// The O^T accumulators (rank_pad x 32 fp32) take half of the register file.
+template <int RP>
+struct AbsorbedLds {
+  static constexpr int kChunks = RP / 16;  // 16-byte pieces of a latent
+  static constexpr int kLat = kLatentTile * RP, kKey = kLatentTile * (int)kLatentRope, kScale = kLatentTile * 8;
+  static constexpr int kTileBytes = kLat + kKey + kScale;
+  static constexpr int kRing = RP >= 384 ? 2 : RP == 256 ? 3 : 4;
+  static constexpr int kPad = 132;  // floats of a column's 128 sums in the final merge
+  static constexpr int kMerge = 4 * (int)kLatentCols * kPad * 4 + 4 * (int)kLatentCols * 8;
+  static constexpr int kBytes = 4 * kRing * kTileBytes > kMerge ? 4 * kRing * kTileBytes : kMerge;
+  static constexpr int kDma = RP / 32 + 3;  // DMA instructions of a tile
+};
+
+// Order of a token's 16-byte pieces in LDS: piece j at j ^ swizzle(token).  Both
+// the reads of one piece of 8 consecutive tokens and those of the 8 tokens of a
+// transposing read (0..3, 8..11 or 4..7, 12..15) fall on different banks.
+__device__ __forceinline__ constexpr uint32_t lat_swizzle(uint32_t tok) {
+  return (tok & 3) | ((((tok >> 2) ^ (tok >> 3)) & 1) << 2);
+}
+
+template <int RP>
+__global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnArgs a) {
+  using L = AbsorbedLds<RP>;
+  constexpr int CH = L::kChunks, kLatSteps = RP / 32, kBlocks = RP / 32;
+  constexpr uint32_t kStride = RP + kLatentRope;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[L::kBytes];
+  const uint32_t lane = threadIdx.x & 63;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t col = lane & 31, half = lane >> 5;
+  const uint32_t unit = blockIdx.x, H = a.d.heads;
+  uint32_t b = 0;
+  while (b + 1 < a.n_seqs && unit >= a.seqs[b + 1].unit_begin) ++b;
+  const LatentSeq& sq = a.seqs[b];
+  const uint32_t cols = a.decode ? H : a.rows * H;
+  const uint32_t blocks = (cols + kLatentCols - 1) / kLatentCols;
+  const uint32_t local = unit - sq.unit_begin, cb = local % blocks, split = local / blocks;
+  // Tokens that a column sees: up to its own row.
+  const uint32_t c_first = cb * kLatentCols, c_last = min(c_first + kLatentCols, cols) - 1, c = c_first + col;
+  const uint32_t lim_min = sq.start + c_first / H + 1, lim_max = sq.start + c_last / H + 1;
+  const uint32_t limit = c <= c_last ? sq.start + c / H + 1 : 0;
+  const uint32_t tiles = (lim_max + kLatentTile - 1) / kLatentTile;
+  const uint32_t t_begin = split * a.tiles_per_split, t_end = min(tiles, t_begin + a.tiles_per_split);
+
+  const size_t block = sq.block_begin + cb;
+  u32x4 qhi[kLatSteps + 2], qlo[kLatSteps + 2];
+  {
+    const uint8_t* dg = a.digits + block * latent_digit_bytes(RP) + lane * 32;
+#pragma unroll
+    for (int s = 0; s < kLatSteps + 2; ++s) {
+      qhi[s] = *(const u32x4*)(dg + s * 2048);
+      qlo[s] = *(const u32x4*)(dg + s * 2048 + 16);
+    }
+  }
+  const float2 qs = limit ? *(const float2*)(a.qscale + (block * kLatentCols + col) * 2) : float2{0.0f, 0.0f};
+  const float lat_scale = qs.x * a.scale * kLog2e, key_scale = qs.y * a.scale * kLog2e;
+
+  uint8_t* ring = lds + wave * (L::kRing * L::kTileBytes);
+  const uint32_t tpi = 64 / CH;  // tokens of a DMA instruction (a whole number but for rank_pad 384)
+  const uint32_t jb = lane % CH, tb = lane / CH;
+  const uint32_t j16 = (jb ^ lat_swizzle(tb)) * 16, tb_off = tb * kStride;
+  const uint32_t key_tok = lane / 4;
+  auto issue = [&](uint32_t tile, uint32_t slot) __attribute__((always_inline)) {
+    uint8_t* to = ring + slot * L::kTileBytes;
+    const auto rows = latent_rsrc(sq.rows.codes + (size_t)tile * kLatentTile * kStride, kLatentTile * kStride);
+#pragma unroll
+    for (int i = 0; i < RP / 32; ++i) {
+      if constexpr (64 % CH == 0) {
+        latent_dma16(rows, to + i * 1024, tb_off + (j16 ^ (lat_swizzle(i * tpi) * 16)), i * tpi * kStride);
+      } else {
+        const uint32_t p = i * 64 + lane, tok = p / CH, j = (p % CH) ^ lat_swizzle(tok);
+        latent_dma16(rows, to + i * 1024, tok * kStride + j * 16, 0);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)  // token i * 16 + lane / 4, piece (lane % 4) ^ (token / 2 % 4)
+      latent_dma16(rows, to + L::kLat + i * 1024,
+                   (i * 16 + key_tok) * kStride + RP + (((lane & 3) ^ ((key_tok >> 1) & 3)) * 16), 0);
+    const auto scales = latent_rsrc(sq.rows.scales + (size_t)tile * kLatentTile * 2, kLatentTile * 8);
+    latent_dma4(scales, to + L::kLat + L::kKey, lane * 4);
+  };
+
+  // LDS offsets of this lane: codes of token `col` (score operand) and of the 8
+  // tokens of a transposing read.
+  const uint32_t sw = lat_swizzle(col);
+  uint32_t ka[4], va[4];
+  const uint32_t trow = (lane & 15) >> 1, vtok = 4 * half + (trow < 4 ? trow : trow + 4);
+#pragma unroll
+  for (uint32_t v = 0; v < 4; ++v) {
+    ka[v] = col * RP + (((2 * v + half) ^ sw) * 16);
+    va[v] = vtok * RP + (((2 * v + ((lane >> 4) & 1)) ^ lat_swizzle(vtok)) * 16) + 8 * (lane & 1);
+  }
+
+  floatx16 O[kBlocks];
+#pragma unroll
+  for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) O[i][j] = 0.0f;
+  float mref = kNoMax, l = 0.0f;
+
+  const uint32_t first = t_begin + wave;
+  const uint32_t count = first < t_end ? (t_end - first + 3) / 4 : 0;
+#pragma unroll
+  for (int i = 0; i < L::kRing - 1; ++i)
+    if ((uint32_t)i < count) issue(first + 4 * i, i);
+  uint32_t slot = 0;
+  for (uint32_t it = 0; it < count; ++it) {
+    const uint32_t tile = first + 4 * it;
+    if (it + L::kRing - 1 < count) {
+      const uint32_t to = slot + L::kRing - 1;
+      issue(tile + 4 * (L::kRing - 1), to >= L::kRing ? to - L::kRing : to);
+      latent_wait_vmcnt<L::kDma*(L::kRing - 1) < 63 ? L::kDma * (L::kRing - 1) : 63>();
+    } else {
+      latent_wait_vmcnt<0>();
+    }
+    const uint8_t* lat = ring + slot * L::kTileBytes;
+    const uint8_t* key = lat + L::kLat;
+    const float* scales = (const float*)(key + L::kKey);
+
+    // Scores: the shared key's part, then the latent's.
+    float S[16];
+    float ts[16];  // this lane's tokens' latent scales
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const floatx4 s0 = *(const floatx4*)(scales + (8 * g + 4 * half) * 2);
+      const floatx4 s1 = *(const floatx4*)(scales + (8 * g + 4 * half) * 2 + 4);
+      ts[4 * g] = s0[0], ts[4 * g + 1] = s0[2], ts[4 * g + 2] = s1[0], ts[4 * g + 3] = s1[2];
+      S[4 * g] = s0[1], S[4 * g + 1] = s0[3], S[4 * g + 2] = s1[1], S[4 * g + 3] = s1[3];
+    }
+    {
+      intx16 hi = {}, lo = {};
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const u32x4 kf = *(const u32x4*)(key + col * kLatentRope + (((2 * s + half) ^ ((col >> 1) & 3)) * 16));
+        hi = mfma32x32x32_i8(kf, qhi[kLatSteps + s], hi);
+        lo = mfma32x32x32_i8(kf, qlo[kLatSteps + s], lo);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) S[i] = fmaf((float)hi[i], 256.0f, (float)lo[i]) * (S[i] * key_scale);
+    }
+    {
+      intx16 hi = {}, lo = {};
+#pragma unroll
+      for (int s = 0; s < kLatSteps; ++s) {
+        const u32x4 kf = *(const u32x4*)(lat + ka[s & 3] + (s >> 2) * 128);
+        hi = mfma32x32x32_i8(kf, qhi[s], hi);
+        lo = mfma32x32x32_i8(kf, qlo[s], lo);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) S[i] = fmaf(fmaf((float)hi[i], 256.0f, (float)lo[i]), ts[i] * lat_scale, S[i]);
+    }
+    const uint32_t tok0 = tile * kLatentTile + 4 * half;
+    const bool whole = (tile + 1) * kLatentTile <= lim_min && c_last - c_first == kLatentCols - 1;
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const bool seen = tok0 + 8 * (i / 4) + i % 4 < limit;
+        S[i] = seen ? S[i] : -INFINITY;
+        ts[i] = seen ? ts[i] : 0.0f;  // nothing of an unseen token, not even a scale that is no number
+      }
+    }
+    float top = S[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, S[i]);
+    top = halves_max(top);
+    if (__any(top > mref + 8.0f)) {
+      const float m = fmaxf(mref, top), f = __builtin_amdgcn_exp2f(mref - m);
+      mref = m;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) O[i][j] *= f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      S[i] = __builtin_amdgcn_exp2f(S[i] - mref);
+      l += S[i];
+      S[i] *= ts[i];
+    }
+    u32x4 p[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[u][i] = to_bf16x2(S[8 * u + 2 * i], S[8 * u + 2 * i + 1]);
+#pragma unroll
+    for (int rb = 0; rb < kBlocks; ++rb)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const u32x2 v = lds_read_tr8(lat + va[rb & 3] + (rb >> 2) * 128 + u * 16 * RP);
+        O[rb] = mfma32x32x16(bytes_to_bf16(v), p[u], O[rb]);
+      }
+    latent_wait_lds();  // before the DMA of a later tile writes here
+    slot = slot + 1 == L::kRing ? 0 : slot + 1;
+  }
+
+  // Merge the four waves: one maximum per column, then the sums, 128 latent
+  // elements at a time.
+  l = halves_sum(l);
+  __syncthreads();
+  float* ml = (float*)(lds + 4 * kLatentCols * L::kPad * 4);
+  if (half == 0) *(float2*)(ml + (wave * kLatentCols + col) * 2) = float2{mref, l};
+  __syncthreads();
+  float m = kNoMax, sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[(w * kLatentCols + col) * 2]);
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+    sum += ml[(w * kLatentCols + col) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * kLatentCols + col) * 2] - m);
+  const float f = __builtin_amdgcn_exp2f(mref - m);
+  if (wave == 0 && half == 0)
+    *(float2*)(a.partials + (size_t)a.units * kLatentCols * RP + ((size_t)unit * kLatentCols + col) * 2) =
+        float2{m, sum};
+  float* buf = (float*)lds;
+#pragma unroll
+  for (int q = 0; q < RP / 128; ++q) {
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        floatx4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = O[4 * q + rb][4 * g + i] * f;
+        *(floatx4*)(buf + (wave * kLatentCols + col) * L::kPad + 32 * rb + 8 * g + 4 * half) = v;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = i * 256 + threadIdx.x, cc = at / 32, r = (at % 32) * 4;
+      if (c_first + cc > c_last) break;
+      floatx4 v = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) v += *(const floatx4*)(buf + (w * kLatentCols + cc) * L::kPad + r);
+      *(floatx4*)(a.partials + ((size_t)unit * kLatentCols + cc) * RP + q * 128 + r) = v;
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Joining the splits, and out of the latent space
+// ---------------------------------------------------------------------------
+// One workgroup per (row, head) column: its splits' sums weighted by 2^(m - M),
+// divided by the joined softmax sum and rounded to bf16 (the operand of the
+// product with W_uv).
+template <int RP>
+__global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnArgs a) {
+  constexpr int kLanes = RP / 4, kGroups = 256 / kLanes;
+  __shared__ floatx4 part[256];
+  const uint32_t H = a.d.heads, m = blockIdx.x / H, h = blockIdx.x - m * H;
+  const LatentSeq& sq = a.seqs[a.decode ? m : 0];
+  const uint32_t cols = a.decode ? H : a.rows * H, blocks = (cols + kLatentCols - 1) / kLatentCols;
+  const uint32_t c = a.decode ? h : blockIdx.x, cb = c / kLatentCols, col = c % kLatentCols;
+  const uint32_t t = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const float* ml = a.partials + (size_t)a.units * kLatentCols * RP;
+  auto at = [&](uint32_t s) { return (size_t)(sq.unit_begin + s * blocks + cb) * kLatentCols + col; };
+  const uint32_t lane = threadIdx.x & 63;
+  float top = kNoMax, sum = 0.0f;
+  for (uint32_t s = lane; s < sq.splits; s += 64) top = fmaxf(top, ml[at(s) * 2]);
+  top = wave_allmax(top);
+  for (uint32_t s = lane; s < sq.splits; s += 64) {
+    const float2 v = *(const float2*)(ml + at(s) * 2);
+    sum += v.y * __builtin_amdgcn_exp2f(v.x - top);
+  }
+  sum = wave_allsum(sum);
+  floatx4 acc = {0, 0, 0, 0};
+  if (group < kGroups)
+    for (uint32_t s = group; s < sq.splits; s += kGroups) {
+      const float w = __builtin_amdgcn_exp2f(ml[at(s) * 2] - top);
+      acc += *(const floatx4*)(a.partials + at(s) * RP + 4 * t) * w;
+    }
+  part[threadIdx.x] = acc;
+  __syncthreads();
+  if (group != 0) return;
+#pragma unroll
+  for (int g = 1; g < kGroups; ++g) acc += part[g * kLanes + t];
+  const float r = 1.0f / sum;
+  *(u32x2*)(a.mixed + (size_t)blockIdx.x * RP + 4 * t) =
+      u32x2{to_bf16x2(acc[0] * r, acc[1] * r), to_bf16x2(acc[2] * r, acc[3] * r)};
+}
+
+// o[m][h][n] = sum_r mixed[m][h][r] W_uv[h][n][r]: workgroup = (16 rows, head),
+// a wave takes a quarter of the head's outputs.
+template <int RP>
+__global__ __launch_bounds__(256) void latent_up_kernel(LatentAttnArgs a) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, kq = lane >> 4;
+  const uint32_t h = blockIdx.y, m0 = blockIdx.x * 16, H = a.d.heads, vp = a.d.v_pad;
+  const uint16_t* up = a.up + ((size_t)h * (a.d.nope_pad + vp) + a.d.nope_pad) * RP;
+  const uint16_t* x = a.mixed + ((size_t)min(m0 + n, a.rows - 1) * H + h) * RP;
+  for (uint32_t n0 = 16 * wave; n0 < vp; n0 += 64) {
+    floatx4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < RP / 32; ++s)
+      acc = mfma16x16x32(*(const u32x4*)(x + 32 * s + 8 * kq), *(const u32x4*)(up + (size_t)(n0 + n) * RP + 32 * s + 8 * kq),
+                         acc);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t m = m0 + 4 * kq + i;
+      if (m < a.rows && n0 + n < a.d.v) a.o[((size_t)m * H + h) * a.d.v + n0 + n] = f32_to_bf16(acc[i]);
+    }
+  }
+}
+
+template <int RP>
+hipError_t absorbed(const LatentAttnArgs& a, hipStream_t st) {
+  const dim3 tiles((a.rows + 15) / 16, a.d.heads);
+  hipLaunchKernelGGL(latent_query_kernel<RP>, tiles, dim3(256), 0, st, a);
+  hipLaunchKernelGGL(latent_attn_kernel<RP>, dim3(a.units), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(latent_join_kernel<RP>, dim3(a.rows * a.d.heads), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(latent_up_kernel<RP>, tiles, dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_latent_absorbed(const LatentAttnArgs& a, hipStream_t st) {
+  switch (a.d.rank_pad) {
+    case 128: return absorbed<128>(a, st);
+    case 256: return absorbed<256>(a, st);
+    case 384: return absorbed<384>(a, st);
+    default: return absorbed<512>(a, st);
+  }
+}
+
+}  // namespace qm

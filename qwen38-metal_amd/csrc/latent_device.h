@@ -1,0 +1,80 @@
+// Device helpers of the latent attention kernels.
+#pragma once
+#include "common.h"
+
+namespace qm {
+
+typedef int intx4 __attribute__((ext_vector_type(4)));
+typedef int intx16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t latent_rsrc(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
+}
+
+// Builtins of the device pass only.
+#if defined(__HIP_DEVICE_COMPILE__)
+#define QM_LDS(T, p) ((__attribute__((address_space(3))) T*)(p))
+// Lane i's bytes at voff + soff land at lds + i * size.
+__device__ __forceinline__ void latent_dma16(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t voff, uint32_t soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, QM_LDS(void, lds), 16, voff, soff, 0, 0);
+}
+__device__ __forceinline__ void latent_dma4(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t voff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, QM_LDS(void, lds), 4, voff, 0, 0, 0);
+}
+// Transposing read of bytes: each 16 lanes read 8 rows of 16 bytes (lanes 2t
+// and 2t + 1 give the address of row t's two halves) and lane i receives byte i
+// of the 8 rows.
+__device__ __forceinline__ u32x2 lds_read_tr8(const uint8_t* lds) {
+  typedef int intx2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(QM_LDS(intx2, lds)));
+}
+__device__ __forceinline__ intx16 mfma32x32x32_i8(u32x4 a, u32x4 b, intx16 c) {
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(intx4, a), __builtin_bit_cast(intx4, b), c, 0, 0, 0);
+}
+#undef QM_LDS
+#else
+__device__ void latent_dma16(__amdgpu_buffer_rsrc_t, void*, uint32_t, uint32_t);
+__device__ void latent_dma4(__amdgpu_buffer_rsrc_t, void*, uint32_t);
+__device__ u32x2 lds_read_tr8(const uint8_t*);
+__device__ intx16 mfma32x32x32_i8(u32x4, u32x4, intx16);
+#endif
+
+// s_waitcnt vmcnt(n) (gfx9 encoding; expcnt and lgkmcnt left at their maxima).
+template <int N>
+__device__ __forceinline__ void latent_wait_vmcnt() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 0xF) | ((N >> 4) << 14));
+  __asm__ volatile("" ::: "memory");
+}
+// s_waitcnt lgkmcnt(0): this wave's LDS reads have returned.
+__device__ __forceinline__ void latent_wait_lds() {
+  __asm__ volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  __asm__ volatile("" ::: "memory");
+}
+
+// Two fp32 values -> packed bf16 (round to nearest even, v_cvt_pk_bf16_f32).
+typedef __bf16 latent_bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t to_bf16x2(float lo, float hi) {
+  const latent_bf16x2 v = {(__bf16)lo, (__bf16)hi};
+  return __builtin_bit_cast(uint32_t, v);
+}
+// 8 signed bytes -> 8 bf16, exact.
+__device__ __forceinline__ u32x4 bytes_to_bf16(u32x2 w) {
+  return u32x4{to_bf16x2((float)(int8_t)w.x, (float)(int8_t)(w.x >> 8)),
+               to_bf16x2((float)(int8_t)(w.x >> 16), (float)(int8_t)(w.x >> 24)),
+               to_bf16x2((float)(int8_t)w.y, (float)(int8_t)(w.y >> 8)),
+               to_bf16x2((float)(int8_t)(w.y >> 16), (float)(int8_t)(w.y >> 24))};
+}
+
+// Maximum of lanes l and l ^ 32, and their sum.
+__device__ __forceinline__ float halves_max(float v) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+}  // namespace qm

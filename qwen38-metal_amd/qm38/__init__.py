@@ -40,6 +40,12 @@ EXPORTS = [
     "qm_kv_create", "qm_kv_destroy", "qm_kv_length", "qm_kv_capacity", "qm_kv_allocated_pages", "qm_kv_page_for_token",
     "qm_kv_reserve", "qm_kv_truncate", "qm_kv_clone", "qm_kv_read",
     "qm_attn_decode", "qm_attn_decode_noalloc", "qm_attn_prefill", "qm_attn_prepare",
+    "qm_rotary",
+    "qm_latent_kv_create", "qm_latent_kv_destroy", "qm_latent_kv_length", "qm_latent_kv_capacity",
+    "qm_latent_kv_reserve", "qm_latent_kv_truncate", "qm_latent_kv_clone", "qm_latent_kv_read",
+    "qm_latent_append", "qm_latent_load",
+    "qm_latent_weights_create", "qm_latent_weights_create_q4", "qm_latent_weights_destroy",
+    "qm_latent_decode", "qm_latent_prefill",
     "qm_dn_weights_create", "qm_dn_weights_destroy", "qm_dn_state_create", "qm_dn_state_destroy",
     "qm_dn_state_clone", "qm_dn_state_read", "qm_dn_state_write", "qm_dn_step", "qm_dn_prefill",
     "qm_dn_snapshots_create", "qm_dn_snapshots_destroy", "qm_dn_prefill_snapshots", "qm_dn_snapshot_restore",
@@ -90,6 +96,33 @@ class RopeConfig(C.Structure):
     """qm_rope_config (RopeParameters, native.rs:119-197)."""
     _fields_ = [("head_dim", C.c_uint32), ("rotary_dim", C.c_uint32), ("rope_theta", C.c_float),
                 ("mrope_section1", C.c_uint32), ("mrope_section2", C.c_uint32), ("has_mrope_sections", C.c_uint32)]
+
+
+class RotaryConfig(C.Structure):
+    """qm_rotary_config: rotary positions on part of a head.  scaling: "none",
+    "linear" or "yarn"; attention_factor 0 takes the scaling's own."""
+    SCALINGS = ("none", "linear", "yarn")
+    _fields_ = [("rotary_dim", C.c_uint32), ("layout", C.c_uint32), ("theta", C.c_float), ("scaling", C.c_uint32),
+                ("factor", C.c_float), ("original_positions", C.c_uint32), ("beta_fast", C.c_float),
+                ("beta_slow", C.c_float), ("attention_factor", C.c_float)]
+
+    def __init__(self, rotary_dim: int, interleaved: bool = False, theta: float = 1e4, scaling: str = "none",
+                 factor: float = 1.0, original_positions: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                 attention_factor: float = 0.0):
+        super().__init__(rotary_dim, int(interleaved), theta, self.SCALINGS.index(scaling), factor,
+                         original_positions, beta_fast, beta_slow, attention_factor)
+
+
+class RotaryTensor(C.Structure):
+    """qm_rotary_tensor"""
+    _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("offset", C.c_uint32), ("in_stride", C.c_uint64), ("out_stride", C.c_uint64)]
+
+
+class LatentConfig(C.Structure):
+    """qm_latent_config: the widths of latent attention and its softmax scale."""
+    _fields_ = [("heads", C.c_uint32), ("rank", C.c_uint32), ("nope_dim", C.c_uint32), ("rope_dim", C.c_uint32),
+                ("v_dim", C.c_uint32), ("softmax_scale", C.c_float)]
 
 
 class DecodeLinearLayer(C.Structure):
@@ -168,6 +201,22 @@ def load(path: str | os.PathLike | None = None) -> C.CDLL:
         "qm_attn_prefill": ([vp, vp, vp, vp, vp, vp, u32, u32, vp], i32),
         "qm_attn_prepare": ([vp, C.POINTER(RopeConfig), u32, u32, u32, vp, vp, vp, vp, C.c_float, vp, u32, vp, vp,
                              vp], i32),
+        "qm_rotary": ([vp, C.POINTER(RotaryConfig), C.POINTER(RotaryTensor), u32, u32, vp, u32], i32),
+        "qm_latent_kv_create": ([vp, u32, u32, u32, C.POINTER(vp)], i32),
+        "qm_latent_kv_destroy": ([vp], None),
+        "qm_latent_kv_length": ([vp], u32),
+        "qm_latent_kv_capacity": ([vp], u32),
+        "qm_latent_kv_reserve": ([vp, u32], i32),
+        "qm_latent_kv_truncate": ([vp, u32], i32),
+        "qm_latent_kv_clone": ([vp, C.POINTER(vp)], i32),
+        "qm_latent_kv_read": ([vp, vp, vp], i32),
+        "qm_latent_append": ([vp, vp, vp, vp, C.c_float, u32], i32),
+        "qm_latent_load": ([vp, vp, u32, u32, vp], i32),
+        "qm_latent_weights_create": ([vp, C.POINTER(LatentConfig), vp, C.POINTER(vp)], i32),
+        "qm_latent_weights_create_q4": ([vp, C.POINTER(LatentConfig), C.POINTER(Q4Job), C.POINTER(vp)], i32),
+        "qm_latent_weights_destroy": ([vp], None),
+        "qm_latent_decode": ([vp, vp, C.POINTER(vp), u32, vp, vp, vp, C.c_float, vp], i32),
+        "qm_latent_prefill": ([vp, vp, vp, vp, vp, vp, C.c_float, u32, vp], i32),
         "qm_dn_weights_create": ([vp, C.POINTER(DnConfig), vp, vp, vp, vp, C.POINTER(vp)], i32),
         "qm_dn_weights_destroy": ([vp], None),
         "qm_dn_state_create": ([vp, vp, C.POINTER(vp)], i32),
@@ -336,6 +385,40 @@ class Runtime:
         _check(self.lib.qm_attn_prepare(self.handle, C.byref(rope), rows, num_heads, kv_heads, _ptr(q_with_gate),
                                         _ptr(k), _ptr(q_norm), _ptr(k_norm), epsilon, _ptr(positions),
                                         position_base, _ptr(q_out), _ptr(gate_out), _ptr(k_out)))
+
+    # ---- rotary positions and latent attention --------------------------------
+    def rotary(self, config: RotaryConfig, tensors, rows: int, positions=None, position_base: int = 0) -> None:
+        """qm_rotary: rotates `rows` rows of up to four tensors in one launch.
+        tensors: (in, out, heads, head_dim, offset[, in_stride, out_stride])
+        each; out may be in (in place).  positions: uint32/int32 [rows] on the
+        device, or None for position_base + row."""
+        arr = (RotaryTensor * len(tensors))()
+        for t, (src, dst, *rest) in zip(arr, tensors):
+            t.in_, t.out = _ptr(src), _ptr(dst)
+            t.heads, t.head_dim, t.offset = rest[:3]
+            t.in_stride, t.out_stride = rest[3:] or (0, 0)
+        _check(self.lib.qm_rotary(self.handle, C.byref(config), arr, len(tensors), rows, _ptr(positions),
+                                  position_base))
+
+    def create_latent_kv(self, rank: int, rope_dim: int, max_tokens: int = 0) -> "LatentKv":
+        """The 8-bit cache of latent attention; max_tokens = 0 grows without limit."""
+        return LatentKv(self, rank, rope_dim, max_tokens)
+
+    def create_latent_weights(self, config: LatentConfig, kv_b) -> "LatentWeights":
+        """kv_b: bf16 [heads][nope_dim + v_dim][rank] on the device, or a Q4Job of those rows."""
+        return LatentWeights(self, config, kv_b)
+
+    def latent_attention(self, weights: "LatentWeights", seqs, q, kv, norm, epsilon: float, o) -> None:
+        """One new token for each sequence of a ragged batch (qm_latent_decode)."""
+        arr = (C.c_void_p * len(seqs))(*[s.handle for s in seqs])
+        _check(self.lib.qm_latent_decode(self.handle, weights.handle, arr, len(seqs), _ptr(q), _ptr(kv), _ptr(norm),
+                                         epsilon, _ptr(o)))
+
+    def latent_attention_prefill(self, weights: "LatentWeights", seq: "LatentKv", q, kv, norm, epsilon: float,
+                                 rows: int, o) -> None:
+        """`rows` new rows of one sequence over its cache (qm_latent_prefill)."""
+        _check(self.lib.qm_latent_prefill(self.handle, weights.handle, seq.handle, _ptr(q), _ptr(kv), _ptr(norm),
+                                          epsilon, rows, _ptr(o)))
 
     # ---- DeltaNet ---------------------------------------------------------
     def create_deltanet_weights(self, config: DnConfig, conv_weight, a_log, dt_bias, norm) -> "DnWeights":
@@ -521,6 +604,94 @@ class KvCache:
         _check(self.rt.lib.qm_kv_read(self.handle, keys.ctypes.data, values.ctypes.data, ks.ctypes.data,
                                       vs.ctypes.data))
         return keys, values, ks, vs
+
+
+class LatentKv:
+    """qm_latent_kv: the 8-bit cache of latent attention."""
+
+    def __init__(self, rt: Runtime, rank: int, rope_dim: int, max_tokens: int, handle=None):
+        self.rt = rt
+        self.rank = rank
+        self.rope_dim = rope_dim
+        self.max_tokens = max_tokens
+        if handle is None:
+            handle = C.c_void_p()
+            _check(rt.lib.qm_latent_kv_create(rt.handle, rank, rope_dim, max_tokens, C.byref(handle)))
+        self.handle = handle
+        rt._children.add(self)
+
+    def close(self) -> None:
+        if self.handle:
+            self.rt.lib.qm_latent_kv_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    @property
+    def sequence_length(self) -> int:
+        return self.rt.lib.qm_latent_kv_length(self.handle)
+
+    @property
+    def capacity_tokens(self) -> int:
+        return self.rt.lib.qm_latent_kv_capacity(self.handle)
+
+    def reserve(self, additional: int) -> None:
+        _check(self.rt.lib.qm_latent_kv_reserve(self.handle, additional))
+
+    def truncate(self, length: int) -> None:
+        _check(self.rt.lib.qm_latent_kv_truncate(self.handle, length))
+
+    def clone(self) -> "LatentKv":
+        h = C.c_void_p()
+        _check(self.rt.lib.qm_latent_kv_clone(self.handle, C.byref(h)))
+        return LatentKv(self.rt, self.rank, self.rope_dim, self.max_tokens, handle=h)
+
+    def append(self, rows, norm, epsilon: float, count: int) -> None:
+        """Quantises `count` rows (bf16 [count][rank + rope_dim]) behind the
+        cached tokens, the latent RMS-normalised with `norm` (None: as given)."""
+        _check(self.rt.lib.qm_latent_append(self.rt.handle, self.handle, _ptr(rows), _ptr(norm), epsilon, count))
+
+    def load(self, first: int, count: int, out) -> None:
+        """Reads tokens first .. first + count - 1 back as bf16 [count][rank + rope_dim]."""
+        _check(self.rt.lib.qm_latent_load(self.rt.handle, self.handle, first, count, _ptr(out)))
+
+    def read(self):
+        """Host copies: (codes int8 [T][rank + rope_dim], scales f32 [T][2])."""
+        import numpy as np
+        codes = np.zeros((self.sequence_length, self.rank + self.rope_dim), np.int8)
+        scales = np.zeros((self.sequence_length, 2), np.float32)
+        _check(self.rt.lib.qm_latent_kv_read(self.handle, codes.ctypes.data, scales.ctypes.data))
+        return codes, scales
+
+
+class LatentWeights:
+    """qm_latent_weights: the projection out of the latent space, laid out for both forms."""
+
+    def __init__(self, rt: Runtime, config: LatentConfig, kv_b):
+        self.rt = rt
+        self.config = config
+        h = C.c_void_p()
+        if isinstance(kv_b, Q4Job):
+            _check(rt.lib.qm_latent_weights_create_q4(rt.handle, C.byref(config), C.byref(kv_b), C.byref(h)))
+        else:
+            _check(rt.lib.qm_latent_weights_create(rt.handle, C.byref(config), _ptr(kv_b), C.byref(h)))
+        self.handle = h
+        rt._children.add(self)
+
+    def close(self) -> None:
+        if self.handle:
+            self.rt.lib.qm_latent_weights_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class DnWeights:

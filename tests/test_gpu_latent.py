@@ -1,0 +1,493 @@
+"""GPU tests of rotary positions, the 8-bit latent cache and latent attention
+against plain forms in 64 bits."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import qm38
+from gpu_util import to_dev, tuned
+from latent_util import HALF, assert_attention, attention, frequencies, quantised, rotated
+from qm38 import synth
+
+pytestmark = pytest.mark.gpu
+
+EPS = 1e-6
+WIDE, SMALL, ODD, TINY = (512, 64, 128, 128), (256, 32, 64, 64), (384, 48, 96, 80), (8, 8, 8, 8)
+
+
+def bf16(gen, *shape, std=1.0):
+    return (torch.randn(shape, generator=gen, device="cuda:0") * std).to(torch.bfloat16)
+
+
+def generator(seed):
+    g = torch.Generator(device="cuda:0")
+    g.manual_seed(seed)
+    return g
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions
+# ---------------------------------------------------------------------------
+def check_rotated(got, x, positions, freq, factor, offset, interleaved):
+    ref = rotated(x, positions, freq, factor, offset, interleaved)
+    rd = 2 * len(freq)
+    inside = torch.zeros(x.shape[-1], dtype=torch.bool, device=x.device)
+    inside[offset:offset + rd] = True
+    assert torch.equal(got[..., ~inside], x[..., ~inside])
+    # fp32 sine, cosine and products of the pair, then half a bf16 step.
+    pair = rotated(x.abs(), torch.zeros_like(positions), freq, 1.0, offset, interleaved)
+    size = (x.double().abs().amax() * factor) * 1e-6
+    err = (got.double() - ref).abs()
+    assert (err <= ref.abs() * HALF + size)[..., inside].all()
+    assert pair.shape == ref.shape
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("rows,heads,width,offset,rd", [
+    (1, 1, 2, 0, 2), (1, 20, 192, 128, 64), (5, 20, 192, 128, 64), (300, 3, 128, 0, 128), (7, 5, 65, 3, 30),
+    (33, 2, 256, 0, 256), (2, 7, 96, 8, 24), (65, 64, 64, 16, 32)])
+@pytest.mark.parametrize("scaling,factor", [("none", 1.0), ("linear", 4.0), ("yarn", 8.0)])
+def test_rotary(rt, interleaved, rows, heads, width, offset, rd, scaling, factor):
+    g = generator(rows + width)
+    x = bf16(g, rows, heads, width)
+    positions = torch.randint(0, 1 << 20, (rows,), generator=g, device="cuda:0", dtype=torch.int32)
+    cfg = qm38.RotaryConfig(rd, interleaved, 1e6, scaling, factor, 4096)
+    freq, mul = frequencies(rd, 1e6, scaling, factor, 4096, device="cuda:0")
+    out = torch.full_like(x, 7.0)
+    rt.rotary(cfg, [(x, out, heads, width, offset)], rows, positions=positions)
+    check_rotated(out, x, positions, freq, mul, offset, interleaved)
+    same = x.clone()
+    rt.rotary(cfg, [(same, same, heads, width, offset)], rows, positions=positions)
+    assert torch.equal(same, out)
+
+
+def test_rotary_of_strided_tensors_in_one_launch(rt):
+    """Queries and key inside one projection row, in place; the rest of the row stays."""
+    g = generator(3)
+    rows, H = 19, 6
+    row = bf16(g, rows, H * 192 + 576 + 40)
+    before = row.clone()
+    base = 2 ** 32 - 19  # the last positions that fit
+    cfg = qm38.RotaryConfig(64, True, 1e4)
+    freq, _ = frequencies(64, 1e4, device="cuda:0")
+    q, kv = row[:, :H * 192], row[:, H * 192:H * 192 + 576]
+    s = row.shape[1]
+    rt.rotary(cfg, [(q, q, H, 192, 128, s, s), (kv, kv, 1, 576, 512, s, s)], rows, position_base=base)
+    positions = torch.arange(rows, device="cuda:0", dtype=torch.float64) + base
+    check_rotated(q.reshape(rows, H, 192), before[:, :H * 192].reshape(rows, H, 192), positions, freq, 1.0, 128, True)
+    check_rotated(kv[:, None], before[:, None, H * 192:H * 192 + 576], positions, freq, 1.0, 512, True)
+    assert torch.equal(row[:, H * 192 + 576:], before[:, H * 192 + 576:])
+    # From one column of a buffer to another: rows interleave, elements do not meet.
+    out = torch.zeros(rows, 2, 64, dtype=torch.bfloat16, device="cuda:0")
+    out[:, 0] = before[:, :64]
+    rt.rotary(qm38.RotaryConfig(64), [(out[:, 0], out[:, 1], 1, 64, 0, 128, 128)], rows)
+    positions = torch.arange(rows, device="cuda:0")
+    check_rotated(out[:, 1:], before[:, None, :64], positions, freq, 1.0, 0, False)
+    assert torch.equal(out[:, 0], before[:, :64])
+
+
+def test_rotary_unaligned_equals_aligned(rt):
+    g = generator(4)
+    flat = bf16(g, 9 * 3 * 96 + 1)
+    x = flat[1:].reshape(9, 3, 96)  # 2-byte aligned
+    y, z = torch.empty_like(x), torch.empty_like(x)
+    for interleaved in (False, True):
+        cfg = qm38.RotaryConfig(32, interleaved)
+        rt.rotary(cfg, [(x, y, 3, 96, 64)], 9, position_base=77)
+        rt.rotary(cfg, [(x.clone(), z, 3, 96, 64)], 9, position_base=77)
+        assert torch.equal(y, z)
+
+
+def test_rotary_captured(rt):
+    """A captured call replayed with other positions in its buffer, with eager calls between."""
+    g = generator(5)
+    x = bf16(g, 33, 8, 192)
+    out = torch.empty_like(x)
+    positions = torch.arange(33, device="cuda:0", dtype=torch.int32)
+    cfg = qm38.RotaryConfig(64, True, 1e6, "yarn", 4.0, 8192)
+    call = lambda o: rt.rotary(cfg, [(x, o, 8, 192, 128)], 33, positions=positions)  # noqa: E731
+    graph = torch.cuda.CUDAGraph()
+    stream = torch.cuda.Stream()
+    try:
+        with torch.cuda.graph(graph, stream=stream):
+            rt.set_stream(stream)
+            call(out)
+    finally:
+        rt.set_stream(torch.cuda.current_stream())
+    for i in range(4):
+        positions += 1000 * i
+        eager = torch.empty_like(x)
+        call(eager)
+        out.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+
+
+# ---------------------------------------------------------------------------
+# The cache
+# ---------------------------------------------------------------------------
+def held(cache):
+    """(latents, keys) float64 that a cache stands for."""
+    codes, scales = (torch.from_numpy(a).to("cuda:0").double() for a in cache.read())
+    return codes[:, :cache.rank] * scales[:, :1], codes[:, cache.rank:] * scales[:, 1:]
+
+
+@pytest.mark.parametrize("widths", [WIDE, SMALL, ODD, TINY, (136, 64, 8, 8)])
+@pytest.mark.parametrize("pieces", [(1,), (3, 1, 60, 1), (64,), (65, 400), (1000,)])
+def test_cache_codes(rt, widths, pieces):
+    rank, rope = widths[:2]
+    g = generator(sum(pieces) + rank)
+    cache = rt.create_latent_kv(rank, rope)
+    rows = bf16(g, sum(pieces), rank + rope)
+    rows[0] = 0  # the smallest scale
+    rows[-1, rank:] *= 1e30
+    at = 0
+    for n in pieces:
+        cache.append(rows[at:at + n].clone(), None, 0.0, n)
+        at += n
+    assert cache.sequence_length == at <= cache.capacity_tokens
+    codes, scales = cache.read()
+    for part, (lo, hi) in enumerate(((0, rank), (rank, rank + rope))):
+        c, s = quantised(rows[:, lo:hi].double())
+        assert np.array_equal(codes[:, lo:hi], c.cpu().numpy())
+        assert np.array_equal(scales[:, part], s[:, 0].cpu().numpy())
+    # Read back: the products rounded once.
+    first = at // 3
+    out = torch.empty(at - first, rank + rope, dtype=torch.bfloat16, device="cuda:0")
+    cache.load(first, at - first, out)
+    want = torch.cat([torch.from_numpy(codes[:, lo:hi]).float() * torch.from_numpy(scales[:, p:p + 1])
+                      for p, (lo, hi) in enumerate(((0, rank), (rank, rank + rope)))], 1)[first:]
+    assert torch.equal(out.cpu(), want.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("widths", [WIDE, SMALL, ODD, TINY])
+def test_cache_normalised(rt, widths):
+    rank, rope = widths[:2]
+    g = generator(rank)
+    rows = bf16(g, 500, rank + rope, std=3.0)
+    norm = torch.rand(rank, generator=g, device="cuda:0") + 0.5
+    cache = rt.create_latent_kv(rank, rope)
+    cache.append(rows, norm, EPS, 500)
+    latent, key = held(cache)
+    x = rows[:, :rank].double()
+    x = x / (x.pow(2).mean(-1, keepdim=True) + EPS).sqrt() * norm.double()
+    # Half a step of the scale, and fp32's error of the norm (a few 2^-24 of the value).
+    step = x.abs().amax(-1, keepdim=True) / 127
+    assert ((latent - x).abs() <= step * (0.5 + 1e-4)).all()
+    c, s = quantised(rows[:, rank:].double())
+    assert torch.equal(key, c * s.double())
+
+
+def test_cache_clone_truncate_reserve(rt):
+    g = generator(9)
+    rows = bf16(g, 300, 576)
+    cache = rt.create_latent_kv(512, 64, max_tokens=300)
+    cache.append(rows, None, 0.0, 100)
+    copy = cache.clone()
+    assert copy.sequence_length == 100 and copy.capacity_tokens == cache.capacity_tokens
+    cache.truncate(10)
+    cache.append(rows[200:], None, 0.0, 100)
+    cache.reserve(190)
+    assert cache.capacity_tokens == 300
+    a, b = cache.read(), copy.read()
+    assert np.array_equal(a[0][:10], b[0][:10]) and not np.array_equal(a[0][10:100], b[0][10:100])
+    with pytest.raises(qm38.QmError) as e:
+        cache.append(rows, None, 0.0, 191)
+    assert e.value.status == "QM_ERR_CAPACITY_EXCEEDED" and cache.sequence_length == 110
+    # The copy's bytes are its own.
+    copy.append(rows[100:], None, 0.0, 200)
+    whole = rt.create_latent_kv(512, 64)
+    whole.append(rows, None, 0.0, 300)
+    for x, y in zip(copy.read(), whole.read()):
+        assert np.array_equal(x, y)
+    for c in (cache, copy, whole):
+        c.close()
+
+
+# ---------------------------------------------------------------------------
+# Attention
+# ---------------------------------------------------------------------------
+def make_weights(rt, g, H, widths, std=None):
+    rank, rope, nope, v = widths
+    kv_b = bf16(g, H, nope + v, rank, std=rank ** -0.5 if std is None else std)
+    scale = (nope + rope) ** -0.5
+    return kv_b, scale, rt.create_latent_weights(qm38.LatentConfig(H, rank, nope, rope, v, scale), kv_b)
+
+
+def filled(rt, g, widths, n, norm):
+    rank, rope = widths[:2]
+    cache = rt.create_latent_kv(rank, rope)
+    if n:
+        cache.append(bf16(g, n, rank + rope), norm, EPS, n)
+    return cache
+
+
+def check_decode(rt, widths, H, lengths, seed, q_std=1.5):
+    rank, rope, nope, v = widths
+    g = generator(seed)
+    kv_b, scale, weights = make_weights(rt, g, H, widths)
+    norm = torch.rand(rank, generator=g, device="cuda:0") + 0.5
+    caches = [filled(rt, g, widths, n, norm) for n in lengths]
+    B = len(lengths)
+    q, kv = bf16(g, B, H, nope + rope, std=q_std), bf16(g, B, rank + rope)
+    o = torch.full((B, H, v), float("nan"), dtype=torch.bfloat16, device="cuda:0")
+    rt.latent_attention(weights, caches, q, kv, norm, EPS, o)
+    for b, cache in enumerate(caches):
+        assert cache.sequence_length == lengths[b] + 1
+        latent, key = held(cache)
+        ref, bound = attention(q[b:b + 1], latent, key, kv_b, nope, scale, lengths[b])
+        assert_attention(o[b:b + 1], ref, bound, f"sequence {b} of {lengths[b]}")
+    again = torch.empty_like(o)
+    for cache, n in zip(caches, lengths):
+        cache.truncate(n)
+    rt.latent_attention(weights, caches, q, kv, norm, EPS, again)
+    assert torch.equal(o, again)
+
+
+@pytest.mark.parametrize("widths", [WIDE, SMALL, ODD, TINY, (128, 16, 24, 128), (264, 64, 128, 8)])
+@pytest.mark.parametrize("H", [1, 5, 32, 33])
+def test_decode_widths(rt, widths, H):
+    check_decode(rt, widths, H, [0, 1, 31, 32, 63, 255, 256, 700], H)
+
+
+@pytest.mark.parametrize("H,lengths", [(128, [4097]), (64, [20000, 3, 8191]), (20, [70001]), (8, [5] * 64),
+                                       (16, [2047, 2048, 2049])])
+def test_decode_lengths(rt, H, lengths):
+    check_decode(rt, WIDE, H, lengths, H)
+
+
+def test_decode_peaked(rt):
+    """Scores of some hundreds: one token takes almost all of a row, the running
+    maximum rises through the cache and falls behind."""
+    check_decode(rt, SMALL, 40, [3000, 10], 1, q_std=60.0)
+
+
+def check_prefill(rt, widths, H, cached, rows, seed, q_std=1.5):
+    rank, rope, nope, v = widths
+    g = generator(seed)
+    kv_b, scale, weights = make_weights(rt, g, H, widths)
+    norm = torch.rand(rank, generator=g, device="cuda:0") + 0.5
+    cache = filled(rt, g, widths, cached, norm)
+    q, kv = bf16(g, rows, H, nope + rope, std=q_std), bf16(g, rows, rank + rope)
+    o = torch.full((rows, H, v), float("nan"), dtype=torch.bfloat16, device="cuda:0")
+    rt.latent_attention_prefill(weights, cache, q, kv, norm, EPS, rows, o)
+    assert cache.sequence_length == cached + rows
+    latent, key = held(cache)
+    ref, bound = attention(q, latent, key, kv_b, nope, scale, cached)
+    assert_attention(o, ref, bound, f"{rows} rows on {cached}")
+    cache.truncate(cached)
+    again = torch.empty_like(o)
+    rt.latent_attention_prefill(weights, cache, q, kv, norm, EPS, rows, again)
+    assert torch.equal(o, again)
+
+
+@pytest.mark.parametrize("widths", [WIDE, SMALL, ODD, TINY])
+@pytest.mark.parametrize("H,cached,rows", [(1, 0, 1), (5, 0, 33), (3, 1000, 7), (20, 31, 130), (33, 64, 65)])
+def test_prefill_widths(rt, widths, H, cached, rows):
+    check_prefill(rt, widths, H, cached, rows, H + rows)
+
+
+@pytest.mark.parametrize("H,cached,rows", [(32, 20001, 5), (64, 0, 300), (8, 4096, 513), (128, 100, 40), (2, 0, 2000)])
+def test_prefill_sizes(rt, H, cached, rows):
+    check_prefill(rt, WIDE, H, cached, rows, H + rows)
+
+
+def test_prefill_peaked(rt):
+    check_prefill(rt, ODD, 12, 700, 300, 2, q_std=60.0)
+
+
+def test_prefill_in_pieces_equals_decode_steps(rt):
+    """A prompt in two chunks and tokens decoded one by one leave the same cache;
+    their outputs agree with one prefill of all rows within both forms' bounds."""
+    rank, rope, nope, v = WIDE
+    g = generator(11)
+    H, rows = 20, 230
+    kv_b, scale, weights = make_weights(rt, g, H, WIDE)
+    norm = torch.rand(rank, generator=g, device="cuda:0") + 0.5
+    q, kv = bf16(g, rows, H, nope + rope, std=1.5), bf16(g, rows, rank + rope)
+    o = torch.empty(rows, H, v, dtype=torch.bfloat16, device="cuda:0")
+    whole, parts = rt.create_latent_kv(rank, rope), rt.create_latent_kv(rank, rope)
+    rt.latent_attention_prefill(weights, whole, q, kv, norm, EPS, rows, o)
+    p = torch.empty_like(o)
+    for lo, hi in ((0, 200), (200, 220)):
+        rt.latent_attention_prefill(weights, parts, q[lo:hi].clone(), kv[lo:hi].clone(), norm, EPS, hi - lo, p[lo:hi])
+    for i in range(220, rows):
+        rt.latent_attention(weights, [parts], q[i:i + 1].clone(), kv[i:i + 1].clone(), norm, EPS, p[i:i + 1])
+    for x, y in zip(whole.read(), parts.read()):
+        assert np.array_equal(x, y)
+    latent, key = held(whole)
+    ref, bound = attention(q, latent, key, kv_b, nope, scale, 0)
+    assert_attention(o, ref, bound, "whole")
+    assert_attention(p, ref, bound, "pieces")
+
+
+def test_weights_from_q4(rt, torch_dev):
+    """kv_b as a Q4 job gives what its values rounded to bf16 give."""
+    rank, rope, nope, v = 256, 64, 64, 48
+    H = 6
+    rng = np.random.default_rng(12)
+    g = generator(12)
+    mat = synth.q4_matrix(rng, H * (nope + v), rank)
+    job = qm38.Runtime.job(*(to_dev(a, torch_dev) for a in mat), mat[0].shape[0])
+    w = synth.unpack_q4(mat[0]).astype(np.float32).reshape(-1, rank // 64, 64)
+    w = w * synth.bf16_to_f32(mat[1])[..., None] + synth.bf16_to_f32(mat[2])[..., None]
+    plain = torch.from_numpy(w.reshape(H, nope + v, rank)).to(torch.bfloat16).to(torch_dev)
+    cfg = qm38.LatentConfig(H, rank, nope, rope, v, 0.1)
+    outs = []
+    q, kv = bf16(g, 40, H, nope + rope), bf16(g, 40, rank + rope)
+    for source in (job, plain):
+        weights = rt.create_latent_weights(cfg, source)
+        cache = rt.create_latent_kv(rank, rope)
+        o = torch.empty(40, H, v, dtype=torch.bfloat16, device=torch_dev)
+        rt.latent_attention_prefill(weights, cache, q, kv, None, 0.0, 40, o)
+        outs.append(o)
+    assert torch.equal(*outs)
+
+
+def test_numbers_that_are_none(rt):
+    """A token whose row holds an infinity or NaN poisons the rows that see it,
+    and no other; a query that does poisons its own row and head."""
+    rank, rope, nope, v = SMALL
+    g = generator(13)
+    H, rows = 5, 40
+    kv_b, scale, weights = make_weights(rt, g, H, SMALL)
+    q, kv = bf16(g, rows, H, nope + rope), bf16(g, rows, rank + rope)
+    kv[30, 3] = float("inf")
+    kv[35, rank + 2] = float("-inf")
+    q[7, 2, 5] = float("nan")
+    q[9, 1, nope + 3] = float("inf")
+    cache = rt.create_latent_kv(rank, rope)
+    o = torch.zeros(rows, H, v, dtype=torch.bfloat16, device="cuda:0")
+    rt.latent_attention_prefill(weights, cache, q, kv, None, 0.0, rows, o)
+    bad = torch.isnan(o).all(-1)
+    want = torch.zeros_like(bad)
+    want[30:] = True
+    want[7, 2] = want[9, 1] = True
+    assert torch.equal(bad, want)
+    assert torch.equal(torch.isfinite(o).all(-1), ~want)
+
+
+def test_streams_in_turn(torch_dev):
+    """Calls of one runtime on several streams share its workspaces; each gives
+    what it gives alone."""
+    rank, rope, nope, v = SMALL
+    with tuned() as rt:
+        g = generator(14)
+        H = 8
+        kv_b, scale, weights = make_weights(rt, g, H, SMALL)
+        streams = [torch.cuda.Stream() for _ in range(3)]
+        caches = [filled(rt, g, SMALL, 900 + 100 * i, None) for i in range(3)]
+        q, kv = bf16(g, 3, H, nope + rope), bf16(g, 3, rank + rope)
+        alone, outs = [], [[torch.empty(1, H, v, dtype=torch.bfloat16, device=torch_dev) for _ in range(6)] for _ in range(3)]
+        for i, cache in enumerate(caches):
+            o = torch.empty(1, H, v, dtype=torch.bfloat16, device=torch_dev)
+            rt.latent_attention(weights, [cache], q[i:i + 1].clone(), kv[i:i + 1].clone(), None, 0.0, o)
+            cache.truncate(cache.sequence_length - 1)
+            alone.append(o)
+        qs, kvs = [q[i:i + 1].clone() for i in range(3)], [kv[i:i + 1].clone() for i in range(3)]
+        busy = torch.randn(2048, 2048, device=torch_dev)
+        torch.cuda.synchronize()
+        for s in streams:
+            with torch.cuda.stream(s):
+                busy @ busy
+        for r in range(6):
+            for i, s in enumerate(streams):
+                rt.set_stream(s)
+                rt.latent_attention(weights, [caches[i]], qs[i], kvs[i], None, 0.0, outs[i][r])
+                caches[i].truncate(caches[i].sequence_length - 1)
+        torch.cuda.synchronize()
+        rt.set_stream(torch.cuda.current_stream())
+        for i in range(3):
+            for o in outs[i]:
+                assert torch.equal(o, alone[i])
+
+
+def test_cache_used_from_another_runtime(rt, torch_dev):
+    """The owner's append comes before another runtime's attention, and after it the owner's read."""
+    rank, rope, nope, v = SMALL
+    with tuned() as other:
+        other.set_stream(torch.cuda.Stream())
+        g = generator(15)
+        kv_b, scale, weights = make_weights(rt, g, 4, SMALL)
+        q, kv = bf16(g, 1, 4, nope + rope), bf16(g, 1, rank + rope)
+        rows = bf16(g, 5000, rank + rope)
+        o = torch.empty(1, 4, v, dtype=torch.bfloat16, device=torch_dev)
+        torch.cuda.synchronize()
+        cache = rt.create_latent_kv(rank, rope)
+        cache.append(rows, None, 0.0, 5000)
+        other.latent_attention(weights, [cache], q, kv, None, 0.0, o)
+        latent, key = held(cache)
+        torch.cuda.synchronize()
+        ref, bound = attention(q, latent, key, kv_b, nope, scale, 5000)
+        assert_attention(o, ref, bound)
+
+
+# ---------------------------------------------------------------------------
+# Refusals
+# ---------------------------------------------------------------------------
+def refused(status, call, *args, **kw):
+    with pytest.raises(qm38.QmError) as e:
+        call(*args, **kw)
+    assert e.value.status == status, e.value
+
+
+def test_refusals(rt):
+    rank, rope, nope, v = SMALL
+    g = generator(16)
+    kv_b, scale, weights = make_weights(rt, g, 4, SMALL)
+    q, kv = bf16(g, 2, 4, nope + rope), bf16(g, 2, rank + rope)
+    o = torch.empty(2, 4, v, dtype=torch.bfloat16, device="cuda:0")
+    a, b, wide = rt.create_latent_kv(rank, rope), rt.create_latent_kv(rank, rope), rt.create_latent_kv(512, rope)
+    refused("QM_ERR_INVALID_ARGUMENT", rt.latent_attention, weights, [a, a], q, kv, None, 0.0, o)
+    refused("QM_ERR_INVALID_ARGUMENT", rt.latent_attention, weights, [], q, kv, None, 0.0, o)
+    refused("QM_ERR_INVALID_ATTENTION_SHAPE", rt.latent_attention, weights, [a, wide], q, kv, None, 0.0, o)
+    refused("QM_ERR_NULL_POINTER", rt.latent_attention, weights, [a, b], q, None, None, 0.0, o)
+    refused("QM_ERR_MISALIGNED", rt.latent_attention, weights, [a, b], q.data_ptr() + 2, kv, None, 0.0, o)
+    refused("QM_ERR_INVALID_ARGUMENT", rt.latent_attention, weights, [a, b], q, kv, kv_b.float(), -1.0, o)
+    refused("QM_ERR_INVALID_ATTENTION_SHAPE", rt.latent_attention_prefill, weights, a, q, kv, None, 0.0, 0, o)
+    refused("QM_ERR_EMPTY_APPEND", a.append, kv, None, 0.0, 0)
+    refused("QM_ERR_INVALID_SEQUENCE_LENGTH", a.load, 0, 1, kv)
+    refused("QM_ERR_INVALID_SEQUENCE_LENGTH", a.truncate, 1)
+    refused("QM_ERR_DIMENSION_OVERFLOW", a.reserve, 2 ** 32 - 1)
+    for bad in ((0, rank, nope, rope, v), (4, 520, nope, rope, v), (4, rank, 136, rope, v), (4, rank, nope, 72, v),
+                (4, rank, nope, rope, 12)):
+        refused("QM_ERR_INVALID_ATTENTION_SHAPE", rt.create_latent_weights, qm38.LatentConfig(*bad, 1.0), kv_b)
+    refused("QM_ERR_INVALID_ARGUMENT", rt.create_latent_weights,
+            qm38.LatentConfig(4, rank, nope, rope, v, float("nan")), kv_b)
+    job = qm38.Runtime.job(kv_b, kv_b, kv_b, 100)
+    refused("QM_ERR_WRONG_LENGTH", rt.create_latent_weights, qm38.LatentConfig(4, rank, nope, rope, v, 1.0), job)
+    refused("QM_ERR_INPUT_NOT_GROUPED", rt.create_latent_weights, qm38.LatentConfig(4, 264, nope, rope, v, 1.0), job)
+    # A failed call leaves the lengths.
+    small = rt.create_latent_kv(rank, rope, max_tokens=1)
+    small.append(kv, None, 0.0, 1)
+    refused("QM_ERR_CAPACITY_EXCEEDED", rt.latent_attention, weights, [a, small], q, kv, None, 0.0, o)
+    assert (a.sequence_length, small.sequence_length) == (0, 1)
+
+
+def test_capture_is_refused(torch_dev):
+    """The calls that move a cache's length do not go into a graph, and say so."""
+    rank, rope, nope, v = SMALL
+    with tuned() as rt:
+        g = generator(17)
+        kv_b, scale, weights = make_weights(rt, g, 4, SMALL)
+        q, kv = bf16(g, 1, 4, nope + rope), bf16(g, 1, rank + rope)
+        o = torch.empty(1, 4, v, dtype=torch.bfloat16, device=torch_dev)
+        cache = filled(rt, g, SMALL, 10, None)
+        x = torch.zeros(4, device=torch_dev)
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            rt.set_stream(stream)
+            x += 1
+            refused("QM_ERR_INVALID_ARGUMENT", rt.latent_attention, weights, [cache], q, kv, None, 0.0, o)
+            refused("QM_ERR_INVALID_ARGUMENT", rt.latent_attention_prefill, weights, cache, q, kv, None, 0.0, 1, o)
+            refused("QM_ERR_INVALID_ARGUMENT", cache.append, kv, None, 0.0, 1)
+            refused("QM_ERR_INVALID_ARGUMENT", cache.load, 0, 1, kv)
+        rt.set_stream(torch.cuda.current_stream())
+        graph.replay()
+        rt.latent_attention(weights, [cache], q, kv, None, 0.0, o)
+        torch.cuda.synchronize()
+        assert cache.sequence_length == 11 and float(x[0]) == 1.0
