@@ -39,6 +39,8 @@ COMMON = [
 # otherwise park them in AGPRs and copy them back every step).
 PER_FILE = {
     "q8_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    # The score products in VGPRs; the sums then take the AGPRs without copies.
+    "latent_absorbed.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -72,7 +72,7 @@ struct LatentAttnArgs {
   uint8_t* digits;        // queries in operand order, [block][rank_pad / 32 + 2][64 lanes][32 bytes]
   float* qscale;          // [block][32][2]
   float* partials;        // O [unit][32][rank_pad], then (max, sum) [unit][32][2]
-  uint16_t* mixed;        // bf16 [rows][H][rank_pad]: the joined sums of latents
+  uint16_t* mixed;        // bf16 [rows][H][2][rank_pad]: the joined sums of latents, and what bf16 leaves of them
   LatentDims d;
   float scale;            // of the scores
   uint32_t rows;          // query rows of the call (decode: sequences)

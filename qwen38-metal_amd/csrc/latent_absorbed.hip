@@ -133,10 +133,14 @@ __global__ __launch_bounds__(256) void latent_query_kernel(LatentAttnArgs a) {
 // other waves before the end.
 //   S^T[token][column] = codes . (hi, lo) on v_mfma_i32_32x32x32_i8, the token's
 //     and the column's scales applied in fp32;
-//   online softmax in fp32 (exp2 domain), the sums rescaled only when a column's
-//     maximum rises by more than 8 (p stays below 2^8);
-//   O^T[latent element][column] += codes^T P'^T on v_mfma_f32_32x32x16_bf16:
-//     P' = p * token scale rounded to bf16 (2^-9 of each term), the codes exact.
+//   online softmax in fp32 (exp2 domain), p = 2^(s - ref): ref is a column's
+//     maximum less 6, moved (and the sums rescaled) only when a maximum passes
+//     ref + 14, so p stays below 2^14 and what is 2^-20 of the largest is still
+//     a normal fp16;
+//   O^T[latent element][column] += codes^T P'^T on v_mfma_f32_32x32x16_f16:
+//     P' = p * token scale / 2^e, 2^e the largest scale's power of two so far,
+//     rounded to fp16 (2^-11 of each term, where bf16 would be 2^-8), the codes
+//     exact.
 //     S^T leaves a lane the P' of its own column in the order that the second
 //     product wants once the tokens of its operand are taken in the same order,
 //     so P' stays in registers; the codes' operand comes by transposing reads.
@@ -238,6 +242,7 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnArgs a) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) O[i][j] = 0.0f;
   float mref = kNoMax, l = 0.0f;
+  uint32_t vexp = 0x00800000u;  // the largest token scale's exponent, as a float's bits: the sums' unit
 
   const uint32_t first = t_begin + wave;
   const uint32_t count = first < t_end ? (t_end - first + 3) / 4 : 0;
@@ -258,16 +263,10 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnArgs a) {
     const uint8_t* key = lat + L::kLat;
     const float* scales = (const float*)(key + L::kKey);
 
-    // Scores: the shared key's part, then the latent's.
+    // Scores: the shared key's part, then the latent's.  The compiler barriers
+    // keep the operands of a few products in flight and no more: the columns'
+    // queries and the sums leave about a hundred registers.
     float S[16];
-    float ts[16];  // this lane's tokens' latent scales
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const floatx4 s0 = *(const floatx4*)(scales + (8 * g + 4 * half) * 2);
-      const floatx4 s1 = *(const floatx4*)(scales + (8 * g + 4 * half) * 2 + 4);
-      ts[4 * g] = s0[0], ts[4 * g + 1] = s0[2], ts[4 * g + 2] = s1[0], ts[4 * g + 3] = s1[2];
-      S[4 * g] = s0[1], S[4 * g + 1] = s0[3], S[4 * g + 2] = s1[1], S[4 * g + 3] = s1[3];
-    }
     {
       intx16 hi = {}, lo = {};
 #pragma unroll
@@ -277,7 +276,10 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnArgs a) {
         lo = mfma32x32x32_i8(kf, qlo[kLatSteps + s], lo);
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) S[i] = fmaf((float)hi[i], 256.0f, (float)lo[i]) * (S[i] * key_scale);
+      for (int i = 0; i < 16; ++i) {
+        const float ks = scales[(8 * (i / 4) + 4 * half + i % 4) * 2 + 1];
+        S[i] = fmaf((float)hi[i], 256.0f, (float)lo[i]) * (ks * key_scale);
+      }
     }
     {
       intx16 hi = {}, lo = {};
@@ -286,51 +288,67 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnArgs a) {
         const u32x4 kf = *(const u32x4*)(lat + ka[s & 3] + (s >> 2) * 128);
         hi = mfma32x32x32_i8(kf, qhi[s], hi);
         lo = mfma32x32x32_i8(kf, qlo[s], lo);
+        if (s % 4 == 3) __asm__ volatile("" ::: "memory");
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) S[i] = fmaf(fmaf((float)hi[i], 256.0f, (float)lo[i]), ts[i] * lat_scale, S[i]);
+      for (int i = 0; i < 16; ++i) {
+        const float ls = scales[(8 * (i / 4) + 4 * half + i % 4) * 2];
+        S[i] = fmaf(fmaf((float)hi[i], 256.0f, (float)lo[i]), ls * lat_scale, S[i]);
+      }
     }
+    // A tile's largest token scale, as a power of two: P' is kept relative to the
+    // largest so far.
     const uint32_t tok0 = tile * kLatentTile + 4 * half;
     const bool whole = (tile + 1) * kLatentTile <= lim_min && c_last - c_first == kLatentCols - 1;
     if (!whole) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const bool seen = tok0 + 8 * (i / 4) + i % 4 < limit;
-        S[i] = seen ? S[i] : -INFINITY;
-        ts[i] = seen ? ts[i] : 0.0f;  // nothing of an unseen token, not even a scale that is no number
-      }
+      for (int i = 0; i < 16; ++i) S[i] = tok0 + 8 * (i / 4) + i % 4 < limit ? S[i] : -INFINITY;
     }
+    // Not of tokens behind the block's last, whose scales are any bits, nor NaN.
+    const float own = tile * kLatentTile + col < lim_max && scales[2 * col] <= FLT_MAX ? scales[2 * col] : 0.0f;
+    const uint32_t big = __float_as_uint(wave_allmax(own)) & 0x7F800000u;
     float top = S[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = fmaxf(top, S[i]);
     top = halves_max(top);
-    if (__any(top > mref + 8.0f)) {
-      const float m = fmaxf(mref, top), f = __builtin_amdgcn_exp2f(mref - m);
+    if (__any(top > mref + 14.0f) || big > vexp) {
+      const float m = fmaxf(mref, top - 6.0f);
+      const uint32_t e = max(big, vexp);
+      float f = __builtin_amdgcn_exp2f(mref - m);
       mref = m;
       l *= f;
+      f *= __uint_as_float(max((int)(vexp - e + 0x3F800000u), 0));  // 2^(old - new)
+      vexp = e;
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) O[i][j] *= f;
     }
+    const float unit_scale = __uint_as_float(0x7F000000u - vexp);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       S[i] = __builtin_amdgcn_exp2f(S[i] - mref);
       l += S[i];
-      S[i] *= ts[i];
+      const float ls = scales[(8 * (i / 4) + 4 * half + i % 4) * 2];
+      S[i] *= (whole || tok0 + 8 * (i / 4) + i % 4 < limit ? ls : 0.0f) * unit_scale;
     }
-    u32x4 p[2];
+    u32x4 p[2];  // pairs in the order of bytes_to_f16
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[u][i] = to_bf16x2(S[8 * u + 2 * i], S[8 * u + 2 * i + 1]);
+      for (int i = 0; i < 2; ++i) {
+        p[u][2 * i] = to_f16x2(S[8 * u + 4 * i], S[8 * u + 4 * i + 2]);
+        p[u][2 * i + 1] = to_f16x2(S[8 * u + 4 * i + 1], S[8 * u + 4 * i + 3]);
+      }
 #pragma unroll
-    for (int rb = 0; rb < kBlocks; ++rb)
+    for (int rb = 0; rb < kBlocks; ++rb) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const u32x2 v = lds_read_tr8(lat + va[rb & 3] + (rb >> 2) * 128 + u * 16 * RP);
-        O[rb] = mfma32x32x16(bytes_to_bf16(v), p[u], O[rb]);
+        O[rb] = mfma32x32x16_f16(bytes_to_f16(v), p[u], O[rb]);
       }
+      if (rb % 2 == 1) __asm__ volatile("" ::: "memory");
+    }
     latent_wait_lds();  // before the DMA of a later tile writes here
     slot = slot + 1 == L::kRing ? 0 : slot + 1;
   }
@@ -348,7 +366,7 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnArgs a) {
 #pragma unroll
   for (int w = 0; w < 4; ++w)
     sum += ml[(w * kLatentCols + col) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * kLatentCols + col) * 2] - m);
-  const float f = __builtin_amdgcn_exp2f(mref - m);
+  const float f = __builtin_amdgcn_exp2f(mref - m) * __uint_as_float(vexp);
   if (wave == 0 && half == 0)
     *(float2*)(a.partials + (size_t)a.units * kLatentCols * RP + ((size_t)unit * kLatentCols + col) * 2) =
         float2{m, sum};
@@ -382,8 +400,8 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnArgs a) {
 // Joining the splits, and out of the latent space
 // ---------------------------------------------------------------------------
 // One workgroup per (row, head) column: its splits' sums weighted by 2^(m - M),
-// divided by the joined softmax sum and rounded to bf16 (the operand of the
-// product with W_uv).
+// divided by the joined softmax sum and written as bf16 and the bf16 of what that
+// leaves (2^-17 in all), the operands of the product with W_uv.
 template <int RP>
 __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnArgs a) {
   constexpr int kLanes = RP / 4, kGroups = 256 / kLanes;
@@ -416,8 +434,15 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnArgs a) {
 #pragma unroll
   for (int g = 1; g < kGroups; ++g) acc += part[g * kLanes + t];
   const float r = 1.0f / sum;
-  *(u32x2*)(a.mixed + (size_t)blockIdx.x * RP + 4 * t) =
-      u32x2{to_bf16x2(acc[0] * r, acc[1] * r), to_bf16x2(acc[2] * r, acc[3] * r)};
+  float x[4], y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] = acc[i] * r;
+    y[i] = x[i] - (float)(__bf16)x[i];
+  }
+  uint16_t* to = a.mixed + (size_t)blockIdx.x * 2 * RP + 4 * t;
+  *(u32x2*)to = u32x2{to_bf16x2(x[0], x[1]), to_bf16x2(x[2], x[3])};
+  *(u32x2*)(to + RP) = u32x2{to_bf16x2(y[0], y[1]), to_bf16x2(y[2], y[3])};
 }
 
 // o[m][h][n] = sum_r mixed[m][h][r] W_uv[h][n][r]: workgroup = (16 rows, head),
@@ -427,13 +452,15 @@ __global__ __launch_bounds__(256) void latent_up_kernel(LatentAttnArgs a) {
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, kq = lane >> 4;
   const uint32_t h = blockIdx.y, m0 = blockIdx.x * 16, H = a.d.heads, vp = a.d.v_pad;
   const uint16_t* up = a.up + ((size_t)h * (a.d.nope_pad + vp) + a.d.nope_pad) * RP;
-  const uint16_t* x = a.mixed + ((size_t)min(m0 + n, a.rows - 1) * H + h) * RP;
+  const uint16_t* x = a.mixed + ((size_t)min(m0 + n, a.rows - 1) * H + h) * 2 * RP;
   for (uint32_t n0 = 16 * wave; n0 < vp; n0 += 64) {
     floatx4 acc = {0, 0, 0, 0};
 #pragma unroll
-    for (int s = 0; s < RP / 32; ++s)
-      acc = mfma16x16x32(*(const u32x4*)(x + 32 * s + 8 * kq), *(const u32x4*)(up + (size_t)(n0 + n) * RP + 32 * s + 8 * kq),
-                         acc);
+    for (int s = 0; s < RP / 32; ++s) {
+      const u32x4 w = *(const u32x4*)(up + (size_t)(n0 + n) * RP + 32 * s + 8 * kq);
+      acc = mfma16x16x32(*(const u32x4*)(x + 32 * s + 8 * kq), w, acc);
+      acc = mfma16x16x32(*(const u32x4*)(x + RP + 32 * s + 8 * kq), w, acc);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t m = m0 + 4 * kq + i;

@@ -53,20 +53,40 @@ __device__ __forceinline__ void latent_wait_lds() {
   __asm__ volatile("" ::: "memory");
 }
 
+// Two fp32 values -> packed fp16 (round to nearest even, v_cvt_pk_f16_f32).
+typedef _Float16 latent_halfx2 __attribute__((ext_vector_type(2)));
+typedef _Float16 latent_halfx4 __attribute__((ext_vector_type(4)));
+typedef _Float16 latent_halfx8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ uint32_t to_f16x2(float lo, float hi) {
+  const latent_halfx2 v = {(_Float16)lo, (_Float16)hi};
+  return __builtin_bit_cast(uint32_t, v);
+}
+// 8 signed bytes -> 8 fp16, exact, in the order 0, 2, 1, 3, 4, 6, 5, 7: 0x6400 | u
+// is the fp16 1024 + u, so each pair takes one AND-OR and one packed subtraction.
+__device__ __forceinline__ u32x4 bytes_to_f16(u32x2 w) {
+  const latent_halfx4 bias = {(_Float16)1152.0f, (_Float16)1152.0f, (_Float16)1152.0f, (_Float16)1152.0f};
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t u = w[i] ^ 0x80808080u;
+    const u32x2 biased = {(u & 0x00FF00FFu) | 0x64006400u, ((u >> 8) & 0x00FF00FFu) | 0x64006400u};
+    const u32x2 v = __builtin_bit_cast(u32x2, __builtin_bit_cast(latent_halfx4, biased) - bias);
+    r[2 * i] = v.x;
+    r[2 * i + 1] = v.y;
+  }
+  return r;
+}
+__device__ __forceinline__ floatx16 mfma32x32x16_f16(u32x4 a, u32x4 b, floatx16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(latent_halfx8, a),
+                                                __builtin_bit_cast(latent_halfx8, b), c, 0, 0, 0);
+}
+
 // Two fp32 values -> packed bf16 (round to nearest even, v_cvt_pk_bf16_f32).
 typedef __bf16 latent_bf16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t to_bf16x2(float lo, float hi) {
   const latent_bf16x2 v = {(__bf16)lo, (__bf16)hi};
   return __builtin_bit_cast(uint32_t, v);
 }
-// 8 signed bytes -> 8 bf16, exact.
-__device__ __forceinline__ u32x4 bytes_to_bf16(u32x2 w) {
-  return u32x4{to_bf16x2((float)(int8_t)w.x, (float)(int8_t)(w.x >> 8)),
-               to_bf16x2((float)(int8_t)(w.x >> 16), (float)(int8_t)(w.x >> 24)),
-               to_bf16x2((float)(int8_t)w.y, (float)(int8_t)(w.y >> 8)),
-               to_bf16x2((float)(int8_t)(w.y >> 16), (float)(int8_t)(w.y >> 24))};
-}
-
 // Maximum of lanes l and l ^ 32, and their sum.
 __device__ __forceinline__ float halves_max(float v) {
   const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);

@@ -278,7 +278,7 @@ void plan_absorbed(const qm_runtime* rt, LatentAttnArgs* a) {
 qm_status absorbed_workspaces(qm_runtime* rt, LatentAttnArgs* a) {
   const LatentDims& d = a->d;
   const size_t digits = a->blocks * latent_digit_bytes(d.rank_pad), scales = (size_t)a->blocks * kLatentCols * 8;
-  const size_t mixed = (size_t)a->rows * d.heads * d.rank_pad * 2;
+  const size_t mixed = (size_t)a->rows * d.heads * d.rank_pad * 4;
   qm_status st = ensure_scratch(rt, digits + scales + mixed);
   if (st != QM_OK) return st;
   if ((st = ensure_partials(rt, (size_t)a->units * kLatentCols * (d.rank_pad + 2) * sizeof(float))) != QM_OK) return st;
