@@ -40,6 +40,7 @@ COMMON = [
 PER_FILE = {
     "q8_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     # The score products in VGPRs; the sums then take the AGPRs without copies.
+    "latent_expanded.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "latent_absorbed.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

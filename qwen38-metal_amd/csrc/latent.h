@@ -86,4 +86,31 @@ struct LatentAttnArgs {
 constexpr uint64_t latent_digit_bytes(uint32_t rank_pad) { return (uint64_t)(rank_pad / 32 + 2) * 64 * 32; }
 hipError_t launch_latent_absorbed(const LatentAttnArgs& a, hipStream_t st);
 
+// Expanded attention: rows 0 .. m - 1 at positions start .. over `tokens` = start
+// + m cached tokens.  The workspaces are in operand order (latent_expanded.hip).
+struct LatentExpandArgs {
+  const uint16_t* q;    // bf16 [m][H][nope + rope]
+  uint16_t* o;          // bf16 [m][H][v]
+  const uint16_t* wop;  // weights (launch_latent_wop)
+  const float* wmul;    // their powers of two [H][2]
+  LatentRows rows;
+  LatentDims d;
+  float scale;
+  uint32_t m, start, tokens;
+  uint32_t padded;       // tokens rounded up to kLatentExpandTokens
+  uint32_t head0, heads; // the launch's heads (filled by the launcher)
+  uint32_t out8;         // o's rows take 8-byte stores
+  uint16_t* latents;     // fp16 [padded / 32][rank_pad / 16][512]
+  uint16_t* keys;        // fp16 [padded / 32][4][512]: the shared key
+  float* fk;             // [padded] factors of a token's keys and values
+  float* fv;
+  float* powers;         // [padded / 32][2]
+  uint16_t* k;           // fp16 [heads][padded / 32][nope_pad / 16][512]
+  uint16_t* v;           // fp16 [heads][padded / 32][v_pad / 16][512]
+};
+constexpr uint32_t kLatentExpandTokens = 128;
+hipError_t launch_latent_expanded(const LatentExpandArgs& a, uint32_t heads_at_once, hipStream_t st);
+// wop fp16 [H * (nope_pad + v_pad) / 32][rank_pad / 16][512] and wmul fp32 [H][2] from `up`.
+hipError_t launch_latent_wop(const LatentDims& d, const uint16_t* up, float* wmul, uint16_t* wop, hipStream_t st);
+
 }  // namespace qm

@@ -30,7 +30,19 @@ struct qm_latent_weights {
   float scale = 0.0f;
   uint16_t* down = nullptr;
   uint16_t* up = nullptr;
+  uint16_t* wop = nullptr;  // up, as the expanded form reads it
+  float* wmul = nullptr;
 };
+
+namespace {
+void free_weights(qm_latent_weights* w) {
+  (void)hipFree(w->down);
+  (void)hipFree(w->up);
+  (void)hipFree(w->wop);
+  (void)hipFree(w->wmul);
+  delete w;
+}
+}  // namespace
 
 namespace {
 
@@ -193,12 +205,13 @@ qm_status create_weights(qm_runtime* rt, const qm_latent_config& c, qm_latent_we
   const size_t up = (size_t)d.heads * (d.nope_pad + d.v_pad) * d.rank_pad * 2;
   hipError_t e = hipMalloc(&w->down, down);
   if (e == hipSuccess) e = hipMalloc(&w->up, up);
+  if (e == hipSuccess) e = hipMalloc(&w->wop, up);
+  if (e == hipSuccess) e = hipMalloc(&w->wmul, (size_t)d.heads * 2 * sizeof(float));
   if (e == hipSuccess) e = launch(d, w->down, w->up);
+  if (e == hipSuccess) e = launch_latent_wop(d, w->up, w->wmul, w->wop, rt->stream);
   if (e == hipSuccess) e = hipStreamSynchronize(rt->stream);
   if (e != hipSuccess) {
-    (void)hipFree(w->down);
-    (void)hipFree(w->up);
-    delete w;
+    free_weights(w);
     return hip_check(e, "latent weights");
   }
   *out = w;
@@ -287,6 +300,57 @@ qm_status absorbed_workspaces(qm_runtime* rt, LatentAttnArgs* a) {
   a->qscale = (float*)(p + digits);
   a->mixed = (uint16_t*)(p + digits + scales);
   a->partials = (float*)rt->partials;
+  return QM_OK;
+}
+
+// Which form a prefill of M rows over T tokens takes: the one with the fewer
+// multiplications.
+bool prefers_expanded(const qm_runtime* rt, const LatentDims& d, uint32_t M, uint64_t T) {
+  if (rt->tune.latent_form) return rt->tune.latent_form == 2;
+  const double pairs = (double)M * ((double)T - 0.5 * M);
+  const double absorbed = pairs * (2.0 * d.rank_pad + kLatentRope);
+  const double expanded = pairs * (d.nope_pad + kLatentRope + d.v_pad) + (double)T * d.rank_pad * (d.nope_pad + d.v_pad);
+  return expanded < absorbed;
+}
+
+// Expanded prefill: workspaces, then the launches (behind the append's).
+struct ExpandedPlan {
+  LatentExpandArgs a{};
+  uint32_t heads_at_once = 0;
+};
+qm_status plan_expanded(qm_runtime* rt, const qm_latent_weights* w, const qm_latent_kv* seq, uint32_t M, uint16_t* o,
+                        const uint16_t* q, ExpandedPlan* p) {
+  LatentExpandArgs& a = p->a;
+  const LatentDims& d = w->d;
+  a.q = q;
+  a.o = o;
+  a.wop = w->wop;
+  a.wmul = w->wmul;
+  a.rows = seq->rows;
+  a.d = d;
+  a.scale = w->scale;
+  a.m = M;
+  a.start = seq->length;
+  a.tokens = seq->length + M;
+  a.padded = (a.tokens + kLatentExpandTokens - 1) / kLatentExpandTokens * kLatentExpandTokens;
+  a.out8 = aligned(o, 8);
+  const uint64_t P = a.padded;
+  const uint64_t latents = P * d.rank_pad * 2, keys = P * kLatentRope * 2, factors = P * 4, powers = P / 32 * 8;
+  const uint64_t k_head = P * d.nope_pad * 2, v_head = P * d.v_pad * 2;
+  const uint64_t budget = (uint64_t)(rt->tune.latent_mb > 0 ? rt->tune.latent_mb : 1024) << 20;
+  p->heads_at_once = (uint32_t)std::min<uint64_t>(d.heads, std::max<uint64_t>(1, budget / (k_head + v_head)));
+  const uint64_t n = p->heads_at_once;
+  qm_status st = ensure_scratch(rt, latents + keys + 2 * factors + powers + n * (k_head + v_head));
+  if (st != QM_OK) return st;
+  uint8_t* at = (uint8_t*)rt->scratch;
+  auto take = [&](uint64_t bytes) { uint8_t* r = at; at += bytes; return r; };
+  a.k = (uint16_t*)take(n * k_head);
+  a.v = (uint16_t*)take(n * v_head);
+  a.latents = (uint16_t*)take(latents);
+  a.keys = (uint16_t*)take(keys);
+  a.fk = (float*)take(factors);
+  a.fv = (float*)take(factors);
+  a.powers = (float*)take(powers);
   return QM_OK;
 }
 
@@ -526,9 +590,7 @@ qm_status qm_latent_weights_create_q4(qm_runtime* rt, const qm_latent_config* cf
 void qm_latent_weights_destroy(qm_latent_weights* w) {
   if (!w) return;
   DeviceGuard g(w->device);
-  (void)hipFree(w->down);
-  (void)hipFree(w->up);
-  delete w;
+  free_weights(w);
 }
 
 qm_status qm_latent_decode(qm_runtime* rt, const qm_latent_weights* w, qm_latent_kv* const* seqs, uint32_t B,
@@ -583,22 +645,30 @@ qm_status qm_latent_prefill(qm_runtime* rt, const qm_latent_weights* w, qm_laten
   LatentAppendArgs ap = append_args(w->d, kv, norm, epsilon, M, false);
   ap.seqs[0] = seq->rows;
   ap.pos[0] = seq->length;
+  const bool expanded = prefers_expanded(rt, w->d, M, (uint64_t)seq->length + M);
   LatentAttnArgs at{};
-  at.q = q;
-  at.o = o;
-  at.down = w->down;
-  at.up = w->up;
-  at.d = w->d;
-  at.scale = w->scale;
-  at.rows = M;
-  at.n_seqs = 1;
-  at.seqs[0].rows = seq->rows;
-  at.seqs[0].start = seq->length;
-  plan_absorbed(rt, &at);
-  if ((st = absorbed_workspaces(rt, &at)) != QM_OK) return st;
+  ExpandedPlan ep;
+  if (expanded) {
+    st = plan_expanded(rt, w, seq, M, o, q, &ep);
+  } else {
+    at.q = q;
+    at.o = o;
+    at.down = w->down;
+    at.up = w->up;
+    at.d = w->d;
+    at.scale = w->scale;
+    at.rows = M;
+    at.n_seqs = 1;
+    at.seqs[0].rows = seq->rows;
+    at.seqs[0].start = seq->length;
+    plan_absorbed(rt, &at);
+    st = absorbed_workspaces(rt, &at);
+  }
+  if (st != QM_OK) return st;
   if ((st = stream_after(rt, seq->rt)) != QM_OK) return st;
   hipError_t e = launch_latent_append(ap, rt->stream);
-  if (e == hipSuccess) e = launch_latent_absorbed(at, rt->stream);
+  if (e == hipSuccess)
+    e = expanded ? launch_latent_expanded(ep.a, ep.heads_at_once, rt->stream) : launch_latent_absorbed(at, rt->stream);
   if (e != hipSuccess) return hip_check(e, "latent attention launch");
   seq->length += M;
   return stream_after(seq->rt, rt);

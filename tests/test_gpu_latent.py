@@ -285,10 +285,16 @@ def check_prefill(rt, widths, H, cached, rows, seed, q_std=1.5):
     assert torch.equal(o, again)
 
 
-@pytest.mark.parametrize("widths", [WIDE, SMALL, ODD, TINY])
+FORMS = {"absorbed": dict(QM38_LATENT_FORM=1), "expanded": dict(QM38_LATENT_FORM=2),
+         "head by head": dict(QM38_LATENT_FORM=2, QM38_LATENT_MB=1)}
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("widths", [WIDE, SMALL, ODD, TINY, (200, 8, 128, 40), (512, 64, 64, 128)])
 @pytest.mark.parametrize("H,cached,rows", [(1, 0, 1), (5, 0, 33), (3, 1000, 7), (20, 31, 130), (33, 64, 65)])
-def test_prefill_widths(rt, widths, H, cached, rows):
-    check_prefill(rt, widths, H, cached, rows, H + rows)
+def test_prefill_widths(torch_dev, form, widths, H, cached, rows):
+    with tuned(**FORMS[form]) as rt:
+        check_prefill(rt, widths, H, cached, rows, H + rows)
 
 
 @pytest.mark.parametrize("H,cached,rows", [(32, 20001, 5), (64, 0, 300), (8, 4096, 513), (128, 100, 40), (2, 0, 2000)])
@@ -296,8 +302,38 @@ def test_prefill_sizes(rt, H, cached, rows):
     check_prefill(rt, WIDE, H, cached, rows, H + rows)
 
 
-def test_prefill_peaked(rt):
-    check_prefill(rt, ODD, 12, 700, 300, 2, q_std=60.0)
+@pytest.mark.parametrize("form", FORMS)
+def test_prefill_peaked(torch_dev, form):
+    with tuned(**FORMS[form]) as rt:
+        check_prefill(rt, ODD, 12, 700, 300, 2, q_std=60.0)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_scales_far_apart(torch_dev, form):
+    """Tokens whose latents and keys are 2^-40 to 2^40 times others', and tokens
+    of zeros, alone in a tile and beside others."""
+    rank, rope, nope, v = SMALL
+    with tuned(**FORMS[form]) as rt:
+        g = generator(18)
+        H, rows = 6, 200
+        kv_b, scale, weights = make_weights(rt, g, H, SMALL)
+        q, kv = bf16(g, rows, H, nope + rope), bf16(g, rows, rank + rope)
+        kv[:40] = 0
+        kv[50:60, :rank] = 0
+        kv[60:70, rank:] = 0
+        kv[70:75] *= 2.0 ** -40
+        kv[100, :rank] *= 2.0 ** 40
+        q[110:115] *= 2.0 ** -30
+        q[116] *= 2.0 ** 20
+        kv[150:152, :rank] *= 2.0 ** 20
+        cache = rt.create_latent_kv(rank, rope)
+        o = torch.full((rows, H, v), float("nan"), dtype=torch.bfloat16, device=torch_dev)
+        rt.latent_attention_prefill(weights, cache, q, kv, None, 0.0, rows, o)
+        latent, key = held(cache)
+        ref, bound = attention(q, latent, key, kv_b, nope, scale, 0)
+        err = (o.double() - ref).abs()
+        assert (err <= bound + 1e-30).all(), float((err / (bound + 1e-30)).max())
+        assert (o[:40] == 0).all()
 
 
 def test_prefill_in_pieces_equals_decode_steps(rt):
@@ -348,7 +384,13 @@ def test_weights_from_q4(rt, torch_dev):
     assert torch.equal(*outs)
 
 
-def test_numbers_that_are_none(rt):
+@pytest.mark.parametrize("form", FORMS)
+def test_numbers_that_are_none(torch_dev, form):
+    with tuned(**FORMS[form]) as rt:
+        check_numbers_that_are_none(rt)
+
+
+def check_numbers_that_are_none(rt):
     """A token whose row holds an infinity or NaN poisons the rows that see it,
     and no other; a query that does poisons its own row and head."""
     rank, rope, nope, v = SMALL
