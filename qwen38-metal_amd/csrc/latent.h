@@ -23,16 +23,18 @@ struct LatentRows {
   float* scales;
 };
 
-struct LatentAppendArgs {
-  const uint16_t* kv;  // bf16 [items][rank + rope]
+// A call's new rows.
+struct LatentNewRows {
+  const uint16_t* kv;  // bf16 [rows][rank + rope]
   const float* norm;   // fp32 [rank] or null: stored as given
   float eps;
   uint32_t rank, rope, rank_pad;
+};
+struct LatentAppendArgs {
+  LatentNewRows rows;
+  LatentRows to;
+  uint32_t first;  // token that row 0 becomes
   uint32_t items;
-  // Item i becomes token pos[i] of seqs[i] (decode), or token pos[0] + i of seqs[0].
-  uint32_t decode;
-  LatentRows seqs[kMaxLatentSeqs];
-  uint32_t pos[kMaxLatentSeqs];
 };
 hipError_t launch_latent_append(const LatentAppendArgs& a, hipStream_t st);
 
@@ -50,6 +52,8 @@ struct LatentDims {
 };
 hipError_t launch_latent_weights(const LatentDims& d, const uint16_t* kv_b, uint16_t* down, uint16_t* up,
                                  hipStream_t st);
+// wnorm[h]: the largest norm of a row of `down` (a column of W_uk), rounded up.
+hipError_t launch_latent_wnorm(const LatentDims& d, const uint16_t* down, float* wnorm, hipStream_t st);
 // The same from an affine-Q4 matrix [H * (nope + v)][rank] (rank a multiple of 64).
 hipError_t launch_latent_weights_q4(const LatentDims& d, const uint32_t* w, const uint16_t* s, const uint16_t* b,
                                     uint16_t* down, uint16_t* up, hipStream_t st);
@@ -69,6 +73,8 @@ struct LatentAttnArgs {
   uint16_t* o;            // bf16 [rows][H][v]
   const uint16_t* down;
   const uint16_t* up;
+  const float* wnorm;     // [H]
+  LatentNewRows new_rows; // appended by the first launch
   uint8_t* digits;        // queries in operand order, [block][rank_pad / 32 + 2][64 lanes][32 bytes]
   float* qscale;          // [block][32][2]
   float* partials;        // O [unit][32][rank_pad], then (max, sum) [unit][32][2]

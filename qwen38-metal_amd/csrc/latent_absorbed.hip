@@ -3,11 +3,13 @@
 // per token, and the sums of latents come out through W_uv.  For decode and
 // for few rows: a token costs 584 bytes (rank 512) whatever the heads.
 //
-// Four launches: latent_query_kernel, latent_attn_kernel (split over the
-// cache's length), latent_join_kernel, latent_up_kernel.
+// Four launches: latent_query_kernel (which also appends the new rows),
+// latent_attn_kernel (split over the cache's length), latent_join_kernel,
+// latent_up_kernel.
 #include <float.h>
 
 #include "latent.h"
+#include "latent_append.h"
 #include "latent_device.h"
 
 namespace qm {
@@ -17,111 +19,132 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -1e30f;  // running maximum before the first visible token
 
 // ---------------------------------------------------------------------------
-// Queries into the latent space, as two 8-bit digits
+// New rows into the cache, queries into the latent space
 // ---------------------------------------------------------------------------
-// qa[h][r] = sum_d q_nope[h][d] W_uk[h][d][r], then the row (and apart from it
-// the rotated part) as 16-bit integers: q = qs * (256 hi + lo), qs = absmax /
-// 32512, hi in -127..127, lo in -128..127.  The scores are then whole-number
+// The first workgroups append the call's rows (four a workgroup); the others
+// form qa[h][r] = sum_d q_nope[h][d] W_uk[h][d][r] and write it, and apart from
+// it the rotated part, as 16-bit integers in two 8-bit digits: q = qs * (256 hi +
+// lo), hi in -127..127, lo in -128..127.  The scores are then whole-number
 // products with the cache's codes on the i8 matrix cores, exact but for this
-// rounding (2^-17 of the row's largest element, where rounding qa to bf16 would
-// be 2^-9 of each), and the cache's bytes need no conversion.  A row with a NaN
+// rounding, and the codes need no conversion.  qs = bound / 32512: for qa the
+// bound is |q_nope| times the head's largest column norm of W_uk (usually 2 or 3
+// times the row's largest element, so qa is rounded to about 2^-15 of that,
+// where bf16 would round each element to 2^-8), which lets the row be cut over
+// workgroups; for the rotated part it is its largest element.  A row with a NaN
 // or an infinity gets a NaN scale, which its scores keep.
 //
-// Workgroup = (16 rows, head); a wave takes a quarter of the latent.
+// Workgroup = (16 rows, head, 128 latent elements), a wave 32 of them: D = W
+// (rows) x queries (columns), so a lane holds four consecutive elements of a
+// row.  One token of 32 heads (4 MB of weights) is bound by latency: 128
+// workgroups of one round trip each.
+__device__ __forceinline__ void two_digits(float v, float s, bool skip, int at, uint32_t* hi, uint32_t* lo) {
+  const int q = skip ? 0 : (int)rintf(fminf(fmaxf(v / s, -32512.0f), 32512.0f));
+  const int h8 = (q + 128) >> 8;
+  *hi |= ((uint32_t)h8 & 255u) << (8 * at);
+  *lo |= ((uint32_t)(q - 256 * h8) & 255u) << (8 * at);
+}
+
 template <int RP>
-__global__ __launch_bounds__(256) void latent_query_kernel(LatentAttnArgs a) {
-  constexpr int kTiles = RP / 64;    // 16-wide tiles of a wave
-  constexpr int kStride = RP + 4;    // floats of a row in LDS
-  __shared__ float buf[16 * kStride];
+__global__ __launch_bounds__(256) void latent_query_kernel(LatentAttnArgs a, uint32_t append_blocks) {
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t h = blockIdx.y, m0 = blockIdx.x * 16;
+  if (blockIdx.x < append_blocks) {
+    const uint32_t item = blockIdx.x * 4 + wave;
+    if (item >= a.rows) return;
+    const LatentSeq& sq = a.seqs[a.decode ? item : 0];
+    latent_append_row(a.new_rows, sq.rows, sq.start + (a.decode ? 0 : item), item, lane);
+    return;
+  }
   const uint32_t H = a.d.heads, nope = a.d.nope, qw = nope + a.d.rope, np = a.d.nope_pad;
-  const uint32_t n = lane & 15, kq = lane >> 4;
-  const uint16_t* down = a.down + (size_t)h * RP * np;
-  const uint16_t* qrow = a.q + ((size_t)min(m0 + n, a.rows - 1) * H + h) * qw;
-  u32x4 qa[4];
+  uint32_t unit = blockIdx.x - append_blocks;
+  const uint32_t chunk = unit % (RP / 128);
+  unit /= RP / 128;
+  const uint32_t h = unit % H, m0 = unit / H * 16;
+  const uint32_t n = lane & 15, kq = lane >> 4, m = m0 + n;
+  const bool live = m < a.rows;
+  const uint16_t* down = a.down + ((size_t)h * RP + chunk * 128 + wave * 32) * np;
+  const uint16_t* qrow = a.q + ((size_t)min(m, a.rows - 1) * H + h) * qw;
+  u32x4 x[4], w[2][4];
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
     const uint32_t k = 32 * s + 8 * kq;
-    qa[s] = k < nope && m0 + n < a.rows ? *(const u32x4*)(qrow + k) : u32x4{0, 0, 0, 0};
+    x[s] = k < nope && live ? *(const u32x4*)(qrow + k) : u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      w[t][s] = 32u * s < np ? *(const u32x4*)(down + (size_t)(16 * t + n) * np + k) : u32x4{0, 0, 0, 0};
   }
+  // |q|, scaled by a power of two against overflow; the largest absolute value
+  // as bits, where NaN and infinity come out on top.
+  uint32_t top = 0;
 #pragma unroll
-  for (int t = 0; t < kTiles; ++t) {
-    const uint32_t r = wave * (RP / 4) + 16 * t;
-    floatx4 acc = {0, 0, 0, 0};
+  for (int s = 0; s < 4; ++s)
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
-      if (32u * s < np) acc = mfma16x16x32(qa[s], *(const u32x4*)(down + (size_t)(r + n) * np + 32 * s + 8 * kq), acc);
+    for (int k = 0; k < 4; ++k) top = max(top, max(x[s][k] & 0x7FFF0000u, (x[s][k] << 16) & 0x7FFF0000u));
+  top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+  top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+  const bool bad = top >= 0x7F800000u;
+  const uint32_t e = min(max(top & 0x7F800000u, 0x01000000u), 0x7E000000u);
+  const float down_scale = __uint_as_float(0x7F000000u - e);
+  float ss = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) buf[(4 * kq + i) * kStride + r + n] = acc[i];
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float lo = __uint_as_float(x[s][k] << 16) * down_scale;
+      const float hi = __uint_as_float(x[s][k] & 0xFFFF0000u) * down_scale;
+      ss = fmaf(lo, lo, fmaf(hi, hi, ss));
+    }
+  ss += __shfl_xor(ss, 16);
+  ss += __shfl_xor(ss, 32);
+  const float qs = fmaxf(sqrtf(ss) * a.wnorm[h] / 32512.0f * __uint_as_float(e), FLT_MIN);
+
+  floatx4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) acc[t] = mfma16x16x32(w[t][s], x[s], acc[t]);
+  const float nan = __uint_as_float(0x7FC00000u);
+  if (live) {
+    const uint32_t c = a.decode ? h : m * H + h, col = c % kLatentCols;
+    const size_t block = a.seqs[a.decode ? m : 0].block_begin + c / kLatentCols;
+    uint8_t* to = a.digits + block * latent_digit_bytes(RP) + col * 32;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      uint32_t hi = 0, lo = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) two_digits(acc[t][i], qs, bad, i, &hi, &lo);
+      // Piece of 16 elements 16 t of the wave's 32: steps are 32 elements, halves 16.
+      uint8_t* at = to + ((chunk * 4 + wave) * 64 + t * 32) * 32 + 4 * kq;
+      *(uint32_t*)at = hi;
+      *(uint32_t*)(at + 16) = lo;
+    }
+    if (chunk == 0 && wave == 0 && kq == 0) a.qscale[(block * kLatentCols + col) * 2] = bad ? nan : qs;
   }
-  __syncthreads();
-  // 16 threads a row.
-  const uint32_t row = threadIdx.x >> 4, t = threadIdx.x & 15, m = m0 + row;
-  const float* x = buf + row * kStride;
-  uint32_t top = 0, top_key = 0;  // largest absolute value, as bits: NaN and infinity come out on top
-#pragma unroll
-  for (int i = 0; i < RP / 16; ++i) top = max(top, __float_as_uint(x[t + 16 * i]) & 0x7FFFFFFFu);
-  const uint16_t* key = a.q + ((size_t)min(m, a.rows - 1) * H + h) * qw + nope;
+  if (chunk != 0) return;
+  // The rotated part: 16 threads a row, 4 elements each.
+  const uint32_t t = threadIdx.x & 15, mk = m0 + (threadIdx.x >> 4);
+  const uint16_t* key = a.q + ((size_t)min(mk, a.rows - 1) * H + h) * qw + nope;
   float k[4];
+  uint32_t top_key = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     k[i] = 4 * t + i < a.d.rope ? bf16_to_f32(key[4 * t + i]) : 0.0f;
     top_key = max(top_key, __float_as_uint(k[i]) & 0x7FFFFFFFu);
   }
 #pragma unroll
-  for (int s = 1; s < 16; s *= 2) {
-    top = max(top, (uint32_t)__shfl_xor((int)top, s));
-    top_key = max(top_key, (uint32_t)__shfl_xor((int)top_key, s));
-  }
-  if (m >= a.rows) return;
-  const float qs = fmaxf(__uint_as_float(top) / 32512.0f, FLT_MIN);
+  for (int s = 1; s < 16; s *= 2) top_key = max(top_key, (uint32_t)__shfl_xor((int)top_key, s));
+  if (mk >= a.rows) return;
   const float ks = fmaxf(__uint_as_float(top_key) / 32512.0f, FLT_MIN);
-  const bool bad = top >= 0x7F800000u, bad_key = top_key >= 0x7F800000u;
-  const uint32_t c = a.decode ? h : m * H + h;
-  const size_t block = a.seqs[a.decode ? m : 0].block_begin + c / kLatentCols;
-  const uint32_t col = c % kLatentCols;
-  uint8_t* to = a.digits + block * latent_digit_bytes(RP);
-  auto digits = [](float v, float s, bool skip, uint32_t* hi, uint32_t* lo) __attribute__((always_inline)) {
-    const int q = skip ? 0 : (int)rintf(fminf(fmaxf(v / s, -32512.0f), 32512.0f));
-    const int h8 = (q + 128) >> 8;
-    *hi = (uint32_t)h8 & 255u;
-    *lo = (uint32_t)(q - 256 * h8) & 255u;
-  };
+  const bool bad_key = top_key >= 0x7F800000u;
+  const uint32_t c = a.decode ? h : mk * H + h, col = c % kLatentCols;
+  const size_t block = a.seqs[a.decode ? mk : 0].block_begin + c / kLatentCols;
+  uint32_t hi = 0, lo = 0;
 #pragma unroll
-  for (int i = 0; i < RP / 256 + 1; ++i) {
-    const uint32_t chunk = t + 16 * i;  // 16 elements
-    if (chunk >= RP / 16) break;
-    uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      uint32_t h8, l8;
-      digits(x[16 * chunk + j], qs, bad, &h8, &l8);
-      hi[j / 4] |= h8 << (8 * (j % 4));
-      lo[j / 4] |= l8 << (8 * (j % 4));
-    }
-    uint8_t* at = to + ((size_t)(chunk / 2) * 64 + (chunk % 2) * 32 + col) * 32;
-    *(u32x4*)at = u32x4{hi[0], hi[1], hi[2], hi[3]};
-    *(u32x4*)(at + 16) = u32x4{lo[0], lo[1], lo[2], lo[3]};
-  }
-  {
-    uint32_t hi = 0, lo = 0;  // the key part: 4 elements a thread
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t h8, l8;
-      digits(k[j], ks, bad_key, &h8, &l8);
-      hi |= h8 << (8 * j);
-      lo |= l8 << (8 * j);
-    }
-    const uint32_t chunk = t / 4;
-    uint8_t* at = to + ((size_t)(RP / 32 + chunk / 2) * 64 + (chunk % 2) * 32 + col) * 32 + 4 * (t % 4);
-    *(uint32_t*)at = hi;
-    *(uint32_t*)(at + 16) = lo;
-  }
-  if (t == 0) {
-    const float nan = __uint_as_float(0x7FC00000u);
-    *(float2*)(a.qscale + (block * kLatentCols + col) * 2) = float2{bad ? nan : qs, bad_key ? nan : ks};
-  }
+  for (int i = 0; i < 4; ++i) two_digits(k[i], ks, bad_key, i, &hi, &lo);
+  uint8_t* at = a.digits + block * latent_digit_bytes(RP) +
+                ((RP / 32 + t / 8) * 64 + (t / 4 % 2) * 32 + col) * 32 + 4 * (t % 4);
+  *(uint32_t*)at = hi;
+  *(uint32_t*)(at + 16) = lo;
+  if (t == 0) a.qscale[(block * kLatentCols + col) * 2 + 1] = bad_key ? nan : ks;
 }
 
 // ---------------------------------------------------------------------------
@@ -263,37 +286,42 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnArgs a) {
     const uint8_t* key = lat + L::kLat;
     const float* scales = (const float*)(key + L::kKey);
 
-    // Scores: the shared key's part, then the latent's.  The compiler barriers
-    // keep the operands of a few products in flight and no more: the columns'
-    // queries and the sums leave about a hundred registers.
+    // Scores: the shared key's part, then the latent's.  A step's operand is read
+    // two steps ahead; the compiler barriers keep that order, and keep the reads
+    // from running further ahead (the columns' queries and the sums leave about a
+    // hundred registers).
     float S[16];
+    auto key_at = [&](int s) __attribute__((always_inline)) {
+      return s < 2 ? *(const u32x4*)(key + col * kLatentRope + (((2 * s + half) ^ ((col >> 1) & 3)) * 16))
+                   : *(const u32x4*)(lat + ka[(s - 2) & 3] + ((s - 2) >> 2) * 128);
+    };
     {
+      constexpr int kAhead = 2;
+      u32x4 kf[kAhead + 1];
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) kf[s] = key_at(s);
       intx16 hi = {}, lo = {};
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const u32x4 kf = *(const u32x4*)(key + col * kLatentRope + (((2 * s + half) ^ ((col >> 1) & 3)) * 16));
-        hi = mfma32x32x32_i8(kf, qhi[kLatSteps + s], hi);
-        lo = mfma32x32x32_i8(kf, qlo[kLatSteps + s], lo);
-      }
+      for (int s = 0; s < kLatSteps + 2; ++s) {
+        if (s + kAhead < kLatSteps + 2) kf[(s + kAhead) % (kAhead + 1)] = key_at(s + kAhead);
+        __asm__ volatile("" ::: "memory");
+        const int qi = s < 2 ? kLatSteps + s : s - 2;
+        hi = mfma32x32x32_i8(kf[s % (kAhead + 1)], qhi[qi], hi);
+        lo = mfma32x32x32_i8(kf[s % (kAhead + 1)], qlo[qi], lo);
+        if (s == 1) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float ks = scales[(8 * (i / 4) + 4 * half + i % 4) * 2 + 1];
-        S[i] = fmaf((float)hi[i], 256.0f, (float)lo[i]) * (ks * key_scale);
-      }
-    }
-    {
-      intx16 hi = {}, lo = {};
-#pragma unroll
-      for (int s = 0; s < kLatSteps; ++s) {
-        const u32x4 kf = *(const u32x4*)(lat + ka[s & 3] + (s >> 2) * 128);
-        hi = mfma32x32x32_i8(kf, qhi[s], hi);
-        lo = mfma32x32x32_i8(kf, qlo[s], lo);
-        if (s % 4 == 3) __asm__ volatile("" ::: "memory");
+          for (int i = 0; i < 16; ++i) {
+            const float ks = scales[(8 * (i / 4) + 4 * half + i % 4) * 2 + 1];
+            S[i] = (float)((hi[i] << 8) + lo[i]) * (ks * key_scale);
+            hi[i] = lo[i] = 0;
+          }
+        }
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float ls = scales[(8 * (i / 4) + 4 * half + i % 4) * 2];
-        S[i] = fmaf(fmaf((float)hi[i], 256.0f, (float)lo[i]), ls * lat_scale, S[i]);
+        // (At most 512 * 127 * 127 * 256 + 512 * 128 * 127 < 2^31.)
+        S[i] = fmaf((float)((hi[i] << 8) + lo[i]), ls * lat_scale, S[i]);
       }
     }
     // A tile's largest token scale, as a power of two: P' is kept relative to the
@@ -340,14 +368,20 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnArgs a) {
         p[u][2 * i] = to_f16x2(S[8 * u + 4 * i], S[8 * u + 4 * i + 2]);
         p[u][2 * i + 1] = to_f16x2(S[8 * u + 4 * i + 1], S[8 * u + 4 * i + 3]);
       }
+    {
+      constexpr int kAhead = 4;
+      u32x2 vf[kAhead + 1];
+      auto value_at = [&](int i) __attribute__((always_inline)) {
+        return lds_read_tr8(lat + va[i / 2 & 3] + (i / 8) * 128 + (i & 1) * 16 * RP);
+      };
 #pragma unroll
-    for (int rb = 0; rb < kBlocks; ++rb) {
+      for (int i = 0; i < kAhead; ++i) vf[i] = value_at(i);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const u32x2 v = lds_read_tr8(lat + va[rb & 3] + (rb >> 2) * 128 + u * 16 * RP);
-        O[rb] = mfma32x32x16_f16(bytes_to_f16(v), p[u], O[rb]);
+      for (int i = 0; i < 2 * kBlocks; ++i) {
+        if (i + kAhead < 2 * kBlocks) vf[(i + kAhead) % (kAhead + 1)] = value_at(i + kAhead);
+        __asm__ volatile("" ::: "memory");
+        O[i / 2] = mfma32x32x16_f16(bytes_to_f16(vf[i % (kAhead + 1)]), p[i & 1], O[i / 2]);
       }
-      if (rb % 2 == 1) __asm__ volatile("" ::: "memory");
     }
     latent_wait_lds();  // before the DMA of a later tile writes here
     slot = slot + 1 == L::kRing ? 0 : slot + 1;
@@ -399,21 +433,21 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnArgs a) {
 // ---------------------------------------------------------------------------
 // Joining the splits, and out of the latent space
 // ---------------------------------------------------------------------------
-// One workgroup per (row, head) column: its splits' sums weighted by 2^(m - M),
-// divided by the joined softmax sum and written as bf16 and the bf16 of what that
-// leaves (2^-17 in all), the operands of the product with W_uv.
+// Workgroup = (one (row, head) column, 128 latent elements): its splits' sums
+// weighted by 2^(m - M), eight splits at a time, divided by the joined softmax
+// sum and written as bf16 and the bf16 of what that leaves (2^-17 in all), the
+// operands of the product with W_uv.
 template <int RP>
 __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnArgs a) {
-  constexpr int kLanes = RP / 4, kGroups = 256 / kLanes;
   __shared__ floatx4 part[256];
-  const uint32_t H = a.d.heads, m = blockIdx.x / H, h = blockIdx.x - m * H;
+  const uint32_t c_all = blockIdx.x / (RP / 128), r0 = blockIdx.x % (RP / 128) * 128;
+  const uint32_t H = a.d.heads, m = c_all / H, h = c_all - m * H;
   const LatentSeq& sq = a.seqs[a.decode ? m : 0];
   const uint32_t cols = a.decode ? H : a.rows * H, blocks = (cols + kLatentCols - 1) / kLatentCols;
-  const uint32_t c = a.decode ? h : blockIdx.x, cb = c / kLatentCols, col = c % kLatentCols;
-  const uint32_t t = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const uint32_t c = a.decode ? h : c_all, cb = c / kLatentCols, col = c % kLatentCols;
+  const uint32_t t = threadIdx.x % 32, group = threadIdx.x / 32, lane = threadIdx.x & 63;
   const float* ml = a.partials + (size_t)a.units * kLatentCols * RP;
   auto at = [&](uint32_t s) { return (size_t)(sq.unit_begin + s * blocks + cb) * kLatentCols + col; };
-  const uint32_t lane = threadIdx.x & 63;
   float top = kNoMax, sum = 0.0f;
   for (uint32_t s = lane; s < sq.splits; s += 64) top = fmaxf(top, ml[at(s) * 2]);
   top = wave_allmax(top);
@@ -423,16 +457,16 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnArgs a) {
   }
   sum = wave_allsum(sum);
   floatx4 acc = {0, 0, 0, 0};
-  if (group < kGroups)
-    for (uint32_t s = group; s < sq.splits; s += kGroups) {
-      const float w = __builtin_amdgcn_exp2f(ml[at(s) * 2] - top);
-      acc += *(const floatx4*)(a.partials + at(s) * RP + 4 * t) * w;
-    }
+#pragma unroll 4
+  for (uint32_t s = group; s < sq.splits; s += 8) {
+    const float w = __builtin_amdgcn_exp2f(ml[at(s) * 2] - top);
+    acc += *(const floatx4*)(a.partials + at(s) * RP + r0 + 4 * t) * w;
+  }
   part[threadIdx.x] = acc;
   __syncthreads();
   if (group != 0) return;
 #pragma unroll
-  for (int g = 1; g < kGroups; ++g) acc += part[g * kLanes + t];
+  for (int g = 1; g < 8; ++g) acc += part[g * 32 + t];
   const float r = 1.0f / sum;
   float x[4], y[4];
 #pragma unroll
@@ -440,42 +474,55 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnArgs a) {
     x[i] = acc[i] * r;
     y[i] = x[i] - (float)(__bf16)x[i];
   }
-  uint16_t* to = a.mixed + (size_t)blockIdx.x * 2 * RP + 4 * t;
+  uint16_t* to = a.mixed + (size_t)c_all * 2 * RP + r0 + 4 * t;
   *(u32x2*)to = u32x2{to_bf16x2(x[0], x[1]), to_bf16x2(x[2], x[3])};
   *(u32x2*)(to + RP) = u32x2{to_bf16x2(y[0], y[1]), to_bf16x2(y[2], y[3])};
 }
 
-// o[m][h][n] = sum_r mixed[m][h][r] W_uv[h][n][r]: workgroup = (16 rows, head),
-// a wave takes a quarter of the head's outputs.
+// o[m][h][n] = sum_r mixed[m][h][r] W_uv[h][n][r]: workgroup = (16 rows, head, 32
+// outputs), a wave takes a quarter of the latent; the quarters are added in
+// order in LDS.
 template <int RP>
 __global__ __launch_bounds__(256) void latent_up_kernel(LatentAttnArgs a) {
+  __shared__ float part[4][16][33];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, kq = lane >> 4;
-  const uint32_t h = blockIdx.y, m0 = blockIdx.x * 16, H = a.d.heads, vp = a.d.v_pad;
-  const uint16_t* up = a.up + ((size_t)h * (a.d.nope_pad + vp) + a.d.nope_pad) * RP;
-  const uint16_t* x = a.mixed + ((size_t)min(m0 + n, a.rows - 1) * H + h) * 2 * RP;
-  for (uint32_t n0 = 16 * wave; n0 < vp; n0 += 64) {
-    floatx4 acc = {0, 0, 0, 0};
+  const uint32_t H = a.d.heads, vp = a.d.v_pad;
+  const uint32_t n0 = blockIdx.x % (vp / 32) * 32, h = blockIdx.x / (vp / 32) % H, m0 = blockIdx.x / (vp / 32) / H * 16;
+  if (n0 >= a.d.v) return;
+  const uint16_t* up = a.up + ((size_t)h * (a.d.nope_pad + vp) + a.d.nope_pad + n0) * RP + wave * (RP / 4) + 8 * kq;
+  const uint16_t* x = a.mixed + ((size_t)min(m0 + n, a.rows - 1) * H + h) * 2 * RP + wave * (RP / 4) + 8 * kq;
+  floatx4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-    for (int s = 0; s < RP / 32; ++s) {
-      const u32x4 w = *(const u32x4*)(up + (size_t)(n0 + n) * RP + 32 * s + 8 * kq);
-      acc = mfma16x16x32(*(const u32x4*)(x + 32 * s + 8 * kq), w, acc);
-      acc = mfma16x16x32(*(const u32x4*)(x + RP + 32 * s + 8 * kq), w, acc);
-    }
+  for (int s = 0; s < RP / 128; ++s) {
+    const u32x4 hi = *(const u32x4*)(x + 32 * s), lo = *(const u32x4*)(x + RP + 32 * s);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t m = m0 + 4 * kq + i;
-      if (m < a.rows && n0 + n < a.d.v) a.o[((size_t)m * H + h) * a.d.v + n0 + n] = f32_to_bf16(acc[i]);
+    for (int t = 0; t < 2; ++t) {
+      const u32x4 w = *(const u32x4*)(up + (size_t)(16 * t + n) * RP + 32 * s);
+      acc[t] = mfma16x16x32(hi, w, acc[t]);
+      acc[t] = mfma16x16x32(lo, w, acc[t]);
     }
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[wave][4 * kq + i][16 * t + n] = acc[t][i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t at = i * 256 + threadIdx.x, mm = at / 32, nn = at % 32;
+    if (m0 + mm >= a.rows || n0 + nn >= a.d.v) continue;
+    const float v = part[0][mm][nn] + part[1][mm][nn] + part[2][mm][nn] + part[3][mm][nn];
+    a.o[((size_t)(m0 + mm) * H + h) * a.d.v + n0 + nn] = f32_to_bf16(v);
   }
 }
 
 template <int RP>
 hipError_t absorbed(const LatentAttnArgs& a, hipStream_t st) {
-  const dim3 tiles((a.rows + 15) / 16, a.d.heads);
-  hipLaunchKernelGGL(latent_query_kernel<RP>, tiles, dim3(256), 0, st, a);
+  const uint32_t tiles = (a.rows + 15) / 16 * a.d.heads, append_blocks = (a.rows + 3) / 4;
+  hipLaunchKernelGGL(latent_query_kernel<RP>, dim3(append_blocks + tiles * (RP / 128)), dim3(256), 0, st, a, append_blocks);
   hipLaunchKernelGGL(latent_attn_kernel<RP>, dim3(a.units), dim3(256), 0, st, a);
-  hipLaunchKernelGGL(latent_join_kernel<RP>, dim3(a.rows * a.d.heads), dim3(256), 0, st, a);
-  hipLaunchKernelGGL(latent_up_kernel<RP>, tiles, dim3(256), 0, st, a);
+  hipLaunchKernelGGL(latent_join_kernel<RP>, dim3(a.rows * a.d.heads * (RP / 128)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(latent_up_kernel<RP>, dim3(tiles * (a.d.v_pad / 32)), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 

@@ -1,92 +1,20 @@
 // The 8-bit cache of latent attention: rows written and read back, and the
 // weights in the kernels' layouts.
 //
-// A token's row is its latent (rank_pad codes) and the shared key (64 codes),
-// each with one fp32 scale: s = max(absmax / 127, FLT_MIN), code = round half
-// away(clamp(x / s, -127, 127)) with IEEE division, the quantiser of the Q8 KV
-// cache (but that a part with a NaN or an infinity stands for NaN).  The latent may be RMS-normalised on its way (x rsqrt(mean x^2 + eps)
-// w), in fp32: the projection's row is read once and nothing else is written
-// but the 8 bits.
-//
-// A wave takes a row: 8 elements per lane of the latent (16 bytes in, 8 out)
-// and 8 per lane of lanes 0..7 of the key.
-#include <float.h>
-
-#include <algorithm>
-
-#include "common.h"
+// A row's layout and quantiser: latent_append.h.
 #include "latent.h"
+#include "latent_append.h"
+#include "latent_device.h"
 
 namespace qm {
 namespace {
 
 constexpr int kWaves = 4;
 
-__device__ __forceinline__ void unpack8(u32x4 v, float (&x)[8]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = bf16_to_f32(v[i] & 0xFFFFu);
-    x[2 * i + 1] = __uint_as_float(v[i] & 0xFFFF0000u);
-  }
-}
-
-// Quantises a wave's row held 8 elements per lane; returns the scale: NaN, with
-// codes of 0, for a row that holds a NaN or an infinity.
-__device__ __forceinline__ float quantise(const float (&x)[8], u32x2* codes) {
-  float amax = 0.0f;
-  bool finite = true;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    amax = fmaxf(amax, fabsf(x[i]));
-    finite = finite && fabsf(x[i]) <= FLT_MAX;
-  }
-  if (__any(!finite)) {
-    *codes = u32x2{0, 0};
-    return __uint_as_float(0x7FC00000u);
-  }
-  amax = wave_allmax(amax);
-  const float s = fmaxf(amax / 127.0f, FLT_MIN);
-  uint32_t w[2] = {0, 0};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int8_t c = (int8_t)roundf(fminf(fmaxf(x[i] / s, -127.0f), 127.0f));
-    w[i / 4] |= (uint32_t)(uint8_t)c << (8 * (i % 4));
-  }
-  *codes = u32x2{w[0], w[1]};
-  return s;
-}
-
 __global__ __launch_bounds__(64 * kWaves) void latent_append_kernel(LatentAppendArgs a) {
-  const uint32_t lane = threadIdx.x & 63;
   const uint32_t item = blockIdx.x * kWaves + (threadIdx.x >> 6);
   if (item >= a.items) return;  // wave-uniform
-  const uint16_t* src = a.kv + (size_t)item * (a.rank + a.rope);
-  const uint32_t e = 8 * lane;
-  const u32x4 none = {0, 0, 0, 0};
-  const u32x4 lat = e < a.rank ? *(const u32x4*)(src + e) : none;
-  const u32x4 key = e < a.rope ? *(const u32x4*)(src + a.rank + e) : none;
-  float w[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = a.norm && e < a.rank ? a.norm[e + i] : 1.0f;
-  float x[8], k[8];
-  unpack8(lat, x);
-  unpack8(key, k);
-  if (a.norm) {
-    float ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
-    const float r = 1.0f / sqrtf(wave_allsum(ss) / (float)a.rank + a.eps);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
-  }
-  u32x2 cx, ck;
-  const float sx = quantise(x, &cx), sk = quantise(k, &ck);
-  const LatentRows& to = a.seqs[a.decode ? item : 0];
-  const size_t token = a.decode ? a.pos[item] : (size_t)a.pos[0] + item;
-  int8_t* row = to.codes + token * (a.rank_pad + kLatentRope);
-  if (e < a.rank_pad) *(u32x2*)(row + e) = cx;
-  if (e < kLatentRope) *(u32x2*)(row + a.rank_pad + e) = ck;
-  if (lane == 0) *(float2*)(to.scales + 2 * token) = float2{sx, sk};
+  latent_append_row(a.rows, a.to, a.first + item, item, threadIdx.x & 63);
 }
 
 __global__ __launch_bounds__(64 * kWaves) void latent_load_kernel(LatentRows rows, uint32_t rank, uint32_t rope,
@@ -145,6 +73,30 @@ __global__ __launch_bounds__(256) void latent_weights_kernel(LatentDims d, From 
   if (key) down[((size_t)h * d.rank_pad + r) * d.nope_pad + n] = v;
 }
 
+// One workgroup per head.  A norm that is no number stays one (compared as bits).
+__global__ __launch_bounds__(256) void latent_wnorm_kernel(LatentDims d, const uint16_t* down, float* wnorm) {
+  __shared__ uint32_t top[256];
+  const uint16_t* w = down + (size_t)blockIdx.x * d.rank_pad * d.nope_pad;
+  uint32_t best = 0;
+  for (uint32_t r = threadIdx.x; r < d.rank_pad; r += 256) {
+    float s = 0.0f;
+    for (uint32_t k = 0; k < d.nope_pad; k += 8) {
+      float x[8];
+      latent_unpack8(*(const u32x4*)(w + (size_t)r * d.nope_pad + k), x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s = fmaf(x[i], x[i], s);
+    }
+    best = max(best, __float_as_uint(s) & 0x7FFFFFFFu);
+  }
+  top[threadIdx.x] = best;
+  __syncthreads();
+  for (uint32_t n = 128; n; n /= 2) {
+    if (threadIdx.x < n) top[threadIdx.x] = max(top[threadIdx.x], top[threadIdx.x + n]);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) wnorm[blockIdx.x] = sqrtf(__uint_as_float(top[0])) * 1.0001f;
+}
+
 template <class From>
 hipError_t weights(const LatentDims& d, From from, uint16_t* down, uint16_t* up, hipStream_t st) {
   const uint32_t n = (d.nope_pad + d.v_pad) * d.rank_pad;
@@ -156,6 +108,11 @@ hipError_t weights(const LatentDims& d, From from, uint16_t* down, uint16_t* up,
 
 hipError_t launch_latent_append(const LatentAppendArgs& a, hipStream_t st) {
   hipLaunchKernelGGL(latent_append_kernel, dim3((a.items + kWaves - 1) / kWaves), dim3(64 * kWaves), 0, st, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_latent_wnorm(const LatentDims& d, const uint16_t* down, float* wnorm, hipStream_t st) {
+  hipLaunchKernelGGL(latent_wnorm_kernel, dim3(d.heads), dim3(256), 0, st, d, down, wnorm);
   return hipGetLastError();
 }
 

@@ -62,14 +62,14 @@ __device__ __forceinline__ uint32_t to_f16x2(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, v);
 }
 // 8 signed bytes -> 8 fp16, exact, in the order 0, 2, 1, 3, 4, 6, 5, 7: 0x6400 | u
-// is the fp16 1024 + u, so each pair takes one AND-OR and one packed subtraction.
+// is the fp16 1024 + u, so each pair takes one permute and one packed subtraction.
 __device__ __forceinline__ u32x4 bytes_to_f16(u32x2 w) {
   const latent_halfx4 bias = {(_Float16)1152.0f, (_Float16)1152.0f, (_Float16)1152.0f, (_Float16)1152.0f};
   u32x4 r;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint32_t u = w[i] ^ 0x80808080u;
-    const u32x2 biased = {(u & 0x00FF00FFu) | 0x64006400u, ((u >> 8) & 0x00FF00FFu) | 0x64006400u};
+    const u32x2 biased = {perm_b32(u, 0x64646464u, 0x00060004u), perm_b32(u, 0x64646464u, 0x00070005u)};
     const u32x2 v = __builtin_bit_cast(u32x2, __builtin_bit_cast(latent_halfx4, biased) - bias);
     r[2 * i] = v.x;
     r[2 * i + 1] = v.y;

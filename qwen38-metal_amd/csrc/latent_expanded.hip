@@ -40,10 +40,13 @@ __global__ __launch_bounds__(256) void latent_wmul_kernel(LatentDims d, const ui
   __shared__ float top[2][4];
   const uint32_t h = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rows = d.nope_pad + d.v_pad;
   float best[2] = {0.0f, 0.0f};
+#pragma unroll 4
   for (uint32_t n = wave; n < rows; n += 4) {
     const uint16_t* w = up + ((size_t)h * rows + n) * d.rank_pad;
+    const u32x4 x = 8 * lane < d.rank_pad ? *(const u32x4*)(w + 8 * lane) : u32x4{0, 0, 0, 0};
     float s = 0.0f;
-    for (uint32_t r = lane; r < d.rank_pad; r += 64) s += fabsf(bf16_to_f32(w[r]));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s += fabsf(bf16_to_f32(x[k] & 0xFFFFu)) + fabsf(__uint_as_float(x[k] & 0xFFFF0000u));
     s = wave_allsum(s);
     const int part = n >= d.nope_pad;
     best[part] = fmaxf(best[part], s);

@@ -32,6 +32,7 @@ struct qm_latent_weights {
   uint16_t* up = nullptr;
   uint16_t* wop = nullptr;  // up, as the expanded form reads it
   float* wmul = nullptr;
+  float* wnorm = nullptr;   // bound of the absorbed form's queries
 };
 
 namespace {
@@ -40,6 +41,7 @@ void free_weights(qm_latent_weights* w) {
   (void)hipFree(w->up);
   (void)hipFree(w->wop);
   (void)hipFree(w->wmul);
+  (void)hipFree(w->wnorm);
   delete w;
 }
 }  // namespace
@@ -207,7 +209,9 @@ qm_status create_weights(qm_runtime* rt, const qm_latent_config& c, qm_latent_we
   if (e == hipSuccess) e = hipMalloc(&w->up, up);
   if (e == hipSuccess) e = hipMalloc(&w->wop, up);
   if (e == hipSuccess) e = hipMalloc(&w->wmul, (size_t)d.heads * 2 * sizeof(float));
+  if (e == hipSuccess) e = hipMalloc(&w->wnorm, (size_t)d.heads * sizeof(float));
   if (e == hipSuccess) e = launch(d, w->down, w->up);
+  if (e == hipSuccess) e = launch_latent_wnorm(d, w->down, w->wnorm, rt->stream);
   if (e == hipSuccess) e = launch_latent_wop(d, w->up, w->wmul, w->wop, rt->stream);
   if (e == hipSuccess) e = hipStreamSynchronize(rt->stream);
   if (e != hipSuccess) {
@@ -237,16 +241,31 @@ qm_status check_attention(const qm_runtime* rt, const qm_latent_weights* w, qm_l
   return check_stream(rt, "latent attention");
 }
 
-LatentAppendArgs append_args(const LatentDims& d, const uint16_t* kv, const float* norm, float epsilon, uint32_t items,
-                             bool decode) {
-  LatentAppendArgs a{};
-  a.kv = kv;
-  a.norm = norm;
-  a.eps = epsilon;
-  a.rank = d.rank;
-  a.rope = d.rope;
-  a.rank_pad = d.rank_pad;
-  a.items = items;
+LatentNewRows new_rows(uint32_t rank, uint32_t rope, const uint16_t* kv, const float* norm, float epsilon) {
+  LatentNewRows n{};
+  n.kv = kv;
+  n.norm = norm;
+  n.eps = epsilon;
+  n.rank = rank;
+  n.rope = rope;
+  n.rank_pad = latent_rank_pad(rank);
+  return n;
+}
+
+// What an absorbed call has from its arguments; the sequences are the caller's.
+LatentAttnArgs absorbed_args(const qm_latent_weights* w, const LatentNewRows& rows, const uint16_t* q, uint16_t* o,
+                             uint32_t M, uint32_t n_seqs, bool decode) {
+  LatentAttnArgs a{};
+  a.q = q;
+  a.o = o;
+  a.down = w->down;
+  a.up = w->up;
+  a.wnorm = w->wnorm;
+  a.new_rows = rows;
+  a.d = w->d;
+  a.scale = w->scale;
+  a.rows = M;
+  a.n_seqs = n_seqs;
   a.decode = decode;
   return a;
 }
@@ -528,11 +547,7 @@ qm_status qm_latent_append(qm_runtime* rt, qm_latent_kv* kv, const uint16_t* row
   if (st != QM_OK) return st;
   if ((st = grow(kv, (uint64_t)kv->length + M)) != QM_OK) return st;
   if ((st = stream_after(rt, kv->rt)) != QM_OK) return st;
-  LatentDims d{};
-  d.rank = kv->rank, d.rope = kv->rope, d.rank_pad = kv->rank_pad;
-  LatentAppendArgs a = append_args(d, rows, norm, epsilon, M, false);
-  a.seqs[0] = kv->rows;
-  a.pos[0] = kv->length;
+  const LatentAppendArgs a{new_rows(kv->rank, kv->rope, rows, norm, epsilon), kv->rows, kv->length, M};
   if ((st = hip_check(launch_latent_append(a, rt->stream), "latent append launch")) != QM_OK) return st;
   kv->length += M;
   return stream_after(kv->rt, rt);
@@ -603,28 +618,17 @@ qm_status qm_latent_decode(qm_runtime* rt, const qm_latent_weights* w, qm_latent
   if (!g.ok()) return no_device();
   for (uint32_t b = 0; b < B; ++b)
     if ((st = grow(seqs[b], (uint64_t)seqs[b]->length + 1)) != QM_OK) return st;
-  LatentAppendArgs ap = append_args(w->d, kv, norm, epsilon, B, true);
-  LatentAttnArgs at{};
-  at.q = q;
-  at.o = o;
-  at.down = w->down;
-  at.up = w->up;
-  at.d = w->d;
-  at.scale = w->scale;
-  at.rows = at.n_seqs = B;
-  at.decode = 1;
+  LatentAttnArgs at = absorbed_args(w, new_rows(w->d.rank, w->d.rope, kv, norm, epsilon), q, o, B, B, true);
   for (uint32_t b = 0; b < B; ++b) {
-    ap.seqs[b] = at.seqs[b].rows = seqs[b]->rows;
-    ap.pos[b] = at.seqs[b].start = seqs[b]->length;
+    at.seqs[b].rows = seqs[b]->rows;
+    at.seqs[b].start = seqs[b]->length;
   }
   plan_absorbed(rt, &at);
   if ((st = absorbed_workspaces(rt, &at)) != QM_OK) return st;
   // Caches owned by another runtime: their pending work comes first.
   for (uint32_t b = 0; b < B; ++b)
     if ((st = stream_after(rt, seqs[b]->rt)) != QM_OK) return st;
-  hipError_t e = launch_latent_append(ap, rt->stream);
-  if (e == hipSuccess) e = launch_latent_absorbed(at, rt->stream);
-  if (e != hipSuccess) return hip_check(e, "latent attention launch");
+  if ((st = hip_check(launch_latent_absorbed(at, rt->stream), "latent attention launch")) != QM_OK) return st;
   for (uint32_t b = 0; b < B; ++b) seqs[b]->length += 1;
   for (uint32_t b = 0; b < B; ++b)
     if ((st = stream_after(seqs[b]->rt, rt)) != QM_OK) return st;
@@ -642,23 +646,14 @@ qm_status qm_latent_prefill(qm_runtime* rt, const qm_latent_weights* w, qm_laten
   DeviceGuard g(rt->device);
   if (!g.ok()) return no_device();
   if ((st = grow(seq, (uint64_t)seq->length + M)) != QM_OK) return st;
-  LatentAppendArgs ap = append_args(w->d, kv, norm, epsilon, M, false);
-  ap.seqs[0] = seq->rows;
-  ap.pos[0] = seq->length;
+  const LatentNewRows rows = new_rows(w->d.rank, w->d.rope, kv, norm, epsilon);
   const bool expanded = prefers_expanded(rt, w->d, M, (uint64_t)seq->length + M);
   LatentAttnArgs at{};
   ExpandedPlan ep;
   if (expanded) {
     st = plan_expanded(rt, w, seq, M, o, q, &ep);
   } else {
-    at.q = q;
-    at.o = o;
-    at.down = w->down;
-    at.up = w->up;
-    at.d = w->d;
-    at.scale = w->scale;
-    at.rows = M;
-    at.n_seqs = 1;
+    at = absorbed_args(w, rows, q, o, M, 1, false);
     at.seqs[0].rows = seq->rows;
     at.seqs[0].start = seq->length;
     plan_absorbed(rt, &at);
@@ -666,9 +661,13 @@ qm_status qm_latent_prefill(qm_runtime* rt, const qm_latent_weights* w, qm_laten
   }
   if (st != QM_OK) return st;
   if ((st = stream_after(rt, seq->rt)) != QM_OK) return st;
-  hipError_t e = launch_latent_append(ap, rt->stream);
-  if (e == hipSuccess)
-    e = expanded ? launch_latent_expanded(ep.a, ep.heads_at_once, rt->stream) : launch_latent_absorbed(at, rt->stream);
+  hipError_t e = hipSuccess;
+  if (expanded) {
+    e = launch_latent_append(LatentAppendArgs{rows, seq->rows, seq->length, M}, rt->stream);
+    if (e == hipSuccess) e = launch_latent_expanded(ep.a, ep.heads_at_once, rt->stream);
+  } else {
+    e = launch_latent_absorbed(at, rt->stream);
+  }
   if (e != hipSuccess) return hip_check(e, "latent attention launch");
   seq->length += M;
   return stream_after(seq->rt, rt);
