@@ -70,6 +70,7 @@ struct Tuning {
   int prefill_splits = 0;   // QM38_PREFILL_SPLITS: workgroups sharing a prefill column block's tiles
   int prefill_waves = 0;    // QM38_PREFILL_WAVES: 4 or 8 waves per prefill workgroup
   int latent_form = 0;      // QM38_LATENT_FORM: 1 absorbed, 2 expanded latent prefill
+  int latent_tiles = 0;     // QM38_LATENT_TILES: tiles of an absorbed split
   int latent_mb = 0;        // QM38_LATENT_MB: workspace of expanded keys and values
   int dn_step_head = -1;    // QM38_DN_STEP_HEAD: 0 forces the split step kernel (-1: default)
   int dn_chunked = -1;      // QM38_DN_CHUNKED: 1 / 0 forces the chunked / token-serial prefill (-1: default)

@@ -8,8 +8,8 @@ namespace qm {
 
 constexpr uint32_t kLatentMaxRank = 512, kLatentMaxNope = 128, kLatentMaxV = 128;
 constexpr uint32_t kLatentRope = 64;   // stored width of the shared key (the extra elements hold zero)
-constexpr uint32_t kLatentTile = 32;   // tokens of a tile; a cache's capacity is a multiple
-constexpr uint32_t kLatentCols = 32;   // (row, head) columns of an absorbed-attention workgroup
+constexpr uint32_t kLatentTile = 64;   // tokens of an absorbed-attention tile; a cache's capacity is a multiple
+constexpr uint32_t kLatentCols = 32;   // (row, head) columns of a block
 constexpr uint32_t kMaxLatentSeqs = 64;
 
 // Stored widths: a latent's (128 .. 512) and an expanded key's or value's (64, 128).
@@ -59,7 +59,7 @@ hipError_t launch_latent_weights_q4(const LatentDims& d, const uint32_t* w, cons
                                     uint16_t* down, uint16_t* up, hipStream_t st);
 
 // Absorbed attention.  Column c = row * H + head of a sequence; 32 columns
-// make a block.  Decode: one row for each sequence, H columns each.  Prefill:
+// make a block, one or two of them a workgroup's group.  Decode: one row for each sequence, H columns each.  Prefill:
 // one sequence of `rows` rows.
 struct LatentSeq {
   LatentRows rows;
@@ -77,7 +77,7 @@ struct LatentAttnArgs {
   LatentNewRows new_rows; // appended by the first launch
   uint8_t* digits;        // queries in operand order, [block][rank_pad / 32 + 2][64 lanes][32 bytes]
   float* qscale;          // [block][32][2]
-  float* partials;        // O [unit][32][rank_pad], then (max, sum) [unit][32][2]
+  float* partials;        // sums [unit][group_cols * rank_pad], then (max, softmax sum) [unit][group_cols][2]
   uint16_t* mixed;        // bf16 [rows][H][2][rank_pad]: the joined sums of latents, and what bf16 leaves of them
   LatentDims d;
   float scale;            // of the scores
@@ -87,6 +87,7 @@ struct LatentAttnArgs {
   uint32_t blocks;        // column blocks of the call
   uint32_t units;         // workgroups of the attention launch
   uint32_t tiles_per_split;
+  uint32_t group_cols;    // columns of an attention workgroup, 32 or 64
   LatentSeq seqs[kMaxLatentSeqs];
 };
 constexpr uint64_t latent_digit_bytes(uint32_t rank_pad) { return (uint64_t)(rank_pad / 32 + 2) * 64 * 32; }

@@ -8,6 +8,8 @@
 // latent_up_kernel.
 #include <float.h>
 
+#include <type_traits>
+
 #include "latent.h"
 #include "latent_append.h"
 #include "latent_device.h"
@@ -150,34 +152,40 @@ __global__ __launch_bounds__(256) void latent_query_kernel(LatentAttnArgs a, uin
 // ---------------------------------------------------------------------------
 // Attention over the cache
 // ---------------------------------------------------------------------------
-// A wave takes 32 columns (heads of a row, or of several rows) and every fourth
-// 32-token tile of its workgroup's share of the cache, alone: it streams the
-// tiles' bytes into its own LDS ring by buffer->LDS DMA and never waits for the
-// other waves before the end.
-//   S^T[token][column] = codes . (hi, lo) on v_mfma_i32_32x32x32_i8, the token's
-//     and the column's scales applied in fp32;
-//   online softmax in fp32 (exp2 domain), p = 2^(s - ref): ref is a column's
-//     maximum less 6, moved (and the sums rescaled) only when a maximum passes
-//     ref + 14, so p stays below 2^14 and what is 2^-20 of the largest is still
-//     a normal fp16;
-//   O^T[latent element][column] += codes^T P'^T on v_mfma_f32_32x32x16_f16:
-//     P' = p * token scale / 2^e, 2^e the largest scale's power of two so far,
-//     rounded to fp16 (2^-11 of each term, where bf16 would be 2^-8), the codes
-//     exact.
-//     S^T leaves a lane the P' of its own column in the order that the second
-//     product wants once the tokens of its operand are taken in the same order,
-//     so P' stays in registers; the codes' operand comes by transposing reads.
-// The O^T accumulators (rank_pad x 32 fp32) take half of the register file.
-template <int RP>
+// Workgroup = (32 NC columns, a share of the cache's 64-token tiles), eight waves,
+// one workgroup a CU.  A column is a head of a row.  The tiles' bytes stream into
+// an LDS ring by buffer->LDS DMA and are read from there as they lie:
+//   scores   S^T[token][column] = codes . (hi, lo) on v_mfma_i32_32x32x32_i8.  A
+//            wave has a column block, 32 of the tokens and a part of the latent
+//            (a half, or a quarter with one column block); the parts exchange
+//            their whole numbers through LDS and each finishes a share of the
+//            tokens, where the token's and the column's scales come in in fp32.
+//            Cutting the latent keeps the queries in registers once.
+//   softmax  online, in fp32: p = 2^(s - ref), ref a column's maximum less 6,
+//            moved (and the sums rescaled) only when a maximum passes ref + 14, so
+//            p stays below 2^14 and what is 2^-20 of the largest is still a normal
+//            fp16.  The waves compute p with the ref they have and publish it with
+//            their maxima; where one passes, all see it behind the same barrier
+//            and do it again.
+//   sums     O^T[latent element][column] += codes^T P'^T on
+//            v_mfma_f32_32x32x16_f16, a wave an eighth of the latent: P' = token
+//            scale * p / 2^w, w moved like ref with the largest p * token scale;
+//            rounded to fp16 (2^-11 of each term, where bf16 would be 2^-8), the
+//            codes exact.  The codes' operand comes by transposing
+//            reads; its conversion is shared by the wave's columns.
+// Two barriers a tile: the scores' exchange, and P'.
+template <int RP, int NC>
 struct AbsorbedLds {
   static constexpr int kChunks = RP / 16;  // 16-byte pieces of a latent
   static constexpr int kLat = kLatentTile * RP, kKey = kLatentTile * (int)kLatentRope, kScale = kLatentTile * 8;
   static constexpr int kTileBytes = kLat + kKey + kScale;
-  static constexpr int kRing = RP >= 384 ? 2 : RP == 256 ? 3 : 4;
-  static constexpr int kPad = 132;  // floats of a column's 128 sums in the final merge
-  static constexpr int kMerge = 4 * (int)kLatentCols * kPad * 4 + 4 * (int)kLatentCols * 8;
-  static constexpr int kBytes = 4 * kRing * kTileBytes > kMerge ? 4 * kRing * kTileBytes : kMerge;
-  static constexpr int kDma = RP / 32 + 3;  // DMA instructions of a tile
+  static constexpr int kRing = 3;
+  static constexpr int kParts = 4 / NC;       // of the contraction
+  static constexpr int kShare = 16 / kParts;  // scores of a lane that a wave finishes
+  static constexpr int kExchange = NC == 1 ? 32768 : 16384;
+  static constexpr int kP = NC * 4096, kMax = 2 * kParts * NC * 32 * 8;
+  static constexpr int kBytes = kRing * kTileBytes + kExchange + kP + kMax;
+  static constexpr int kDma = RP / 128 + 2;  // DMA instructions of a wave and tile
 };
 
 // Order of a token's 16-byte pieces in LDS: piece j at j ^ swizzle(token).  Both
@@ -187,12 +195,17 @@ __device__ __forceinline__ constexpr uint32_t lat_swizzle(uint32_t tok) {
   return (tok & 3) | ((((tok >> 2) ^ (tok >> 3)) & 1) << 2);
 }
 
-template <int RP>
-__global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnArgs a) {
-  using L = AbsorbedLds<RP>;
-  constexpr int CH = L::kChunks, kLatSteps = RP / 32, kBlocks = RP / 32;
-  constexpr uint32_t kStride = RP + kLatentRope;
+template <int RP, int NC>
+__global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
+  using L = AbsorbedLds<RP, NC>;
+  constexpr int CH = L::kChunks, kParts = L::kParts, kShare = L::kShare;
+  constexpr int kLatSteps = RP / 32 / kParts;       // a wave's
+  constexpr int kAll = RP / 32, kBlocks = (kAll + 7) / 8;  // blocks of 32 latent elements: all, a wave's
+  constexpr uint32_t kStride = RP + kLatentRope, kCols = 32 * NC;
   __shared__ __attribute__((aligned(16))) uint8_t lds[L::kBytes];
+  uint8_t* const exchange = lds + L::kRing * L::kTileBytes;
+  uint8_t* const pbuf = exchange + L::kExchange;
+  float2* const maxima = (float2*)(pbuf + L::kP);  // [token block][part][column]: of s, of p * token scale
   const uint32_t lane = threadIdx.x & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t col = lane & 31, half = lane >> 5;
@@ -201,272 +214,350 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnArgs a) {
   while (b + 1 < a.n_seqs && unit >= a.seqs[b + 1].unit_begin) ++b;
   const LatentSeq& sq = a.seqs[b];
   const uint32_t cols = a.decode ? H : a.rows * H;
-  const uint32_t blocks = (cols + kLatentCols - 1) / kLatentCols;
-  const uint32_t local = unit - sq.unit_begin, cb = local % blocks, split = local / blocks;
+  const uint32_t groups = (cols + kCols - 1) / kCols;
+  const uint32_t local = unit - sq.unit_begin, cg = local % groups, split = local / groups;
+  // The wave's scores: a block of tokens, a column block, a part of the contraction.
+  const uint32_t tb = wave & 1, my_block = NC == 1 ? 0 : (wave >> 1) & 1, part = wave / (2 * NC);
   // Tokens that a column sees: up to its own row.
-  const uint32_t c_first = cb * kLatentCols, c_last = min(c_first + kLatentCols, cols) - 1, c = c_first + col;
+  const uint32_t c_first = cg * kCols, c_last = min(c_first + kCols, cols) - 1, c = c_first + 32 * my_block + col;
   const uint32_t lim_min = sq.start + c_first / H + 1, lim_max = sq.start + c_last / H + 1;
   const uint32_t limit = c <= c_last ? sq.start + c / H + 1 : 0;
   const uint32_t tiles = (lim_max + kLatentTile - 1) / kLatentTile;
   const uint32_t t_begin = split * a.tiles_per_split, t_end = min(tiles, t_begin + a.tiles_per_split);
 
-  const size_t block = sq.block_begin + cb;
-  u32x4 qhi[kLatSteps + 2], qlo[kLatSteps + 2];
+  // A tile's bytes, an eighth a wave: pieces of 1 KB of the latents, 512 bytes of
+  // the shared keys, 64 of the scales.
+  auto issue = [&](uint32_t tile, uint32_t slot) __attribute__((always_inline)) {
+    uint8_t* to = lds + slot * L::kTileBytes;
+    const auto rows = latent_rsrc(sq.rows.codes + (size_t)tile * kLatentTile * kStride, kLatentTile * kStride);
+#pragma unroll
+    for (int i = 0; i < RP / 128; ++i) {
+      const uint32_t p0 = (wave * (RP / 128) + i) * 64;
+      if constexpr (64 % CH == 0) {  // whole tokens: piece j of token p0 / CH + lane / CH
+        const uint32_t t0 = lane / CH, j = (lane % CH) ^ lat_swizzle(t0) ^ lat_swizzle(p0 / CH);
+        latent_dma16(rows, to + p0 * 16, t0 * kStride + j * 16, p0 / CH * kStride);
+      } else {
+        const uint32_t tok = (p0 + lane) / CH, j = ((p0 + lane) % CH) ^ lat_swizzle(tok);
+        latent_dma16(rows, to + p0 * 16, tok * kStride + j * 16, 0);
+      }
+    }
+    if (lane < 32) {  // token 8 wave + lane / 4, piece (lane % 4) ^ (token / 2 % 4)
+      const uint32_t tok = lane / 4;
+      latent_dma16(rows, to + L::kLat + wave * 512, tok * kStride + RP + (((lane & 3) ^ ((tok >> 1) & 3)) * 16),
+                   8 * wave * kStride);
+    }
+    const auto scales = latent_rsrc(sq.rows.scales + (size_t)tile * kLatentTile * 2, kLatentTile * 8);
+    if (lane < 16) latent_dma4(scales, to + L::kLat + L::kKey + wave * 64, wave * 64 + lane * 4);
+  };
+#pragma unroll
+  for (int i = 0; i < L::kRing - 1; ++i)
+    if (t_begin + i < t_end) issue(t_begin + i, i);
+
+  // (A group's last block may be one that does not exist; its columns have no tokens.)
+  const size_t block = sq.block_begin + min(cg * NC + my_block, (cols - 1) / 32);
+  u32x4 qhi[kLatSteps + 2], qlo[kLatSteps + 2];  // the shared key's last
   {
     const uint8_t* dg = a.digits + block * latent_digit_bytes(RP) + lane * 32;
 #pragma unroll
     for (int s = 0; s < kLatSteps + 2; ++s) {
-      qhi[s] = *(const u32x4*)(dg + s * 2048);
-      qlo[s] = *(const u32x4*)(dg + s * 2048 + 16);
+      const uint32_t step = s < kLatSteps ? part * kLatSteps + s : kAll + s - kLatSteps;
+      qhi[s] = *(const u32x4*)(dg + step * 2048);
+      qlo[s] = *(const u32x4*)(dg + step * 2048 + 16);
     }
   }
   const float2 qs = limit ? *(const float2*)(a.qscale + (block * kLatentCols + col) * 2) : float2{0.0f, 0.0f};
   const float lat_scale = qs.x * a.scale * kLog2e, key_scale = qs.y * a.scale * kLog2e;
 
-  uint8_t* ring = lds + wave * (L::kRing * L::kTileBytes);
-  const uint32_t tpi = 64 / CH;  // tokens of a DMA instruction (a whole number but for rank_pad 384)
-  const uint32_t jb = lane % CH, tb = lane / CH;
-  const uint32_t j16 = (jb ^ lat_swizzle(tb)) * 16, tb_off = tb * kStride;
-  const uint32_t key_tok = lane / 4;
-  auto issue = [&](uint32_t tile, uint32_t slot) __attribute__((always_inline)) {
-    uint8_t* to = ring + slot * L::kTileBytes;
-    const auto rows = latent_rsrc(sq.rows.codes + (size_t)tile * kLatentTile * kStride, kLatentTile * kStride);
-#pragma unroll
-    for (int i = 0; i < RP / 32; ++i) {
-      if constexpr (64 % CH == 0) {
-        latent_dma16(rows, to + i * 1024, tb_off + (j16 ^ (lat_swizzle(i * tpi) * 16)), i * tpi * kStride);
-      } else {
-        const uint32_t p = i * 64 + lane, tok = p / CH, j = (p % CH) ^ lat_swizzle(tok);
-        latent_dma16(rows, to + i * 1024, tok * kStride + j * 16, 0);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)  // token i * 16 + lane / 4, piece (lane % 4) ^ (token / 2 % 4)
-      latent_dma16(rows, to + L::kLat + i * 1024,
-                   (i * 16 + key_tok) * kStride + RP + (((lane & 3) ^ ((key_tok >> 1) & 3)) * 16), 0);
-    const auto scales = latent_rsrc(sq.rows.scales + (size_t)tile * kLatentTile * 2, kLatentTile * 8);
-    latent_dma4(scales, to + L::kLat + L::kKey, lane * 4);
-  };
-
-  // LDS offsets of this lane: codes of token `col` (score operand) and of the 8
+  // LDS offsets of this lane: codes of its token (score operands) and of the 8
   // tokens of a transposing read.
-  const uint32_t sw = lat_swizzle(col);
-  uint32_t ka[4], va[4];
+  const uint32_t tok0 = 32 * tb + col;
   const uint32_t trow = (lane & 15) >> 1, vtok = 4 * half + (trow < 4 ? trow : trow + 4);
-#pragma unroll
-  for (uint32_t v = 0; v < 4; ++v) {
-    ka[v] = col * RP + (((2 * v + half) ^ sw) * 16);
-    va[v] = vtok * RP + (((2 * v + ((lane >> 4) & 1)) ^ lat_swizzle(vtok)) * 16) + 8 * (lane & 1);
-  }
+  const uint32_t ka = tok0 * RP + ((half ^ lat_swizzle(tok0)) * 16);
+  const uint32_t kk = tok0 * kLatentRope + ((half ^ ((tok0 >> 1) & 3)) * 16);
+  const uint32_t va = vtok * RP + ((((lane >> 4) & 1) ^ lat_swizzle(vtok)) * 16) + 8 * (lane & 1);
 
-  floatx16 O[kBlocks];
+  floatx16 O[kBlocks][NC];
 #pragma unroll
   for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) O[i][j] = 0.0f;
-  float mref = kNoMax, l = 0.0f;
-  uint32_t vexp = 0x00800000u;  // the largest token scale's exponent, as a float's bits: the sums' unit
-
-  const uint32_t first = t_begin + wave;
-  const uint32_t count = first < t_end ? (t_end - first + 3) / 4 : 0;
+    for (int n = 0; n < NC; ++n)
 #pragma unroll
-  for (int i = 0; i < L::kRing - 1; ++i)
-    if ((uint32_t)i < count) issue(first + 4 * i, i);
+      for (int j = 0; j < 16; ++j) O[i][n][j] = 0.0f;
+  float mref[NC], w2[NC], l = 0.0f;  // ref, w
+#pragma unroll
+  for (int n = 0; n < NC; ++n) mref[n] = kNoMax, w2[n] = 0.0f;
+
+  latent_wait_vmcnt<0>();
+  lds_barrier();
   uint32_t slot = 0;
-  for (uint32_t it = 0; it < count; ++it) {
-    const uint32_t tile = first + 4 * it;
-    if (it + L::kRing - 1 < count) {
-      const uint32_t to = slot + L::kRing - 1;
-      issue(tile + 4 * (L::kRing - 1), to >= L::kRing ? to - L::kRing : to);
-      latent_wait_vmcnt<L::kDma*(L::kRing - 1) < 63 ? L::kDma * (L::kRing - 1) : 63>();
-    } else {
-      latent_wait_vmcnt<0>();
-    }
-    const uint8_t* lat = ring + slot * L::kTileBytes;
+  for (uint32_t tile = t_begin; tile < t_end; ++tile) {
+    const uint8_t* lat = lds + slot * L::kTileBytes;
     const uint8_t* key = lat + L::kLat;
     const float* scales = (const float*)(key + L::kKey);
 
-    // Scores: the shared key's part, then the latent's.  A step's operand is read
-    // two steps ahead; the compiler barriers keep that order, and keep the reads
-    // from running further ahead (the columns' queries and the sums leave about a
-    // hundred registers).
-    float S[16];
-    auto key_at = [&](int s) __attribute__((always_inline)) {
-      return s < 2 ? *(const u32x4*)(key + col * kLatentRope + (((2 * s + half) ^ ((col >> 1) & 3)) * 16))
-                   : *(const u32x4*)(lat + ka[(s - 2) & 3] + ((s - 2) >> 2) * 128);
-    };
+    // The wave's part of the latent's products, then all of the shared key's: 256
+    // hi + lo in whole numbers (at most 512 * 127 * 127 * 256 + 512 * 128 * 127 <
+    // 2^31).
+    int kdot[kShare], ldot[kShare];
     {
-      constexpr int kAhead = 2;
-      u32x4 kf[kAhead + 1];
-#pragma unroll
-      for (int s = 0; s < kAhead; ++s) kf[s] = key_at(s);
       intx16 hi = {}, lo = {};
 #pragma unroll
-      for (int s = 0; s < kLatSteps + 2; ++s) {
-        if (s + kAhead < kLatSteps + 2) kf[(s + kAhead) % (kAhead + 1)] = key_at(s + kAhead);
-        __asm__ volatile("" ::: "memory");
-        const int qi = s < 2 ? kLatSteps + s : s - 2;
-        hi = mfma32x32x32_i8(kf[s % (kAhead + 1)], qhi[qi], hi);
-        lo = mfma32x32x32_i8(kf[s % (kAhead + 1)], qlo[qi], lo);
-        if (s == 1) {
+      for (int s = 0; s < kLatSteps; ++s) {
+        const uint32_t step = part * kLatSteps + s;
+        const u32x4 kf = *(const u32x4*)(lat + (ka ^ ((step & 3) * 32)) + (step >> 2) * 128);
+        hi = mfma32x32x32_i8(kf, qhi[s], hi);
+        lo = mfma32x32x32_i8(kf, qlo[s], lo);
+      }
+      // Shares of the other parts' waves: [column block][token block][to][from], 64
+      // lanes x 4 scores a KB.
+      const uint32_t tile_at = (my_block * 2 + tb) * kParts;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float ks = scales[(8 * (i / 4) + 4 * half + i % 4) * 2 + 1];
-            S[i] = (float)((hi[i] << 8) + lo[i]) * (ks * key_scale);
-            hi[i] = lo[i] = 0;
+      for (int q = 0; q < kParts; ++q) {
+        int d[kShare];
+#pragma unroll
+        for (int i = 0; i < kShare; ++i) d[i] = (hi[q * kShare + i] << 8) + lo[q * kShare + i];
+        if (part == (uint32_t)q) {
+#pragma unroll
+          for (int i = 0; i < kShare; ++i) ldot[i] = d[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < kShare / 4; ++i) {
+            const uint32_t at = NC == 1 ? (tile_at + q) * 4 + part : (tile_at + q) * 2 + i;
+            *(intx4*)(exchange + at * 1024 + lane * 16) = intx4{d[4 * i], d[4 * i + 1], d[4 * i + 2], d[4 * i + 3]};
           }
         }
       }
+      __asm__ volatile("" ::: "memory");  // not both products' sums at once: registers
+      intx16 khi = {}, klo = {};
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float ls = scales[(8 * (i / 4) + 4 * half + i % 4) * 2];
-        // (At most 512 * 127 * 127 * 256 + 512 * 128 * 127 < 2^31.)
-        S[i] = fmaf((float)((hi[i] << 8) + lo[i]), ls * lat_scale, S[i]);
+      for (int s = 0; s < 2; ++s) {
+        const u32x4 kf = *(const u32x4*)(key + (kk ^ (s * 32)));
+        khi = mfma32x32x32_i8(kf, qhi[kLatSteps + s], khi);
+        klo = mfma32x32x32_i8(kf, qlo[kLatSteps + s], klo);
+      }
+#pragma unroll
+      for (int q = 0; q < kParts; ++q)
+        if (part == (uint32_t)q)
+#pragma unroll
+          for (int i = 0; i < kShare; ++i) kdot[i] = (khi[q * kShare + i] << 8) + klo[q * kShare + i];
+      lds_barrier();  // scores exchanged; every wave is done with the tile before
+      if (tile + L::kRing - 1 < t_end) issue(tile + L::kRing - 1, slot == 0 ? L::kRing - 1 : slot - 1);
+#pragma unroll
+      for (int f = 0; f < (NC == 1 ? 4 : 2); ++f) {
+        if (NC == 1 && part == (uint32_t)f) continue;
+        const uint32_t at = NC == 1 ? (tile_at + part) * 4 + f : (tile_at + part) * 2 + f;
+        const intx4 v = *(const intx4*)(exchange + at * 1024 + lane * 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ldot[(NC == 1 ? 0 : 4 * f) + j] += v[j];
       }
     }
-    // A tile's largest token scale, as a power of two: P' is kept relative to the
-    // largest so far.
-    const uint32_t tok0 = tile * kLatentTile + 4 * half;
-    const bool whole = (tile + 1) * kLatentTile <= lim_min && c_last - c_first == kLatentCols - 1;
+
+    // The wave's share: scores i of a lane are tokens 8 (i / 4) + 4 half + i % 4 of
+    // its token block, its own from part * kShare on.
+    const uint32_t first = part * kShare;
+    float S[kShare], ts[kShare];
+#pragma unroll
+    for (int g = 0; g < kShare / 4; ++g) {
+      const float* at = scales + tb * 64 + (2 * (first / 4 + g) + half) * 8;
+      const floatx4 s0 = *(const floatx4*)at, s1 = *(const floatx4*)(at + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = 4 * g + j;
+        ts[i] = j < 2 ? s0[2 * j] : s1[2 * j - 4];
+        S[i] = fmaf((float)ldot[i], ts[i] * lat_scale, (float)kdot[i] * ((j < 2 ? s0[2 * j + 1] : s1[2 * j - 3]) * key_scale));
+      }
+    }
+    const bool whole = (tile + 1) * kLatentTile <= lim_min && c_last - c_first == kCols - 1;
     if (!whole) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) S[i] = tok0 + 8 * (i / 4) + i % 4 < limit ? S[i] : -INFINITY;
+      for (int i = 0; i < kShare; ++i) {
+        const uint32_t tok = tile * kLatentTile + 32 * tb + 8 * (first / 4 + i / 4) + 4 * half + i % 4;
+        S[i] = tok < limit ? S[i] : -INFINITY;
+        ts[i] = tok < limit ? ts[i] : 0.0f;  // nothing of it, not even a scale that is no number
+      }
     }
-    // Not of tokens behind the block's last, whose scales are any bits, nor NaN.
-    const float own = tile * kLatentTile + col < lim_max && scales[2 * col] <= FLT_MAX ? scales[2 * col] : 0.0f;
-    const uint32_t big = __float_as_uint(wave_allmax(own)) & 0x7F800000u;
     float top = S[0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, S[i]);
+    for (int i = 1; i < kShare; ++i) top = fmaxf(top, S[i]);
     top = halves_max(top);
-    if (__any(top > mref + 14.0f) || big > vexp) {
-      const float m = fmaxf(mref, top - 6.0f);
-      const uint32_t e = max(big, vexp);
-      float f = __builtin_amdgcn_exp2f(mref - m);
-      mref = m;
-      l *= f;
-      f *= __uint_as_float(max((int)(vexp - e + 0x3F800000u), 0));  // 2^(old - new)
-      vexp = e;
+    const uint32_t at_max = (tb * kParts + part) * kCols + 32 * my_block + col;
+    float sum, top_pt;
+    auto publish = [&]() __attribute__((always_inline)) {
+      float p[kShare];
+      const bool lower = NC == 1 || my_block == 0;
+      const float ref = lower ? mref[0] : mref[NC - 1], unit = __builtin_amdgcn_exp2f(-(lower ? w2[0] : w2[NC - 1]));
+      sum = top_pt = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kBlocks; ++i)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) O[i][j] *= f;
-    }
-    const float unit_scale = __uint_as_float(0x7F000000u - vexp);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      S[i] = __builtin_amdgcn_exp2f(S[i] - mref);
-      l += S[i];
-      const float ls = scales[(8 * (i / 4) + 4 * half + i % 4) * 2];
-      S[i] *= (whole || tok0 + 8 * (i / 4) + i % 4 < limit ? ls : 0.0f) * unit_scale;
-    }
-    u32x4 p[2];  // pairs in the order of bytes_to_f16
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        p[u][2 * i] = to_f16x2(S[8 * u + 4 * i], S[8 * u + 4 * i + 2]);
-        p[u][2 * i + 1] = to_f16x2(S[8 * u + 4 * i + 1], S[8 * u + 4 * i + 3]);
+      for (int i = 0; i < kShare; ++i) {
+        const float e = __builtin_amdgcn_exp2f(S[i] - ref);
+        sum += e;
+        p[i] = e * ts[i] * unit;
+        top_pt = fmaxf(top_pt, p[i]);
       }
-    {
-      constexpr int kAhead = 4;
-      u32x2 vf[kAhead + 1];
-      auto value_at = [&](int i) __attribute__((always_inline)) {
-        return lds_read_tr8(lat + va[i / 2 & 3] + (i / 8) * 128 + (i & 1) * 16 * RP);
-      };
+      // Pairs in the order of bytes_to_f16; scores 8 u .. 8 u + 7 are contraction block u.
+      uint8_t* to = pbuf + (tb * NC + my_block) * 2048 + lane * 16;
+      if constexpr (NC == 1)
+        *(u32x2*)(to + (part / 2) * 1024 + (part % 2) * 8) = u32x2{to_f16x2(p[0], p[2]), to_f16x2(p[1], p[3])};
+      else
+        *(u32x4*)(to + part * 1024) =
+            u32x4{to_f16x2(p[0], p[2]), to_f16x2(p[1], p[3]), to_f16x2(p[4], p[6]), to_f16x2(p[5], p[7])};
+    };
+    publish();
+    top_pt = halves_max(top_pt);
+    if (half == 0) maxima[at_max] = float2{top, top_pt};
+    if (tile + 2 < t_end) latent_wait_vmcnt<L::kDma>();  // the next tile's bytes
+    else latent_wait_vmcnt<0>();
+    lds_barrier();  // P', the maxima and the next tile are in LDS
+    bool passed = false;
+    float tops[NC];
+    auto read_maxima = [&](int n, float* y) __attribute__((always_inline)) {
+      float2 m = maxima[32 * n + col];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) vf[i] = value_at(i);
-#pragma unroll
-      for (int i = 0; i < 2 * kBlocks; ++i) {
-        if (i + kAhead < 2 * kBlocks) vf[(i + kAhead) % (kAhead + 1)] = value_at(i + kAhead);
-        __asm__ volatile("" ::: "memory");
-        O[i / 2] = mfma32x32x16_f16(bytes_to_f16(vf[i % (kAhead + 1)]), p[i & 1], O[i / 2]);
+      for (int q = 1; q < 2 * kParts; ++q) {
+        const float2 v = maxima[q * kCols + 32 * n + col];
+        m.x = fmaxf(m.x, v.x), m.y = fmaxf(m.y, v.y);
       }
+      *y = m.y;
+      return m.x;
+    };
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      float pt;
+      tops[n] = read_maxima(n, &pt);
+      passed = passed || tops[n] > mref[n] + 14.0f || pt > 16384.0f;
     }
-    latent_wait_lds();  // before the DMA of a later tile writes here
+    if (__any(passed)) {  // the same in every wave
+      float m[NC];
+#pragma unroll
+      for (int n = 0; n < NC; ++n) m[n] = fmaxf(mref[n], tops[n] - 6.0f);
+      // log2(p * token scale) with the new ref: the waves' maxima again.
+      const float own = NC == 1 || my_block == 0 ? m[0] : m[NC - 1];
+      float top_w = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kShare; ++i) top_w = fmaxf(top_w, S[i] - own + __log2f(ts[i]));
+      top_w = halves_max(top_w);
+      lds_barrier();
+      if (half == 0) maxima[at_max].y = top_w;
+      lds_barrier();
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        float w;
+        (void)read_maxima(n, &w);
+        const float moved = mref[n] - m[n];
+        w = fmaxf(fmaxf(w2[n] + moved, w - 6.0f), -100.0f);  // 2^-w stays a number
+        const float f = __builtin_amdgcn_exp2f(moved + (w2[n] - w));
+        if (NC == 1 || my_block == (uint32_t)n) l *= __builtin_amdgcn_exp2f(moved);
+        mref[n] = m[n];
+        w2[n] = w;
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) O[i][n][j] *= f;
+      }
+      publish();
+      lds_barrier();
+    }
+    l += sum;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        u32x4 p[NC];
+#pragma unroll
+        for (int n = 0; n < NC; ++n) p[n] = *(const u32x4*)(pbuf + ((t * NC + n) * 2 + u) * 1024 + lane * 16);
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+          const uint32_t rb = wave + 8 * i;
+          if (kAll % 8 != 0 && rb >= kAll) break;
+          const u32x4 v = bytes_to_f16(lds_read_tr8(lat + (va ^ ((rb & 3) * 32)) + (rb >> 2) * 128 + (32 * t + 16 * u) * RP));
+#pragma unroll
+          for (int n = 0; n < NC; ++n) O[i][n] = mfma32x32x16_f16(v, p[n], O[i][n]);
+        }
+      }
     slot = slot + 1 == L::kRing ? 0 : slot + 1;
   }
 
-  // Merge the four waves: one maximum per column, then the sums, 128 latent
-  // elements at a time.
+  // The columns' softmax sums from the other waves, and the sums of latents as the
+  // lanes hold them (1 KB a store; the join reads them likewise).
   l = halves_sum(l);
-  __syncthreads();
-  float* ml = (float*)(lds + 4 * kLatentCols * L::kPad * 4);
-  if (half == 0) *(float2*)(ml + (wave * kLatentCols + col) * 2) = float2{mref, l};
-  __syncthreads();
-  float m = kNoMax, sum = 0.0f;
+  lds_barrier();
+  if (half == 0) maxima[(tb * kParts + part) * kCols + 32 * my_block + col].x = l;
+  lds_barrier();
+  float* out = a.partials + (size_t)unit * kCols * RP;
+  float* ml = a.partials + (size_t)a.units * kCols * RP + (size_t)unit * kCols * 2;
+  if (wave < NC && half == 0) {
+    float total = 0.0f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[(w * kLatentCols + col) * 2]);
+    for (int q = 0; q < 2 * kParts; ++q) total += maxima[q * kCols + 32 * wave + col].x;
+    *(float2*)(ml + (32 * wave + col) * 2) = float2{wave == 0 ? mref[0] : mref[NC - 1], total};
+  }
 #pragma unroll
-  for (int w = 0; w < 4; ++w)
-    sum += ml[(w * kLatentCols + col) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * kLatentCols + col) * 2] - m);
-  const float f = __builtin_amdgcn_exp2f(mref - m) * __uint_as_float(vexp);
-  if (wave == 0 && half == 0)
-    *(float2*)(a.partials + (size_t)a.units * kLatentCols * RP + ((size_t)unit * kLatentCols + col) * 2) =
-        float2{m, sum};
-  float* buf = (float*)lds;
+  for (int n = 0; n < NC; ++n) {
+    if (c_first + 32 * n > c_last) break;
+    const float f = __builtin_amdgcn_exp2f(w2[n]);
 #pragma unroll
-  for (int q = 0; q < RP / 128; ++q) {
+    for (int i = 0; i < kBlocks; ++i) {
+      const uint32_t rb = wave + 8 * i;
+      if (kAll % 8 != 0 && rb >= kAll) break;
 #pragma unroll
-    for (int rb = 0; rb < 4; ++rb)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        floatx4 v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = O[4 * q + rb][4 * g + i] * f;
-        *(floatx4*)(buf + (wave * kLatentCols + col) * L::kPad + 32 * rb + 8 * g + 4 * half) = v;
-      }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t at = i * 256 + threadIdx.x, cc = at / 32, r = (at % 32) * 4;
-      if (c_first + cc > c_last) break;
-      floatx4 v = {0, 0, 0, 0};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) v += *(const floatx4*)(buf + (w * kLatentCols + cc) * L::kPad + r);
-      *(floatx4*)(a.partials + ((size_t)unit * kLatentCols + cc) * RP + q * 128 + r) = v;
+      for (int g = 0; g < 4; ++g)
+        *(floatx4*)(out + (((size_t)n * kAll + rb) * 4 + g) * 256 + lane * 4) =
+            floatx4{O[i][n][4 * g] * f, O[i][n][4 * g + 1] * f, O[i][n][4 * g + 2] * f, O[i][n][4 * g + 3] * f};
     }
-    __syncthreads();
   }
 }
 
 // ---------------------------------------------------------------------------
 // Joining the splits, and out of the latent space
 // ---------------------------------------------------------------------------
-// Workgroup = (one (row, head) column, 128 latent elements): its splits' sums
-// weighted by 2^(m - M), eight splits at a time, divided by the joined softmax
-// sum and written as bf16 and the bf16 of what that leaves (2^-17 in all), the
-// operands of the product with W_uv.
-template <int RP>
-__global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnArgs a) {
-  __shared__ floatx4 part[256];
-  const uint32_t c_all = blockIdx.x / (RP / 128), r0 = blockIdx.x % (RP / 128) * 128;
-  const uint32_t H = a.d.heads, m = c_all / H, h = c_all - m * H;
-  const LatentSeq& sq = a.seqs[a.decode ? m : 0];
-  const uint32_t cols = a.decode ? H : a.rows * H, blocks = (cols + kLatentCols - 1) / kLatentCols;
-  const uint32_t c = a.decode ? h : c_all, cb = c / kLatentCols, col = c % kLatentCols;
-  const uint32_t t = threadIdx.x % 32, group = threadIdx.x / 32, lane = threadIdx.x & 63;
-  const float* ml = a.partials + (size_t)a.units * kLatentCols * RP;
-  auto at = [&](uint32_t s) { return (size_t)(sq.unit_begin + s * blocks + cb) * kLatentCols + col; };
+// Workgroup = (32 columns, 8 latent elements: one store of the attention's): the
+// splits' sums weighted by 2^(m - M), a wave every sixteenth split, added in
+// wave order, divided by the joined softmax sum and written as bf16 and the bf16
+// of what that leaves (2^-17 in all), the operands of the product with W_uv.
+template <int RP, int NC>
+__global__ __launch_bounds__(1024) void latent_join_kernel(LatentAttnArgs a) {
+  constexpr uint32_t kWaves = 16, kCols = 32 * NC;
+  __shared__ floatx4 part[kWaves][64];
+  __shared__ float2 red[kWaves][32];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31;
+  const uint32_t H = a.d.heads, cols = a.decode ? H : a.rows * H, blocks = (cols + 31) / 32;
+  const uint32_t piece = blockIdx.x % (RP / 8), block = blockIdx.x / (RP / 8);
+  const uint32_t b = a.decode ? block / blocks : 0, cb = block - b * blocks;
+  const LatentSeq& sq = a.seqs[b];
+  const uint32_t groups = (cols + kCols - 1) / kCols, n = cb % NC;
+  const size_t u0 = sq.unit_begin + cb / NC;
+  const float* ml = a.partials + (size_t)a.units * kCols * RP;
+  const float* o = a.partials + ((size_t)n * (RP / 8) + piece) * 256 + lane * 4;
+  // The wave's splits, relative to their own maximum.
   float top = kNoMax, sum = 0.0f;
-  for (uint32_t s = lane; s < sq.splits; s += 64) top = fmaxf(top, ml[at(s) * 2]);
-  top = wave_allmax(top);
-  for (uint32_t s = lane; s < sq.splits; s += 64) {
-    const float2 v = *(const float2*)(ml + at(s) * 2);
-    sum += v.y * __builtin_amdgcn_exp2f(v.x - top);
-  }
-  sum = wave_allsum(sum);
   floatx4 acc = {0, 0, 0, 0};
 #pragma unroll 4
-  for (uint32_t s = group; s < sq.splits; s += 8) {
-    const float w = __builtin_amdgcn_exp2f(ml[at(s) * 2] - top);
-    acc += *(const floatx4*)(a.partials + at(s) * RP + r0 + 4 * t) * w;
+  for (uint32_t s = wave; s < sq.splits; s += kWaves) {
+    const size_t u = u0 + (size_t)s * groups;
+    const float2 v = *(const float2*)(ml + (u * kCols + 32 * n + col) * 2);
+    const floatx4 x = *(const floatx4*)(o + u * kCols * RP);
+    const float m = fmaxf(top, v.x), f = __builtin_amdgcn_exp2f(top - m), g = __builtin_amdgcn_exp2f(v.x - m);
+    top = m;
+    sum = sum * f + v.y * g;
+    acc = acc * f + x * g;
   }
-  part[threadIdx.x] = acc;
+  part[wave][lane] = acc;
+  if (lane < 32) red[wave][lane] = float2{top, sum};
   __syncthreads();
-  if (group != 0) return;
+  if (wave != 0) return;
+  float m = kNoMax;
 #pragma unroll
-  for (int g = 1; g < 8; ++g) acc += part[g * 32 + t];
+  for (uint32_t w = 0; w < kWaves; ++w) m = fmaxf(m, red[w][col].x);
+  sum = 0.0f;
+  acc = floatx4{0, 0, 0, 0};
+#pragma unroll
+  for (uint32_t w = 0; w < kWaves; ++w) {
+    const float f = __builtin_amdgcn_exp2f(red[w][col].x - m);
+    sum += red[w][col].y * f;
+    acc += part[w][lane] * f;
+  }
+  const uint32_t c = cb * 32 + col;
+  if (c >= cols) return;
   const float r = 1.0f / sum;
   float x[4], y[4];
 #pragma unroll
@@ -474,7 +565,7 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnArgs a) {
     x[i] = acc[i] * r;
     y[i] = x[i] - (float)(__bf16)x[i];
   }
-  uint16_t* to = a.mixed + (size_t)c_all * 2 * RP + r0 + 4 * t;
+  uint16_t* to = a.mixed + ((size_t)b * cols + c) * 2 * RP + piece * 8 + 4 * (lane >> 5);
   *(u32x2*)to = u32x2{to_bf16x2(x[0], x[1]), to_bf16x2(x[2], x[3])};
   *(u32x2*)(to + RP) = u32x2{to_bf16x2(y[0], y[1]), to_bf16x2(y[2], y[3])};
 }
@@ -516,24 +607,28 @@ __global__ __launch_bounds__(256) void latent_up_kernel(LatentAttnArgs a) {
   }
 }
 
-template <int RP>
+template <int RP, int NC>
 hipError_t absorbed(const LatentAttnArgs& a, hipStream_t st) {
   const uint32_t tiles = (a.rows + 15) / 16 * a.d.heads, append_blocks = (a.rows + 3) / 4;
   hipLaunchKernelGGL(latent_query_kernel<RP>, dim3(append_blocks + tiles * (RP / 128)), dim3(256), 0, st, a, append_blocks);
-  hipLaunchKernelGGL(latent_attn_kernel<RP>, dim3(a.units), dim3(256), 0, st, a);
-  hipLaunchKernelGGL(latent_join_kernel<RP>, dim3(a.rows * a.d.heads * (RP / 128)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((latent_attn_kernel<RP, NC>), dim3(a.units), dim3(512), 0, st, a);
+  hipLaunchKernelGGL((latent_join_kernel<RP, NC>), dim3(a.blocks * (RP / 8)), dim3(1024), 0, st, a);
   hipLaunchKernelGGL(latent_up_kernel<RP>, dim3(tiles * (a.d.v_pad / 32)), dim3(256), 0, st, a);
   return hipGetLastError();
+}
+template <int RP>
+hipError_t absorbed_cols(const LatentAttnArgs& a, hipStream_t st) {
+  return a.group_cols == 32 ? absorbed<RP, 1>(a, st) : absorbed<RP, 2>(a, st);
 }
 
 }  // namespace
 
 hipError_t launch_latent_absorbed(const LatentAttnArgs& a, hipStream_t st) {
   switch (a.d.rank_pad) {
-    case 128: return absorbed<128>(a, st);
-    case 256: return absorbed<256>(a, st);
-    case 384: return absorbed<384>(a, st);
-    default: return absorbed<512>(a, st);
+    case 128: return absorbed_cols<128>(a, st);
+    case 256: return absorbed_cols<256>(a, st);
+    case 384: return absorbed_cols<384>(a, st);
+    default: return absorbed_cols<512>(a, st);
   }
 }
 

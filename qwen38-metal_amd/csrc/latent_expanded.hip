@@ -103,9 +103,10 @@ __global__ __launch_bounds__(256) void latent_unpack_kernel(LatentExpandArgs a) 
     float topv = s.x <= FLT_MAX ? s.x : 0.0f;
     top = wave_allmax(top), topv = wave_allmax(topv);
     // 2^g as a float's bits: the exponent field, plus one (at most 2^122: scales
-    // end at FLT_MAX / 127).  2^g is kept from vanishing in the scores' factor.
+    // end at FLT_MAX / 127).  Both are kept from vanishing: 2^g is in the scores'
+    // factor, the softmax sum is over 2^gv.
     const uint32_t g = max(__float_as_uint(top) & 0x7F800000u, 0x21800000u) + 0x00800000u;
-    const uint32_t gv = max(__float_as_uint(topv) & 0x7F800000u, 0x00800000u) + 0x00800000u;
+    const uint32_t gv = max(__float_as_uint(topv) & 0x7F800000u, 0x21800000u) + 0x00800000u;
     const float ig = __uint_as_float(0x7F000000u - g), igv = __uint_as_float(0x7F000000u - gv);
     if (lane < 32) {
       sk[lane] = s.y * ig;
@@ -266,9 +267,9 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(LatentExpandArgs 
 //   S^T[token][row] = K Q^T, online softmax in fp32 with a lane's column to
 //   itself, O^T[v][row] += V^T P^T with P (fp16) straight from the registers that
 //   held S.  Tiles of 32 tokens stream through LDS by DMA, shared by the waves.
-// p = 2^(s - ref) with ref the row's maximum less 6, moved when a maximum passes
-// ref + 14, as in the absorbed form; a tile's power of two for the values goes
-// into P where it is not the sums' own.
+// P = 2^(s + gv - ref), 2^gv the tile's power of two of the values and ref the
+// row's maximum of s + gv less 6, moved (and the sums rescaled) when one passes
+// ref + 14; the softmax sum takes a tile's sum of P over 2^gv.
 template <int NP, int VP, int W>
 struct FlashLds {
   static constexpr int kKSteps = NP / 16 + 4, kVBlocks = VP / 32;
@@ -370,7 +371,6 @@ __global__ __launch_bounds__(64 * W, 2) void latent_flash_kernel(LatentExpandArg
 #pragma unroll
     for (int j = 0; j < 16; ++j) O[i][j] = 0.0f;
   float mref = kNoMax, l = 0.0f;
-  uint32_t vexp = 0x00800000u;  // the sums' unit, a power of two as a float's bits
 
   issue(0, 0);
   if (stages > 1) issue(1, 1);
@@ -398,31 +398,24 @@ __global__ __launch_bounds__(64 * W, 2) void latent_flash_kernel(LatentExpandArg
       float top = S[0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) top = fmaxf(top, S[i]);
-      top = halves_max(top) * ct;
-      const uint32_t big = __float_as_uint(pw.y);
-      if (__any(top > mref + 14.0f) || big > vexp) {
-        const float m = fmaxf(mref, top - 6.0f);
-        const uint32_t e = max(big, vexp);
-        float f = __builtin_amdgcn_exp2f(mref - m);
+      const float gv = (float)(int)(__float_as_uint(pw.y) >> 23) - 127.0f;
+      top = fmaf(halves_max(top), ct, gv);
+      if (__any(top > mref + 14.0f)) {
+        const float m = fmaxf(mref, top - 6.0f), f = __builtin_amdgcn_exp2f(mref - m);
         mref = m;
         l *= f;
-        f *= __uint_as_float(max((int)(vexp - e + 0x3F800000u), 0));
-        vexp = e;
 #pragma unroll
         for (int i = 0; i < VB; ++i)
 #pragma unroll
           for (int j = 0; j < 16; ++j) O[i][j] *= f;
       }
+      float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        S[i] = __builtin_amdgcn_exp2f(fmaf(S[i], ct, -mref));
-        l += S[i];
+        S[i] = __builtin_amdgcn_exp2f(fmaf(S[i], ct, gv - mref));
+        sum += S[i];
       }
-      if (big != vexp) {
-        const float f = __uint_as_float(max((int)(big - vexp + 0x3F800000u), 0));
-#pragma unroll
-        for (int i = 0; i < 16; ++i) S[i] *= f;
-      }
+      l = fmaf(sum, __uint_as_float(0x7F000000u - __float_as_uint(pw.y)), l);
       u32x4 p[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -438,7 +431,7 @@ __global__ __launch_bounds__(64 * W, 2) void latent_flash_kernel(LatentExpandArg
   }
 
   l = halves_sum(l);
-  const float r = __uint_as_float(vexp) / a.wmul[2 * h + 1] / l;
+  const float r = 1.0f / (a.wmul[2 * h + 1] * l);
   if (!live) return;
   uint16_t* o = a.o + ((size_t)row * H + h) * a.d.v;
 #pragma unroll

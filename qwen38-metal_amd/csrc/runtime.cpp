@@ -291,6 +291,7 @@ qm::Tuning qm::read_tuning(int cu_count) {
   t.prefill_splits = get("QM38_PREFILL_SPLITS", 0);
   t.prefill_waves = get("QM38_PREFILL_WAVES", 0);
   t.latent_form = get("QM38_LATENT_FORM", 0);
+  t.latent_tiles = get("QM38_LATENT_TILES", 0);
   t.latent_mb = get("QM38_LATENT_MB", 0);
   t.dn_step_head = get("QM38_DN_STEP_HEAD", -1);
   t.dn_chunked = get("QM38_DN_CHUNKED", -1);

@@ -80,7 +80,7 @@ qm_status grow(qm_latent_kv* kv, uint64_t tokens) {
   constexpr uint64_t kMost = 1ull << 30;  // 576 GB at rank 512; token arithmetic stays within 32 bits
   if (tokens > kMost)
     return fail(QM_ERR_DIMENSION_OVERFLOW, "latent cache of %llu tokens", (unsigned long long)tokens);
-  uint64_t cap = 2 * kLatentTile;
+  uint64_t cap = kLatentTile;
   while (cap < tokens) cap <<= 1;
   if (kv->max_tokens) cap = std::min<uint64_t>(cap, kv->max_tokens);
   cap = (cap + kLatentTile - 1) / kLatentTile * kLatentTile;
@@ -270,28 +270,31 @@ LatentAttnArgs absorbed_args(const qm_latent_weights* w, const LatentNewRows& ro
   return a;
 }
 
-// Splits of the absorbed attention.  A workgroup's four waves take a column
-// block's tiles in turn; as many splits as fill the chip once, none below 8
-// tiles (the join costs more than a shorter walk saves).
+// Splits of the absorbed attention: as many as fill the chip once (a workgroup a
+// CU), none below 2 tiles (the join costs more than a shorter walk
+// saves).
 void plan_absorbed(const qm_runtime* rt, LatentAttnArgs* a) {
   const uint32_t cols = a->decode ? a->d.heads : a->rows * a->d.heads;
-  const uint32_t blocks = (cols + kLatentCols - 1) / kLatentCols;
+  a->group_cols = cols <= kLatentCols ? kLatentCols : 2 * kLatentCols;
+  const uint32_t groups = (cols + a->group_cols - 1) / a->group_cols, blocks = (cols + kLatentCols - 1) / kLatentCols;
   auto tiles = [&](uint32_t b) {
     return ((uint64_t)a->seqs[b].start + (a->decode ? 1 : a->rows) + kLatentTile - 1) / kLatentTile;
   };
   auto units = [&](uint64_t per) {
     uint64_t u = 0;
-    for (uint32_t b = 0; b < a->n_seqs; ++b) u += (tiles(b) + per - 1) / per * blocks;
+    for (uint32_t b = 0; b < a->n_seqs; ++b) u += (tiles(b) + per - 1) / per * groups;
     return u;
   };
   uint64_t most = 1;
   for (uint32_t b = 0; b < a->n_seqs; ++b) most = std::max(most, tiles(b));
-  uint64_t lo = std::min<uint64_t>(8, most), hi = most;  // the least tiles a split that fit one round
+  const int forced = rt->tune.latent_tiles;
+  uint64_t lo = std::min<uint64_t>(2, most), hi = most;  // the least tiles a split that fit one round
   while (lo < hi) {
     const uint64_t mid = (lo + hi) / 2;
     if (units(mid) <= (uint64_t)rt->cu_count) hi = mid;
     else lo = mid + 1;
   }
+  if (forced > 0) lo = std::min<uint64_t>(forced, most);
   a->tiles_per_split = (uint32_t)lo;
   uint32_t u = 0, block = 0;
   for (uint32_t b = 0; b < a->n_seqs; ++b) {
@@ -299,7 +302,7 @@ void plan_absorbed(const qm_runtime* rt, LatentAttnArgs* a) {
     s.unit_begin = u;
     s.block_begin = block;
     s.splits = (uint32_t)((tiles(b) + lo - 1) / lo);
-    u += s.splits * blocks;
+    u += s.splits * groups;
     block += blocks;
   }
   a->units = u;
@@ -313,7 +316,7 @@ qm_status absorbed_workspaces(qm_runtime* rt, LatentAttnArgs* a) {
   const size_t mixed = (size_t)a->rows * d.heads * d.rank_pad * 4;
   qm_status st = ensure_scratch(rt, digits + scales + mixed);
   if (st != QM_OK) return st;
-  if ((st = ensure_partials(rt, (size_t)a->units * kLatentCols * (d.rank_pad + 2) * sizeof(float))) != QM_OK) return st;
+  if ((st = ensure_partials(rt, (size_t)a->units * a->group_cols * (d.rank_pad + 2) * sizeof(float))) != QM_OK) return st;
   uint8_t* p = (uint8_t*)rt->scratch;
   a->digits = p;
   a->qscale = (float*)(p + digits);

@@ -336,6 +336,30 @@ def test_scales_far_apart(torch_dev, form):
         assert (o[:40] == 0).all()
 
 
+@pytest.mark.parametrize("form", FORMS)
+def test_a_large_token_that_is_not_attended(torch_dev, form):
+    """A token whose latent is 2^20 times the others' but whose score leaves it
+    nothing (the shared key's part decides) costs the others no precision, and
+    rows that do not see it none either."""
+    rank, rope, nope, v = SMALL
+    with tuned(**FORMS[form]) as rt:
+        g = generator(19)
+        H, rows = 6, 200
+        kv_b, scale, weights = make_weights(rt, g, H, SMALL)
+        q, kv = bf16(g, rows, H, nope + rope), bf16(g, rows, rank + rope)
+        q[..., :nope] = 0
+        q[..., nope:] = 1
+        kv[5, :rank] *= 2.0 ** 20
+        kv[110, :rank] *= 2.0 ** 20
+        kv[[5, 110], rank:] = -100.0
+        cache = rt.create_latent_kv(rank, rope)
+        o = torch.full((rows, H, v), float("nan"), dtype=torch.bfloat16, device=torch_dev)
+        rt.latent_attention_prefill(weights, cache, q, kv, None, 0.0, rows, o)
+        latent, key = held(cache)
+        ref, bound = attention(q, latent, key, kv_b, nope, scale, 0)
+        assert_attention(o, ref, bound)
+
+
 def test_prefill_in_pieces_equals_decode_steps(rt):
     """A prompt in two chunks and tokens decoded one by one leave the same cache;
     their outputs agree with one prefill of all rows within both forms' bounds."""
