@@ -8,7 +8,7 @@ namespace qm {
 
 constexpr uint32_t kLatentMaxRank = 512, kLatentMaxNope = 128, kLatentMaxV = 128;
 constexpr uint32_t kLatentRope = 64;   // stored width of the shared key (the extra elements hold zero)
-constexpr uint32_t kLatentTile = 64;   // tokens of an absorbed-attention tile; a cache's capacity is a multiple
+constexpr uint32_t kLatentTile = 32;   // tokens of an absorbed-attention block; a cache's capacity is a multiple
 constexpr uint32_t kLatentCols = 32;   // (row, head) columns of a block
 constexpr uint32_t kMaxLatentSeqs = 64;
 

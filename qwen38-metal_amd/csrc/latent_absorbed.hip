@@ -152,48 +152,71 @@ __global__ __launch_bounds__(256) void latent_query_kernel(LatentAttnArgs a, uin
 // ---------------------------------------------------------------------------
 // Attention over the cache
 // ---------------------------------------------------------------------------
-// Workgroup = (32 NC columns, a share of the cache's 64-token tiles), eight waves,
-// one workgroup a CU.  A column is a head of a row.  The tiles' bytes stream into
-// an LDS ring by buffer->LDS DMA and are read from there as they lie:
+// Workgroup = (32 NC columns, a share of the cache's 32-token blocks), eight waves,
+// one workgroup a CU.  A column is a head of a row.  The blocks' bytes stream into
+// an LDS ring by buffer->LDS DMA and are read from there as they lie, two blocks
+// (64 tokens) at a time:
 //   scores   S^T[token][column] = codes . (hi, lo) on v_mfma_i32_32x32x32_i8.  A
-//            wave has a column block, 32 of the tokens and a part of the latent
-//            (a half, or a quarter with one column block); the parts exchange
-//            their whole numbers through LDS and each finishes a share of the
-//            tokens, where the token's and the column's scales come in in fp32.
-//            Cutting the latent keeps the queries in registers once.
-//   softmax  online, in fp32: p = 2^(s - ref), ref a column's maximum less 6,
-//            moved (and the sums rescaled) only when a maximum passes ref + 14, so
-//            p stays below 2^14 and what is 2^-20 of the largest is still a normal
-//            fp16.  The waves compute p with the ref they have and publish it with
-//            their maxima; where one passes, all see it behind the same barrier
-//            and do it again.
+//            wave has a block, a column block and a part of the latent (a half, or
+//            a quarter with one column block), which keeps the queries in registers
+//            once; the parts exchange their whole numbers through LDS and each
+//            finishes a share of the tokens,
+//   softmax  where the token's and the column's scales come in in fp32; online: p =
+//            2^(s - ref), ref a column's maximum less 6, moved (and the sums
+//            rescaled) only when a maximum passes ref + 14, so p stays below 2^14
+//            and what is 2^-20 of the largest is still a normal fp16.  The waves
+//            compute p with the ref they have and publish it; where a maximum
+//            passes, a flag says so behind the same barrier and it is done again.
 //   sums     O^T[latent element][column] += codes^T P'^T on
 //            v_mfma_f32_32x32x16_f16, a wave an eighth of the latent: P' = token
 //            scale * p / 2^w, w moved like ref with the largest p * token scale;
 //            rounded to fp16 (2^-11 of each term, where bf16 would be 2^-8), the
-//            codes exact.  The codes' operand comes by transposing
-//            reads; its conversion is shared by the wave's columns.
-// Two barriers a tile: the scores' exchange, and P'.
+//            codes exact.  The codes' operand comes by transposing reads; its
+//            conversion is shared by the wave's columns.
+// Two barriers for 64 tokens.  Between the first (scores exchanged) and the second
+// (P' written) the softmax's vector work runs mixed with the latent's part of the
+// next scores, behind the second the sums' products and the shared key's part.
+//
+// With 128 heads and 131072
+// tokens the loop takes about 5000 cycles for 64 tokens of 64 columns, 2304 of them
+// the matrix cores'; before it 5 us until the first blocks are there, behind it
+// 33 MB of partial sums.  56 us in all, 75 MB read.  With softmax and all
+// products in phases of their own: 59; waits of LDS reads for the copies in flight
+// (what the compiler makes of its own copy builtin): 71.
 template <int RP, int NC>
 struct AbsorbedLds {
   static constexpr int kChunks = RP / 16;  // 16-byte pieces of a latent
   static constexpr int kLat = kLatentTile * RP, kKey = kLatentTile * (int)kLatentRope, kScale = kLatentTile * 8;
   static constexpr int kTileBytes = kLat + kKey + kScale;
-  static constexpr int kRing = 3;
+  static constexpr int kRing = 6;
   static constexpr int kParts = 4 / NC;       // of the contraction
   static constexpr int kShare = 16 / kParts;  // scores of a lane that a wave finishes
   static constexpr int kExchange = NC == 1 ? 32768 : 16384;
   static constexpr int kP = NC * 4096, kMax = 2 * kParts * NC * 32 * 8;
-  static constexpr int kBytes = kRing * kTileBytes + kExchange + kP + kMax;
-  static constexpr int kDma = RP / 128 + 2;  // DMA instructions of a wave and tile
+  static constexpr int kKeyDigits = NC * 4096;  // of the queries' rotated part [block][step][hi, lo][lane]
+  // The ring last: the others are then in reach of an instruction's offset.
+  static constexpr int kAtP = kExchange, kAtMax = kAtP + kP, kAtKeys = kAtMax + kMax, kAtFlag = kAtKeys + kKeyDigits;
+  // Registers: at rank 512 one of the queries' 16 operands of a wave lives here.
+  static constexpr bool kLowInLds = RP / 32 / kParts >= 8 && NC == 2;
+  static constexpr int kAtLow = kAtFlag + 16, kLow = kLowInLds ? 4096 : 0;
+  static constexpr int kAtRing = kAtLow + kLow, kBytes = kAtRing + kRing * kTileBytes;
+  static_assert(kAtRing < 65536, "the offsets' range");
+  static constexpr int kPieces = (RP / 32 + 7) / 8;  // KB of the latents that a wave brings
+  static constexpr int kDma = kPieces + 1;           // DMA instructions of a wave and block, at most
 };
 
-// Order of a token's 16-byte pieces in LDS: piece j at j ^ swizzle(token).  Both
-// the reads of one piece of 8 consecutive tokens and those of the 8 tokens of a
-// transposing read (0..3, 8..11 or 4..7, 12..15) fall on different banks.
-__device__ __forceinline__ constexpr uint32_t lat_swizzle(uint32_t tok) {
-  return (tok & 3) | ((((tok >> 2) ^ (tok >> 3)) & 1) << 2);
+// Order of a token's 16-byte pieces in LDS: piece j at j ^ swizzle(token).  The
+// banks repeat after 16 pieces.  Reads of one piece of 16 consecutive tokens, and
+// transposing reads of two adjacent pieces of 8 tokens (0..3, 8..11 or 4..7, 12..15),
+// fall on different ones.  Rows of an odd number of 8 pieces (rank_pad 128, 384)
+// alternate between the halves by themselves.
+template <int CH>
+__device__ __forceinline__ constexpr uint32_t lat_swizzle(uint32_t t) {
+  const uint32_t b0 = t & 1, b1 = (t >> 1) & 1, b2 = (t >> 2) & 1, b3 = (t >> 3) & 1;
+  return CH % 16 == 0 ? b3 | (b0 << 1) | (b1 << 2) | ((b2 ^ b3) << 3) : b2 | (b1 << 1) | ((b2 ^ b3) << 2);
 }
+// The shared key's four pieces: four tokens to a round of banks.
+__device__ __forceinline__ constexpr uint32_t key_swizzle(uint32_t t) { return (t >> 2) & 3; }
 
 template <int RP, int NC>
 __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
@@ -203,9 +226,11 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
   constexpr int kAll = RP / 32, kBlocks = (kAll + 7) / 8;  // blocks of 32 latent elements: all, a wave's
   constexpr uint32_t kStride = RP + kLatentRope, kCols = 32 * NC;
   __shared__ __attribute__((aligned(16))) uint8_t lds[L::kBytes];
-  uint8_t* const exchange = lds + L::kRing * L::kTileBytes;
-  uint8_t* const pbuf = exchange + L::kExchange;
-  float2* const maxima = (float2*)(pbuf + L::kP);  // [token block][part][column]: of s, of p * token scale
+  uint8_t* const exchange = lds;
+  uint8_t* const pbuf = lds + L::kAtP;
+  float2* const maxima = (float2*)(lds + L::kAtMax);  // [token block][part][column]: of s, of p * token scale
+  uint8_t* const key_digits = lds + L::kAtKeys;
+  uint32_t* const flag = (uint32_t*)(lds + L::kAtFlag);  // a maximum has passed
   const uint32_t lane = threadIdx.x & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t col = lane & 31, half = lane >> 5;
@@ -216,65 +241,85 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
   const uint32_t cols = a.decode ? H : a.rows * H;
   const uint32_t groups = (cols + kCols - 1) / kCols;
   const uint32_t local = unit - sq.unit_begin, cg = local % groups, split = local / groups;
-  // The wave's scores: a block of tokens, a column block, a part of the contraction.
-  const uint32_t tb = wave & 1, my_block = NC == 1 ? 0 : (wave >> 1) & 1, part = wave / (2 * NC);
+  // The wave's scores: one of the two blocks, a column block, a part of the contraction.
+  const uint32_t tb = wave >> 2, my_block = NC == 1 ? 0 : wave & 1, part = NC == 1 ? wave & 3 : (wave >> 1) & 1;
   // Tokens that a column sees: up to its own row.
   const uint32_t c_first = cg * kCols, c_last = min(c_first + kCols, cols) - 1, c = c_first + 32 * my_block + col;
-  const uint32_t lim_min = sq.start + c_first / H + 1, lim_max = sq.start + c_last / H + 1;
-  const uint32_t limit = c <= c_last ? sq.start + c / H + 1 : 0;
+  const uint32_t lim_max = sq.start + c_last / H + 1;
   const uint32_t tiles = (lim_max + kLatentTile - 1) / kLatentTile;
   const uint32_t t_begin = split * a.tiles_per_split, t_end = min(tiles, t_begin + a.tiles_per_split);
+  const uint32_t n = t_begin < t_end ? t_end - t_begin : 0;
+  const uint32_t lim_min = min(sq.start + c_first / H + 1, t_end * kLatentTile);
+  const uint32_t limit = c <= c_last ? min(sq.start + c / H + 1, t_end * kLatentTile) : 0;
 
-  // A tile's bytes, an eighth a wave: pieces of 1 KB of the latents, 512 bytes of
-  // the shared keys, 64 of the scales.
-  auto issue = [&](uint32_t tile, uint32_t slot) __attribute__((always_inline)) {
-    uint8_t* to = lds + slot * L::kTileBytes;
-    const auto rows = latent_rsrc(sq.rows.codes + (size_t)tile * kLatentTile * kStride, kLatentTile * kStride);
+  const int8_t* const codes = sq.rows.codes;
+  const float* const row_scales = sq.rows.scales;
+  // A block's bytes, in pieces of 1 KB: the latents' over all waves (some twice
+  // where eight do not divide them), two of the shared keys, and the scales.
+  constexpr bool kAlike = 512 % CH == 0 && 512 / CH % 16 == 0;  // a wave's pieces differ by whole periods of the swizzle
+  constexpr int kFrom = kAlike ? 1 : L::kPieces;
+  uint32_t from[kFrom];
 #pragma unroll
-    for (int i = 0; i < RP / 128; ++i) {
-      const uint32_t p0 = (wave * (RP / 128) + i) * 64;
-      if constexpr (64 % CH == 0) {  // whole tokens: piece j of token p0 / CH + lane / CH
-        const uint32_t t0 = lane / CH, j = (lane % CH) ^ lat_swizzle(t0) ^ lat_swizzle(p0 / CH);
-        latent_dma16(rows, to + p0 * 16, t0 * kStride + j * 16, p0 / CH * kStride);
-      } else {
-        const uint32_t tok = (p0 + lane) / CH, j = ((p0 + lane) % CH) ^ lat_swizzle(tok);
-        latent_dma16(rows, to + p0 * 16, tok * kStride + j * 16, 0);
-      }
+  for (int k = 0; k < kFrom; ++k) {
+    const uint32_t at = (wave + 8 * k) % (RP / 32) * 64 + lane, tok = at / CH;
+    from[k] = tok * kStride + ((at % CH) ^ lat_swizzle<CH>(tok)) * 16;
+  }
+  uint32_t from_other = wave == 2 ? lane * 4 : (16 * wave + lane / 4) * kStride + RP + ((lane & 3) ^ key_swizzle(lane / 4)) * 16;
+  // Instruction k of kDma; a block that is not `there` reads as zero.
+  auto issue = [&](uint32_t tile, uint32_t slot, bool there, int k) __attribute__((always_inline)) {  // slot: its offset
+    uint8_t* to = lds + L::kAtRing + slot;
+    const auto rows = latent_rsrc(codes + (size_t)tile * kLatentTile * kStride, there ? kLatentTile * kStride : 0);
+    if (k < L::kPieces) {
+      latent_dma16(rows, to + (wave + 8 * k) % (RP / 32) * 1024, from[kAlike ? 0 : k], kAlike ? k * (512 / CH) * kStride : 0);
+    } else if (wave < 2) {
+      latent_dma16(rows, to + L::kLat + wave * 1024, from_other, 0);
+    } else if (wave == 2) {
+      const auto scales = latent_rsrc(row_scales + (size_t)tile * kLatentTile * 2, there ? kLatentTile * 8 : 0);
+      latent_dma4(scales, to + L::kLat + L::kKey, from_other);
     }
-    if (lane < 32) {  // token 8 wave + lane / 4, piece (lane % 4) ^ (token / 2 % 4)
-      const uint32_t tok = lane / 4;
-      latent_dma16(rows, to + L::kLat + wave * 512, tok * kStride + RP + (((lane & 3) ^ ((tok >> 1) & 3)) * 16),
-                   8 * wave * kStride);
-    }
-    const auto scales = latent_rsrc(sq.rows.scales + (size_t)tile * kLatentTile * 2, kLatentTile * 8);
-    if (lane < 16) latent_dma4(scales, to + L::kLat + L::kKey + wave * 64, wave * 64 + lane * 4);
   };
-#pragma unroll
-  for (int i = 0; i < L::kRing - 1; ++i)
-    if (t_begin + i < t_end) issue(t_begin + i, i);
-
   // (A group's last block may be one that does not exist; its columns have no tokens.)
   const size_t block = sq.block_begin + min(cg * NC + my_block, (cols - 1) / 32);
-  u32x4 qhi[kLatSteps + 2], qlo[kLatSteps + 2];  // the shared key's last
+  u32x4 qhi[kLatSteps], qlo[kLatSteps];
   {
     const uint8_t* dg = a.digits + block * latent_digit_bytes(RP) + lane * 32;
 #pragma unroll
-    for (int s = 0; s < kLatSteps + 2; ++s) {
-      const uint32_t step = s < kLatSteps ? part * kLatSteps + s : kAll + s - kLatSteps;
-      qhi[s] = *(const u32x4*)(dg + step * 2048);
-      qlo[s] = *(const u32x4*)(dg + step * 2048 + 16);
+    for (int s = 0; s < kLatSteps; ++s) {
+      qhi[s] = *(const u32x4*)(dg + (part * kLatSteps + s) * 2048);
+      qlo[s] = *(const u32x4*)(dg + (part * kLatSteps + s) * 2048 + 16);
     }
+  }
+  const bool brings = tb == 0 && part < 2;  // the rotated part's digits into LDS, once for all waves of a column block
+  u32x4 kd[2];
+  if (brings) {
+    const uint8_t* dg = a.digits + block * latent_digit_bytes(RP) + lane * 32 + (kAll + part) * 2048;
+    kd[0] = *(const u32x4*)dg;
+    kd[1] = *(const u32x4*)(dg + 16);
   }
   const float2 qs = limit ? *(const float2*)(a.qscale + (block * kLatentCols + col) * 2) : float2{0.0f, 0.0f};
   const float lat_scale = qs.x * a.scale * kLog2e, key_scale = qs.y * a.scale * kLog2e;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int k = 0; k < L::kDma; ++k) issue(t_begin + i, i * L::kTileBytes, t_begin + i < t_end, k);
+  if (brings) {  // (the loads before it are waited for, not the blocks behind them)
+    if constexpr (L::kLowInLds) *(u32x4*)(lds + L::kAtLow + wave * 1024 + lane * 16) = qlo[0];
+    uint8_t* to = key_digits + (my_block * 2 + part) * 2048 + lane * 16;
+    *(u32x4*)to = kd[0];
+    *(u32x4*)(to + 1024) = kd[1];
+  }
 
   // LDS offsets of this lane: codes of its token (score operands) and of the 8
   // tokens of a transposing read.
-  const uint32_t tok0 = 32 * tb + col;
   const uint32_t trow = (lane & 15) >> 1, vtok = 4 * half + (trow < 4 ? trow : trow + 4);
-  const uint32_t ka = tok0 * RP + ((half ^ lat_swizzle(tok0)) * 16);
-  const uint32_t kk = tok0 * kLatentRope + ((half ^ ((tok0 >> 1) & 3)) * 16);
-  const uint32_t va = vtok * RP + ((((lane >> 4) & 1) ^ lat_swizzle(vtok)) * 16) + 8 * (lane & 1);
+  const uint32_t ka = col * RP + ((half ^ lat_swizzle<CH>(col)) * 16);
+  // Pieces 2 n + .. of a row: the swizzle reaches over 16 (or 8) of them.
+  constexpr uint32_t kSpan = CH % 16 == 0 ? 8 : 4;
+  auto piece = [](uint32_t at, uint32_t n) __attribute__((always_inline)) {
+    return (at ^ ((n % kSpan) * 32)) + n / kSpan * (kSpan * 32);
+  };
+  const uint32_t va = L::kAtRing + piece(vtok * RP + ((((lane >> 4) & 1) ^ lat_swizzle<CH>(vtok)) * 16) + 8 * (lane & 1), wave);
+  static_assert(8 % kSpan == 0, "eight blocks on, the pieces are eight blocks on");
 
   floatx16 O[kBlocks][NC];
 #pragma unroll
@@ -287,194 +332,274 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
 #pragma unroll
   for (int n = 0; n < NC; ++n) mref[n] = kNoMax, w2[n] = 0.0f;
 
-  latent_wait_vmcnt<0>();
-  lds_barrier();
-  uint32_t slot = 0;
-  for (uint32_t tile = t_begin; tile < t_end; ++tile) {
-    const uint8_t* lat = lds + slot * L::kTileBytes;
-    const uint8_t* key = lat + L::kLat;
-    const float* scales = (const float*)(key + L::kKey);
-
-    // The wave's part of the latent's products, then all of the shared key's: 256
-    // hi + lo in whole numbers (at most 512 * 127 * 127 * 256 + 512 * 128 * 127 <
-    // 2^31).
-    int kdot[kShare], ldot[kShare];
-    {
-      intx16 hi = {}, lo = {};
+  // The wave's part of a block's score products: 256 hi + lo in whole numbers (at
+  // most 512 * 127 * 127 * 256 + 512 * 128 * 127 < 2^31) of the latent, and all of
+  // the shared key's.
+  auto score_step = [](u32x4 kf, u32x4 qh, u32x4 ql, bool start, intx16& hi, intx16& lo) __attribute__((always_inline)) {
+    hi = mfma32x32x32_i8(kf, qh, start ? intx16{} : hi);
+    lo = mfma32x32x32_i8(kf, ql, start ? intx16{} : lo);
+  };
+  // The wave's share of its current block, in turn: whole numbers of the
+  // latent's and the key's products; scores and token scales (as bits).
+  int ldot[kShare] = {}, kdot[kShare] = {};
+  auto take_keys = [&](const intx16& hi, const intx16& lo) __attribute__((always_inline)) {
 #pragma unroll
-      for (int s = 0; s < kLatSteps; ++s) {
-        const uint32_t step = part * kLatSteps + s;
-        const u32x4 kf = *(const u32x4*)(lat + (ka ^ ((step & 3) * 32)) + (step >> 2) * 128);
-        hi = mfma32x32x32_i8(kf, qhi[s], hi);
-        lo = mfma32x32x32_i8(kf, qlo[s], lo);
-      }
-      // Shares of the other parts' waves: [column block][token block][to][from], 64
-      // lanes x 4 scores a KB.
-      const uint32_t tile_at = (my_block * 2 + tb) * kParts;
+    for (int q = 0; q < kParts; ++q)
+      if (part == (uint32_t)q)
 #pragma unroll
-      for (int q = 0; q < kParts; ++q) {
-        int d[kShare];
+        for (int i = 0; i < kShare; ++i) kdot[i] = (hi[q * kShare + i] << 8) + lo[q * kShare + i];
+  };
+  // Shares of the other parts' waves: [column block][block][to][from], 64 lanes x 4
+  // scores a KB.
+  const uint32_t tile_at = (my_block * 2 + tb) * kParts * (NC == 1 ? 4096 : 2048) + lane * 16;
+  auto exchange_scores = [&](const intx16& hi, const intx16& lo) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < kShare; ++i) d[i] = (hi[q * kShare + i] << 8) + lo[q * kShare + i];
-        if (part == (uint32_t)q) {
+    for (int q = 0; q < kParts; ++q) {
+      int d[kShare];
 #pragma unroll
-          for (int i = 0; i < kShare; ++i) ldot[i] = d[i];
-        } else {
+      for (int i = 0; i < kShare; ++i) d[i] = (hi[q * kShare + i] << 8) + lo[q * kShare + i];
+      if (part == (uint32_t)q) {
 #pragma unroll
-          for (int i = 0; i < kShare / 4; ++i) {
-            const uint32_t at = NC == 1 ? (tile_at + q) * 4 + part : (tile_at + q) * 2 + i;
-            *(intx4*)(exchange + at * 1024 + lane * 16) = intx4{d[4 * i], d[4 * i + 1], d[4 * i + 2], d[4 * i + 3]};
-          }
+        for (int i = 0; i < kShare; ++i) ldot[i] = d[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < kShare / 4; ++i) {
+          const uint32_t at = NC == 1 ? q * 4096 + part * 1024 : q * 2048 + i * 1024;
+          *(intx4*)(exchange + tile_at + at) = intx4{d[4 * i], d[4 * i + 1], d[4 * i + 2], d[4 * i + 3]};
         }
       }
-      __asm__ volatile("" ::: "memory");  // not both products' sums at once: registers
-      intx16 khi = {}, klo = {};
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const u32x4 kf = *(const u32x4*)(key + (kk ^ (s * 32)));
-        khi = mfma32x32x32_i8(kf, qhi[kLatSteps + s], khi);
-        klo = mfma32x32x32_i8(kf, qlo[kLatSteps + s], klo);
-      }
-#pragma unroll
-      for (int q = 0; q < kParts; ++q)
-        if (part == (uint32_t)q)
-#pragma unroll
-          for (int i = 0; i < kShare; ++i) kdot[i] = (khi[q * kShare + i] << 8) + klo[q * kShare + i];
-      lds_barrier();  // scores exchanged; every wave is done with the tile before
-      if (tile + L::kRing - 1 < t_end) issue(tile + L::kRing - 1, slot == 0 ? L::kRing - 1 : slot - 1);
-#pragma unroll
-      for (int f = 0; f < (NC == 1 ? 4 : 2); ++f) {
-        if (NC == 1 && part == (uint32_t)f) continue;
-        const uint32_t at = NC == 1 ? (tile_at + part) * 4 + f : (tile_at + part) * 2 + f;
-        const intx4 v = *(const intx4*)(exchange + at * 1024 + lane * 16);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) ldot[(NC == 1 ? 0 : 4 * f) + j] += v[j];
-      }
     }
+  };
 
-    // The wave's share: scores i of a lane are tokens 8 (i / 4) + 4 half + i % 4 of
-    // its token block, its own from part * kShare on.
-    const uint32_t first = part * kShare;
-    float S[kShare], ts[kShare];
+  float sum = 0.0f, top = 0.0f, top_pt = 0.0f;
+  const uint32_t lane16 = lane * 16;
+  const bool lower = NC == 1 || my_block == 0;
+  auto& S = ldot;  // scores
+  auto& T = kdot;  // token scales
+  const uint32_t first = part * kShare;  // scores i of a lane are tokens 8 (i / 4) + 4 half + i % 4, its own from here on
+  const uint32_t at_max = (tb * kParts + part) * kCols + 32 * my_block + col;
+  float p[kShare];
+  auto store_p = [&]() __attribute__((always_inline)) {
+    // Pairs in the order of bytes_to_f16; scores 8 u .. 8 u + 7 are contraction block u.
+    uint8_t* to = pbuf + (tb * NC + my_block) * 2048 + lane16;
+    if constexpr (NC == 1)
+      *(u32x2*)(to + (part / 2) * 1024 + (part % 2) * 8) = u32x2{to_f16x2(p[0], p[2]), to_f16x2(p[1], p[3])};
+    else
+      *(u32x4*)(to + part * 1024) =
+          u32x4{to_f16x2(p[0], p[2]), to_f16x2(p[1], p[3]), to_f16x2(p[4], p[6]), to_f16x2(p[5], p[7])};
+  };
+  auto weigh = [&](int i, float ref, float unit) __attribute__((always_inline)) {
+    const float e = __builtin_amdgcn_exp2f(__int_as_float(S[i]) - ref);
+    sum += e;
+    p[i] = e * __int_as_float(T[i]) * unit;
+  };
+  // What a wave reads from LDS for four scores of its block: the other parts'
+  // numbers, the tokens' scales.
+  constexpr int kOthers = kParts - 1;
+  struct SoftmaxIn {
+    intx4 d[kOthers];
+    floatx4 s[2];
+  };
+  auto read_softmax = [&](uint32_t slot, int g) __attribute__((always_inline)) {
+    SoftmaxIn r;
 #pragma unroll
-    for (int g = 0; g < kShare / 4; ++g) {
-      const float* at = scales + tb * 64 + (2 * (first / 4 + g) + half) * 8;
-      const floatx4 s0 = *(const floatx4*)at, s1 = *(const floatx4*)(at + 4);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = 4 * g + j;
-        ts[i] = j < 2 ? s0[2 * j] : s1[2 * j - 4];
-        S[i] = fmaf((float)ldot[i], ts[i] * lat_scale, (float)kdot[i] * ((j < 2 ? s0[2 * j + 1] : s1[2 * j - 3]) * key_scale));
-      }
+    for (int f = 0; f < kOthers; ++f) {
+      const uint32_t at = NC == 1 ? part * 4096 + ((part + 1 + f) & 3) * 1024 : part * 2048 + g * 1024;
+      r.d[f] = *(const intx4*)(exchange + tile_at + at);
     }
-    const bool whole = (tile + 1) * kLatentTile <= lim_min && c_last - c_first == kCols - 1;
+    const float* at = (const float*)(lds + L::kAtRing + slot + L::kLat + L::kKey) + (2 * (first / 4 + g) + half) * 8;
+    r.s[0] = *(const floatx4*)at;
+    r.s[1] = *(const floatx4*)(at + 4);
+    return r;
+  };
+  // Score i of the wave's share: its value, and what it gives with the references there are.
+  auto softmax = [&](int i, const SoftmaxIn& r, uint32_t tile, bool whole, float ref, float unit) __attribute__((always_inline)) {
+    const int g = i / 4, j = i % 4;
+    const floatx4 s0 = r.s[0], s1 = r.s[1];
+    int dot = ldot[i];
+#pragma unroll
+    for (int f = 0; f < kOthers; ++f) dot += r.d[f][j];
+    float t = j < 2 ? s0[2 * j] : s1[2 * j - 4];
+    float v = fmaf((float)dot, t * lat_scale, (float)kdot[i] * ((j < 2 ? s0[2 * j + 1] : s1[2 * j - 3]) * key_scale));
     if (!whole) {
-#pragma unroll
-      for (int i = 0; i < kShare; ++i) {
-        const uint32_t tok = tile * kLatentTile + 32 * tb + 8 * (first / 4 + i / 4) + 4 * half + i % 4;
-        S[i] = tok < limit ? S[i] : -INFINITY;
-        ts[i] = tok < limit ? ts[i] : 0.0f;  // nothing of it, not even a scale that is no number
-      }
+      const bool seen = tile * kLatentTile + 8 * (first / 4 + g) + 4 * half + j < limit;
+      v = seen ? v : -INFINITY;
+      t = seen ? t : 0.0f;  // nothing of it, not even a scale that is no number
     }
-    float top = S[0];
-#pragma unroll
-    for (int i = 1; i < kShare; ++i) top = fmaxf(top, S[i]);
-    top = halves_max(top);
-    const uint32_t at_max = (tb * kParts + part) * kCols + 32 * my_block + col;
-    float sum, top_pt;
-    auto publish = [&]() __attribute__((always_inline)) {
-      float p[kShare];
-      const bool lower = NC == 1 || my_block == 0;
-      const float ref = lower ? mref[0] : mref[NC - 1], unit = __builtin_amdgcn_exp2f(-(lower ? w2[0] : w2[NC - 1]));
-      sum = top_pt = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kShare; ++i) {
-        const float e = __builtin_amdgcn_exp2f(S[i] - ref);
-        sum += e;
-        p[i] = e * ts[i] * unit;
-        top_pt = fmaxf(top_pt, p[i]);
-      }
-      // Pairs in the order of bytes_to_f16; scores 8 u .. 8 u + 7 are contraction block u.
-      uint8_t* to = pbuf + (tb * NC + my_block) * 2048 + lane * 16;
-      if constexpr (NC == 1)
-        *(u32x2*)(to + (part / 2) * 1024 + (part % 2) * 8) = u32x2{to_f16x2(p[0], p[2]), to_f16x2(p[1], p[3])};
-      else
-        *(u32x4*)(to + part * 1024) =
-            u32x4{to_f16x2(p[0], p[2]), to_f16x2(p[1], p[3]), to_f16x2(p[4], p[6]), to_f16x2(p[5], p[7])};
-    };
-    publish();
-    top_pt = halves_max(top_pt);
-    if (half == 0) maxima[at_max] = float2{top, top_pt};
-    if (tile + 2 < t_end) latent_wait_vmcnt<L::kDma>();  // the next tile's bytes
-    else latent_wait_vmcnt<0>();
-    lds_barrier();  // P', the maxima and the next tile are in LDS
-    bool passed = false;
-    float tops[NC];
-    auto read_maxima = [&](int n, float* y) __attribute__((always_inline)) {
-      float2 m = maxima[32 * n + col];
+    top = fmaxf(top, v);
+    S[i] = __float_as_int(v);
+    T[i] = __float_as_int(t);
+    weigh(i, ref, unit);
+    top_pt = fmaxf(top_pt, p[i]);
+  };
+  // Moves the references to the maxima and publishes again.
+  auto move = [&]() __attribute__((always_inline)) {
+    auto column_max = [&](int n, float2* m) __attribute__((always_inline)) {
+      *m = maxima[32 * n + col];
 #pragma unroll
       for (int q = 1; q < 2 * kParts; ++q) {
         const float2 v = maxima[q * kCols + 32 * n + col];
-        m.x = fmaxf(m.x, v.x), m.y = fmaxf(m.y, v.y);
+        m->x = fmaxf(m->x, v.x), m->y = fmaxf(m->y, v.y);
       }
-      *y = m.y;
-      return m.x;
     };
+    const float t = halves_max(top);
+    if (half == 0) maxima[at_max].x = t;
+    lds_barrier();
+    float m[NC];
+    float2 v;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-      float pt;
-      tops[n] = read_maxima(n, &pt);
-      passed = passed || tops[n] > mref[n] + 14.0f || pt > 16384.0f;
+      column_max(n, &v);
+      m[n] = fmaxf(mref[n], v.x - 6.0f);
     }
-    if (__any(passed)) {  // the same in every wave
-      float m[NC];
+    // log2(p * token scale) with the new ref.
+    const float own = lower ? m[0] : m[NC - 1];
+    float top_w = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < NC; ++n) m[n] = fmaxf(mref[n], tops[n] - 6.0f);
-      // log2(p * token scale) with the new ref: the waves' maxima again.
-      const float own = NC == 1 || my_block == 0 ? m[0] : m[NC - 1];
-      float top_w = -INFINITY;
+    for (int i = 0; i < kShare; ++i) top_w = fmaxf(top_w, __int_as_float(S[i]) - own + __log2f(__int_as_float(T[i])));
+    top_w = halves_max(top_w);
+    if (half == 0) maxima[at_max].y = top_w;
+    lds_barrier();
+    if (threadIdx.x == 0) *flag = 0;
 #pragma unroll
-      for (int i = 0; i < kShare; ++i) top_w = fmaxf(top_w, S[i] - own + __log2f(ts[i]));
-      top_w = halves_max(top_w);
-      lds_barrier();
-      if (half == 0) maxima[at_max].y = top_w;
-      lds_barrier();
+    for (int n = 0; n < NC; ++n) {
+      column_max(n, &v);
+      const float moved = mref[n] - m[n], w = fmaxf(fmaxf(w2[n] + moved, v.y - 6.0f), -100.0f);  // 2^-w stays a number
+      const float f = __builtin_amdgcn_exp2f(moved + (w2[n] - w));
+      if (NC == 1 || my_block == (uint32_t)n) l *= __builtin_amdgcn_exp2f(moved);
+      mref[n] = m[n];
+      w2[n] = w;
 #pragma unroll
-      for (int n = 0; n < NC; ++n) {
-        float w;
-        (void)read_maxima(n, &w);
-        const float moved = mref[n] - m[n];
-        w = fmaxf(fmaxf(w2[n] + moved, w - 6.0f), -100.0f);  // 2^-w stays a number
-        const float f = __builtin_amdgcn_exp2f(moved + (w2[n] - w));
-        if (NC == 1 || my_block == (uint32_t)n) l *= __builtin_amdgcn_exp2f(moved);
-        mref[n] = m[n];
-        w2[n] = w;
+      for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-        for (int i = 0; i < kBlocks; ++i)
+        for (int j = 0; j < 16; ++j) O[i][n][j] *= f;
+    }
+    const float ref = lower ? mref[0] : mref[NC - 1], unit = __builtin_amdgcn_exp2f(-(lower ? w2[0] : w2[NC - 1]));
+    sum = 0.0f;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) O[i][n][j] *= f;
+    for (int i = 0; i < kShare; ++i) weigh(i, ref, unit);
+    store_p();
+    lds_barrier();
+  };
+  struct KeyOperands {
+    u32x4 k, hi, lo;
+  };
+  auto read_key = [&](uint32_t slot, int s) __attribute__((always_inline)) {
+    uint32_t col = lane & 31, half = lane >> 5;
+    __asm__ volatile("" : "+v"(col), "+v"(half));
+    const uint32_t kk = col * kLatentRope + ((half ^ key_swizzle(col)) * 16);
+    const uint8_t* kd = key_digits + my_block * 4096 + lane16 + s * 2048;
+    return KeyOperands{*(const u32x4*)(lds + (L::kAtRing + L::kLat + slot + (kk ^ (32 * s)))), *(const u32x4*)kd,
+                       *(const u32x4*)(kd + 1024)};
+  };
+  auto low = [&](int s) __attribute__((always_inline)) {
+    return L::kLowInLds && s == 0 ? *(const u32x4*)(lds + L::kAtLow + (wave & 3) * 1024 + lane16) : qlo[s];
+  };
+  auto score_codes = [&](uint32_t slot, int s) __attribute__((always_inline)) {
+    return *(const u32x4*)(lds + (L::kAtRing + slot + piece(ka, part * kLatSteps + s)));
+  };
+  // The sums' products of the two blocks at `now`.  A step takes one operand of codes
+  // and the columns' P'; its operands are read a step ahead, and no further
+  // (registers).
+  auto products = [&](uint32_t now, uint32_t next, const KeyOperands& key) __attribute__((always_inline)) {
+    constexpr int kFrags = 4 * kBlocks;
+    u32x2 codes_at[2];
+    u32x4 pf[2][NC];
+    auto read = [&](int f) __attribute__((always_inline)) {
+      const int t = f / (2 * kBlocks), u = f / kBlocks % 2;
+      codes_at[f % 2] = lds_read_tr8(lds + now + va + t * L::kTileBytes + 16 * u * RP + f % kBlocks * 256);
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+        if (f % kBlocks == 0) pf[u][n] = *(const u32x4*)(pbuf + ((t * NC + n) * 2 + u) * 1024 + lane16);
+    };
+    {
+      intx16 hi, lo;
+      const KeyOperands second = read_key(next, 1);
+      score_step(key.k, key.hi, key.lo, true, hi, lo);
+      read(0);
+      score_step(second.k, second.hi, second.lo, false, hi, lo);
+      take_keys(hi, lo);
+    }
+#pragma unroll
+    for (int f = 0; f < kFrags; ++f) {
+      __builtin_amdgcn_sched_barrier(0);
+      const u32x2 now_codes = codes_at[f % 2];
+      if (f + 1 < kFrags) read(f + 1);
+      const int i = f % kBlocks;
+      if (kAll % 8 == 0 || wave + 8 * i < kAll) {
+        const u32x4 v = bytes_to_f16(now_codes);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) O[i][n] = mfma32x32x16_f16(v, pf[f / kBlocks % 2][n], O[i][n]);
       }
-      publish();
-      lds_barrier();
     }
-    l += sum;
+  };
+
+  if (threadIdx.x == 0) *flag = 0;
+  latent_wait_vmcnt<2 * L::kPieces>();  // the first two blocks
+  lds_barrier();
+  if (n) {
+    intx16 hi, lo;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int s = 0; s < kLatSteps; ++s) score_step(score_codes(tb * L::kTileBytes, s), qhi[s], low(s), s == 0, hi, lo);
+    exchange_scores(hi, lo);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        u32x4 p[NC];
+    for (int s = 0; s < 2; ++s) {
+      const KeyOperands key = read_key(tb * L::kTileBytes, s);
+      score_step(key.k, key.hi, key.lo, s == 0, hi, lo);
+    }
+    take_keys(hi, lo);
+  }
+  latent_wait_vmcnt<0>();
+  uint32_t now = 0, next = 2 * L::kTileBytes, free = 4 * L::kTileBytes;  // two blocks of the ring each
+  for (uint32_t i = 0; i < n; i += 2) {
+    lds_barrier();  // scores exchanged, the next blocks in LDS; every wave is done with the blocks before
+    SoftmaxIn in = read_softmax(now + tb * L::kTileBytes, 0);
 #pragma unroll
-        for (int n = 0; n < NC; ++n) p[n] = *(const u32x4*)(pbuf + ((t * NC + n) * 2 + u) * 1024 + lane * 16);
+    for (int b = 0; b < 2; ++b) issue(t_begin + i + 4 + b, free + b * L::kTileBytes, i + 4 + b < n, L::kPieces);
+    // The softmax, and mixed with it the latent's part of the scores of the next two
+    // blocks.  Behind the last block these are of whatever the ring holds and go
+    // nowhere: a second form of the loop without them took more registers than there
+    // are.
+    intx16 hi, lo;
+    KeyOperands key;
+    {
+      const uint32_t tile = t_begin + i + tb;
+      const bool whole = (tile + 1) * kLatentTile <= lim_min && c_last - c_first == kCols - 1;
+      const float ref = lower ? mref[0] : mref[NC - 1], unit = __builtin_amdgcn_exp2f(-(lower ? w2[0] : w2[NC - 1]));
+      top = -INFINITY, top_pt = sum = 0.0f;
+      u32x4 k = score_codes(next + tb * L::kTileBytes, 0);
+      const u32x4 low0 = low(0);
 #pragma unroll
-        for (int i = 0; i < kBlocks; ++i) {
-          const uint32_t rb = wave + 8 * i;
-          if (kAll % 8 != 0 && rb >= kAll) break;
-          const u32x4 v = bytes_to_f16(lds_read_tr8(lat + (va ^ ((rb & 3) * 32)) + (rb >> 2) * 128 + (32 * t + 16 * u) * RP));
+      for (int s = 0; s < kLatSteps; ++s) {
+        __builtin_amdgcn_sched_barrier(0);
+        const u32x4 k_now = k;
+        if (s + 1 < kLatSteps) k = score_codes(next + tb * L::kTileBytes, s + 1);
+        score_step(k_now, qhi[s], s == 0 ? low0 : qlo[s], s == 0, hi, lo);
+        // The DMA of the two blocks behind the next two, an instruction or two a step.
 #pragma unroll
-          for (int n = 0; n < NC; ++n) O[i][n] = mfma32x32x16_f16(v, p[n], O[i][n]);
+        for (int d = s * 2 * L::kPieces / kLatSteps; d < (s + 1) * 2 * L::kPieces / kLatSteps; ++d) {
+          const uint32_t b = d / L::kPieces, to = i + 4 + b;
+          issue(t_begin + to, free + b * L::kTileBytes, to < n, d % L::kPieces);
+        }
+#pragma unroll
+        for (int j = s * kShare / kLatSteps; j < (s + 1) * kShare / kLatSteps; ++j) {
+          softmax(j, in, tile, whole, ref, unit);
+          if (j % 4 == 3 && j + 1 < kShare) in = read_softmax(now + tb * L::kTileBytes, (j + 1) / 4);
         }
       }
-    slot = slot + 1 == L::kRing ? 0 : slot + 1;
+      __builtin_amdgcn_sched_barrier(0);
+      key = read_key(next + tb * L::kTileBytes, 0);
+      store_p();
+      if (top > ref + 14.0f || top_pt > 16384.0f) *flag = 1;
+    }
+    lds_barrier();  // P' and the flag
+    if (__builtin_amdgcn_readfirstlane(*flag)) move();
+    l += sum;
+    products(now, next + tb * L::kTileBytes, key);
+    exchange_scores(hi, lo);
+    latent_wait_vmcnt<0>();
+    const uint32_t t = now;
+    now = next, next = free, free = t;
   }
 
   // The columns' softmax sums from the other waves, and the sums of latents as the

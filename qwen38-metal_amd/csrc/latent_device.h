@@ -7,20 +7,38 @@ namespace qm {
 typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef int intx16 __attribute__((ext_vector_type(16)));
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t latent_rsrc(const void* base, uint32_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
+// A buffer descriptor (uniform): reads beyond its bytes give zero.
+__device__ __forceinline__ u32x4 latent_rsrc(const void* base, uint32_t bytes) {
+  const uint64_t p = (uint64_t)base;
+  return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)p),
+               (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(p >> 32)) & 0xFFFFu,
+               (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
 }
 
 // Builtins of the device pass only.
 #if defined(__HIP_DEVICE_COMPILE__)
 #define QM_LDS(T, p) ((__attribute__((address_space(3))) T*)(p))
-// Lane i's bytes at voff + soff land at lds + i * size.
-__device__ __forceinline__ void latent_dma16(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t voff, uint32_t soff) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, QM_LDS(void, lds), 16, voff, soff, 0, 0);
+// Buffer -> LDS copies: lane i's bytes at voff + soff land at lds + i * size (lds
+// and soff uniform).  In asm, because the compiler lets every LDS read that
+// follows the builtin wait for the copy (any LDS address may be the one it
+// writes) and so ends the overlap; the waits are latent_wait_vmcnt's.  The copies
+// have no register output, and the waits that the compiler counts for its own
+// loads only become stricter by them.  s_nop: M0, and scalar registers that a vector
+// instruction wrote, have to settle before a memory instruction reads them.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 among the clobbers
+__device__ __forceinline__ uint32_t latent_lds_address(const void* lds) {
+  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);  // a generic LDS address' lower half is the offset
 }
-__device__ __forceinline__ void latent_dma4(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t voff) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, QM_LDS(void, lds), 4, voff, 0, 0, 0);
+__device__ __forceinline__ void latent_dma16(u32x4 r, void* lds, uint32_t voff, uint32_t soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :: "s"(latent_lds_address(lds)), "v"(voff), "s"(r), "s"(__builtin_amdgcn_readfirstlane(soff)) : "memory", "m0");
 }
+__device__ __forceinline__ void latent_dma4(u32x4 r, void* lds, uint32_t voff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :: "s"(latent_lds_address(lds)), "v"(voff), "s"(r) : "memory", "m0");
+}
+#pragma clang diagnostic pop
 // Transposing read of bytes: each 16 lanes read 8 rows of 16 bytes (lanes 2t
 // and 2t + 1 give the address of row t's two halves) and lane i receives byte i
 // of the 8 rows.
@@ -33,8 +51,8 @@ __device__ __forceinline__ intx16 mfma32x32x32_i8(u32x4 a, u32x4 b, intx16 c) {
 }
 #undef QM_LDS
 #else
-__device__ void latent_dma16(__amdgpu_buffer_rsrc_t, void*, uint32_t, uint32_t);
-__device__ void latent_dma4(__amdgpu_buffer_rsrc_t, void*, uint32_t);
+__device__ void latent_dma16(u32x4, void*, uint32_t, uint32_t);
+__device__ void latent_dma4(u32x4, void*, uint32_t);
 __device__ u32x2 lds_read_tr8(const uint8_t*);
 __device__ intx16 mfma32x32x32_i8(u32x4, u32x4, intx16);
 #endif

@@ -353,17 +353,26 @@ __global__ __launch_bounds__(64 * W, 2) void latent_flash_kernel(LatentExpandArg
   const uint8_t* kb = (const uint8_t*)a.k + (size_t)hc * all_tiles * (NP / 16) * 1024;
   const uint8_t* vb = (const uint8_t*)a.v + (size_t)hc * all_tiles * (2 * VB) * 1024;
   const uint8_t* sb = (const uint8_t*)a.keys;
-  auto issue = [&](uint32_t stage, uint32_t buf) __attribute__((always_inline)) {
+  // What this wave copies of a stage: addresses in the next stage to issue.
+  const uint8_t* from[L::kDma];
+  uint32_t step[L::kDma];
+#pragma unroll
+  for (int i = 0; i < L::kDma; ++i) {
+    const uint32_t kbyte = i * W + wave, t = kbyte / (L::kTile / 1024), at = kbyte - t * (L::kTile / 1024);
+    const uint32_t per = at < NP / 16 ? NP / 16 : at < KS ? 4 : 2 * VB;
+    const uint8_t* part = at < NP / 16 ? kb + at * 1024 : at < KS ? sb + (at - NP / 16) * 1024 : vb + (at - KS) * 1024;
+    from[i] = part + (size_t)t * per * 1024;
+    step[i] = L::kTiles * per * 1024;
+  }
+  auto issue = [&](uint32_t buf) __attribute__((always_inline)) {  // within the padding: padded is a multiple of 128
 #pragma unroll
     for (int i = 0; i < L::kDma; ++i) {
-      const uint32_t kbyte = i * W + wave, t = kbyte / (L::kTile / 1024), at = kbyte - t * (L::kTile / 1024);
-      const size_t tile = stage * L::kTiles + t;  // within the padding: padded is a multiple of 128
-      const uint8_t* from = at < NP / 16 ? kb + (tile * (NP / 16) + at) * 1024
-                            : at < KS    ? sb + (tile * 4 + at - NP / 16) * 1024
-                                         : vb + (tile * (2 * VB) + at - KS) * 1024;
-      latent_dma16(latent_rsrc(from, 1024), lds + buf * L::kStage + kbyte * 1024, lane * 16, 0);
+      latent_dma16(latent_rsrc(from[i], 1024), lds + buf * L::kStage + (i * W + wave) * 1024, lane * 16, 0);
+      from[i] += step[i];
     }
   };
+  // Scalar loads: a vector load's wait would wait for the copies before it too.
+  const auto* powers = (const __attribute__((address_space(4))) float*)(uintptr_t)a.powers;
 
   floatx16 O[VB];
 #pragma unroll
@@ -372,20 +381,20 @@ __global__ __launch_bounds__(64 * W, 2) void latent_flash_kernel(LatentExpandArg
     for (int j = 0; j < 16; ++j) O[i][j] = 0.0f;
   float mref = kNoMax, l = 0.0f;
 
-  issue(0, 0);
-  if (stages > 1) issue(1, 1);
+  issue(0);
+  if (stages > 1) issue(1);
   uint32_t buf = 0;
   for (uint32_t st = 0; st < stages; ++st) {
     if (st + 1 < stages) latent_wait_vmcnt<L::kDma>();
     else latent_wait_vmcnt<0>();
     lds_barrier();
-    if (st + 2 < stages) issue(st + 2, buf == 0 ? 2 : buf - 1);
+    if (st + 2 < stages) issue(buf == 0 ? 2 : buf - 1);
 #pragma unroll
     for (int tt = 0; tt < L::kTiles; ++tt) {
       const uint32_t tile = st * L::kTiles + tt;
       if (tile * 32 >= wave_limit) break;  // wave-uniform
       const uint8_t* base = lds + buf * L::kStage + tt * L::kTile + lane * 16;
-      const float2 pw = *(const float2*)(a.powers + 2 * tile);
+      const float2 pw = {powers[2 * tile], powers[2 * tile + 1]};
       floatx16 S = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
       for (int s = 0; s < KS; ++s) S = mfma32x32x16_f16(*(const u32x4*)(base + s * 1024), Q[s], S);

@@ -80,7 +80,7 @@ qm_status grow(qm_latent_kv* kv, uint64_t tokens) {
   constexpr uint64_t kMost = 1ull << 30;  // 576 GB at rank 512; token arithmetic stays within 32 bits
   if (tokens > kMost)
     return fail(QM_ERR_DIMENSION_OVERFLOW, "latent cache of %llu tokens", (unsigned long long)tokens);
-  uint64_t cap = kLatentTile;
+  uint64_t cap = 2 * kLatentTile;
   while (cap < tokens) cap <<= 1;
   if (kv->max_tokens) cap = std::min<uint64_t>(cap, kv->max_tokens);
   cap = (cap + kLatentTile - 1) / kLatentTile * kLatentTile;
@@ -271,7 +271,7 @@ LatentAttnArgs absorbed_args(const qm_latent_weights* w, const LatentNewRows& ro
 }
 
 // Splits of the absorbed attention: as many as fill the chip once (a workgroup a
-// CU), none below 2 tiles (the join costs more than a shorter walk
+// CU), none below 4 blocks (the join costs more than a shorter walk
 // saves).
 void plan_absorbed(const qm_runtime* rt, LatentAttnArgs* a) {
   const uint32_t cols = a->decode ? a->d.heads : a->rows * a->d.heads;
@@ -288,7 +288,7 @@ void plan_absorbed(const qm_runtime* rt, LatentAttnArgs* a) {
   uint64_t most = 1;
   for (uint32_t b = 0; b < a->n_seqs; ++b) most = std::max(most, tiles(b));
   const int forced = rt->tune.latent_tiles;
-  uint64_t lo = std::min<uint64_t>(2, most), hi = most;  // the least tiles a split that fit one round
+  uint64_t lo = std::min<uint64_t>(4, most), hi = most;  // the least tiles a split that fit one round
   while (lo < hi) {
     const uint64_t mid = (lo + hi) / 2;
     if (units(mid) <= (uint64_t)rt->cu_count) hi = mid;
