@@ -116,7 +116,7 @@ struct LatentExpandArgs {
   uint16_t* v;           // fp16 [heads][padded / 32][v_pad / 16][512]
 };
 constexpr uint32_t kLatentExpandTokens = 128;
-hipError_t launch_latent_expanded(const LatentExpandArgs& a, uint32_t heads_at_once, hipStream_t st);
+hipError_t launch_latent_expanded(const LatentExpandArgs& a, uint32_t heads_at_once, uint32_t cu_count, hipStream_t st);
 // wop fp16 [H * (nope_pad + v_pad) / 32][rank_pad / 16][512] and wmul fp32 [H][2] from `up`.
 hipError_t launch_latent_wop(const LatentDims& d, const uint16_t* up, float* wmul, uint16_t* wop, hipStream_t st);
 

@@ -8,6 +8,7 @@
 // latent_up_kernel.
 #include <float.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "latent.h"
@@ -635,18 +636,18 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
 // ---------------------------------------------------------------------------
 // Joining the splits, and out of the latent space
 // ---------------------------------------------------------------------------
-// Workgroup = (32 columns, 8 latent elements: one store of the attention's): the
-// splits' sums weighted by 2^(m - M), a wave every sixteenth split, added in
-// wave order, divided by the joined softmax sum and written as bf16 and the bf16
+// P waves take (32 columns, 8 latent elements: one store of the attention's), a
+// workgroup 16 / P neighbours of them: the splits' sums weighted by 2^(m - M), a
+// wave every P-th split, added in wave order, divided by the joined softmax sum and written as bf16 and the bf16
 // of what that leaves (2^-17 in all), the operands of the product with W_uv.
-template <int RP, int NC>
+template <int RP, int NC, int P>
 __global__ __launch_bounds__(1024) void latent_join_kernel(LatentAttnArgs a) {
-  constexpr uint32_t kWaves = 16, kCols = 32 * NC;
-  __shared__ floatx4 part[kWaves][64];
-  __shared__ float2 red[kWaves][32];
+  constexpr uint32_t kCols = 32 * NC, kPieces = 16 / P;
+  __shared__ floatx4 part[16][64];
+  __shared__ float2 red[16][32];
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31;
   const uint32_t H = a.d.heads, cols = a.decode ? H : a.rows * H, blocks = (cols + 31) / 32;
-  const uint32_t piece = blockIdx.x % (RP / 8), block = blockIdx.x / (RP / 8);
+  const uint32_t piece = blockIdx.x % (RP / 8 / kPieces) * kPieces + wave / P, block = blockIdx.x / (RP / 8 / kPieces);
   const uint32_t b = a.decode ? block / blocks : 0, cb = block - b * blocks;
   const LatentSeq& sq = a.seqs[b];
   const uint32_t groups = (cols + kCols - 1) / kCols, n = cb % NC;
@@ -657,7 +658,7 @@ __global__ __launch_bounds__(1024) void latent_join_kernel(LatentAttnArgs a) {
   float top = kNoMax, sum = 0.0f;
   floatx4 acc = {0, 0, 0, 0};
 #pragma unroll 4
-  for (uint32_t s = wave; s < sq.splits; s += kWaves) {
+  for (uint32_t s = wave % P; s < sq.splits; s += P) {
     const size_t u = u0 + (size_t)s * groups;
     const float2 v = *(const float2*)(ml + (u * kCols + 32 * n + col) * 2);
     const floatx4 x = *(const floatx4*)(o + u * kCols * RP);
@@ -669,17 +670,17 @@ __global__ __launch_bounds__(1024) void latent_join_kernel(LatentAttnArgs a) {
   part[wave][lane] = acc;
   if (lane < 32) red[wave][lane] = float2{top, sum};
   __syncthreads();
-  if (wave != 0) return;
+  if (wave % P != 0) return;
   float m = kNoMax;
 #pragma unroll
-  for (uint32_t w = 0; w < kWaves; ++w) m = fmaxf(m, red[w][col].x);
+  for (uint32_t w = 0; w < P; ++w) m = fmaxf(m, red[wave + w][col].x);
   sum = 0.0f;
   acc = floatx4{0, 0, 0, 0};
 #pragma unroll
-  for (uint32_t w = 0; w < kWaves; ++w) {
-    const float f = __builtin_amdgcn_exp2f(red[w][col].x - m);
-    sum += red[w][col].y * f;
-    acc += part[w][lane] * f;
+  for (uint32_t w = 0; w < P; ++w) {
+    const float f = __builtin_amdgcn_exp2f(red[wave + w][col].x - m);
+    sum += red[wave + w][col].y * f;
+    acc += part[wave + w][lane] * f;
   }
   const uint32_t c = cb * 32 + col;
   if (c >= cols) return;
@@ -737,7 +738,11 @@ hipError_t absorbed(const LatentAttnArgs& a, hipStream_t st) {
   const uint32_t tiles = (a.rows + 15) / 16 * a.d.heads, append_blocks = (a.rows + 3) / 4;
   hipLaunchKernelGGL(latent_query_kernel<RP>, dim3(append_blocks + tiles * (RP / 128)), dim3(256), 0, st, a, append_blocks);
   hipLaunchKernelGGL((latent_attn_kernel<RP, NC>), dim3(a.units), dim3(512), 0, st, a);
-  hipLaunchKernelGGL((latent_join_kernel<RP, NC>), dim3(a.blocks * (RP / 8)), dim3(1024), 0, st, a);
+  // Up to 8 splits two waves have few to go through, and idle ones would cost more.
+  uint32_t splits = 1;
+  for (uint32_t b = 0; b < a.n_seqs; ++b) splits = std::max(splits, a.seqs[b].splits);
+  if (splits > 8) hipLaunchKernelGGL((latent_join_kernel<RP, NC, 16>), dim3(a.blocks * (RP / 8)), dim3(1024), 0, st, a);
+  else hipLaunchKernelGGL((latent_join_kernel<RP, NC, 2>), dim3(a.blocks * (RP / 64)), dim3(1024), 0, st, a);
   hipLaunchKernelGGL(latent_up_kernel<RP>, dim3(tiles * (a.d.v_pad / 32)), dim3(256), 0, st, a);
   return hipGetLastError();
 }

@@ -268,13 +268,21 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(LatentExpandArgs 
 //   itself, O^T[v][row] += V^T P^T with P (fp16) straight from the registers that
 //   held S.  Tiles of 32 tokens stream through LDS by DMA, shared by the waves.
 // P = 2^(s + gv - ref), 2^gv the tile's power of two of the values and ref the
-// row's maximum of s + gv less 6, moved (and the sums rescaled) when one passes
-// ref + 14; the softmax sum takes a tile's sum of P over 2^gv.
+// row's maximum of s + gv less 6; the softmax sum takes a tile's sum of P over
+// 2^gv.  A tile is weighed with the ref there is; only where a lane's sum of P
+// passes 2^14 (so that no P can have passed fp16) is its maximum looked for, ref
+// moved, the sums rescaled and the tile weighed again.
+//
+// Bound by the matrix cores and the vector unit together (640 and 480 cycles a wave
+// and tile, two waves a SIMD): 2048 rows of 128 heads on 4096 tokens take 885 us,
+// 57% of the matrix cores' cycles at the clock it runs at.  The next tile's key
+// products go between the exponentials; with each phase by itself, and a maximum
+// for every tile: 945.
 template <int NP, int VP, int W>
 struct FlashLds {
   static constexpr int kKSteps = NP / 16 + 4, kVBlocks = VP / 32;
   static constexpr int kTile = (kKSteps + 2 * kVBlocks) * 1024;
-  static constexpr int kTiles = W == 8 ? 2 : 1;   // of a stage
+  static constexpr int kTiles = 2;  // of a stage
   static constexpr int kBufs = 3;
   static constexpr int kStage = kTiles * kTile;
   static constexpr int kDma = kStage / 1024 / W;  // DMA instructions of a wave
@@ -381,62 +389,95 @@ __global__ __launch_bounds__(64 * W, 2) void latent_flash_kernel(LatentExpandArg
     for (int j = 0; j < 16; ++j) O[i][j] = 0.0f;
   float mref = kNoMax, l = 0.0f;
 
+  // A tile's scores are formed while the tile before is in its softmax: the products
+  // of a turn are the next tile's KS of keys, then 2 VB of values.  Their operands
+  // are read kAhead products before, into the next turn.
+  constexpr int kOps = KS + 2 * VB, kAhead = 4;
+  static_assert(kOps % kAhead == 0 && L::kTiles == 2, "registers of the operands and scores by turn");
+  u32x4 ring[kAhead];
+  floatx16 S[2];
   issue(0);
   if (stages > 1) issue(1);
+  if (stages > 1) latent_wait_vmcnt<L::kDma>();
+  else latent_wait_vmcnt<0>();
+  lds_barrier();
+  const uint8_t* const mine = lds + lane * 16;
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+    S[0] = mfma32x32x16_f16(*(const u32x4*)(mine + s * 1024), Q[s], s ? S[0] : floatx16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0});
+#pragma unroll
+  for (int s = 0; s < kAhead; ++s) ring[s] = *(const u32x4*)(mine + L::kTile + s * 1024);
   uint32_t buf = 0;
+  float2 pw = {powers[0], powers[1]};
   for (uint32_t st = 0; st < stages; ++st) {
-    if (st + 1 < stages) latent_wait_vmcnt<L::kDma>();
-    else latent_wait_vmcnt<0>();
-    lds_barrier();
+    const uint32_t next_buf = buf == 2 ? 0 : buf + 1;
+    latent_wait_vmcnt<0>();
+    lds_barrier();  // stage st + 1 is in LDS; every wave is done with stage st - 1
     if (st + 2 < stages) issue(buf == 0 ? 2 : buf - 1);
 #pragma unroll
     for (int tt = 0; tt < L::kTiles; ++tt) {
       const uint32_t tile = st * L::kTiles + tt;
       if (tile * 32 >= wave_limit) break;  // wave-uniform
-      const uint8_t* base = lds + buf * L::kStage + tt * L::kTile + lane * 16;
-      const float2 pw = {powers[2 * tile], powers[2 * tile + 1]};
-      floatx16 S = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-      for (int s = 0; s < KS; ++s) S = mfma32x32x16_f16(*(const u32x4*)(base + s * 1024), Q[s], S);
-      const float ct = fmaxf(c * pw.x, FLT_MIN);  // a masked score stays -infinity times more than nothing
+      floatx16 &C = S[tt], &N = S[1 - tt];
+      const uint8_t* base = mine + buf * L::kStage + tt * L::kTile;
+      // (Behind the last tile: whatever is there, used for nothing.)
+      const uint8_t* next = tt == 0 ? base + L::kTile : mine + next_buf * L::kStage;
+      const uint8_t* after = tt == 0 ? mine + next_buf * L::kStage : next + L::kTile;
+      const uint32_t ahead = min(tile + 1, all_tiles - 1);
+      const float2 now = pw;
+      pw = {powers[2 * ahead], powers[2 * ahead + 1]};
       if ((tile + 1) * 32 > wave_whole) {
         const uint32_t tok0 = tile * 32 + 4 * half;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) S[i] = tok0 + 8 * (i / 4) + i % 4 < limit ? S[i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) C[i] = tok0 + 8 * (i / 4) + i % 4 < limit ? C[i] : -INFINITY;
       }
-      float top = S[0];
+      const float ct = fmaxf(c * now.x, FLT_MIN);  // a masked score stays -infinity times more than nothing
+      const float gv = (float)(int)(__float_as_uint(now.y) >> 23) - 127.0f;
+      float sum = 0.0f, off = gv - mref;
+      u32x4 p[2];
+      auto weigh = [&](int i) __attribute__((always_inline)) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(C[2 * i], ct, off)), p1 = __builtin_amdgcn_exp2f(fmaf(C[2 * i + 1], ct, off));
+        sum += p0 + p1;
+        p[i / 4][i % 4] = to_f16x2(p0, p1);
+      };
+      auto take = [&](int q) __attribute__((always_inline)) {  // operand q; q + kAhead goes into its place
+        const u32x4 v = ring[q % kAhead];
+        const int r = q + kAhead;
+        ring[q % kAhead] = *(const u32x4*)(r < KS ? next + r * 1024 : r < kOps ? base + r * 1024 : after + (r - kOps) * 1024);
+        return v;
+      };
 #pragma unroll
-      for (int i = 1; i < 16; ++i) top = fmaxf(top, S[i]);
-      const float gv = (float)(int)(__float_as_uint(pw.y) >> 23) - 127.0f;
-      top = fmaf(halves_max(top), ct, gv);
-      if (__any(top > mref + 14.0f)) {
-        const float m = fmaxf(mref, top - 6.0f), f = __builtin_amdgcn_exp2f(mref - m);
+      for (int s = 0; s < KS; ++s) {
+        __builtin_amdgcn_sched_barrier(0);
+        N = mfma32x32x16_f16(take(s), Q[s], s ? N : floatx16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0});
+#pragma unroll
+        for (int i = s * 8 / KS; i < (s + 1) * 8 / KS; ++i) weigh(i);
+      }
+      // No P above 2^14: then fp16 holds them.
+      if (__any(!(sum <= 16384.0f))) {
+        float top = C[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, C[i]);
+        const float m = fmaxf(mref, fmaf(halves_max(top), ct, gv) - 6.0f), f = __builtin_amdgcn_exp2f(mref - m);
         mref = m;
         l *= f;
 #pragma unroll
         for (int i = 0; i < VB; ++i)
 #pragma unroll
           for (int j = 0; j < 16; ++j) O[i][j] *= f;
+        off = gv - m;
+        sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) weigh(i);
       }
-      float sum = 0.0f;
+      l = fmaf(sum, __uint_as_float(0x7F000000u - __float_as_uint(now.y)), l);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        S[i] = __builtin_amdgcn_exp2f(fmaf(S[i], ct, gv - mref));
-        sum += S[i];
+      for (int n = 0; n < 2 * VB; ++n) {
+        __builtin_amdgcn_sched_barrier(0);
+        O[n / 2] = mfma32x32x16_f16(take(KS + n), p[n % 2], O[n / 2]);
       }
-      l = fmaf(sum, __uint_as_float(0x7F000000u - __float_as_uint(pw.y)), l);
-      u32x4 p[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[u][i] = to_f16x2(S[8 * u + 2 * i], S[8 * u + 2 * i + 1]);
-#pragma unroll
-      for (int n = 0; n < VB; ++n)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          O[n] = mfma32x32x16_f16(*(const u32x4*)(base + (KS + 2 * n + u) * 1024), p[u], O[n]);
     }
-    buf = buf == 2 ? 0 : buf + 1;
+    buf = next_buf;
   }
 
   l = halves_sum(l);
@@ -459,10 +500,14 @@ __global__ __launch_bounds__(64 * W, 2) void latent_flash_kernel(LatentExpandArg
     }
 }
 
+// Eight waves a workgroup share the tiles' way through LDS; four where that gives
+// more workgroups and each still a CU to itself (512 rows of 16 heads on 60000
+// tokens: 1100 us, with eight waves 1490; 1024 rows of 64 heads: 46 with eight).
 template <int NP, int VP>
-hipError_t flash(const LatentExpandArgs& a, hipStream_t st) {
-  constexpr int W = 8;
-  hipLaunchKernelGGL((latent_flash_kernel<NP, VP, W>), dim3((a.m + 32 * W - 1) / (32 * W) * a.heads), dim3(64 * W), 0, st, a);
+hipError_t flash(const LatentExpandArgs& a, uint32_t cu_count, hipStream_t st) {
+  const uint32_t small = (a.m + 127) / 128 * a.heads;
+  if (a.m > 128 && small <= cu_count) hipLaunchKernelGGL((latent_flash_kernel<NP, VP, 4>), dim3(small), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((latent_flash_kernel<NP, VP, 8>), dim3((a.m + 255) / 256 * a.heads), dim3(512), 0, st, a);
   return hipGetLastError();
 }
 
@@ -475,7 +520,7 @@ hipError_t launch_latent_wop(const LatentDims& d, const uint16_t* up, float* wmu
   return hipGetLastError();
 }
 
-hipError_t launch_latent_expanded(const LatentExpandArgs& args, uint32_t heads_at_once, hipStream_t st) {
+hipError_t launch_latent_expanded(const LatentExpandArgs& args, uint32_t heads_at_once, uint32_t cu_count, hipStream_t st) {
   LatentExpandArgs a = args;
   hipLaunchKernelGGL(latent_unpack_kernel, dim3(a.padded / 32), dim3(256), 0, st, a);
   hipError_t e = hipGetLastError();
@@ -491,8 +536,8 @@ hipError_t launch_latent_expanded(const LatentExpandArgs& args, uint32_t heads_a
       default: hipLaunchKernelGGL(latent_expand_kernel<512>, grid, dim3(256), 0, st, a); break;
     }
     if ((e = hipGetLastError()) != hipSuccess) break;
-    if (a.d.nope_pad == 64) e = a.d.v_pad == 64 ? flash<64, 64>(a, st) : flash<64, 128>(a, st);
-    else e = a.d.v_pad == 64 ? flash<128, 64>(a, st) : flash<128, 128>(a, st);
+    if (a.d.nope_pad == 64) e = a.d.v_pad == 64 ? flash<64, 64>(a, cu_count, st) : flash<64, 128>(a, cu_count, st);
+    else e = a.d.v_pad == 64 ? flash<128, 64>(a, cu_count, st) : flash<128, 128>(a, cu_count, st);
   }
   return e;
 }

@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <cmath>
 #include <new>
 #include <vector>
 
@@ -270,9 +271,12 @@ LatentAttnArgs absorbed_args(const qm_latent_weights* w, const LatentNewRows& ro
   return a;
 }
 
-// Splits of the absorbed attention: as many as fill the chip once (a workgroup a
-// CU), none below 4 blocks (the join costs more than a shorter walk
-// saves).
+// Splits of the absorbed attention: the least blocks a split that go through the
+// chip (a workgroup a CU) in one round, or in two to four where that ends sooner, a
+// workgroup's start and end costing as much as 7 blocks.  512 rows of 20 heads on
+// 20000 tokens are 160 groups of columns: one round of them 656 us, two rounds of
+// 480 workgroups 500.  None below 4 blocks: the join costs more than a shorter
+// walk saves.
 void plan_absorbed(const qm_runtime* rt, LatentAttnArgs* a) {
   const uint32_t cols = a->decode ? a->d.heads : a->rows * a->d.heads;
   a->group_cols = cols <= kLatentCols ? kLatentCols : 2 * kLatentCols;
@@ -288,11 +292,16 @@ void plan_absorbed(const qm_runtime* rt, LatentAttnArgs* a) {
   uint64_t most = 1;
   for (uint32_t b = 0; b < a->n_seqs; ++b) most = std::max(most, tiles(b));
   const int forced = rt->tune.latent_tiles;
-  uint64_t lo = std::min<uint64_t>(4, most), hi = most;  // the least tiles a split that fit one round
-  while (lo < hi) {
-    const uint64_t mid = (lo + hi) / 2;
-    if (units(mid) <= (uint64_t)rt->cu_count) hi = mid;
-    else lo = mid + 1;
+  uint64_t lo = most, best = UINT64_MAX;
+  for (uint64_t rounds = 1; rounds <= 4; ++rounds) {
+    uint64_t least = std::min<uint64_t>(4, most), hi = most;
+    while (least < hi) {
+      const uint64_t mid = (least + hi) / 2;
+      if (units(mid) <= rounds * rt->cu_count) hi = mid;
+      else least = mid + 1;
+    }
+    const uint64_t taken = (units(least) + rt->cu_count - 1) / rt->cu_count;
+    if (taken * (least + 7) < best) best = taken * (least + 7), lo = least;
   }
   if (forced > 0) lo = std::min<uint64_t>(forced, most);
   a->tiles_per_split = (uint32_t)lo;
@@ -325,13 +334,23 @@ qm_status absorbed_workspaces(qm_runtime* rt, LatentAttnArgs* a) {
   return QM_OK;
 }
 
-// Which form a prefill of M rows over T tokens takes: the one with the fewer
-// multiplications.
+// Which form a prefill of M rows over T tokens takes, by what each was measured to
+// cost in us (16 and 128 heads, 2 to 512 rows on 0 to 60000 tokens, ranks 384 and
+// 512; the two lie within a tenth where the sums cross):
+//   absorbed  20, 0.006 a column of rank 512 (queries in, sums out), and 0.46
+//             multiplications a fs;
+//   expanded  26, forming keys and values at 0.44 a fs, and 0.6 a 32-token tile of
+//             a workgroup's walk, which stays however few rows or workgroups there
+//             are (1.0 a round where 128 rows of a head are not a CU's alone).
 bool prefers_expanded(const qm_runtime* rt, const LatentDims& d, uint32_t M, uint64_t T) {
   if (rt->tune.latent_form) return rt->tune.latent_form == 2;
-  const double pairs = (double)M * ((double)T - 0.5 * M);
-  const double absorbed = pairs * (2.0 * d.rank_pad + kLatentRope);
-  const double expanded = pairs * (d.nope_pad + kLatentRope + d.v_pad) + (double)T * d.rank_pad * (d.nope_pad + d.v_pad);
+  const double pairs = (double)M * ((double)T - 0.5 * M) * d.heads;
+  const double cols = (double)M * d.heads;
+  const double absorbed = 20.0 + cols * d.rank_pad * (0.006 / 512) + pairs * (2.0 * d.rank_pad + kLatentRope) / 0.46e9;
+  const bool alone = std::ceil(M / 128.0) * d.heads <= rt->cu_count;
+  const double walk = alone ? 0.6 : std::max(1.0, std::ceil(M / 256.0) * d.heads / rt->cu_count);
+  const double expanded = 26.0 + (double)T * d.rank_pad * (d.nope_pad + d.v_pad) * d.heads / 0.44e9 +
+                          walk * ((double)T - 0.5 * M) / 32;
   return expanded < absorbed;
 }
 
@@ -667,7 +686,7 @@ qm_status qm_latent_prefill(qm_runtime* rt, const qm_latent_weights* w, qm_laten
   hipError_t e = hipSuccess;
   if (expanded) {
     e = launch_latent_append(LatentAppendArgs{rows, seq->rows, seq->length, M}, rt->stream);
-    if (e == hipSuccess) e = launch_latent_expanded(ep.a, ep.heads_at_once, rt->stream);
+    if (e == hipSuccess) e = launch_latent_expanded(ep.a, ep.heads_at_once, rt->cu_count, rt->stream);
   } else {
     e = launch_latent_absorbed(at, rt->stream);
   }
