@@ -302,6 +302,61 @@ def test_prefill_sizes(rt, H, cached, rows):
     check_prefill(rt, WIDE, H, cached, rows, H + rows)
 
 
+# Workgroups of eight waves (300 rows of 130 heads, 520 of 66) and of four; rows end inside a wave, a workgroup and a tile.
+@pytest.mark.parametrize("widths", [WIDE, SMALL, (128, 64, 64, 128), (128, 64, 128, 64)])
+@pytest.mark.parametrize("H,cached,rows", [(130, 20, 300), (66, 1, 520), (20, 333, 300), (1, 0, 1025)])
+def test_prefill_workgroups(torch_dev, widths, H, cached, rows):
+    with tuned(QM38_LATENT_FORM=2) as rt:
+        check_prefill(rt, widths, H, cached, rows, H + rows)
+
+
+# Columns' groups that fill the chip once with one split (160), more than once
+# (1280), and with 9 splits and more.
+@pytest.mark.parametrize("H,cached,rows", [(20, 3000, 512), (20, 100, 4096), (64, 2500, 24), (2, 0, 700)])
+def test_absorbed_splits(torch_dev, H, cached, rows):
+    with tuned(QM38_LATENT_FORM=1) as rt:
+        check_prefill(rt, SMALL, H, cached, rows, H + rows)
+
+
+def test_cache_beyond_32_bit_offsets(rt):
+    """7.5 million tokens, 4.4 GB of codes: all but the last hundred alike, so that
+    the softmax over them is that over 101 tokens, one of them weighing 7.5 million."""
+    rank, rope, nope, v = WIDE
+    g = generator(31)
+    H, alike, chunk = 8, 7_500_000, 500_000
+    kv_b, scale, weights = make_weights(rt, g, H, WIDE)
+    one, others = bf16(g, 1, rank + rope, std=0.01), bf16(g, 100, rank + rope)
+    cache, few = rt.create_latent_kv(rank, rope), rt.create_latent_kv(rank, rope)
+    cache.reserve(alike + 100)
+    many = one.expand(chunk, -1).contiguous()
+    for _ in range(alike // chunk):
+        cache.append(many, None, 0.0, chunk)
+    cache.append(others, None, 0.0, 97)
+    few.append(torch.cat([one, others]), None, 0.0, 101)
+    latent, key = held(few)
+    w = kv_b.double()
+    k, values = latent @ w[:, :nope].transpose(1, 2), latent @ w[:, nope:].transpose(1, 2)  # [H][101][nope], [H][101][v]
+    weigh = torch.zeros(101, dtype=torch.float64, device="cuda:0")
+    weigh[0] = np.log(alike)
+    q = bf16(g, 3, H, nope + rope, std=8.0)
+    x = q.double().transpose(0, 1)
+    score = (x[..., :nope] @ k.transpose(1, 2) + x[..., nope:] @ key.T) * scale + weigh  # [H][3][101]
+    o = torch.empty(3, H, v, dtype=torch.bfloat16, device="cuda:0")
+    rt.latent_attention(weights, [cache], q[:1], others[97:98], None, 0.0, o[:1])
+    rt.latent_attention_prefill(weights, cache, q[1:], others[98:], None, 0.0, 2, o[1:])
+    assert cache.sequence_length == alike + 100
+    for row in range(3):
+        p = torch.softmax(score[:, row:row + 1, :99 + row], -1)
+        assert 0.01 < float(p[..., 1:].sum(-1).mean()) < 0.99  # both kinds count
+        ref = (p @ values[:, :99 + row]).transpose(0, 1)
+        assert_attention(o[row:row + 1], ref, torch.full_like(ref, torch.inf), f"row {row}")
+    out = torch.empty(1, rank + rope, dtype=torch.bfloat16, device="cuda:0")
+    near = torch.empty_like(out)
+    cache.load(alike + 50, 1, out)
+    few.load(51, 1, near)
+    assert torch.equal(out, near)
+    cache.close()
+
 @pytest.mark.parametrize("form", FORMS)
 def test_prefill_peaked(torch_dev, form):
     with tuned(**FORMS[form]) as rt:
@@ -557,3 +612,72 @@ def test_capture_is_refused(torch_dev):
         rt.latent_attention(weights, [cache], q, kv, None, 0.0, o)
         torch.cuda.synchronize()
         assert cache.sequence_length == 11 and float(x[0]) == 1.0
+
+
+# ---------------------------------------------------------------------------
+# Together
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("rows", [19, 300])
+def test_a_layer_of_them(rt, torch_dev, rows):
+    """Quantised projections, positions turned in place, the latent cache and its
+    attention, the output projection: a prompt, then two sequences decoded together.
+    Each operator against its formula on what the one before it gave."""
+    E, H = 512, 12
+    rank, rope, nope, v = 256, 64, 64, 64
+    rng, g = np.random.default_rng(21), generator(21)
+
+    def matrix(n, k):
+        mat = synth.q4_matrix(rng, n, k)
+        w = synth.unpack_q4(mat[0]).astype(np.float32).reshape(-1, k // 64, 64)
+        w = w * synth.bf16_to_f32(mat[1])[..., None] + synth.bf16_to_f32(mat[2])[..., None]
+        dev = tuple(to_dev(a, torch_dev) for a in mat)
+        return dev, qm38.Runtime.job(*dev, n), torch.from_numpy(w.reshape(n, k)).to(torch_dev).double()
+
+    held_q, q_job, _ = matrix(H * (nope + rope), E)
+    held_kv, kv_job, _ = matrix(rank + rope, E)
+    held_b, b_job, b_plain = matrix(H * (nope + v), rank)
+    held_o, o_job, o_plain = matrix(E, H * v)
+    norm = torch.rand(rank, generator=g, device=torch_dev) + 0.5
+    scale = (nope + rope) ** -0.5
+    weights = rt.create_latent_weights(qm38.LatentConfig(H, rank, nope, rope, v, scale), b_job)
+    kv_b = b_plain.to(torch.bfloat16).reshape(H, nope + v, rank)
+    turn = qm38.RotaryConfig(rope, interleaved=True, theta=1e4)
+    freq, factor = frequencies(rope, 1e4, device=torch_dev)
+
+    def layer(x, positions, attend):
+        n = x.shape[0]
+        q = torch.empty(n, H, nope + rope, dtype=torch.bfloat16, device=torch_dev)
+        kv = torch.empty(n, rank + rope, dtype=torch.bfloat16, device=torch_dev)
+        rt.q4_project([q_job, kv_job], x, E, n, [q, kv])
+        rt.synchronize()
+        before = q.clone(), kv.clone()
+        rt.rotary(turn, [(q, q, H, nope + rope, nope), (kv, kv, 1, rank + rope, rank)], n, positions=positions)
+        o = torch.empty(n, H, v, dtype=torch.bfloat16, device=torch_dev)
+        attend(q, kv, o)
+        y = torch.empty(n, E, dtype=torch.bfloat16, device=torch_dev)
+        rt.q4_project([o_job], o, H * v, n, [y])
+        rt.synchronize()
+        check_rotated(q, before[0], positions, freq, factor, nope, True)
+        check_rotated(kv[:, None], before[1][:, None], positions, freq, factor, rank, True)
+        plain = o.reshape(n, H * v).double() @ o_plain.T
+        # Weights in 4 bits are exact; a sum of bf16 products, then half a bf16 step.
+        size = o.reshape(n, H * v).double().abs() @ o_plain.abs().T
+        assert ((y.double() - plain).abs() <= plain.abs() * HALF + size * 2.0 ** -11).all()
+        return q, o
+
+    first, second = rt.create_latent_kv(rank, rope), rt.create_latent_kv(rank, rope)
+    x = bf16(g, rows, E, std=0.3)
+    at = torch.arange(rows, dtype=torch.int32, device=torch_dev)
+    q, o = layer(x, at, lambda q, kv, o: rt.latent_attention_prefill(weights, first, q, kv, norm, EPS, rows, o))
+    ref, bound = attention(q, *held(first), kv_b, nope, scale, 0)
+    assert_attention(o, ref, bound, "prompt")
+    for step in range(3):
+        at = torch.tensor([rows + step, step], dtype=torch.int32, device=torch_dev)
+        q, o = layer(bf16(g, 2, E, std=0.3), at,
+                     lambda q, kv, o: rt.latent_attention(weights, [first, second], q, kv, norm, EPS, o))
+        for b, (cache, start) in enumerate(((first, rows + step), (second, step))):
+            assert cache.sequence_length == start + 1
+            ref, bound = attention(q[b:b + 1], *held(cache), kv_b, nope, scale, start)
+            assert_attention(o[b:b + 1], ref, bound, f"step {step} of sequence {b}")
+    for c in (first, second):
+        c.close()
