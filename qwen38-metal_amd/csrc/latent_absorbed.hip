@@ -54,7 +54,7 @@ __global__ __launch_bounds__(256) void latent_query_kernel(LatentAttnArgs a, uin
     const uint32_t item = blockIdx.x * 4 + wave;
     if (item >= a.rows) return;
     const LatentSeq& sq = a.seqs[a.decode ? item : 0];
-    latent_append_row(a.new_rows, sq.rows, sq.start + (a.decode ? 0 : item), item, lane);
+    latent_append_rows<1>(a.new_rows, sq.rows, sq.start + (a.decode ? 0 : item), item, item + 1, lane);
     return;
   }
   const uint32_t H = a.d.heads, nope = a.d.nope, qw = nope + a.d.rope, np = a.d.nope_pad;

@@ -11,10 +11,11 @@ namespace {
 
 constexpr int kWaves = 4;
 
+template <int R>
 __global__ __launch_bounds__(64 * kWaves) void latent_append_kernel(LatentAppendArgs a) {
-  const uint32_t item = blockIdx.x * kWaves + (threadIdx.x >> 6);
+  const uint32_t item = (blockIdx.x * kWaves + (threadIdx.x >> 6)) * R;
   if (item >= a.items) return;  // wave-uniform
-  latent_append_row(a.rows, a.to, a.first + item, item, threadIdx.x & 63);
+  latent_append_rows<R>(a.rows, a.to, a.first + item, item, a.items, threadIdx.x & 63);
 }
 
 __global__ __launch_bounds__(64 * kWaves) void latent_load_kernel(LatentRows rows, uint32_t rank, uint32_t rope,
@@ -106,8 +107,12 @@ hipError_t weights(const LatentDims& d, From from, uint16_t* down, uint16_t* up,
 
 }  // namespace
 
+// A wave a row while there are no more rows than the chip has waves at once (four a
+// A wave a row while the chip holds four waves a SIMD of them, then four rows a wave.
 hipError_t launch_latent_append(const LatentAppendArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(latent_append_kernel, dim3((a.items + kWaves - 1) / kWaves), dim3(64 * kWaves), 0, st, a);
+  constexpr int kMany = 4;
+  if (a.items <= 4096) hipLaunchKernelGGL(latent_append_kernel<1>, dim3((a.items + kWaves - 1) / kWaves), dim3(64 * kWaves), 0, st, a);
+  else hipLaunchKernelGGL(latent_append_kernel<kMany>, dim3((a.items + kWaves * kMany - 1) / (kWaves * kMany)), dim3(64 * kWaves), 0, st, a);
   return hipGetLastError();
 }
 

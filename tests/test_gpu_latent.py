@@ -164,6 +164,30 @@ def test_cache_codes(rt, widths, pieces):
     assert torch.equal(out.cpu(), want.to(torch.bfloat16))
 
 
+@pytest.mark.parametrize("n", [3, 5000])
+def test_codes_between_two_steps(rt, n):
+    """Quotients at a half and one bf16 step beside it, at scales of every size; rows
+    with numbers that are none among them; 5000 rows end inside a wave's four."""
+    g = generator(n)
+    power = torch.randint(-100, 100, (n, 1), generator=g, device="cuda:0").double()
+    half = torch.randint(0, 63, (n, 576), generator=g, device="cuda:0").double() + 0.5
+    x = (half * torch.where(torch.rand((n, 576), generator=g, device="cuda:0") < 0.5, 1.0, -1.0)).to(torch.bfloat16)
+    beside = (x.view(torch.int16) + torch.randint(-1, 2, (n, 576), generator=g, device="cuda:0").to(torch.int16)).view(torch.bfloat16)
+    x = beside.double()
+    x[:, 5], x[:, 520] = 127.0, -127.0  # the scale is the power of two
+    rows = (x * 2.0 ** power).to(torch.bfloat16)
+    rows[1, 3], rows[2, 570] = float("nan"), float("inf")
+    cache = rt.create_latent_kv(512, 64)
+    cache.append(rows, None, 0.0, n)
+    codes, scales = cache.read()
+    for part, (lo, hi) in enumerate(((0, 512), (512, 576))):
+        c, s = quantised(rows[:, lo:hi].double())
+        none = ~torch.isfinite(rows[:, lo:hi]).all(1).cpu().numpy()
+        assert np.isnan(scales[none, part]).all() and (codes[none, lo:hi] == 0).all() and none.sum() == 1
+        assert np.array_equal(codes[~none, lo:hi], c.cpu().numpy()[~none])
+        assert np.array_equal(scales[~none, part], s[:, 0].cpu().numpy()[~none])
+
+
 @pytest.mark.parametrize("widths", [WIDE, SMALL, ODD, TINY])
 def test_cache_normalised(rt, widths):
     rank, rope = widths[:2]
