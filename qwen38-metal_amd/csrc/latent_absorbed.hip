@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256) void latent_query_kernel(LatentAttnArgs a, uin
 //
 // With 128 heads and 131072
 // tokens the loop takes about 5000 cycles for 64 tokens of 64 columns, 2304 of them
-// the matrix cores'; before it 5 us until the first blocks are there, behind it
+// the matrix cores'; before it 5 us until queries and first blocks are there, behind it
 // 33 MB of partial sums.  56 us in all, 75 MB read.  With softmax and all
 // products in phases of their own: 59; waits of LDS reads for the copies in flight
 // (what the compiler makes of its own copy builtin): 71.
@@ -279,6 +279,15 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
       latent_dma4(scales, to + L::kLat + L::kKey, from_other);
     }
   };
+  // Two blocks before the queries, so that one trip to memory brings both; the next
+  // two behind them.
+  auto issue_two = [&](uint32_t i) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t j = i; j < i + 2; ++j)
+#pragma unroll
+      for (int k = 0; k < L::kDma; ++k) issue(t_begin + j, j * L::kTileBytes, t_begin + j < t_end, k);
+  };
+  issue_two(0);
   // (A group's last block may be one that does not exist; its columns have no tokens.)
   const size_t block = sq.block_begin + min(cg * NC + my_block, (cols - 1) / 32);
   u32x4 qhi[kLatSteps], qlo[kLatSteps];
@@ -299,11 +308,7 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
   }
   const float2 qs = limit ? *(const float2*)(a.qscale + (block * kLatentCols + col) * 2) : float2{0.0f, 0.0f};
   const float lat_scale = qs.x * a.scale * kLog2e, key_scale = qs.y * a.scale * kLog2e;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int k = 0; k < L::kDma; ++k) issue(t_begin + i, i * L::kTileBytes, t_begin + i < t_end, k);
-  if (brings) {  // (the loads before it are waited for, not the blocks behind them)
+  if (brings) {
     if constexpr (L::kLowInLds) *(u32x4*)(lds + L::kAtLow + wave * 1024 + lane * 16) = qlo[0];
     uint8_t* to = key_digits + (my_block * 2 + part) * 2048 + lane * 16;
     *(u32x4*)to = kd[0];
@@ -536,7 +541,8 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
   };
 
   if (threadIdx.x == 0) *flag = 0;
-  latent_wait_vmcnt<2 * L::kPieces>();  // the first two blocks
+  latent_wait_vmcnt<0>();  // the first two blocks
+  issue_two(2);
   lds_barrier();
   if (n) {
     intx16 hi, lo;
