@@ -167,7 +167,8 @@ __global__ __launch_bounds__(256) void latent_query_kernel(LatentAttnArgs a, uin
 //            rescaled) only when a maximum passes ref + 14, so p stays below 2^14
 //            and what is 2^-20 of the largest is still a normal fp16.  The waves
 //            compute p with the ref they have and publish it; where a maximum
-//            passes, a flag says so behind the same barrier and it is done again.
+//            passes 2^14, a flag says so behind the same barrier and it is done
+//            again; so is, at once, a block that some column does not see whole.
 //   sums     O^T[latent element][column] += codes^T P'^T on
 //            v_mfma_f32_32x32x16_f16, a wave an eighth of the latent: P' = token
 //            scale * p / 2^w, w moved like ref with the largest p * token scale;
@@ -178,12 +179,13 @@ __global__ __launch_bounds__(256) void latent_query_kernel(LatentAttnArgs a, uin
 // (P' written) the softmax's vector work runs mixed with the latent's part of the
 // next scores, behind the second the sums' products and the shared key's part.
 //
-// With 128 heads and 131072
-// tokens the loop takes about 5000 cycles for 64 tokens of 64 columns, 2304 of them
-// the matrix cores'; before it 5 us until queries and first blocks are there, behind it
-// 33 MB of partial sums.  56 us in all, 75 MB read.  With softmax and all
-// products in phases of their own: 59; waits of LDS reads for the copies in flight
-// (what the compiler makes of its own copy builtin): 71.
+// With 128 heads and 131072 tokens the loop takes about 4800 cycles for 64 tokens of
+// 64 columns, 2304 of them the matrix cores' and as many the vector unit's, which two
+// waves a SIMD overlap in part; before it 4 us until queries and first blocks are
+// there, behind it 33 MB of partial sums.  54 us in all, 75 MB read (1.4 TB/s).  With
+// masks and maxima for every block: 55; with softmax and all products in phases of
+// their own: 59; waits of LDS reads for the copies in flight (what the compiler makes
+// of its own copy builtin): 71.
 template <int RP, int NC>
 struct AbsorbedLds {
   static constexpr int kChunks = RP / 16;  // 16-byte pieces of a latent
@@ -197,9 +199,10 @@ struct AbsorbedLds {
   static constexpr int kKeyDigits = NC * 4096;  // of the queries' rotated part [block][step][hi, lo][lane]
   // The ring last: the others are then in reach of an instruction's offset.
   static constexpr int kAtP = kExchange, kAtMax = kAtP + kP, kAtKeys = kAtMax + kMax, kAtFlag = kAtKeys + kKeyDigits;
-  // Registers: at rank 512 one of the queries' 16 operands of a wave lives here.
-  static constexpr bool kLowInLds = RP / 32 / kParts >= 8 && NC == 2;
-  static constexpr int kAtLow = kAtFlag + 16, kLow = kLowInLds ? 4096 : 0;
+  // Registers: with two column blocks and many steps the lower digits of a wave's
+  // first steps live here.
+  static constexpr int kLowSteps = NC == 2 && RP / 32 / kParts >= 6 ? RP / 32 / kParts / 2 : 0;
+  static constexpr int kAtLow = kAtFlag + 16, kLow = kLowSteps * 4096;
   static constexpr int kAtRing = kAtLow + kLow, kBytes = kAtRing + kRing * kTileBytes;
   static_assert(kAtRing < 65536, "the offsets' range");
   static constexpr int kPieces = (RP / 32 + 7) / 8;  // KB of the latents that a wave brings
@@ -309,7 +312,8 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
   const float2 qs = limit ? *(const float2*)(a.qscale + (block * kLatentCols + col) * 2) : float2{0.0f, 0.0f};
   const float lat_scale = qs.x * a.scale * kLog2e, key_scale = qs.y * a.scale * kLog2e;
   if (brings) {
-    if constexpr (L::kLowInLds) *(u32x4*)(lds + L::kAtLow + wave * 1024 + lane * 16) = qlo[0];
+#pragma unroll
+    for (int s = 0; s < L::kLowSteps; ++s) *(u32x4*)(lds + L::kAtLow + s * 4096 + wave * 1024 + lane * 16) = qlo[s];
     uint8_t* to = key_digits + (my_block * 2 + part) * 2048 + lane * 16;
     *(u32x4*)to = kd[0];
     *(u32x4*)(to + 1024) = kd[1];
@@ -346,7 +350,7 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
     lo = mfma32x32x32_i8(kf, ql, start ? intx16{} : lo);
   };
   // The wave's share of its current block, in turn: whole numbers of the
-  // latent's and the key's products; scores and token scales (as bits).
+  // latent's and the key's products; then scores (as bits).
   int ldot[kShare] = {}, kdot[kShare] = {};
   auto take_keys = [&](const intx16& hi, const intx16& lo) __attribute__((always_inline)) {
 #pragma unroll
@@ -377,11 +381,10 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
     }
   };
 
-  float sum = 0.0f, top = 0.0f, top_pt = 0.0f;
+  float sum = 0.0f, top_pt = 0.0f;
   const uint32_t lane16 = lane * 16;
   const bool lower = NC == 1 || my_block == 0;
   auto& S = ldot;  // scores
-  auto& T = kdot;  // token scales
   const uint32_t first = part * kShare;  // scores i of a lane are tokens 8 (i / 4) + 4 half + i % 4, its own from here on
   const uint32_t at_max = (tb * kParts + part) * kCols + 32 * my_block + col;
   float p[kShare];
@@ -394,10 +397,10 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
       *(u32x4*)(to + part * 1024) =
           u32x4{to_f16x2(p[0], p[2]), to_f16x2(p[1], p[3]), to_f16x2(p[4], p[6]), to_f16x2(p[5], p[7])};
   };
-  auto weigh = [&](int i, float ref, float unit) __attribute__((always_inline)) {
+  auto weigh = [&](int i, float t, float ref, float unit) __attribute__((always_inline)) {
     const float e = __builtin_amdgcn_exp2f(__int_as_float(S[i]) - ref);
     sum += e;
-    p[i] = e * __int_as_float(T[i]) * unit;
+    p[i] = e * t * unit;
   };
   // What a wave reads from LDS for four scores of its block: the other parts'
   // numbers, the tokens' scales.
@@ -406,6 +409,11 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
     intx4 d[kOthers];
     floatx4 s[2];
   };
+  auto read_scales = [&](uint32_t slot, int g, floatx4 (&s)[2]) __attribute__((always_inline)) {
+    const float* at = (const float*)(lds + L::kAtRing + slot + L::kLat + L::kKey) + (2 * (first / 4 + g) + half) * 8;
+    s[0] = *(const floatx4*)at;
+    s[1] = *(const floatx4*)(at + 4);
+  };
   auto read_softmax = [&](uint32_t slot, int g) __attribute__((always_inline)) {
     SoftmaxIn r;
 #pragma unroll
@@ -413,33 +421,52 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
       const uint32_t at = NC == 1 ? part * 4096 + ((part + 1 + f) & 3) * 1024 : part * 2048 + g * 1024;
       r.d[f] = *(const intx4*)(exchange + tile_at + at);
     }
-    const float* at = (const float*)(lds + L::kAtRing + slot + L::kLat + L::kKey) + (2 * (first / 4 + g) + half) * 8;
-    r.s[0] = *(const floatx4*)at;
-    r.s[1] = *(const floatx4*)(at + 4);
+    read_scales(slot, g, r.s);
     return r;
   };
+  auto latent_scale = [](const floatx4 (&s)[2], int j) __attribute__((always_inline)) { return j < 2 ? s[0][2 * j] : s[1][2 * j - 4]; };
+  auto key_token_scale = [](const floatx4 (&s)[2], int j) __attribute__((always_inline)) { return j < 2 ? s[0][2 * j + 1] : s[1][2 * j - 3]; };
   // Score i of the wave's share: its value, and what it gives with the references there are.
-  auto softmax = [&](int i, const SoftmaxIn& r, uint32_t tile, bool whole, float ref, float unit) __attribute__((always_inline)) {
-    const int g = i / 4, j = i % 4;
-    const floatx4 s0 = r.s[0], s1 = r.s[1];
+  auto softmax = [&](int i, const SoftmaxIn& r, float ref, float unit) __attribute__((always_inline)) {
+    const int j = i % 4;
     int dot = ldot[i];
 #pragma unroll
     for (int f = 0; f < kOthers; ++f) dot += r.d[f][j];
-    float t = j < 2 ? s0[2 * j] : s1[2 * j - 4];
-    float v = fmaf((float)dot, t * lat_scale, (float)kdot[i] * ((j < 2 ? s0[2 * j + 1] : s1[2 * j - 3]) * key_scale));
-    if (!whole) {
-      const bool seen = tile * kLatentTile + 8 * (first / 4 + g) + 4 * half + j < limit;
-      v = seen ? v : -INFINITY;
-      t = seen ? t : 0.0f;  // nothing of it, not even a scale that is no number
-    }
-    top = fmaxf(top, v);
-    S[i] = __float_as_int(v);
-    T[i] = __float_as_int(t);
-    weigh(i, ref, unit);
+    const float t = latent_scale(r.s, j);
+    S[i] = __float_as_int(fmaf((float)dot, t * lat_scale, (float)kdot[i] * (key_token_scale(r.s, j) * key_scale)));
+    weigh(i, t, ref, unit);
     top_pt = fmaxf(top_pt, p[i]);
   };
+  // The same of a block that some columns do not see to its end.
+  auto masked = [&](uint32_t slot, uint32_t tile, float ref, float unit) __attribute__((always_inline)) {
+    sum = top_pt = 0.0f;
+#pragma unroll
+    for (int g = 0; g < kShare / 4; ++g) {
+      floatx4 s[2];
+      read_scales(slot, g, s);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = 4 * g + j;
+        const bool seen = tile * kLatentTile + 8 * (first / 4 + g) + 4 * half + j < limit;
+        S[i] = __float_as_int(seen ? __int_as_float(S[i]) : -INFINITY);
+        weigh(i, seen ? latent_scale(s, j) : 0.0f, ref, unit);  // nothing of it, not even a scale that is no number
+        top_pt = fmaxf(top_pt, p[i]);
+      }
+    }
+  };
   // Moves the references to the maxima and publishes again.
-  auto move = [&]() __attribute__((always_inline)) {
+  auto move = [&](uint32_t slot, uint32_t tile) __attribute__((always_inline)) {
+    float T[kShare], top = -INFINITY;  // token scales
+#pragma unroll
+    for (int g = 0; g < kShare / 4; ++g) {
+      floatx4 s[2];
+      read_scales(slot, g, s);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        T[4 * g + j] = tile * kLatentTile + 8 * (first / 4 + g) + 4 * half + j < limit ? latent_scale(s, j) : 0.0f;
+        top = fmaxf(top, __int_as_float(S[4 * g + j]));
+      }
+    }
     auto column_max = [&](int n, float2* m) __attribute__((always_inline)) {
       *m = maxima[32 * n + col];
 #pragma unroll
@@ -462,7 +489,7 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
     const float own = lower ? m[0] : m[NC - 1];
     float top_w = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kShare; ++i) top_w = fmaxf(top_w, __int_as_float(S[i]) - own + __log2f(__int_as_float(T[i])));
+    for (int i = 0; i < kShare; ++i) top_w = fmaxf(top_w, __int_as_float(S[i]) - own + __log2f(T[i]));
     top_w = halves_max(top_w);
     if (half == 0) maxima[at_max].y = top_w;
     lds_barrier();
@@ -483,7 +510,7 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
     const float ref = lower ? mref[0] : mref[NC - 1], unit = __builtin_amdgcn_exp2f(-(lower ? w2[0] : w2[NC - 1]));
     sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kShare; ++i) weigh(i, ref, unit);
+    for (int i = 0; i < kShare; ++i) weigh(i, T[i], ref, unit);
     store_p();
     lds_barrier();
   };
@@ -499,7 +526,7 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
                        *(const u32x4*)(kd + 1024)};
   };
   auto low = [&](int s) __attribute__((always_inline)) {
-    return L::kLowInLds && s == 0 ? *(const u32x4*)(lds + L::kAtLow + (wave & 3) * 1024 + lane16) : qlo[s];
+    return s < L::kLowSteps ? *(const u32x4*)(lds + L::kAtLow + s * 4096 + (wave & 3) * 1024 + lane16) : qlo[s];
   };
   auto score_codes = [&](uint32_t slot, int s) __attribute__((always_inline)) {
     return *(const u32x4*)(lds + (L::kAtRing + slot + piece(ka, part * kLatSteps + s)));
@@ -507,7 +534,7 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
   // The sums' products of the two blocks at `now`.  A step takes one operand of codes
   // and the columns' P'; its operands are read a step ahead, and no further
   // (registers).
-  auto products = [&](uint32_t now, uint32_t next, const KeyOperands& key) __attribute__((always_inline)) {
+  auto products = [&](uint32_t now, uint32_t next, const KeyOperands& key, auto move) __attribute__((always_inline)) {
     constexpr int kFrags = 4 * kBlocks;
     u32x2 codes_at[2];
     u32x4 pf[2][NC];
@@ -520,12 +547,18 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
     };
     {
       intx16 hi, lo;
+      const uint32_t passed = *flag;
       const KeyOperands second = read_key(next, 1);
       score_step(key.k, key.hi, key.lo, true, hi, lo);
-      read(0);
       score_step(second.k, second.hi, second.lo, false, hi, lo);
+      read(0);
       take_keys(hi, lo);
+      if (__builtin_amdgcn_readfirstlane(passed)) {
+        move();
+        read(0);
+      }
     }
+    l += sum;
 #pragma unroll
     for (int f = 0; f < kFrags; ++f) {
       __builtin_amdgcn_sched_barrier(0);
@@ -573,15 +606,16 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
       const uint32_t tile = t_begin + i + tb;
       const bool whole = (tile + 1) * kLatentTile <= lim_min && c_last - c_first == kCols - 1;
       const float ref = lower ? mref[0] : mref[NC - 1], unit = __builtin_amdgcn_exp2f(-(lower ? w2[0] : w2[NC - 1]));
-      top = -INFINITY, top_pt = sum = 0.0f;
+      top_pt = sum = 0.0f;
       u32x4 k = score_codes(next + tb * L::kTileBytes, 0);
-      const u32x4 low0 = low(0);
+      u32x4 lo_digits = low(0);
 #pragma unroll
       for (int s = 0; s < kLatSteps; ++s) {
         __builtin_amdgcn_sched_barrier(0);
         const u32x4 k_now = k;
-        if (s + 1 < kLatSteps) k = score_codes(next + tb * L::kTileBytes, s + 1);
-        score_step(k_now, qhi[s], s == 0 ? low0 : qlo[s], s == 0, hi, lo);
+        const u32x4 lo_now = lo_digits;
+        if (s + 1 < kLatSteps) k = score_codes(next + tb * L::kTileBytes, s + 1), lo_digits = low(s + 1);
+        score_step(k_now, qhi[s], lo_now, s == 0, hi, lo);
         // The DMA of the two blocks behind the next two, an instruction or two a step.
 #pragma unroll
         for (int d = s * 2 * L::kPieces / kLatSteps; d < (s + 1) * 2 * L::kPieces / kLatSteps; ++d) {
@@ -590,19 +624,20 @@ __global__ __launch_bounds__(512, 2) void latent_attn_kernel(LatentAttnArgs a) {
         }
 #pragma unroll
         for (int j = s * kShare / kLatSteps; j < (s + 1) * kShare / kLatSteps; ++j) {
-          softmax(j, in, tile, whole, ref, unit);
+          softmax(j, in, ref, unit);
           if (j % 4 == 3 && j + 1 < kShare) in = read_softmax(now + tb * L::kTileBytes, (j + 1) / 4);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
+      if (!whole) masked(now + tb * L::kTileBytes, tile, ref, unit);
       key = read_key(next + tb * L::kTileBytes, 0);
       store_p();
-      if (top > ref + 14.0f || top_pt > 16384.0f) *flag = 1;
+      if (fmaxf(sum, top_pt) > 16384.0f) *flag = 1;
     }
     lds_barrier();  // P' and the flag
-    if (__builtin_amdgcn_readfirstlane(*flag)) move();
-    l += sum;
-    products(now, next + tb * L::kTileBytes, key);
+    products(now, next + tb * L::kTileBytes, key, [&]() __attribute__((always_inline)) {
+      move(now + tb * L::kTileBytes, t_begin + i + tb);
+    });
     exchange_scores(hi, lo);
     latent_wait_vmcnt<0>();
     const uint32_t t = now;
