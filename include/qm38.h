@@ -474,7 +474,8 @@ void qm_latent_weights_destroy(qm_latent_weights* w);
 qm_status qm_latent_decode(qm_runtime* rt, const qm_latent_weights* w, qm_latent_kv* const* seqs, uint32_t B,
                            const uint16_t* q, const uint16_t* kv, const float* norm, float epsilon, uint16_t* o);
 /* M new rows of one sequence, row i attending over the cached tokens and the
- * new rows up to itself.  Layouts as above with M in the place of B. */
+ * new rows up to itself.  Layouts as above with M in the place of B.  In both
+ * calls o overlaps no input; 2-byte alignment of it is enough. */
 qm_status qm_latent_prefill(qm_runtime* rt, const qm_latent_weights* w, qm_latent_kv* seq, const uint16_t* q,
                             const uint16_t* kv, const float* norm, float epsilon, uint32_t M, uint16_t* o);
 

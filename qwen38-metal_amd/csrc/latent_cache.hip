@@ -2,6 +2,8 @@
 // weights in the kernels' layouts.
 //
 // A row's layout and quantiser: latent_append.h.
+#include <algorithm>
+
 #include "latent.h"
 #include "latent_append.h"
 #include "latent_device.h"
@@ -107,13 +109,25 @@ hipError_t weights(const LatentDims& d, From from, uint16_t* down, uint16_t* up,
 
 }  // namespace
 
-// A wave a row while there are no more rows than the chip has waves at once (four a
+constexpr uint32_t kMostRows = 1u << 22;  // of a launch, whose threads stay below 2^32
+
 // A wave a row while the chip holds four waves a SIMD of them, then four rows a wave.
-hipError_t launch_latent_append(const LatentAppendArgs& a, hipStream_t st) {
+hipError_t launch_latent_append(const LatentAppendArgs& args, hipStream_t st) {
   constexpr int kMany = 4;
-  if (a.items <= 4096) hipLaunchKernelGGL(latent_append_kernel<1>, dim3((a.items + kWaves - 1) / kWaves), dim3(64 * kWaves), 0, st, a);
-  else hipLaunchKernelGGL(latent_append_kernel<kMany>, dim3((a.items + kWaves * kMany - 1) / (kWaves * kMany)), dim3(64 * kWaves), 0, st, a);
-  return hipGetLastError();
+  LatentAppendArgs a = args;
+  for (uint64_t r0 = 0; r0 < args.items; r0 += kMostRows) {
+    a.rows.kv = args.rows.kv + r0 * (args.rows.rank + args.rows.rope);
+    a.first = args.first + (uint32_t)r0;
+    a.items = (uint32_t)std::min<uint64_t>(kMostRows, args.items - r0);
+    if (a.items <= 4096)
+      hipLaunchKernelGGL(latent_append_kernel<1>, dim3((a.items + kWaves - 1) / kWaves), dim3(64 * kWaves), 0, st, a);
+    else
+      hipLaunchKernelGGL(latent_append_kernel<kMany>, dim3((a.items + kWaves * kMany - 1) / (kWaves * kMany)),
+                         dim3(64 * kWaves), 0, st, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_latent_wnorm(const LatentDims& d, const uint16_t* down, float* wnorm, hipStream_t st) {
@@ -123,9 +137,14 @@ hipError_t launch_latent_wnorm(const LatentDims& d, const uint16_t* down, float*
 
 hipError_t launch_latent_load(const LatentRows& rows, uint32_t rank, uint32_t rope, uint32_t rank_pad, uint32_t first,
                               uint32_t count, uint16_t* out, hipStream_t st) {
-  hipLaunchKernelGGL(latent_load_kernel, dim3((count + kWaves - 1) / kWaves), dim3(64 * kWaves), 0, st, rows, rank,
-                     rope, rank_pad, first, count, out);
-  return hipGetLastError();
+  for (uint64_t r0 = 0; r0 < count; r0 += kMostRows) {
+    const uint32_t n = (uint32_t)std::min<uint64_t>(kMostRows, count - r0);
+    hipLaunchKernelGGL(latent_load_kernel, dim3((n + kWaves - 1) / kWaves), dim3(64 * kWaves), 0, st, rows, rank, rope,
+                       rank_pad, first + (uint32_t)r0, n, out + r0 * (rank + rope));
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_latent_weights(const LatentDims& d, const uint16_t* kv_b, uint16_t* down, uint16_t* up,

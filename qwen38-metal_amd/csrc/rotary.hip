@@ -123,12 +123,12 @@ hipError_t launch_rotary(const RotaryArgs& args, uint32_t M, bool interleaved, b
     items += (uint64_t)a.t[k].heads * a.t[k].head_dim / (vec ? 8 : 1);
   }
   a.items = (uint32_t)items;
-  constexpr uint32_t kMaxRows = 1u << 30;  // a grid's blocks
+  constexpr uint32_t kMaxRows = 1u << 23;  // a launch's threads stay below 2^32
   auto kernel = interleaved ? (vec ? rotary_kernel<true, true> : rotary_kernel<true, false>)
                             : (vec ? rotary_kernel<false, true> : rotary_kernel<false, false>);
-  for (uint32_t r0 = 0; r0 < M; r0 += kMaxRows) {
-    a.row0 = r0;
-    const uint32_t rows = std::min(kMaxRows, M - r0);
+  for (uint64_t r0 = 0; r0 < M; r0 += kMaxRows) {
+    a.row0 = (uint32_t)r0;
+    const uint32_t rows = (uint32_t)std::min<uint64_t>(kMaxRows, M - r0);
     // Blocks of a row: one for many rows, more where the rows alone leave CUs idle.
     const uint32_t most = (a.items + kThreads - 1) / kThreads;
     const uint32_t groups = std::max(1u, std::min(most, (1024u + rows - 1) / rows));

@@ -343,7 +343,9 @@ qm_status absorbed_workspaces(qm_runtime* rt, LatentAttnArgs* a) {
 //             a workgroup's walk, which stays however few rows or workgroups there
 //             are (1.0 a round where 128 rows of a head are not a CU's alone).
 bool prefers_expanded(const qm_runtime* rt, const LatentDims& d, uint32_t M, uint64_t T) {
+  if (T > 1u << 28) return false;  // its launches' threads
   if (rt->tune.latent_form) return rt->tune.latent_form == 2;
+  if ((uint64_t)M * d.heads > 1u << 20) return true;  // the absorbed form's partial sums: 2 GB at rank 512
   const double pairs = (double)M * ((double)T - 0.5 * M) * d.heads;
   const double cols = (double)M * d.heads;
   const double absorbed = 20.0 + cols * d.rank_pad * (0.006 / 512) + pairs * (2.0 * d.rank_pad + kLatentRope) / 0.46e9;

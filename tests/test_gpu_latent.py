@@ -638,6 +638,54 @@ def test_capture_is_refused(torch_dev):
         assert cache.sequence_length == 11 and float(x[0]) == 1.0
 
 
+def test_more_rows_than_a_launch_takes(rt):
+    """2^23 + 5 rows turned, 2^22 + 5 appended and read back: the rows at the ends
+    and where one launch follows another."""
+    n = (1 << 23) + 5
+    g = generator(41)
+    x = bf16(g, n, 1, 8)
+    y = torch.empty_like(x)
+    rt.rotary(qm38.RotaryConfig(4, interleaved=True, theta=100.0), [(x, y, 1, 8, 2)], n, position_base=7)
+    freq, factor = frequencies(4, 100.0, device="cuda:0")
+    for lo in (0, (1 << 23) - 4, n - 4):
+        check_rotated(y[lo:lo + 4], x[lo:lo + 4], torch.arange(lo + 7, lo + 11, device="cuda:0"), freq, factor, 2, True)
+    n = (1 << 22) + 5
+    rows = x[:n, 0].repeat(1, 2).contiguous()  # rank 8, rope_dim 8
+    cache = rt.create_latent_kv(8, 8)
+    cache.append(rows, None, 0.0, n)
+    assert cache.sequence_length == n
+    out = torch.empty_like(rows)
+    cache.load(0, n, out)
+    c, s = quantised(rows[:, :8].double())
+    want = (c * s.double()).to(torch.bfloat16)
+    assert torch.equal(out[:, :8], want) and torch.equal(out[:, 8:], want)
+    cache.close()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("widths", [WIDE, ODD])
+def test_output_of_any_alignment(torch_dev, form, widths):
+    """An o on 2 bytes holds what an aligned one does, and nothing around it changes."""
+    rank, rope, nope, v = widths
+    H, rows = 6, 70
+    with tuned(**FORMS[form]) as rt:
+        g = generator(43)
+        _, _, weights = make_weights(rt, g, H, widths)
+        q, kv = bf16(g, rows, H, nope + rope), bf16(g, rows, rank + rope)
+        outs = []
+        for shift in (0, 1):
+            flat = torch.full((rows * H * v + 16,), 7.0, dtype=torch.bfloat16, device=torch_dev)
+            o = flat[8 + shift:8 + shift + rows * H * v].view(rows, H, v)
+            cache = rt.create_latent_kv(rank, rope)
+            rt.latent_attention_prefill(weights, cache, q[:rows - 1], kv[:rows - 1], None, 0.0, rows - 1, o[:rows - 1])
+            rt.latent_attention(weights, [cache], q[rows - 1:].clone(), kv[rows - 1:].clone(), None, 0.0, o[rows - 1:])
+            rt.synchronize()
+            outs.append(o.clone())
+            assert (flat[:8 + shift] == 7).all() and (flat[8 + shift + rows * H * v:] == 7).all()
+            cache.close()
+        assert torch.equal(*outs)
+
+
 # ---------------------------------------------------------------------------
 # Together
 # ---------------------------------------------------------------------------
