@@ -5,7 +5,7 @@
 //
 // Three launches, the last two for as many heads at a time as the workspace
 // holds: latent_unpack_kernel, latent_expand_kernel (the GEMM), and
-// latent_flash_kernel.
+// latent_prompt_kernel.
 //
 // Everything between them lies in global memory in operand order: a block of 32
 // rows (tokens, or weight rows) x 16 contraction elements is 1 KB in which lane
@@ -92,6 +92,8 @@ __global__ __launch_bounds__(256) void latent_wop_kernel(LatentDims d, const uin
 //   fv = s_lat / 2^gv, powers = {2^g, 2^gv}.
 // A token that stands for NaN keeps it in its key (fk or the operand) and has fv
 // = 0: rows that do not see it multiply its value by 0.
+// 6144 tokens of 512 + 64 (3.6 MB in, 7.2 MB out): 9.4 us; 1024: 5.7, a launch and a
+// chain of two loads.
 __global__ __launch_bounds__(256) void latent_unpack_kernel(LatentExpandArgs a) {
   __shared__ float sl[32], sk[32];
   const uint32_t tile = blockIdx.x, tid = threadIdx.x, rp = a.d.rank_pad, stride = rp + kLatentRope;
@@ -138,10 +140,14 @@ __global__ __launch_bounds__(256) void latent_unpack_kernel(LatentExpandArgs a) 
 // through LDS, 32 contraction elements a stage, by buffer->LDS DMA.
 //   Keys: D = W (rows) x latents (columns): a lane holds, for its token, the key
 //   elements 16 u + 4 h + {0..3}, + 8 + {0..3} (h = lane / 32) in eight registers:
-//   the 16 bytes of contraction block u of the flash kernel's key operand, whose
+//   the 16 bytes of contraction block u of the prompt kernel's key operand, whose
 //   queries are read in the same order.
 //   Values: D = latents (rows) x W (columns): a lane holds, for its value
-//   element, the tokens in the order in which the flash kernel's weights P lie.
+//   element, the tokens in the order in which the prompt kernel's weights P lie.
+// Bound by the loop of a stage (barrier, LDS reads of 12 KB a wave, 16 products):
+// 6144 tokens x 32768 rows x 512 take 240 us, 860 TFLOP/s, the matrix cores 44% busy
+// at two workgroups a CU; 393 MB are written meanwhile, without which a like loop
+// took a tenth less.
 constexpr int kExpRows = 256, kExpTokens = 128, kExpStages = 3;
 constexpr int kExpStageBytes = (kExpTokens + kExpRows) * 64;
 
@@ -279,7 +285,7 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(LatentExpandArgs 
 // products go between the exponentials; with each phase by itself, and a maximum
 // for every tile: 945.
 template <int NP, int VP, int W>
-struct FlashLds {
+struct PromptLds {
   static constexpr int kKSteps = NP / 16 + 4, kVBlocks = VP / 32;
   static constexpr int kTile = (kKSteps + 2 * kVBlocks) * 1024;
   static constexpr int kTiles = 2;  // of a stage
@@ -290,8 +296,8 @@ struct FlashLds {
 };
 
 template <int NP, int VP, int W>
-__global__ __launch_bounds__(64 * W, 2) void latent_flash_kernel(LatentExpandArgs a) {
-  using L = FlashLds<NP, VP, W>;
+__global__ __launch_bounds__(64 * W, 2) void latent_prompt_kernel(LatentExpandArgs a) {
+  using L = PromptLds<NP, VP, W>;
   constexpr int KS = L::kKSteps, VB = L::kVBlocks;
   __shared__ __attribute__((aligned(16))) uint8_t lds[L::kBufs * L::kStage];
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -504,10 +510,10 @@ __global__ __launch_bounds__(64 * W, 2) void latent_flash_kernel(LatentExpandArg
 // more workgroups and each still a CU to itself (512 rows of 16 heads on 60000
 // tokens: 1100 us, with eight waves 1490; 1024 rows of 64 heads: 46 with eight).
 template <int NP, int VP>
-hipError_t flash(const LatentExpandArgs& a, uint32_t cu_count, hipStream_t st) {
+hipError_t prompt(const LatentExpandArgs& a, uint32_t cu_count, hipStream_t st) {
   const uint32_t small = (a.m + 127) / 128 * a.heads;
-  if (a.m > 128 && small <= cu_count) hipLaunchKernelGGL((latent_flash_kernel<NP, VP, 4>), dim3(small), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((latent_flash_kernel<NP, VP, 8>), dim3((a.m + 255) / 256 * a.heads), dim3(512), 0, st, a);
+  if (a.m > 128 && small <= cu_count) hipLaunchKernelGGL((latent_prompt_kernel<NP, VP, 4>), dim3(small), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((latent_prompt_kernel<NP, VP, 8>), dim3((a.m + 255) / 256 * a.heads), dim3(512), 0, st, a);
   return hipGetLastError();
 }
 
@@ -536,8 +542,8 @@ hipError_t launch_latent_expanded(const LatentExpandArgs& args, uint32_t heads_a
       default: hipLaunchKernelGGL(latent_expand_kernel<512>, grid, dim3(256), 0, st, a); break;
     }
     if ((e = hipGetLastError()) != hipSuccess) break;
-    if (a.d.nope_pad == 64) e = a.d.v_pad == 64 ? flash<64, 64>(a, cu_count, st) : flash<64, 128>(a, cu_count, st);
-    else e = a.d.v_pad == 64 ? flash<128, 64>(a, cu_count, st) : flash<128, 128>(a, cu_count, st);
+    if (a.d.nope_pad == 64) e = a.d.v_pad == 64 ? prompt<64, 64>(a, cu_count, st) : prompt<64, 128>(a, cu_count, st);
+    else e = a.d.v_pad == 64 ? prompt<128, 64>(a, cu_count, st) : prompt<128, 128>(a, cu_count, st);
   }
   return e;
 }
