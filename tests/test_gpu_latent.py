@@ -284,6 +284,12 @@ def test_decode_lengths(rt, H, lengths):
     check_decode(rt, WIDE, H, lengths, H)
 
 
+@pytest.mark.parametrize("widths,H,lengths", [(TINY, 1024, [100, 0, 33]), (SMALL, 1024, [70]), (TINY, 1024, list(range(64))),
+                                              (WIDE, 1023, [2000])])
+def test_decode_most_heads(rt, widths, H, lengths):
+    check_decode(rt, widths, H, lengths, H + len(lengths))
+
+
 def test_decode_peaked(rt):
     """Scores of some hundreds: one token takes almost all of a row, the running
     maximum rises through the cache and falls behind."""
@@ -380,6 +386,13 @@ def test_cache_beyond_32_bit_offsets(rt):
     few.load(51, 1, near)
     assert torch.equal(out, near)
     cache.close()
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("widths,H,cached,rows", [(TINY, 1024, 5, 70), (SMALL, 1000, 0, 40)])
+def test_prefill_most_heads(torch_dev, form, widths, H, cached, rows):
+    with tuned(**FORMS[form]) as rt:
+        check_prefill(rt, widths, H, cached, rows, H + rows)
+
 
 @pytest.mark.parametrize("form", FORMS)
 def test_prefill_peaked(torch_dev, form):
