@@ -106,7 +106,8 @@ struct LatentExpandArgs {
   uint32_t m, start, tokens;
   uint32_t padded;       // tokens rounded up to kLatentExpandTokens
   uint32_t head0, heads; // the launch's heads (filled by the launcher)
-  uint32_t out8;         // o's rows take 8-byte stores
+  uint32_t out16;        // o's rows take 16-byte stores
+  uint32_t paired;       // rows of a workgroup: from both ends (filled by the launcher)
   uint16_t* latents;     // fp16 [padded / 32][rank_pad / 16][512]
   uint16_t* keys;        // fp16 [padded / 32][4][512]: the shared key
   float* fk;             // [padded] factors of a token's keys and values

@@ -105,6 +105,11 @@ __device__ __forceinline__ uint32_t to_bf16x2(float lo, float hi) {
   const latent_bf16x2 v = {(__bf16)lo, (__bf16)hi};
   return __builtin_bit_cast(uint32_t, v);
 }
+// The upper lanes' `a` and the lower lanes' `b` change places.
+__device__ __forceinline__ void swap_halves(uint32_t& a, uint32_t& b) {
+  const auto p = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = p[0], b = p[1];
+}
 // Maximum of lanes l and l ^ 32, and their sum.
 __device__ __forceinline__ float halves_max(float v) {
   const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);

@@ -304,63 +304,18 @@ __global__ __launch_bounds__(64 * W, 2) void latent_prompt_kernel(LatentExpandAr
   const uint32_t col = lane & 31, half = lane >> 5;
   const uint32_t hc = blockIdx.x % a.heads, rb = gridDim.x / a.heads - 1 - blockIdx.x / a.heads;
   const uint32_t h = a.head0 + hc, H = a.d.heads, nope = a.d.nope, qw = nope + a.d.rope;
-  const uint32_t r_first = rb * 32 * W, r0 = r_first + 32 * wave, row = r0 + col;
+  // Paired: 128 rows from the end for waves 0..3, as many from the start for 4..7 (of
+  // an odd number of such blocks the middle one has a workgroup's first waves alone).
+  const uint32_t halves = (a.m + 127) / 128, last = halves - 1 - rb;
+  const bool none = a.paired && wave >= 4 && rb == last;
+  const uint32_t r0 = none ? a.m : !a.paired ? (rb * W + wave) * 32 : (wave < 4 ? last : rb) * 128 + wave % 4 * 32;
+  const uint32_t r_end = a.paired ? (last + 1) * 128 : (rb + 1) * 32 * W, row = r0 + col;
   const bool live = row < a.m;
   // Tokens that the workgroup, the wave and the lane see.
-  const uint32_t wg_limit = a.start + min(r_first + 32 * W, a.m);
+  const uint32_t wg_limit = a.start + min(r_end, a.m);
   const uint32_t wave_limit = r0 < a.m ? a.start + min(r0 + 32, a.m) : 0;
   const uint32_t wave_whole = r0 < a.m ? a.start + r0 + 1 : 0;  // every row sees what is below
   const uint32_t limit = live ? a.start + row + 1 : 0;
-
-  // Queries, in the key operand's order: fp16 times 2^f, the expanded part divided
-  // by the weights' power as well, f the largest that keeps both parts below 16.
-  // (The part that f leaves small adds less than the other to the scores by as
-  // much.)  The scale goes in with its mantissa, so that products become exponents
-  // of two by a power of two alone: p = 2^(S ct - ref) is then one fused step
-  // whose product is exact, at scores of any size.  A row with a NaN or an
-  // infinity keeps it.
-  u32x4 Q[KS];
-  float c;  // the power of two, but for the tile's
-  {
-    const uint16_t* q = a.q + ((size_t)min(row, a.m - 1) * H + h) * qw;
-    u32x2 x[2 * KS];
-    uint32_t top[2] = {0, 0};
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        // Four elements: of the expanded part in its order, of the shared key's in sequence.
-        constexpr int kParts = NP / 16;
-        const bool shared = s >= kParts;
-        const uint32_t e = shared ? 16 * (s - kParts) + 8 * half + 4 * j : 16 * s + 8 * j + 4 * half;
-        const bool in = live && e < (shared ? a.d.rope : nope);
-        x[2 * s + j] = in ? *(const u32x2*)(q + (shared ? nope : 0) + e) : u32x2{0, 0};
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          top[shared] = max(top[shared], x[2 * s + j][k] & 0x7FFF0000u);
-          top[shared] = max(top[shared], (x[2 * s + j][k] << 16) & 0x7FFF0000u);
-        }
-      }
-    int room[2];  // 2^room times the part stays below 16
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const auto o = __builtin_amdgcn_permlane32_swap(top[k], top[k], false, false);
-      room[k] = 130 - min(max((int)(max(o[0], o[1]) >> 23), 4), 252);
-    }
-    const int w = ilogbf(a.wmul[2 * h]), f = min(room[1], room[0] + w);
-    const float s0 = a.scale * kLog2e;
-    const int se = ilogbf(s0);
-    c = ldexpf(1.0f, se - f);
-    const float mul[2] = {ldexpf(s0, f - w - se), ldexpf(s0, f - se)};
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          Q[s][2 * j + k] = to_f16x2(__uint_as_float(x[2 * s + j][k] << 16) * mul[s >= NP / 16],
-                                     __uint_as_float(x[2 * s + j][k] & 0xFFFF0000u) * mul[s >= NP / 16]);
-  }
 
   const uint32_t tiles = (wg_limit + 31) / 32, stages = (tiles + L::kTiles - 1) / L::kTiles;
   const uint32_t all_tiles = a.padded / 32;
@@ -385,6 +340,62 @@ __global__ __launch_bounds__(64 * W, 2) void latent_prompt_kernel(LatentExpandAr
       from[i] += step[i];
     }
   };
+  issue(0);
+  if (stages > 1) issue(1);
+
+  // Queries, in the key operand's order: fp16 times 2^f, the expanded part divided
+  // by the weights' power as well, f the largest that keeps both parts below 16.
+  // (The part that f leaves small adds less than the other to the scores by as
+  // much.)  The scale goes in with its mantissa, so that products become exponents
+  // of two by a power of two alone: p = 2^(S ct - ref) is then one fused step
+  // whose product is exact, at scores of any size.  A row with a NaN or an
+  // infinity keeps it.
+  u32x4 Q[KS];
+  float c;  // the power of two, but for the tile's
+  {
+    const uint16_t* q = a.q + ((size_t)min(row, a.m - 1) * H + h) * qw;
+    u32x2 x[2 * KS];
+    uint32_t top[2] = {0, 0};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      // Eight elements in sequence; of the expanded part the lanes of a row exchange
+      // four, which leaves each with its order.
+      const bool shared = s >= NP / 16;
+      const uint32_t e = (shared ? 16 * (s - NP / 16) : 16 * s) + 8 * half;
+      const u32x4 y = live && e < (shared ? a.d.rope : nope) ? *(const u32x4*)(q + (shared ? nope : 0) + e) : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint32_t first = y[k], second = y[2 + k];
+        if (!shared) swap_halves(first, second);
+        x[2 * s][k] = first, x[2 * s + 1][k] = second;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          top[shared] = max(top[shared], x[2 * s + j][k] & 0x7FFF0000u);
+          top[shared] = max(top[shared], (x[2 * s + j][k] << 16) & 0x7FFF0000u);
+        }
+      }
+    }
+    int room[2];  // 2^room times the part stays below 16
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const auto o = __builtin_amdgcn_permlane32_swap(top[k], top[k], false, false);
+      room[k] = 130 - min(max((int)(max(o[0], o[1]) >> 23), 4), 252);
+    }
+    const int w = ilogbf(a.wmul[2 * h]), f = min(room[1], room[0] + w);
+    const float s0 = a.scale * kLog2e;
+    const int se = ilogbf(s0);
+    c = ldexpf(1.0f, se - f);
+    const float mul[2] = {ldexpf(s0, f - w - se), ldexpf(s0, f - se)};
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          Q[s][2 * j + k] = to_f16x2(__uint_as_float(x[2 * s + j][k] << 16) * mul[s >= NP / 16],
+                                     __uint_as_float(x[2 * s + j][k] & 0xFFFF0000u) * mul[s >= NP / 16]);
+  }
+
   // Scalar loads: a vector load's wait would wait for the copies before it too.
   const auto* powers = (const __attribute__((address_space(4))) float*)(uintptr_t)a.powers;
 
@@ -402,8 +413,6 @@ __global__ __launch_bounds__(64 * W, 2) void latent_prompt_kernel(LatentExpandAr
   static_assert(kOps % kAhead == 0 && L::kTiles == 2, "registers of the operands and scores by turn");
   u32x4 ring[kAhead];
   floatx16 S[2];
-  issue(0);
-  if (stages > 1) issue(1);
   if (stages > 1) latent_wait_vmcnt<L::kDma>();
   else latent_wait_vmcnt<0>();
   lds_barrier();
@@ -488,20 +497,28 @@ __global__ __launch_bounds__(64 * W, 2) void latent_prompt_kernel(LatentExpandAr
 
   l = halves_sum(l);
   const float r = 1.0f / (a.wmul[2 * h + 1] * l);
-  if (!live) return;
   uint16_t* o = a.o + ((size_t)row * H + h) * a.d.v;
+  // Lanes l and l ^ 32 hold alternating fours of a row's elements; they exchange
+  // theirs, so that each stores eight in sequence.
 #pragma unroll
   for (int n = 0; n < VB; ++n)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const uint32_t e = 32 * n + 8 * g + 4 * half;
-      const u32x2 v = {to_bf16x2(O[n][4 * g] * r, O[n][4 * g + 1] * r), to_bf16x2(O[n][4 * g + 2] * r, O[n][4 * g + 3] * r)};
-      if (e >= a.d.v) continue;
-      if (a.out8) {
-        *(u32x2*)(o + e) = v;
+    for (int g = 0; g < 4; g += 2) {
+      const uint32_t e = 32 * n + 8 * g + 8 * half;
+      u32x4 v;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint32_t first = to_bf16x2(O[n][4 * g + 2 * k] * r, O[n][4 * g + 2 * k + 1] * r);
+        uint32_t second = to_bf16x2(O[n][4 * g + 4 + 2 * k] * r, O[n][4 * g + 5 + 2 * k] * r);
+        swap_halves(first, second);
+        v[k] = first, v[2 + k] = second;
+      }
+      if (!live || e >= a.d.v) continue;
+      if (a.out16) {
+        *(u32x4*)(o + e) = v;
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[e + i] = (uint16_t)(v[i / 2] >> (16 * (i % 2)));
+        for (int i = 0; i < 8; ++i) o[e + i] = (uint16_t)(v[i / 2] >> (16 * (i % 2)));
       }
     }
 }
@@ -512,8 +529,14 @@ __global__ __launch_bounds__(64 * W, 2) void latent_prompt_kernel(LatentExpandAr
 template <int NP, int VP>
 hipError_t prompt(const LatentExpandArgs& a, uint32_t cu_count, hipStream_t st) {
   const uint32_t small = (a.m + 127) / 128 * a.heads;
-  if (a.m > 128 && small <= cu_count) hipLaunchKernelGGL((latent_prompt_kernel<NP, VP, 4>), dim3(small), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((latent_prompt_kernel<NP, VP, 8>), dim3((a.m + 255) / 256 * a.heads), dim3(512), 0, st, a);
+  if (a.m > 128 && small <= cu_count) {
+    hipLaunchKernelGGL((latent_prompt_kernel<NP, VP, 4>), dim3(small), dim3(256), 0, st, a);
+  } else {
+    const uint32_t large = (a.m + 255) / 256 * a.heads;
+    LatentExpandArgs b = a;
+    b.paired = large <= cu_count;
+    hipLaunchKernelGGL((latent_prompt_kernel<NP, VP, 8>), dim3(large), dim3(512), 0, st, b);
+  }
   return hipGetLastError();
 }
 

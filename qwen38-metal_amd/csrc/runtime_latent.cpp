@@ -376,7 +376,7 @@ qm_status plan_expanded(qm_runtime* rt, const qm_latent_weights* w, const qm_lat
   a.start = seq->length;
   a.tokens = seq->length + M;
   a.padded = (a.tokens + kLatentExpandTokens - 1) / kLatentExpandTokens * kLatentExpandTokens;
-  a.out8 = aligned(o, 8);
+  a.out16 = aligned(o, 16);
   const uint64_t P = a.padded;
   const uint64_t latents = P * d.rank_pad * 2, keys = P * kLatentRope * 2, factors = P * 4, powers = P / 32 * 8;
   const uint64_t k_head = P * d.nope_pad * 2, v_head = P * d.v_pad * 2;
