@@ -280,10 +280,11 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(LatentExpandArgs 
 // moved, the sums rescaled and the tile weighed again.
 //
 // Bound by the matrix cores and the vector unit together (640 and 480 cycles a wave
-// and tile, two waves a SIMD): 2048 rows of 128 heads on 4096 tokens take 885 us,
+// and tile, two waves a SIMD): 2048 rows of 128 heads on 4096 tokens take 872 us,
 // 57% of the matrix cores' cycles at the clock it runs at.  The next tile's key
 // products go between the exponentials; with each phase by itself, and a maximum
-// for every tile: 945.
+// for every tile: 945.  1024 rows of 64 heads take 38 us, 6 of them until the queries
+// (25 MB, all at once) are there.
 template <int NP, int VP, int W>
 struct PromptLds {
   static constexpr int kKSteps = NP / 16 + 4, kVBlocks = VP / 32;
@@ -525,7 +526,11 @@ __global__ __launch_bounds__(64 * W, 2) void latent_prompt_kernel(LatentExpandAr
 
 // Eight waves a workgroup share the tiles' way through LDS; four where that gives
 // more workgroups and each still a CU to itself (512 rows of 16 heads on 60000
-// tokens: 1100 us, with eight waves 1490; 1024 rows of 64 heads: 46 with eight).
+// tokens: 1100 us, with eight waves 1490; 2048 rows of 128 heads on 4096: 1130 with
+// four, 901 with eight).  Where one round holds all workgroups of eight, the longest
+// would be walked by 256 rows while others' CUs idle: each takes 128 rows from the
+// prompt's end and 128 from its start (1024 rows of 64 heads 46 -> 41 us).  In
+// several rounds the blocks go longest first.
 template <int NP, int VP>
 hipError_t prompt(const LatentExpandArgs& a, uint32_t cu_count, hipStream_t st) {
   const uint32_t small = (a.m + 127) / 128 * a.heads;
