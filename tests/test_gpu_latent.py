@@ -332,9 +332,11 @@ def test_prefill_sizes(rt, H, cached, rows):
     check_prefill(rt, WIDE, H, cached, rows, H + rows)
 
 
-# Workgroups of eight waves (300 rows of 130 heads, 520 of 66) and of four; rows end inside a wave, a workgroup and a tile.
+# Workgroups of eight waves, of one end (300 rows of 130 heads) or both ends of the
+# prompt (520 of 66, whose middle has one, 250 of 130), and of four; rows end inside a
+# wave, a workgroup and a tile.
 @pytest.mark.parametrize("widths", [WIDE, SMALL, (128, 64, 64, 128), (128, 64, 128, 64)])
-@pytest.mark.parametrize("H,cached,rows", [(130, 20, 300), (66, 1, 520), (20, 333, 300), (1, 0, 1025)])
+@pytest.mark.parametrize("H,cached,rows", [(130, 20, 300), (66, 1, 520), (130, 7, 250), (20, 333, 300), (1, 0, 1025)])
 def test_prefill_workgroups(torch_dev, widths, H, cached, rows):
     with tuned(QM38_LATENT_FORM=2) as rt:
         check_prefill(rt, widths, H, cached, rows, H + rows)
