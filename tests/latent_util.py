@@ -61,7 +61,7 @@ def attention(q, latent, key, kv_b, nope, scale, start):
     p = torch.softmax(torch.where(seen, score, -math.inf), -1)
     o = p @ v
     # Errors, each rounding at its largest.  Scores: the expanded form rounds its
-    # keys to bf16; the absorbed one the queries in the latent space to 1 / 65024
+    # keys (to fp16; half a step of bf16 is allowed); the absorbed one the queries in the latent space to 1 / 65024
     # of their largest element (and the rotated part likewise).
     absorbed = q[..., :nope] @ w[:, :nope]
     a = (q[..., :nope].abs() @ k.abs().transpose(1, 2)) * HALF
