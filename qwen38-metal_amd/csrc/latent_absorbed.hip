@@ -34,7 +34,8 @@ constexpr float kNoMax = -1e30f;  // running maximum before the first visible to
 // times the row's largest element, so qa is rounded to about 2^-15 of that,
 // where bf16 would round each element to 2^-8), which lets the row be cut over
 // workgroups; for the rotated part it is its largest element.  A row with a NaN
-// or an infinity gets a NaN scale, which its scores keep.
+// or an infinity gets a NaN scale, which its scores keep; so does every row of a
+// head whose W_uk holds one (its norm is no finite number).
 //
 // Workgroup = (16 rows, head, 128 latent elements), a wave 32 of them: D = W
 // (rows) x queries (columns), so a lane holds four consecutive elements of a
@@ -85,7 +86,8 @@ __global__ __launch_bounds__(256) void latent_query_kernel(LatentAttnArgs a, uin
     for (int k = 0; k < 4; ++k) top = max(top, max(x[s][k] & 0x7FFF0000u, (x[s][k] << 16) & 0x7FFF0000u));
   top = max(top, (uint32_t)__shfl_xor((int)top, 16));
   top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-  const bool bad = top >= 0x7F800000u;
+  const float wnorm = a.wnorm[h];
+  const bool bad = top >= 0x7F800000u || !(wnorm <= FLT_MAX);  // (fmaxf below would drop a NaN)
   const uint32_t e = min(max(top & 0x7F800000u, 0x01000000u), 0x7E000000u);
   const float down_scale = __uint_as_float(0x7F000000u - e);
   float ss = 0.0f;
@@ -99,7 +101,7 @@ __global__ __launch_bounds__(256) void latent_query_kernel(LatentAttnArgs a, uin
     }
   ss += __shfl_xor(ss, 16);
   ss += __shfl_xor(ss, 32);
-  const float qs = fmaxf(sqrtf(ss) * a.wnorm[h] / 32512.0f * __uint_as_float(e), FLT_MIN);
+  const float qs = fmaxf(sqrtf(ss) * wnorm / 32512.0f * __uint_as_float(e), FLT_MIN);
 
   floatx4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll

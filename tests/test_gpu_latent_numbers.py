@@ -1,0 +1,50 @@
+"""GPU tests of latent attention on weights and rows at the ends of their types:
+numbers that are none, and scales far from one."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import qm38
+from gpu_util import tuned
+from test_gpu_latent import FORMS, SMALL, bf16, generator
+
+pytestmark = pytest.mark.gpu
+
+
+def outputs(rt, widths, kv_b, q, kv, decode):
+    """All rows as a prompt, or the last one decoded behind the others."""
+    rank, rope, nope, v = widths
+    rows, H = q.shape[:2]
+    weights = rt.create_latent_weights(qm38.LatentConfig(H, rank, nope, rope, v, (nope + rope) ** -0.5), kv_b)
+    cache = rt.create_latent_kv(rank, rope)
+    o = torch.zeros(rows, H, v, dtype=torch.bfloat16, device="cuda:0")
+    if decode:
+        cache.append(kv, None, 0.0, rows - 1)
+        rt.latent_attention(weights, [cache], q[rows - 1:].clone(), kv[rows - 1:].clone(), None, 0.0, o[rows - 1:])
+        o = o[rows - 1:]
+    else:
+        rt.latent_attention_prefill(weights, cache, q, kv, None, 0.0, rows, o)
+    torch.cuda.synchronize()
+    weights.close()
+    cache.close()
+    return o
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("form", [*FORMS, "decode"])
+def test_key_weights_that_are_none(torch_dev, form, value):
+    """A NaN or an infinity among a head's W_uk is in every score of that head, and
+    in nothing of the others."""
+    rank, rope, nope, v = SMALL
+    g = generator(51)
+    H, rows = 5, 40
+    kv_b = bf16(g, H, nope + v, rank, std=rank ** -0.5)
+    q, kv = bf16(g, rows, H, nope + rope), bf16(g, rows, rank + rope)
+    worse = kv_b.clone()
+    worse[3, 7, 200] = value
+    with tuned(**FORMS.get(form, {})) as rt:
+        o, clean = (outputs(rt, SMALL, w, q, kv, form == "decode") for w in (worse, kv_b))
+    assert torch.isnan(o[:, 3]).all()
+    others = [0, 1, 2, 4]
+    assert torch.isfinite(clean).all() and torch.equal(o[:, others], clean[:, others])
