@@ -78,20 +78,31 @@ __global__ __launch_bounds__(256) void latent_weights_kernel(LatentDims d, From 
   if (key) down[((size_t)h * d.rank_pad + r) * d.nope_pad + n] = v;
 }
 
-// One workgroup per head.  A norm that is no number stays one (compared as bits).
+// One workgroup per head.  A row's squares are summed relative to its largest
+// element's power of two, so that weights of any size keep their norm; one that
+// passes fp32, or is no number, stays so (compared as bits).
 __global__ __launch_bounds__(256) void latent_wnorm_kernel(LatentDims d, const uint16_t* down, float* wnorm) {
   __shared__ uint32_t top[256];
   const uint16_t* w = down + (size_t)blockIdx.x * d.rank_pad * d.nope_pad;
   uint32_t best = 0;
   for (uint32_t r = threadIdx.x; r < d.rank_pad; r += 256) {
+    const uint16_t* row = w + (size_t)r * d.nope_pad;
+    uint32_t most = 0;
+    for (uint32_t k = 0; k < d.nope_pad; k += 8) {
+      float x[8];
+      latent_unpack8(*(const u32x4*)(row + k), x);
+      most = max(most, latent_top(x));
+    }
+    const uint32_t e = min(max(most & 0x7F800000u, 0x01000000u), 0x7E000000u);
+    const float scale = __uint_as_float(0x7F000000u - e);
     float s = 0.0f;
     for (uint32_t k = 0; k < d.nope_pad; k += 8) {
       float x[8];
-      latent_unpack8(*(const u32x4*)(w + (size_t)r * d.nope_pad + k), x);
+      latent_unpack8(*(const u32x4*)(row + k), x);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s = fmaf(x[i], x[i], s);
+      for (int i = 0; i < 8; ++i) s = fmaf(x[i] * scale, x[i] * scale, s);
     }
-    best = max(best, __float_as_uint(s) & 0x7FFFFFFFu);
+    best = max(best, __float_as_uint(sqrtf(s) * __uint_as_float(e)) & 0x7FFFFFFFu);
   }
   top[threadIdx.x] = best;
   __syncthreads();
@@ -99,7 +110,7 @@ __global__ __launch_bounds__(256) void latent_wnorm_kernel(LatentDims d, const u
     if (threadIdx.x < n) top[threadIdx.x] = max(top[threadIdx.x], top[threadIdx.x + n]);
     __syncthreads();
   }
-  if (threadIdx.x == 0) wnorm[blockIdx.x] = sqrtf(__uint_as_float(top[0])) * 1.0001f;
+  if (threadIdx.x == 0) wnorm[blockIdx.x] = __uint_as_float(top[0]) * 1.0001f;
 }
 
 template <class From>

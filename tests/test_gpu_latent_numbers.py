@@ -48,3 +48,21 @@ def test_key_weights_that_are_none(torch_dev, form, value):
     assert torch.isnan(o[:, 3]).all()
     others = [0, 1, 2, 4]
     assert torch.isfinite(clean).all() and torch.equal(o[:, others], clean[:, others])
+
+
+@pytest.mark.parametrize("power", [-80, -60, 64, 80])
+@pytest.mark.parametrize("form", [*FORMS, "decode"])
+def test_key_weights_of_any_size(torch_dev, form, power):
+    """W_uk times 2^power and queries times 2^-power have the same scores, formed
+    by the same steps: no bit of the outputs differs."""
+    rank, rope, nope, v = SMALL
+    g = generator(52)
+    H, rows = 5, 40
+    kv_b = bf16(g, H, nope + v, rank, std=rank ** -0.5)
+    q, kv = bf16(g, rows, H, nope + rope), bf16(g, rows, rank + rope)
+    scaled, scaled_q = kv_b.clone(), q.clone()
+    scaled[:, :nope] *= 2.0 ** power
+    scaled_q[..., :nope] *= 2.0 ** -power
+    with tuned(**FORMS.get(form, {})) as rt:
+        o, plain = (outputs(rt, SMALL, w, x, kv, form == "decode") for w, x in ((scaled, scaled_q), (kv_b, q)))
+    assert torch.isfinite(plain).all() and torch.equal(o, plain)
