@@ -35,7 +35,8 @@ constexpr float kNoMax = -1e30f;
 // Weights
 // ---------------------------------------------------------------------------
 // wmul[h] = {W_uk's power of two, W_uv's}: 127 * (largest row sum of |W|) * wmul
-// in (2^14, 2^15].
+// in [2^14, 2^15).  Rows with a number that is none have no say: what they give is
+// none at any power, and the head's other values keep their bits.
 __global__ __launch_bounds__(256) void latent_wmul_kernel(LatentDims d, const uint16_t* up, float* wmul) {
   __shared__ float top[2][4];
   const uint32_t h = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rows = d.nope_pad + d.v_pad;
@@ -49,7 +50,7 @@ __global__ __launch_bounds__(256) void latent_wmul_kernel(LatentDims d, const ui
     for (int k = 0; k < 4; ++k) s += fabsf(bf16_to_f32(x[k] & 0xFFFFu)) + fabsf(__uint_as_float(x[k] & 0xFFFF0000u));
     s = wave_allsum(s);
     const int part = n >= d.nope_pad;
-    best[part] = fmaxf(best[part], s);
+    best[part] = fmaxf(best[part], s <= FLT_MAX ? s : 0.0f);
   }
   if (lane == 0) top[0][wave] = best[0], top[1][wave] = best[1];
   __syncthreads();
@@ -57,7 +58,7 @@ __global__ __launch_bounds__(256) void latent_wmul_kernel(LatentDims d, const ui
     float s = 0.0f;
     for (int w = 0; w < 4; ++w) s = fmaxf(s, top[threadIdx.x][w]);
     int e = 0;
-    // Rows of nothing, or of what is no number: any power will do.
+    // (Rows of nothing: any power will do.)
     if (s > 0.0f && s <= FLT_MAX / 127.0f) e = 14 - ilogbf(s * 127.0f);
     wmul[2 * h + threadIdx.x] = ldexpf(1.0f, std::min(std::max(e, -120), 120));
   }

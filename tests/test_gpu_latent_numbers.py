@@ -66,3 +66,27 @@ def test_key_weights_of_any_size(torch_dev, form, power):
     with tuned(**FORMS.get(form, {})) as rt:
         o, plain = (outputs(rt, SMALL, w, x, kv, form == "decode") for w, x in ((scaled, scaled_q), (kv_b, q)))
     assert torch.isfinite(plain).all() and torch.equal(o, plain)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("power", [-20, 0, 12])
+@pytest.mark.parametrize("form", [*FORMS, "decode"])
+def test_value_weights_that_are_none(torch_dev, form, power, value):
+    """A NaN or an infinity in a row of W_uv is in that element of the head's outputs;
+    the others, at weights of any size, keep every bit."""
+    rank, rope, nope, v = SMALL
+    g = generator(53)
+    H, rows = 5, 40
+    kv_b = bf16(g, H, nope + v, rank, std=rank ** -0.5)
+    kv_b[:, nope:] *= 2.0 ** power
+    q, kv = bf16(g, rows, H, nope + rope), bf16(g, rows, rank + rope)
+    # Not the row that is the head's largest, which the finite ones would lose too.
+    element = int(kv_b[3, nope:].double().abs().sum(1).argmin())
+    worse = kv_b.clone()
+    worse[3, nope + element, 200] = value
+    with tuned(**FORMS.get(form, {})) as rt:
+        o, clean = (outputs(rt, SMALL, w, q, kv, form == "decode") for w in (worse, kv_b))
+    assert torch.isfinite(clean).all()
+    assert not torch.isfinite(o[:, 3, element]).any()
+    o[:, 3, element] = clean[:, 3, element]
+    assert torch.equal(o, clean)
