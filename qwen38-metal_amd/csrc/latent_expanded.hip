@@ -35,8 +35,9 @@ constexpr float kNoMax = -1e30f;
 // Weights
 // ---------------------------------------------------------------------------
 // wmul[h] = {W_uk's power of two, W_uv's}: 127 * (largest row sum of |W|) * wmul
-// in [2^14, 2^15).  Rows with a number that is none have no say: what they give is
-// none at any power, and the head's other values keep their bits.
+// in [2^14, 2^15), or up to a quarter of that where the sum times 127 would pass fp32.  Rows with
+// a number that is none have no say: what they give is none at any power, and the
+// head's other values keep their bits.
 __global__ __launch_bounds__(256) void latent_wmul_kernel(LatentDims d, const uint16_t* up, float* wmul) {
   __shared__ float top[2][4];
   const uint32_t h = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rows = d.nope_pad + d.v_pad;
@@ -59,7 +60,7 @@ __global__ __launch_bounds__(256) void latent_wmul_kernel(LatentDims d, const ui
     for (int w = 0; w < 4; ++w) s = fmaxf(s, top[threadIdx.x][w]);
     int e = 0;
     // (Rows of nothing: any power will do.)
-    if (s > 0.0f && s <= FLT_MAX / 127.0f) e = 14 - ilogbf(s * 127.0f);
+    if (s > 0.0f) e = s <= FLT_MAX / 127.0f ? 14 - ilogbf(s * 127.0f) : 7 - ilogbf(s);
     wmul[2 * h + threadIdx.x] = ldexpf(1.0f, std::min(std::max(e, -120), 120));
   }
 }

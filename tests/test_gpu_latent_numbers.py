@@ -90,3 +90,27 @@ def test_value_weights_that_are_none(torch_dev, form, power, value):
     assert not torch.isfinite(o[:, 3, element]).any()
     o[:, 3, element] = clean[:, 3, element]
     assert torch.equal(o, clean)
+
+
+@pytest.mark.parametrize("form", [*FORMS, "decode"])
+def test_weights_near_the_largest(torch_dev, form):
+    """Weights whose row sums times 127 pass fp32, with cached tokens and queries as
+    far below one: what weights near one give, times a power of two."""
+    rank, rope, nope, v = SMALL
+    g = generator(54)
+    H, rows = 5, 40
+    kv_b = bf16(g, H, nope + v, rank, std=rank ** -0.5)
+    q, kv = bf16(g, rows, H, nope + rope), bf16(g, rows, rank + rope)
+    scaled, scaled_q, scaled_kv = kv_b * 2.0 ** 118, q.clone(), kv * 2.0 ** -60
+    assert float(scaled.double().abs().sum(2).amin()) * 127 > torch.finfo(torch.float32).max
+    scaled_q[..., :nope] *= 2.0 ** -58  # W_uk 2^118, latents 2^-60
+    scaled_q[..., nope:] *= 2.0 ** 60   # keys 2^-60
+    with tuned(**FORMS.get(form, {})) as rt:
+        o = outputs(rt, SMALL, scaled, scaled_q, scaled_kv, form == "decode").double() * 2.0 ** -58
+        plain = outputs(rt, SMALL, kv_b, q, kv, form == "decode").double()
+    # The same but for the powers under which fp16 holds P and the expanded keys and
+    # values, which need not be the same: 2^-11 in each of P and V, of sum p |v|, and
+    # about as much of the scores; at most 40 tokens make that sqrt(40) of |o|.  Then
+    # two roundings to bf16 of 2^-8: 4 * 6.4 * 2^-11 + 2^-7 < 2^-5.5.
+    assert torch.isfinite(plain).all()
+    assert ((o - plain).norm(dim=-1) <= 2.0 ** -5.5 * plain.norm(dim=-1)).all()
