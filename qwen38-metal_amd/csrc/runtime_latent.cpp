@@ -334,14 +334,30 @@ qm_status absorbed_workspaces(qm_runtime* rt, LatentAttnArgs* a) {
   return QM_OK;
 }
 
+// Tokens of the expanded form's workspaces.
+uint64_t expanded_tokens(uint64_t T) { return (T + kLatentExpandTokens - 1) / kLatentExpandTokens * kLatentExpandTokens; }
+
+// Heads whose keys and values are formed and attended over at a time: what the
+// workspace holds.
+uint32_t heads_of_a_pass(const qm_runtime* rt, const LatentDims& d, uint64_t T) {
+  const uint64_t budget = (uint64_t)(rt->tune.latent_mb > 0 ? rt->tune.latent_mb : 1024) << 20;
+  const uint64_t head = expanded_tokens(T) * (d.nope_pad + d.v_pad) * 2;
+  return (uint32_t)std::min<uint64_t>(d.heads, std::max<uint64_t>(1, budget / head));
+}
+
 // Which form a prefill of M rows over T tokens takes, by what each was measured to
-// cost in us (16 and 128 heads, 2 to 512 rows on 0 to 60000 tokens, ranks 384 and
-// 512; the two lie within a tenth where the sums cross):
+// cost in us:
 //   absorbed  20, 0.006 a column of rank 512 (queries in, sums out), and 0.46
 //             multiplications a fs;
-//   expanded  26, forming keys and values at 0.44 a fs, and 0.6 a 32-token tile of
-//             a workgroup's walk, which stays however few rows or workgroups there
-//             are (1.0 a round where 128 rows of a head are not a CU's alone).
+//   expanded  26, forming keys and values at 0.44 a fs, and for each pass of heads
+//             0.6 a 32-token tile of a workgroup's walk, which stays however few
+//             rows or workgroups there are (1.0 a round where 128 rows of a head are
+//             not a CU's alone).
+// Over 4 to 2048 rows of 8 to 128 heads on 0 to 262144 tokens, at four sets of widths
+// of ranks 256 to 512 (631 cases), the form taken was the faster one or within 22 %
+// of it, within 10 % in all but 7.  With one walk for all passes, as if every head
+// were resident: 256 rows of 128 heads on 131072 tokens 29.0 ms expanded instead of
+// 10.0 absorbed, on 262144 up to 6.7 times the absorbed form's time.
 bool prefers_expanded(const qm_runtime* rt, const LatentDims& d, uint32_t M, uint64_t T) {
   if (T > 1u << 28) return false;  // its launches' threads
   if (rt->tune.latent_form) return rt->tune.latent_form == 2;
@@ -349,10 +365,15 @@ bool prefers_expanded(const qm_runtime* rt, const LatentDims& d, uint32_t M, uin
   const double pairs = (double)M * ((double)T - 0.5 * M) * d.heads;
   const double cols = (double)M * d.heads;
   const double absorbed = 20.0 + cols * d.rank_pad * (0.006 / 512) + pairs * (2.0 * d.rank_pad + kLatentRope) / 0.46e9;
-  const bool alone = std::ceil(M / 128.0) * d.heads <= rt->cu_count;
-  const double walk = alone ? 0.6 : std::max(1.0, std::ceil(M / 256.0) * d.heads / rt->cu_count);
+  const uint32_t most = heads_of_a_pass(rt, d, T);
+  double walks = 0.0;  // a tile's cost in every pass
+  for (uint32_t h0 = 0; h0 < d.heads; h0 += most) {
+    const uint32_t heads = std::min(most, d.heads - h0);
+    const bool alone = std::ceil(M / 128.0) * heads <= rt->cu_count;
+    walks += alone ? 0.6 : std::max(1.0, std::ceil(M / 256.0) * heads / rt->cu_count);
+  }
   const double expanded = 26.0 + (double)T * d.rank_pad * (d.nope_pad + d.v_pad) * d.heads / 0.44e9 +
-                          walk * ((double)T - 0.5 * M) / 32;
+                          walks * ((double)T - 0.5 * M) / 32;
   return expanded < absorbed;
 }
 
@@ -375,13 +396,12 @@ qm_status plan_expanded(qm_runtime* rt, const qm_latent_weights* w, const qm_lat
   a.m = M;
   a.start = seq->length;
   a.tokens = seq->length + M;
-  a.padded = (a.tokens + kLatentExpandTokens - 1) / kLatentExpandTokens * kLatentExpandTokens;
+  a.padded = (uint32_t)expanded_tokens(a.tokens);
   a.out16 = aligned(o, 16);
   const uint64_t P = a.padded;
   const uint64_t latents = P * d.rank_pad * 2, keys = P * kLatentRope * 2, factors = P * 4, powers = P / 32 * 8;
   const uint64_t k_head = P * d.nope_pad * 2, v_head = P * d.v_pad * 2;
-  const uint64_t budget = (uint64_t)(rt->tune.latent_mb > 0 ? rt->tune.latent_mb : 1024) << 20;
-  p->heads_at_once = (uint32_t)std::min<uint64_t>(d.heads, std::max<uint64_t>(1, budget / (k_head + v_head)));
+  p->heads_at_once = heads_of_a_pass(rt, d, a.tokens);
   const uint64_t n = p->heads_at_once;
   qm_status st = ensure_scratch(rt, latents + keys + 2 * factors + powers + n * (k_head + v_head));
   if (st != QM_OK) return st;
