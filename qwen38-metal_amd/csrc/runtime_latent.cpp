@@ -318,14 +318,27 @@ void plan_absorbed(const qm_runtime* rt, LatentAttnArgs* a) {
   a->blocks = block;
 }
 
+// Grows one of the runtime's workspaces to the next power of two of `bytes` (as the
+// caches grow), or to `bytes` where that cannot be had.  Growing synchronises and
+// allocates, and what a call needs rises with its tokens: sized exactly, every chunk
+// of a prompt would pay for it (16 chunks of 512 rows of 64 heads on a new runtime
+// took 9.0 ms, 4.7 with this).
+qm_status ensure_growing(qm_runtime* rt, qm_status (*ensure)(qm_runtime*, size_t), size_t held, size_t bytes) {
+  size_t want = 1;
+  while (want < bytes) want <<= 1;
+  if (held < bytes && ensure(rt, want) == QM_OK) return QM_OK;
+  return ensure(rt, bytes);
+}
+
 // The workspaces of a planned call, set up in `a`.
 qm_status absorbed_workspaces(qm_runtime* rt, LatentAttnArgs* a) {
   const LatentDims& d = a->d;
   const size_t digits = a->blocks * latent_digit_bytes(d.rank_pad), scales = (size_t)a->blocks * kLatentCols * 8;
   const size_t mixed = (size_t)a->rows * d.heads * d.rank_pad * 4;
-  qm_status st = ensure_scratch(rt, digits + scales + mixed);
+  const size_t partials = (size_t)a->units * a->group_cols * (d.rank_pad + 2) * sizeof(float);
+  qm_status st = ensure_growing(rt, ensure_scratch, rt->scratch_bytes, digits + scales + mixed);
   if (st != QM_OK) return st;
-  if ((st = ensure_partials(rt, (size_t)a->units * a->group_cols * (d.rank_pad + 2) * sizeof(float))) != QM_OK) return st;
+  if ((st = ensure_growing(rt, ensure_partials, rt->partial_bytes, partials)) != QM_OK) return st;
   uint8_t* p = (uint8_t*)rt->scratch;
   a->digits = p;
   a->qscale = (float*)(p + digits);
@@ -403,7 +416,8 @@ qm_status plan_expanded(qm_runtime* rt, const qm_latent_weights* w, const qm_lat
   const uint64_t k_head = P * d.nope_pad * 2, v_head = P * d.v_pad * 2;
   p->heads_at_once = heads_of_a_pass(rt, d, a.tokens);
   const uint64_t n = p->heads_at_once;
-  qm_status st = ensure_scratch(rt, latents + keys + 2 * factors + powers + n * (k_head + v_head));
+  qm_status st = ensure_growing(rt, ensure_scratch, rt->scratch_bytes,
+                                latents + keys + 2 * factors + powers + n * (k_head + v_head));
   if (st != QM_OK) return st;
   uint8_t* at = (uint8_t*)rt->scratch;
   auto take = [&](uint64_t bytes) { uint8_t* r = at; at += bytes; return r; };
