@@ -89,7 +89,10 @@ void qm_runtime_destroy(qm_runtime* rt);
  * the null stream).  The stream must belong to the runtime's device.  Calls on
  * different streams overlap, except that a call which uses the runtime's
  * workspaces (split sums, converted activations, intermediate rows) waits on
- * the device for what was enqueued on the stream left before it. */
+ * the device for what was enqueued on the stream left before it.  A captured
+ * call's graph uses the workspaces of its capture on every replay, which the
+ * caller orders; they stay until the runtime is destroyed, also where later
+ * calls need larger ones. */
 qm_status qm_runtime_set_stream(qm_runtime* rt, void* hip_stream);
 /* Blocks until all work enqueued by `rt` has finished; surfaces asynchronous
  * kernel failures as QM_ERR_COMMAND_FAILED (the reference checks

@@ -63,6 +63,22 @@ static qm_status capture_guard(qm_runtime* rt, const char* what) {
   return QM_OK;
 }
 
+// A call uses a workspace that is there: one that is being captured keeps its address.
+static qm_status use_buffer(qm_runtime* rt, size_t bytes, bool* kept) {
+  if (bytes && !*kept && rt->device >= 0 && qm::stream_capturing(rt->stream)) *kept = true;
+  return QM_OK;
+}
+
+// Gives up a workspace that is to be replaced.
+static void replace_buffer(qm_runtime* rt, void* p, bool* kept) {
+  if (!*kept) {
+    (void)hipFree(p);
+    return;
+  }
+  *kept = false;
+  if (qm_retired_buffer* r = new (std::nothrow) qm_retired_buffer{p, rt->retired}) rt->retired = r;
+}
+
 qm_status qm::order_workspaces(qm_runtime* rt) {
   if (rt->ws_used && !rt->ws_wait && !rt->ws_sync) return QM_OK;
   // A captured use runs when its graph does; the caller orders that.
@@ -103,14 +119,14 @@ static void leave_stream(qm_runtime* rt) {
 qm_status qm::ensure_scratch(qm_runtime* rt, size_t bytes) {
   if (bytes)
     if (qm_status st_ord = order_workspaces(rt); st_ord != QM_OK) return st_ord;
-  if (rt->scratch_bytes >= bytes) return QM_OK;
+  if (rt->scratch_bytes >= bytes) return use_buffer(rt, bytes, &rt->scratch_kept);
   if (rt->device < 0) return no_device();
   if (qm_status st_cap = capture_guard(rt, "ensure_scratch"); st_cap != QM_OK) return st_cap;
   if (rt->scratch) {
     // Work already enqueued may still use the old buffer.
     hipError_t e = hipStreamSynchronize(rt->stream);
     if (e != hipSuccess) return hip_check(e, "scratch resize sync");
-    (void)hipFree(rt->scratch);
+    replace_buffer(rt, rt->scratch, &rt->scratch_kept);
     rt->scratch = nullptr;
     rt->scratch_bytes = 0;
   }
@@ -125,13 +141,13 @@ qm_status qm::ensure_scratch(qm_runtime* rt, size_t bytes) {
 qm_status qm::ensure_partials(qm_runtime* rt, size_t bytes) {
   if (bytes)
     if (qm_status st_ord = order_workspaces(rt); st_ord != QM_OK) return st_ord;
-  if (rt->partial_bytes >= bytes) return QM_OK;
+  if (rt->partial_bytes >= bytes) return use_buffer(rt, bytes, &rt->partials_kept);
   if (rt->device < 0) return no_device();
   if (qm_status st_cap = capture_guard(rt, "ensure_partials"); st_cap != QM_OK) return st_cap;
   if (rt->partials) {
     hipError_t e = hipStreamSynchronize(rt->stream);
     if (e != hipSuccess) return hip_check(e, "partials resize sync");
-    (void)hipFree(rt->partials);
+    replace_buffer(rt, rt->partials, &rt->partials_kept);
     rt->partials = nullptr;
     rt->partial_bytes = 0;
   }
@@ -146,13 +162,13 @@ qm_status qm::ensure_partials(qm_runtime* rt, size_t bytes) {
 qm_status qm::ensure_xh(qm_runtime* rt, size_t bytes) {
   if (bytes)
     if (qm_status st_ord = order_workspaces(rt); st_ord != QM_OK) return st_ord;
-  if (rt->xh_bytes >= bytes) return QM_OK;
+  if (rt->xh_bytes >= bytes) return use_buffer(rt, bytes, &rt->xh_kept);
   if (rt->device < 0) return no_device();
   if (qm_status st_cap = capture_guard(rt, "ensure_xh"); st_cap != QM_OK) return st_cap;
   if (rt->xh) {
     hipError_t e = hipStreamSynchronize(rt->stream);
     if (e != hipSuccess) return hip_check(e, "xh resize sync");
-    (void)hipFree(rt->xh);
+    replace_buffer(rt, rt->xh, &rt->xh_kept);
     rt->xh = nullptr;
     rt->xh_bytes = 0;
   }
@@ -166,13 +182,13 @@ qm_status qm::ensure_xh(qm_runtime* rt, size_t bytes) {
 qm_status qm::ensure_counters(qm_runtime* rt, size_t count) {
   if (count)
     if (qm_status st_ord = order_workspaces(rt); st_ord != QM_OK) return st_ord;
-  if (rt->counter_count >= count) return QM_OK;
+  if (rt->counter_count >= count) return use_buffer(rt, count, &rt->counters_kept);
   if (rt->device < 0) return no_device();
   if (qm_status st_cap = capture_guard(rt, "ensure_counters"); st_cap != QM_OK) return st_cap;
   if (rt->counters) {
     hipError_t e = hipStreamSynchronize(rt->stream);
     if (e != hipSuccess) return hip_check(e, "counters resize sync");
-    (void)hipFree(rt->counters);
+    replace_buffer(rt, rt->counters, &rt->counters_kept);
     rt->counters = nullptr;
     rt->counter_count = 0;
   }
@@ -239,7 +255,13 @@ void qm::release_buffers(qm_runtime* rt) {
   if (rt->partials) (void)hipFree(rt->partials);
   if (rt->xh) (void)hipFree(rt->xh);
   if (rt->keys) (void)hipFree(rt->keys);
+  while (qm_retired_buffer* r = rt->retired) {
+    rt->retired = r->next;
+    (void)hipFree(r->p);
+    delete r;
+  }
   rt->keys = nullptr;
+  rt->scratch_kept = rt->counters_kept = rt->partials_kept = rt->xh_kept = false;
   rt->scratch = rt->counters = nullptr;
   rt->partials = rt->xh = nullptr;
   rt->scratch_bytes = rt->counter_count = rt->partial_bytes = rt->xh_bytes = 0;

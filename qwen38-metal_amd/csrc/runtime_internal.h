@@ -5,6 +5,13 @@
 #include "../../include/qm38.h"
 #include "internal.h"
 
+// A workspace that a captured call uses, replaced by a larger one: the graph keeps its
+// address, so it is freed with the runtime.
+struct qm_retired_buffer {
+  void* p;
+  qm_retired_buffer* next;
+};
+
 struct qm_runtime {
   int device = 0;
   int cu_count = 256;
@@ -33,6 +40,9 @@ struct qm_runtime {
   // hold the MLP's h while h itself is converted).
   void* xh = nullptr;
   size_t xh_bytes = 0;
+  // Whether a captured call uses the current scratch, counters, partials, xh.
+  bool scratch_kept = false, counters_kept = false, partials_kept = false, xh_kept = false;
+  qm_retired_buffer* retired = nullptr;
   // Argmax keys of qm_q4_argmax (one uint64 per row of a 16-row chunk); zero
   // between calls, like the counters.
   unsigned long long* keys = nullptr;

@@ -41,12 +41,12 @@ qm_status validate_job(const qm_q4_job* job, uint32_t in_elems, const char* name
 // device-pointer form of validate_mapped_q4_affine_shape's buffer checks
 // (metal_runtime.rs:8868-8895).  A runtime without a device has no
 // allocations to resolve and skips it.
-qm_status check_range(const qm_runtime* rt, const void* p, uint64_t bytes, const char* what) {
-  if (rt->device < 0) return QM_OK;
-  // The lookup is not allowed while the stream is being captured (HIP treats
-  // it as touching the legacy stream); captured calls were checked when the
-  // capture's caller validated its jobs (qm_decode_graph_create does).
-  if (stream_capturing(rt->stream)) return QM_OK;
+// The lookup is not allowed while the stream is being captured (HIP treats
+// it as touching the legacy stream); captured calls were checked when the
+// capture's caller validated its jobs (qm_decode_graph_create does).
+bool ranges_known(const qm_runtime* rt) { return rt->device >= 0 && !stream_capturing(rt->stream); }
+
+qm_status in_range(const void* p, uint64_t bytes, const char* what) {
   hipDeviceptr_t base = nullptr;
   size_t size = 0;
   if (hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)p) != hipSuccess || !base) {
@@ -63,19 +63,24 @@ qm_status check_range(const qm_runtime* rt, const void* p, uint64_t bytes, const
   return QM_OK;
 }
 
+qm_status check_range(const qm_runtime* rt, const void* p, uint64_t bytes, const char* what) {
+  return ranges_known(rt) ? in_range(p, bytes, what) : QM_OK;
+}
+
 }  // namespace
 
 qm_status qm::q4_job_ranges(const qm_runtime* rt, const qm_q4_job& j, uint32_t in_elems, const char* name) {
+  if (!ranges_known(rt)) return QM_OK;
   char what[96];
   const uint64_t wbytes = (uint64_t)j.out_rows * (in_elems / 8) * 4;
   const uint64_t abytes = (uint64_t)j.out_rows * (in_elems / kGroup) * 2;
   qm_status st;
   snprintf(what, sizeof(what), "%s weights", name);
-  if ((st = check_range(rt, j.weights, wbytes, what)) != QM_OK) return st;
+  if ((st = in_range(j.weights, wbytes, what)) != QM_OK) return st;
   snprintf(what, sizeof(what), "%s scales", name);
-  if ((st = check_range(rt, j.scales, abytes, what)) != QM_OK) return st;
+  if ((st = in_range(j.scales, abytes, what)) != QM_OK) return st;
   snprintf(what, sizeof(what), "%s biases", name);
-  return check_range(rt, j.biases, abytes, what);
+  return in_range(j.biases, abytes, what);
 }
 
 namespace {
