@@ -114,3 +114,40 @@ def test_weights_near_the_largest(torch_dev, form):
     # two roundings to bf16 of 2^-8: 4 * 6.4 * 2^-11 + 2^-7 < 2^-5.5.
     assert torch.isfinite(plain).all()
     assert ((o - plain).norm(dim=-1) <= 2.0 ** -5.5 * plain.norm(dim=-1)).all()
+
+
+def test_rows_that_are_none_in_a_batch(rt):
+    """Of a batch, the sequences that hold a NaN or an infinity, cached or new, are none
+    in every head, a head whose query does in itself alone; the others keep every bit."""
+    rank, rope, nope, v = SMALL
+    g = generator(55)
+    H, cached = 40, 70
+    lengths = [cached] * 6
+    kv_b = bf16(g, H, nope + v, rank, std=rank ** -0.5)
+    weights = rt.create_latent_weights(qm38.LatentConfig(H, rank, nope, rope, v, (nope + rope) ** -0.5), kv_b)
+    old, q, kv = bf16(g, cached, rank + rope), bf16(g, 6, H, nope + rope), bf16(g, 6, rank + rope)
+    bad_old, bad_q, bad_kv = old.clone(), q.clone(), kv.clone()
+    bad_old[31, 5] = float("nan")           # sequence 0: a latent among its tokens,
+    bad_old[64, rank + 1] = float("inf")    # and a key
+    bad_kv[2, 100] = -float("inf")          # sequence 2: its new latent
+    bad_kv[3, rank + 7] = float("nan")      # sequence 3: its new key
+    bad_q[4, 33, 9] = float("nan")
+    bad_q[5, 2, nope + 1] = float("inf")
+    outs = []
+    for first, x, rows in ((old, q, kv), (bad_old, bad_q, bad_kv)):
+        caches = [rt.create_latent_kv(rank, rope) for _ in lengths]
+        for b, cache in enumerate(caches):
+            cache.append(first if b == 0 else old, None, 0.0, cached)
+        o = torch.zeros(6, H, v, dtype=torch.bfloat16, device="cuda:0")
+        rt.latent_attention(weights, caches, x, rows, None, 0.0, o)
+        outs.append(o)
+        torch.cuda.synchronize()
+        for cache in caches:
+            cache.close()
+    clean, o = outs
+    none = torch.zeros(6, H, dtype=torch.bool, device="cuda:0")
+    none[[0, 2, 3]] = True
+    none[4, 33] = none[5, 2] = True
+    assert torch.isfinite(clean).all()
+    assert torch.isnan(o[none]).all() and torch.equal(o[~none], clean[~none])
+    weights.close()
