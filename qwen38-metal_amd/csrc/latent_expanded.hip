@@ -30,6 +30,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -1e30f;
+constexpr int kKeyPower = 8;
 
 // ---------------------------------------------------------------------------
 // Weights
@@ -90,8 +91,9 @@ __global__ __launch_bounds__(256) void latent_wop_kernel(LatentDims d, const uin
 // the shared key scaled, likewise; the tokens' factors.  Tokens behind the last
 // become zeros.
 //   g = 1 + exponent of the tile's largest scale (latent or key), gv of its
-//   largest latent scale; key operand code * s_key / 2^g, fk = s_lat / 2^g,
-//   fv = s_lat / 2^gv, powers = {2^g, 2^gv}.
+//   largest latent scale; key operand 2^8 code * s_key / 2^g (kKeyPower: below 2^15,
+//   as the expanded keys are), fk = s_lat / 2^g, fv = s_lat / 2^gv, powers = {2^g,
+//   2^gv}.
 // A token that stands for NaN keeps it in its key (fk or the operand) and has fv
 // = 0: rows that do not see it multiply its value by 0.
 // 6144 tokens of 512 + 64 (3.6 MB in, 7.2 MB out): 9.4 us; 1024: 5.7, a launch and a
@@ -113,7 +115,7 @@ __global__ __launch_bounds__(256) void latent_unpack_kernel(LatentExpandArgs a) 
     const uint32_t gv = max(__float_as_uint(topv) & 0x7F800000u, 0x21800000u) + 0x00800000u;
     const float ig = __uint_as_float(0x7F000000u - g), igv = __uint_as_float(0x7F000000u - gv);
     if (lane < 32) {
-      sk[lane] = s.y * ig;
+      sk[lane] = s.y * ig * (float)(1 << kKeyPower);
       a.fk[tok] = s.x * ig;
       a.fv[tok] = s.x <= FLT_MAX ? s.x * igv : 0.0f;
     }
@@ -347,9 +349,10 @@ __global__ __launch_bounds__(64 * W, 2) void latent_prompt_kernel(LatentExpandAr
   if (stages > 1) issue(1);
 
   // Queries, in the key operand's order: fp16 times 2^f, the expanded part divided
-  // by the weights' power as well, f the largest that keeps both parts below 16.
-  // (The part that f leaves small adds less than the other to the scores by as
-  // much.)  The scale goes in with its mantissa, so that products become exponents
+  // by the weights' power as well and the shared one by the key operand's, f the
+  // largest that keeps both parts below 2^15.  With keys as large, the smaller part
+  // of a query and the smaller of a token may be 2^20 below the larger ones before
+  // fp16 holds them in fewer than 11 bits.  The scale goes in with its mantissa, so that products become exponents
   // of two by a power of two alone: p = 2^(S ct - ref) is then one fused step
   // whose product is exact, at scores of any size.  A row with a NaN or an
   // infinity keeps it.
@@ -378,17 +381,17 @@ __global__ __launch_bounds__(64 * W, 2) void latent_prompt_kernel(LatentExpandAr
         }
       }
     }
-    int room[2];  // 2^room times the part stays below 16
+    int room[2];  // 2^room times the part stays below 2^14, the scale's mantissa below 2
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const auto o = __builtin_amdgcn_permlane32_swap(top[k], top[k], false, false);
-      room[k] = 130 - min(max((int)(max(o[0], o[1]) >> 23), 4), 252);
+      room[k] = 140 - min(max((int)(max(o[0], o[1]) >> 23), 14), 254);
     }
-    const int w = ilogbf(a.wmul[2 * h]), f = min(room[1], room[0] + w);
+    const int w = ilogbf(a.wmul[2 * h]), f = min(room[1] + kKeyPower, room[0] + w);
     const float s0 = a.scale * kLog2e;
     const int se = ilogbf(s0);
     c = ldexpf(1.0f, se - f);
-    const float mul[2] = {ldexpf(s0, f - w - se), ldexpf(s0, f - se)};
+    const float mul[2] = {ldexpf(s0, f - w - se), ldexpf(s0, f - kKeyPower - se)};
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll

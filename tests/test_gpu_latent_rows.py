@@ -207,3 +207,46 @@ def test_every_pair_of_rotary_positions(rt, interleaved, rows, heads, width, off
     pair = pair.repeat_interleave(2, -1) if interleaved else pair.repeat(1, 1, 2)
     got, ref = out[..., offset:offset + rd].double(), ref[..., offset:offset + rd]
     assert ((got - ref).abs() <= (ref.abs() * HALF + pair * factor * 2.0 ** -20) * (1 + HALF)).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("power", [-10, 10])
+def test_parts_of_a_score_of_different_sizes(torch_dev, form, power):
+    """Latents 2^power and keys 2^-power of the usual size, the two parts of a query the
+    other way round: neither part of a score loses precision."""
+    rank, rope, nope, v = SMALL
+    g = generator(85)
+    H, rows = 6, 200
+    with tuned(**FORMS[form]) as rt:
+        kv_b, scale, weights = make_weights(rt, g, H, SMALL)
+        q, kv = bf16(g, rows, H, nope + rope), bf16(g, rows, rank + rope)
+        kv[:, :rank] *= 2.0 ** power
+        kv[:, rank:] *= 2.0 ** -power
+        q[..., :nope] *= 2.0 ** -power
+        q[..., nope:] *= 2.0 ** power
+        cache = rt.create_latent_kv(rank, rope)
+        o = torch.empty(rows, H, v, dtype=torch.bfloat16, device=torch_dev)
+        rt.latent_attention_prefill(weights, cache, q, kv, None, 0.0, rows, o)
+        ref, bounds = attention_rows(q, *held(cache), kv_b, nope, scale, 0, form.replace("head by head", "expanded"))
+        assert_attention_rows(o, ref, bounds)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_tokens_of_different_sizes_in_a_tile(torch_dev, form):
+    """A token whose latent is 2^16 times its neighbours', and which rows leave nothing
+    (the shared key's part decides), costs no row precision."""
+    rank, rope, nope, v = SMALL
+    g = generator(86)
+    H, rows = 6, 200
+    with tuned(**FORMS[form]) as rt:
+        kv_b, scale, weights = make_weights(rt, g, H, SMALL)
+        q, kv = bf16(g, rows, H, nope + rope), bf16(g, rows, rank + rope)
+        q[..., :nope] = 0
+        q[..., nope:] = 1
+        kv[[5, 110], :rank] *= 2.0 ** 16
+        kv[[5, 110], rank:] = -100.0
+        cache = rt.create_latent_kv(rank, rope)
+        o = torch.empty(rows, H, v, dtype=torch.bfloat16, device=torch_dev)
+        rt.latent_attention_prefill(weights, cache, q, kv, None, 0.0, rows, o)
+        ref, bounds = attention_rows(q, *held(cache), kv_b, nope, scale, 0, form.replace("head by head", "expanded"))
+        assert_attention_rows(o, ref, bounds)
