@@ -347,6 +347,10 @@ qm_status absorbed_workspaces(qm_runtime* rt, LatentAttnArgs* a) {
   return QM_OK;
 }
 
+// Whether the absorbed form takes a prompt of M rows: its partial sums are 2 GB at
+// rank 512 then.
+bool absorbed_fits(const LatentDims& d, uint32_t M) { return (uint64_t)M * d.heads <= 1u << 20; }
+
 // Tokens of the expanded form's workspaces.
 uint64_t expanded_tokens(uint64_t T) { return (T + kLatentExpandTokens - 1) / kLatentExpandTokens * kLatentExpandTokens; }
 
@@ -374,7 +378,7 @@ uint32_t heads_of_a_pass(const qm_runtime* rt, const LatentDims& d, uint64_t T) 
 bool prefers_expanded(const qm_runtime* rt, const LatentDims& d, uint32_t M, uint64_t T) {
   if (T > 1u << 28) return false;  // its launches' threads
   if (rt->tune.latent_form) return rt->tune.latent_form == 2;
-  if ((uint64_t)M * d.heads > 1u << 20) return true;  // the absorbed form's partial sums: 2 GB at rank 512
+  if (!absorbed_fits(d, M)) return true;
   const double pairs = (double)M * ((double)T - 0.5 * M) * d.heads;
   const double cols = (double)M * d.heads;
   const double absorbed = 20.0 + cols * d.rank_pad * (0.006 / 512) + pairs * (2.0 * d.rank_pad + kLatentRope) / 0.46e9;
@@ -705,12 +709,15 @@ qm_status qm_latent_prefill(qm_runtime* rt, const qm_latent_weights* w, qm_laten
   if (!g.ok()) return no_device();
   if ((st = grow(seq, (uint64_t)seq->length + M)) != QM_OK) return st;
   const LatentNewRows rows = new_rows(w->d.rank, w->d.rope, kv, norm, epsilon);
-  const bool expanded = prefers_expanded(rt, w->d, M, (uint64_t)seq->length + M);
+  bool expanded = prefers_expanded(rt, w->d, M, (uint64_t)seq->length + M);
   LatentAttnArgs at{};
   ExpandedPlan ep;
   if (expanded) {
     st = plan_expanded(rt, w, seq, M, o, q, &ep);
-  } else {
+    // Its workspace is a multiple of the cache; the other form's is not.
+    if (st == QM_ERR_OUT_OF_MEMORY && absorbed_fits(w->d, M)) expanded = false;
+  }
+  if (!expanded) {
     at = absorbed_args(w, rows, q, o, M, 1, false);
     at.seqs[0].rows = seq->rows;
     at.seqs[0].start = seq->length;

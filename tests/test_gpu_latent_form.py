@@ -41,3 +41,36 @@ def test_form_of_a_prompt(torch_dev, widths, H, cached, rows, form):
         assert torch.equal(taken, absorbed if form == "absorbed" else expanded)
         weights.close()
         cache.close()
+
+
+def test_prompt_whose_workspace_does_not_fit(torch_dev):
+    """Keys and values of all heads at once (a workspace of 400 GB allowed) pass the
+    device's memory: the call takes the other form instead of failing, and later calls
+    go on."""
+    rank, rope, nope, v = SMALL
+    g = generator(62)
+    H, cached, rows = 256, 6_000_000, 256
+    if torch.cuda.mem_get_info()[1] > (cached * H * 256 * 9) // 10:
+        pytest.skip("the device holds them")
+    with tuned(QM38_LATENT_MB=400_000) as rt, tuned(QM38_LATENT_FORM=1) as one:
+        _, _, weights = make_weights(rt, g, H, SMALL)
+        cache = rt.create_latent_kv(rank, rope)
+        cache.reserve(cached + rows)
+        many = bf16(g, 500_000, rank + rope)
+        for _ in range(cached // len(many)):
+            cache.append(many, None, 0.0, len(many))
+        q, kv = bf16(g, rows, H, nope + rope), bf16(g, rows, rank + rope)
+        outs = []
+        for r in (rt, one):
+            outs.append(torch.empty(rows, H, v, dtype=torch.bfloat16, device=torch_dev))
+            r.latent_attention_prefill(weights, cache, q, kv, None, 0.0, rows, outs[-1])
+            torch.cuda.synchronize()
+            assert cache.sequence_length == cached + rows
+            cache.truncate(cached)
+        assert torch.isfinite(outs[0]).all() and torch.equal(*outs)
+        cache.truncate(1000)  # a prompt whose workspace is there again
+        rt.latent_attention_prefill(weights, cache, q, kv, None, 0.0, rows, outs[0])
+        torch.cuda.synchronize()
+        assert cache.sequence_length == 1000 + rows and torch.isfinite(outs[0]).all()
+        weights.close()
+        cache.close()
