@@ -478,7 +478,11 @@ qm_status qm_latent_decode(qm_runtime* rt, const qm_latent_weights* w, qm_latent
                            const uint16_t* q, const uint16_t* kv, const float* norm, float epsilon, uint16_t* o);
 /* M new rows of one sequence, row i attending over the cached tokens and the
  * new rows up to itself.  Layouts as above with M in the place of B.  In both
- * calls o overlaps no input; 2-byte alignment of it is enough. */
+ * calls o overlaps no input; 2-byte alignment of it is enough.
+ * Takes the absorbed form, or forms the heads' keys and values once for all rows,
+ * whichever was measured to be faster at these sizes.  The latter holds them in
+ * fp16 under a power of two for every 32 tokens: values of a token whose latent
+ * is more than 2^19 below the largest of its 32 lose bits. */
 qm_status qm_latent_prefill(qm_runtime* rt, const qm_latent_weights* w, qm_latent_kv* seq, const uint16_t* q,
                             const uint16_t* kv, const float* norm, float epsilon, uint32_t M, uint16_t* o);
 

@@ -29,7 +29,7 @@ COMMON = [
     "-Wno-unused-function",
     "-Wno-unused-variable",
     # Packed fp32 VALU ops stay disabled: some of their forms have given
-    # wrong results on this hardware pool; hipcc emits plain fp32 ops instead.
+    # wrong results on this hardware; hipcc emits plain fp32 ops instead.
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     f"-I{PKG.parent / 'include'}",
 ]

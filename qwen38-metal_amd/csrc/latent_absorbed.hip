@@ -40,8 +40,8 @@ constexpr float kNoMax = -1e30f;  // running maximum before the first visible to
 // Workgroup = (16 rows, head, 128 latent elements), a wave 32 of them: D = W
 // (rows) x queries (columns), so a lane holds four consecutive elements of a
 // row.  One token of 32 heads (4 MB of weights) is bound by latency: 128
-// workgroups of one round trip each, 6.5 us with the launch; of 128 heads (17 MB)
-// 7.1.
+// workgroups of one round trip each, 6.8 us with the launch; of 128 heads (17 MB)
+// 7.2.
 __device__ __forceinline__ void two_digits(float v, float s, bool skip, int at, uint32_t* hi, uint32_t* lo) {
   const int q = skip ? 0 : (int)rintf(fminf(fmaxf(v / s, -32512.0f), 32512.0f));
   const int h8 = (q + 128) >> 8;

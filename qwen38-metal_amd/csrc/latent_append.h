@@ -12,7 +12,7 @@
 // bound it, not the memory, so codes come from x times 1 / s wherever that cannot
 // differ from the division's: only a quotient within 10^-4 of a half could round
 // otherwise (the product is off by 3 * 2^-24 of at most 127), and is divided.  8192
-// rows of 512 + 64 with norm, 9.4 MB in and 4.8 out: 10.3 us (one row a wave 12.8;
+// rows of 512 + 64 with norm, 9.4 MB in and 4.8 out: 10.2 us (one row a wave 12.8;
 // dividing always, with a key to a wave, 14.2).
 #pragma once
 #include <float.h>

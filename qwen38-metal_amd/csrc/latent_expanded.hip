@@ -16,7 +16,10 @@
 // Keys and values are fp16 (2^-11 of each; bf16 would be 2^-8), kept in its
 // range by powers of two: the weights' per head (wmul: 127 sum |W| of a row stays
 // below 2^15), the tokens' per tile of 32 (2^g: the largest scale is below 1),
-// and each query row's.  The powers come back exactly in fp32.
+// and each query row's.  The powers come back exactly in fp32.  Under a tile's
+// power the values of a token whose latent scale is more than 2^19 below the largest
+// of its 32 lose bits; so does a part of a score (nope, rope) that is 2^20 below the
+// other in the query and above it in the token.
 #include <float.h>
 
 #include <algorithm>
@@ -96,7 +99,7 @@ __global__ __launch_bounds__(256) void latent_wop_kernel(LatentDims d, const uin
 //   2^gv}.
 // A token that stands for NaN keeps it in its key (fk or the operand) and has fv
 // = 0: rows that do not see it multiply its value by 0.
-// 6144 tokens of 512 + 64 (3.6 MB in, 7.2 MB out): 9.4 us; 1024: 5.7, a launch and a
+// 6144 tokens of 512 + 64 (3.6 MB in, 7.2 MB out): 9.0 us; 1024: 5.8, a launch and a
 // chain of two loads.
 __global__ __launch_bounds__(256) void latent_unpack_kernel(LatentExpandArgs a) {
   __shared__ float sl[32], sk[32];
@@ -284,11 +287,11 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(LatentExpandArgs 
 // moved, the sums rescaled and the tile weighed again.
 //
 // Bound by the matrix cores and the vector unit together (640 and 480 cycles a wave
-// and tile, two waves a SIMD): 2048 rows of 128 heads on 4096 tokens take 872 us,
-// 57% of the matrix cores' cycles at the clock it runs at.  The next tile's key
+// and tile, two waves a SIMD): 2048 rows of 128 heads on 4096 tokens take about 900
+// us (853 at the least), 58% of the matrix cores' cycles.  The next tile's key
 // products go between the exponentials; with each phase by itself, and a maximum
-// for every tile: 945.  1024 rows of 64 heads take 38 us, 6 of them until the queries
-// (25 MB, all at once) are there.
+// for every tile: 7% more.  1024 rows of 64 heads take 38 to 40 us, 6 of them until
+// the queries (25 MB, all at once) are there.
 template <int NP, int VP, int W>
 struct PromptLds {
   static constexpr int kKSteps = NP / 16 + 4, kVBlocks = VP / 32;

@@ -276,7 +276,8 @@ LatentAttnArgs absorbed_args(const qm_latent_weights* w, const LatentNewRows& ro
 // workgroup's start and end costing as much as 7 blocks.  512 rows of 20 heads on
 // 20000 tokens are 160 groups of columns: one round of them 656 us, two rounds of
 // 480 workgroups 500.  None below 4 blocks: the join costs more than a shorter
-// walk saves.
+// walk saves.  (What a further split adds to the join, 64 KB of sums at rank 512, is
+// not counted.)
 void plan_absorbed(const qm_runtime* rt, LatentAttnArgs* a) {
   const uint32_t cols = a->decode ? a->d.heads : a->rows * a->d.heads;
   a->group_cols = cols <= kLatentCols ? kLatentCols : 2 * kLatentCols;
