@@ -119,3 +119,27 @@ def test_a_graph_keeps_the_workspaces_that_latent_attention_outgrows(torch_dev, 
         del graph
         weights.close()
         cache.close()
+
+
+def test_a_large_workspace_is_not_doubled(torch_dev):
+    """Above 2 GB a workspace is what the call needs, rounded up to a GB."""
+    rank, rope, nope, v = WIDE
+    g = generator(74)
+    H, rows, cached = 64, 2048, 80000
+    with tuned(QM38_LATENT_FORM=2, QM38_LATENT_MB=8192) as rt:
+        _, _, weights = make_weights(rt, g, H, WIDE)
+        cache = rt.create_latent_kv(rank, rope)
+        cache.reserve(cached + rows)
+        cache.append(bf16(g, cached, rank + rope), None, 0.0, cached)
+        q, kv = bf16(g, rows, H, nope + rope), bf16(g, rows, rank + rope)
+        o = torch.empty(rows, H, v, dtype=torch.bfloat16, device=torch_dev)
+        before = free_bytes()
+        rt.latent_attention_prefill(weights, cache, q, kv, None, 0.0, rows, o)
+        taken = before - free_bytes()
+        if taken == 0:
+            pytest.skip("free-memory reading did not see the workspace")
+        # Keys and values of 64 heads, 512 bytes a token each, and the unpacked cache.
+        need = (cached + rows) * (64 * 512 + 1024 + 128 + 8)
+        assert need <= taken <= need + (1 << 30) + (64 << 20)
+        weights.close()
+        cache.close()
