@@ -270,6 +270,72 @@ qm_status qm_kv_clone(const qm_kv* src, qm_kv** out);
 qm_status qm_kv_read(const qm_kv* kv, int8_t* keys, int8_t* values,
                      float* key_scales, float* value_scales);
 
+/* The same cache in 4 bits (no counterpart in the reference).  Keys and values of
+ * a (token, KV head) are groups of 64 elements (the last one may be shorter), each
+ * with a bf16 scale s and offset m:
+ *   s = bf16(max((max - min) / 15, FLT_MIN)), m = bf16(min + 8 s),
+ *   code = round half to even(clamp((x - m) / s, -8, 7)), x ~ s code + m,
+ * all in fp32 from rows that are fp32 or widened to it: off by at most s/2, and
+ * s/64 + |m|/256 more at the ends of the range.  A group that holds a NaN or an
+ * infinity stands for NaN.  4.5 bits an element where head_dim is its storage
+ * width (Dp as above), kept as one block per (page, KV head).  Every call below
+ * that takes a qm_kv takes either kind, and so does a decode layer; one call takes
+ * caches of one kind. */
+qm_status qm_kv_create_q4(qm_runtime* rt, uint32_t kv_heads, uint32_t head_dim,
+                          uint32_t page_tokens, uint32_t max_tokens, qm_kv** out);
+uint32_t qm_kv_bits(const qm_kv* kv); /* 8 or 4; 0 for NULL */
+/* qm_kv_read of a 4-bit cache (each refuses the other kind): codes int8
+ * [len][kv_heads][head_dim], scales bf16 [len][kv_heads][groups][2] = (s, m). */
+qm_status qm_kv_read_q4(const qm_kv* kv, int8_t* keys, int8_t* values,
+                        uint16_t* key_scales, uint16_t* value_scales);
+
+/* Rows of a fused or separate projection for qm_kv_append, bf16 device pointers;
+ * strides are the elements between rows (0: heads * head_dim).  With `rotary`
+ * set, elements offset .. offset + rotary_dim - 1 of every key are rotated on the
+ * way, in fp64 and rounded once to fp32, and of every query, into q_out (bf16,
+ * the bits of qm_rotary).  positions: device uint32 per row, or NULL for the
+ * row's place in its cache; read with `rotary` only. */
+typedef struct qm_rotary_config qm_rotary_config; /* Rotary positions, below */
+typedef struct qm_kv_rows {
+  const uint16_t* k; /* [rows][kv_heads][head_dim] */
+  const uint16_t* v;
+  uint64_t k_stride, v_stride;
+  const qm_rotary_config* rotary; /* NULL: keys as given, and no queries */
+  uint32_t offset;
+  const uint32_t* positions;
+  const uint16_t* q; /* [rows][heads][head_dim], or NULL */
+  uint16_t* q_out;
+  uint32_t heads;
+  uint64_t q_stride, q_out_stride;
+} qm_kv_rows;
+
+/* Appends counts[b] >= 0 rows to sequence b, for B <= 64 sequences of one shape
+ * and kind, none twice: the rows follow one another in sequence order.  Keys
+ * rotate and both are quantised in the launch that writes them.  q_out may be q
+ * (with equal strides: in place) and otherwise overlaps no input.  Caches grow as
+ * needed.  No row at all: QM_ERR_EMPTY_APPEND; over 2^20 rows, or more than one
+ * launch takes: QM_ERR_DIMENSION_OVERFLOW.  2-byte alignment is enough; rows and
+ * heads on 8 bytes (queries: 16) are faster.  This and the three calls below
+ * refuse a stream that is being captured and the per-thread default stream
+ * (QM_ERR_INVALID_ARGUMENT): what they do depends on the length when they are
+ * made. */
+qm_status qm_kv_append(qm_runtime* rt, qm_kv* const* seqs, const uint32_t* counts, uint32_t B,
+                       const qm_kv_rows* rows);
+/* Reads tokens first .. first + count - 1 back, what their codes stand for rounded
+ * to bf16: k and v [count][kv_heads][head_dim], either may be NULL.  Past the
+ * length: QM_ERR_INVALID_SEQUENCE_LENGTH. */
+qm_status qm_kv_load(qm_runtime* rt, const qm_kv* kv, uint32_t first, uint32_t count,
+                     uint16_t* k, uint16_t* v);
+/* qm_attn_decode of tokens that are in their caches already (qm_kv_append): the
+ * query of every sequence's last token over all its tokens.  A sequence without a
+ * token: QM_ERR_INVALID_SEQUENCE_LENGTH. */
+qm_status qm_attn_decode_cached(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, const uint16_t* q,
+                                const uint16_t* gate, uint32_t H, uint16_t* o);
+/* qm_attn_prefill of the last M tokens, in the cache already; M <= length, else
+ * QM_ERR_INVALID_SEQUENCE_LENGTH. */
+qm_status qm_attn_prefill_cached(qm_runtime* rt, qm_kv* seq, const uint16_t* q, const uint16_t* gate,
+                                 uint32_t H, uint32_t M, uint16_t* o);
+
 /* Decode attention for a ragged batch of B sequences (B <= 64): appends one
  * token per sequence (quantised K/V, qwen38_q8_kv_append, qwen38.metal:
  * 5031-5080) and attends over the whole cache including it.
@@ -364,7 +430,7 @@ qm_status qm_attn_prefill(qm_runtime* rt, qm_kv* seq, const uint16_t* q,
 #define QM_ROTARY_YARN 2        /* f_i where a frequency turns more than beta_fast times within
                                    original_positions, f_i / factor where it turns less than
                                    beta_slow times, a linear ramp over i between the two */
-typedef struct qm_rotary_config {
+struct qm_rotary_config {
   uint32_t rotary_dim;         /* rotated elements of a head: even, 2..256 */
   uint32_t layout;             /* QM_ROTARY_HALF or _INTERLEAVED */
   float theta;                 /* > 1 */
@@ -373,7 +439,7 @@ typedef struct qm_rotary_config {
   uint32_t original_positions; /* YARN: positions the model was trained on, > 0 */
   float beta_fast, beta_slow;  /* YARN: beta_fast > beta_slow > 0 (usually 32 and 1) */
   float attention_factor;      /* of sine and cosine; 0: 0.1 ln(factor) + 1 with YARN, else 1 */
-} qm_rotary_config;
+};
 
 /* bf16 rows of `heads` heads of `head_dim` elements; elements offset ..
  * offset + rotary_dim - 1 of each head are rotated, the others copied.  Strides

@@ -19,7 +19,7 @@ inline uint32_t attn_padded_dim(uint32_t d) { return d <= 64 ? 64 : d <= 128 ? 1
 constexpr int attn_prefill_waves(uint32_t D, int W) { return D == 64 ? 3 : D == 256 && W == 4 ? 1 : 2; }
 
 struct AttnSeq {
-  int8_t* k;          // K pages   [page][kv_head][16][D]
+  int8_t* k;          // K pages   [page][kv_head][16][D]; 4-bit caches: [page][kv_head] blocks, v, ks and vs unused
   int8_t* v;          // V pages   [page][kv_head][D][16]
   float* ks;          // K scales  [page][kv_head][16]
   float* vs;          // V scales  [page][kv_head][16]
@@ -49,7 +49,7 @@ struct AttnArgs {
   const uint16_t* gate;  // bf16 [rows][H][D] or null
   uint16_t* o;           // bf16 [rows][H][D]
   float* partials;       // split partials: O [split rows][H][Dp], then (m, l) [split rows][H][2]
-  const float* k_new;    // decode: fp32 [n_seqs][kv_heads][D] rows appended by the kernel
+  const float* k_new;    // decode: fp32 [n_seqs][kv_heads][D] rows appended by the kernel, or null: none
   const float* v_new;
   uint32_t heads;
   uint32_t kv_heads;
@@ -89,5 +89,7 @@ hipError_t launch_q8_append(const AppendArgs& a, uint32_t items, hipStream_t st)
 // Decode: `units` workgroups; when need_combine, q8_combine_kernel merges the
 // split partials (which must be set) in a second launch.
 hipError_t launch_q8_attention(const AttnArgs& a, uint32_t units, bool need_combine, hipStream_t st);
+// The same over 4-bit caches (q4kv_attention.hip).
+hipError_t launch_q4kv_attention(const AttnArgs& a, uint32_t units, bool need_combine, hipStream_t st);
 
 }  // namespace qm

@@ -40,6 +40,7 @@
 
 #include "attention.h"
 #include "common.h"
+#include "kv_quant.h"
 
 namespace qm {
 namespace {
@@ -59,29 +60,10 @@ __device__ __forceinline__ void q8_load_row(const float* src, uint32_t dr, int l
   }
 }
 
-// Quantises one row held 4 values per lane as qwen38_q8_kv_append does:
-// s = max(absmax / 127, FLT_MIN), q = round-half-away(clamp(x / s, -127,
-// 127)), IEEE division.  Returns s.
-__device__ __forceinline__ float q8_quant_vals(const float (&vals)[4], int8_t (&qv)[4]) {
-  float amax = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(vals[i]));
-  amax = wave_allmax(amax);
-  const float s = fmaxf(amax / 127.0f, FLT_MIN);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) qv[i] = (int8_t)roundf(fminf(fmaxf(vals[i] / s, -127.0f), 127.0f));
-  return s;
-}
-
 __device__ __forceinline__ float q8_quant_row(const float* src, uint32_t dr, int lane, int8_t (&qv)[4]) {
   float vals[4];
   q8_load_row(src, dr, lane, vals);
   return q8_quant_vals(vals, qv);
-}
-
-__device__ __forceinline__ uint32_t pack_q8x4(const int8_t (&qv)[4]) {
-  return (uint32_t)(uint8_t)qv[0] | ((uint32_t)(uint8_t)qv[1] << 8) | ((uint32_t)(uint8_t)qv[2] << 16) |
-         ((uint32_t)(uint8_t)qv[3] << 24);
 }
 
 // Quantises one (token, kv_head) row of K (kind 0) or V (kind 1) with one
@@ -368,7 +350,7 @@ __global__ __launch_bounds__(64 * W) void q8_decode_kernel(AttnArgs args) {
   // (waves 0 and 1 quantise K and V); the barrier below orders those stores
   // before any wave's DMA of the last page.  KV head 0 also records pages
   // materialised by this call in the page table.
-  if (split + 1 == sq.nsplit) {
+  if (split + 1 == sq.nsplit && args.k_new) {
     const uint32_t token = sq.len - 1;
     if (wave < 2) {
       const float* src = (wave == 0 ? args.k_new : args.v_new) + ((size_t)b * KVH + kvh) * dr;

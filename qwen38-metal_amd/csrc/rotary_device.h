@@ -1,0 +1,93 @@
+// Device side of rotary positions, shared by the stand-alone kernel (rotary.hip)
+// and the appends that rotate on the way (kv_append.hip).
+#pragma once
+#include "common.h"
+#include "rotary.h"
+
+namespace qm {
+
+__device__ __forceinline__ void unpack8(u32x4 v, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = bf16_to_f32(v[i] & 0xFFFFu);
+    x[2 * i + 1] = __uint_as_float(v[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
+  u32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = f32_to_bf16(x[2 * i]) | ((uint32_t)f32_to_bf16(x[2 * i + 1]) << 16);
+  return v;
+}
+
+// Sines and cosines of one position, times `factor`, by `threads` threads: the angle
+// in fp64, reduced modulo 2 pi there.
+__device__ __forceinline__ void rotary_table(const double* freq, uint32_t half, uint32_t position, float factor,
+                                             uint32_t threads, float* cos_s, float* sin_s) {
+  for (uint32_t i = threadIdx.x; i < half; i += threads) {
+    const double angle = (double)position * freq[i];
+    const double turns = rint(angle * 0.15915494309189535);
+    double r = fma(-turns, 6.283185307179586, angle);  // 2 pi in two parts
+    r = fma(-turns, 2.4492935982947064e-16, r);
+    float sn, cs;
+    sincosf((float)r, &sn, &cs);
+    cos_s[i] = cs * factor;
+    sin_s[i] = sn * factor;
+  }
+}
+
+// Work item `local` of one row of a tensor: 8 elements of a head (VEC) or one.
+template <bool INTERLEAVED, bool VEC>
+__device__ __forceinline__ void rotary_item(const RotaryTensor& t, const uint16_t* in, uint16_t* out, uint32_t local,
+                                            uint32_t rd, const float* cos_s, const float* sin_s) {
+  const uint32_t half = rd / 2;
+  if constexpr (VEC) {
+    const uint32_t per = t.head_dim / 8, head = local / per, e = (local - head * per) * 8;
+    const size_t at = (size_t)head * t.head_dim + e;
+    const uint32_t c = e - t.offset;  // element of the rotated part (wraps below it)
+    if (e < t.offset || c >= rd) {
+      if (out != in) *(u32x4*)(out + at) = *(const u32x4*)(in + at);
+      return;
+    }
+    float x[8], y[8];
+    if constexpr (INTERLEAVED) {
+      unpack8(*(const u32x4*)(in + at), x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float cs = cos_s[c / 2 + j], sn = sin_s[c / 2 + j];
+        y[2 * j] = x[2 * j] * cs - x[2 * j + 1] * sn;
+        y[2 * j + 1] = x[2 * j + 1] * cs + x[2 * j] * sn;
+      }
+      *(u32x4*)(out + at) = pack8(y);
+    } else {
+      if (c >= half) return;  // its partner's item takes it
+      float z[8], w[8];
+      unpack8(*(const u32x4*)(in + at), x);
+      unpack8(*(const u32x4*)(in + at + half), z);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float cs = cos_s[c + j], sn = sin_s[c + j];
+        y[j] = x[j] * cs - z[j] * sn;
+        w[j] = z[j] * cs + x[j] * sn;
+      }
+      *(u32x4*)(out + at) = pack8(y);
+      *(u32x4*)(out + at + half) = pack8(w);
+    }
+  } else {
+    const uint32_t head = local / t.head_dim, e = local - head * t.head_dim;
+    const size_t at = (size_t)head * t.head_dim + e;
+    const uint32_t c = e - t.offset;
+    if (e < t.offset || c >= rd) {
+      if (out != in) out[at] = in[at];
+      return;
+    }
+    // The first element of a pair takes its second along.
+    if (INTERLEAVED ? c % 2 != 0 : c >= half) return;
+    const uint32_t f = INTERLEAVED ? c / 2 : c, step = INTERLEAVED ? 1 : half;
+    const float x = bf16_to_f32(in[at]), z = bf16_to_f32(in[at + step]);
+    out[at] = f32_to_bf16(x * cos_s[f] - z * sin_s[f]);
+    out[at + step] = f32_to_bf16(z * cos_s[f] + x * sin_s[f]);
+  }
+}
+
+}  // namespace qm

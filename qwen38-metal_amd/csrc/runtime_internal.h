@@ -120,6 +120,34 @@ uint32_t kv_heads_of(const qm_kv* kv);
 uint32_t kv_head_dim_of(const qm_kv* kv);
 const qm_runtime* kv_runtime_of(const qm_kv* kv);
 
+// A call whose position is fixed when it is made, and whose workspaces belong
+// to one stream's order: neither a capture (its graph would keep the position
+// and buffers that growth frees) nor the per-thread stream (one handle, several
+// streams).
+qm_status check_stream(const qm_runtime* rt, const char* what);
+// Radians per position of every frequency, and the factor of sine and cosine.
+qm_status rotary_frequencies(const qm_rotary_config& c, double* freq, float* factor);
+
+// Byte ranges of M rows of `width` elements, `stride` apart.
+struct Extent {
+  uintptr_t base;
+  uint64_t stride, width, bytes;
+};
+inline Extent extent(const void* p, uint64_t stride, uint64_t width, uint64_t M) {
+  return Extent{(uintptr_t)p, 2 * stride, 2 * width, 2 * (stride * (M - 1) + width)};
+}
+// Whether two sets of rows share memory.  With equal strides two columns of one
+// buffer do not, though their extents overlap.
+inline bool overlap(const Extent& x, const Extent& y) {
+  if (x.base + x.bytes <= y.base || y.base + y.bytes <= x.base) return false;
+  if (x.stride != y.stride) return true;
+  const uint64_t d = (x.base > y.base ? x.base - y.base : y.base - x.base) % x.stride;
+  const uint64_t low = x.base > y.base ? y.width : x.width, high = x.base > y.base ? x.width : y.width;
+  return d < low || x.stride - d < high;
+}
+
+inline bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+
 // Makes `device` current for its scope.  ok() is false for a runtime
 // without a device (QM_DEVICE_NONE), whose calls stop at no_device().
 class DeviceGuard {

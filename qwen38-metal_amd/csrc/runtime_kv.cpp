@@ -12,35 +12,22 @@
 #include <algorithm>
 #include <vector>
 
-#include "attention.h"
+#include "kv_append.h"
+#include "kv_internal.h"
 #include "prepare.h"
-#include "runtime_internal.h"
+#include "q4kv.h"
 
 using namespace qm;
 
-struct qm_kv {
-  qm_runtime* rt = nullptr;
-  uint32_t kv_heads = 0;
-  uint32_t head_dim = 0;  // the caller's head dimension
-  uint32_t dp = 0;        // storage width of a page row (attn_padded_dim)
-  uint32_t page_tokens = 16;
-  uint32_t max_tokens = 0;  // hard limit (LogicalPageTable capacity); 0 = grow without limit
-  uint32_t cap_pages = 0;   // physical pages allocated
-  uint32_t length = 0;
-  std::vector<int32_t> pages;  // logical page -> physical id, -1 if not materialised [cap_pages]
-  int32_t next_page_id = 0;
-  int32_t* d_pt = nullptr;  // device page table [cap_pages]
-  int8_t* k = nullptr;      // [cap_pages][kv_heads][16][dp]
-  int8_t* v = nullptr;      // [cap_pages][kv_heads][dp][16]
-  float* ks = nullptr;      // [cap_pages][kv_heads][16]
-  float* vs = nullptr;
-};
-
 namespace {
 
-
-size_t kv_page_bytes(const qm_kv* kv) { return (size_t)kv->kv_heads * kv->page_tokens * kv->dp; }
-size_t scale_page_count(const qm_kv* kv) { return (size_t)kv->kv_heads * kv->page_tokens; }
+// Bytes of a page in `k` (the whole page with 4 bits) and in `v`, and scales in
+// `ks` and in `vs`.
+size_t k_page_bytes(const qm_kv* kv) {
+  return kv->bits == 4 ? (size_t)kv->kv_heads * q4kv_block_bytes(kv->dp) : (size_t)kv->kv_heads * kv->page_tokens * kv->dp;
+}
+size_t v_page_bytes(const qm_kv* kv) { return kv->bits == 4 ? 0 : k_page_bytes(kv); }
+size_t scale_page_count(const qm_kv* kv) { return kv->bits == 4 ? 0 : (size_t)kv->kv_heads * kv->page_tokens; }
 
 struct KvBuffers {
   int32_t* pt = nullptr;
@@ -61,19 +48,17 @@ void free_buffers(const KvBuffers& b) {
 // and are never read (only pages below the length are).
 qm_status alloc_buffers(const qm_kv* kv, uint32_t pages, KvBuffers* out) {
   KvBuffers b;
-  const size_t pb = kv_page_bytes(kv) * pages;
-  const size_t sb = scale_page_count(kv) * pages * sizeof(float);
   hipStream_t s = kv->rt->stream;
-  hipError_t e = hipMalloc(&b.pt, (size_t)pages * sizeof(int32_t));
-  if (e == hipSuccess) e = hipMalloc(&b.k, pb);
-  if (e == hipSuccess) e = hipMalloc(&b.v, pb);
-  if (e == hipSuccess) e = hipMalloc(&b.ks, sb);
-  if (e == hipSuccess) e = hipMalloc(&b.vs, sb);
-  if (e == hipSuccess) e = hipMemsetAsync(b.pt, 0, (size_t)pages * sizeof(int32_t), s);
-  if (e == hipSuccess) e = hipMemsetAsync(b.k, 0, pb, s);
-  if (e == hipSuccess) e = hipMemsetAsync(b.v, 0, pb, s);
-  if (e == hipSuccess) e = hipMemsetAsync(b.ks, 0, sb, s);
-  if (e == hipSuccess) e = hipMemsetAsync(b.vs, 0, sb, s);
+  hipError_t e = hipSuccess;
+  auto take = [&](auto** p, size_t bytes) {
+    if (e != hipSuccess || bytes == 0) return;
+    if ((e = hipMalloc(p, bytes)) == hipSuccess) e = hipMemsetAsync(*p, 0, bytes, s);
+  };
+  take(&b.pt, (size_t)pages * sizeof(int32_t));
+  take(&b.k, k_page_bytes(kv) * pages);
+  take(&b.v, v_page_bytes(kv) * pages);
+  take(&b.ks, scale_page_count(kv) * pages * sizeof(float));
+  take(&b.vs, scale_page_count(kv) * pages * sizeof(float));
   if (e != hipSuccess) {
     (void)hipGetLastError();
     free_buffers(b);
@@ -82,6 +67,21 @@ qm_status alloc_buffers(const qm_kv* kv, uint32_t pages, KvBuffers* out) {
   }
   *out = b;
   return QM_OK;
+}
+
+// The pages materialised in `kv`, copied on the stream.
+hipError_t copy_pages(const qm_kv* kv, const KvBuffers& to, hipStream_t s) {
+  const size_t n = (size_t)kv->next_page_id;
+  hipError_t e = hipSuccess;
+  auto copy = [&](void* dst, const void* src, size_t bytes) {
+    if (e == hipSuccess && bytes) e = hipMemcpyAsync(dst, src, bytes, hipMemcpyDeviceToDevice, s);
+  };
+  copy(to.pt, kv->d_pt, (size_t)kv->cap_pages * sizeof(int32_t));
+  copy(to.k, kv->k, n * k_page_bytes(kv));
+  copy(to.v, kv->v, n * v_page_bytes(kv));
+  copy(to.ks, kv->ks, n * scale_page_count(kv) * 4);
+  copy(to.vs, kv->vs, n * scale_page_count(kv) * 4);
+  return e;
 }
 
 void free_kv(qm_kv* kv) {
@@ -100,10 +100,9 @@ qm_status validate_kv_shape(uint32_t kv_heads, uint32_t head_dim, uint32_t page_
   return QM_OK;
 }
 
-// Physical capacity for `tokens` tokens: the next power of two (at least 16
-// tokens), clamped to the hard limit, copying the materialised pages.
-// Synchronous when it grows; a no-op otherwise.
-qm_status kv_grow(qm_kv* kv, uint64_t tokens) {
+}  // namespace
+
+qm_status qm::kv_grow(qm_kv* kv, uint64_t tokens) {
   if (kv->max_tokens && tokens > kv->max_tokens)
     return fail(QM_ERR_CAPACITY_EXCEEDED, "token range ending at %llu exceeds page table capacity %u",
                 (unsigned long long)tokens, kv->max_tokens);
@@ -113,24 +112,15 @@ qm_status kv_grow(qm_kv* kv, uint64_t tokens) {
   while (cap_tokens < tokens) cap_tokens <<= 1;
   if (kv->max_tokens) cap_tokens = std::min<uint64_t>(cap_tokens, kv->max_tokens);
   const uint64_t new_pages = (cap_tokens + kv->page_tokens - 1) / kv->page_tokens;
-  if (new_pages > (uint64_t)kMaxSplits * kMaxPagesPerSplit || new_pages * kv_page_bytes(kv) > (1ull << 40))
-    return fail(QM_ERR_DIMENSION_OVERFLOW, "Q8 KV token capacity %llu", (unsigned long long)cap_tokens);
+  if (new_pages > (uint64_t)kMaxSplits * kMaxPagesPerSplit || new_pages * k_page_bytes(kv) > (1ull << 40))
+    return fail(QM_ERR_DIMENSION_OVERFLOW, "KV token capacity %llu", (unsigned long long)cap_tokens);
   DeviceGuard g(kv->rt->device);
   if (!g.ok()) return no_device();
   KvBuffers nb;
   qm_status st = alloc_buffers(kv, (uint32_t)new_pages, &nb);
   if (st != QM_OK) return st;
   hipStream_t s = kv->rt->stream;
-  const size_t n = (size_t)kv->next_page_id;
-  hipError_t e = hipSuccess;
-  if (kv->cap_pages)
-    e = hipMemcpyAsync(nb.pt, kv->d_pt, (size_t)kv->cap_pages * sizeof(int32_t), hipMemcpyDeviceToDevice, s);
-  if (e == hipSuccess && n) e = hipMemcpyAsync(nb.k, kv->k, n * kv_page_bytes(kv), hipMemcpyDeviceToDevice, s);
-  if (e == hipSuccess && n) e = hipMemcpyAsync(nb.v, kv->v, n * kv_page_bytes(kv), hipMemcpyDeviceToDevice, s);
-  if (e == hipSuccess && n)
-    e = hipMemcpyAsync(nb.ks, kv->ks, n * scale_page_count(kv) * 4, hipMemcpyDeviceToDevice, s);
-  if (e == hipSuccess && n)
-    e = hipMemcpyAsync(nb.vs, kv->vs, n * scale_page_count(kv) * 4, hipMemcpyDeviceToDevice, s);
+  hipError_t e = copy_pages(kv, nb, s);
   if (e == hipSuccess) e = hipStreamSynchronize(s);
   if (e != hipSuccess) {
     free_buffers(nb);
@@ -152,11 +142,8 @@ qm_status kv_grow(qm_kv* kv, uint64_t tokens) {
   return QM_OK;
 }
 
-// The pages an append of [start, end) would materialise, without changing
-// the table: the first new logical page, how many, and the first new id
-// (ids are sequential, LogicalPageTable::append).
-void plan_pages(const qm_kv* kv, uint32_t start, uint32_t end, int32_t* first_new, int32_t* count,
-                int32_t* first_id) {
+void qm::plan_pages(const qm_kv* kv, uint32_t start, uint32_t end, int32_t* first_new, int32_t* count,
+                    int32_t* first_id) {
   *first_new = -1;
   *count = 0;
   *first_id = -1;
@@ -172,19 +159,20 @@ void plan_pages(const qm_kv* kv, uint32_t start, uint32_t end, int32_t* first_ne
     }
 }
 
-// Records a planned append in the host table.  Materialised pages form a
-// prefix of the logical pages (appends are sequential and truncation keeps
-// pages), so the new ones are consecutive.
-void commit_pages(qm_kv* kv, int32_t first_new, int32_t count) {
+// Materialised pages form a prefix of the logical pages (appends are
+// sequential and truncation keeps pages), so the new ones are consecutive.
+void qm::commit_pages(qm_kv* kv, int32_t first_new, int32_t count) {
   for (int32_t i = 0; i < count; ++i) kv->pages[first_new + i] = kv->next_page_id++;
 }
 
-void rollback_pages(qm_kv* kv, int32_t first_new, int32_t count) {
+void qm::rollback_pages(qm_kv* kv, int32_t first_new, int32_t count) {
   for (int32_t i = count - 1; i >= 0; --i) {
     kv->pages[first_new + i] = -1;
     --kv->next_page_id;
   }
 }
+
+namespace {
 
 AttnSeq seq_desc(const qm_kv* kv) {
   AttnSeq s{};
@@ -199,8 +187,6 @@ AttnSeq seq_desc(const qm_kv* kv) {
   s.new_page_id = -1;
   return s;
 }
-
-bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 qm_status check_heads(uint32_t H, uint32_t KVH) {
   if (H == 0 || H % KVH != 0 || H / KVH > 16)
@@ -229,7 +215,8 @@ struct DecodeChunk {
 // kernel's page limits, and all splits should run in one residency round:
 // one 8-wave workgroup per CU if the splits fit that (measured faster at 32K:
 // the CU's waves share one split), else two 4-wave workgroups per CU.
-qm_status plan_decode_chunk(qm_runtime* rt, qm_kv* const* seqs, uint32_t nb, DecodeChunk* c) {
+// `extra`: tokens that the call appends to each sequence (1 or 0).
+qm_status plan_decode_chunk(qm_runtime* rt, qm_kv* const* seqs, uint32_t nb, uint32_t extra, DecodeChunk* c) {
   const uint32_t KVH = seqs[0]->kv_heads;
   AttnArgs& at = c->at;
   uint64_t total_pages = 0;
@@ -237,8 +224,8 @@ qm_status plan_decode_chunk(qm_runtime* rt, qm_kv* const* seqs, uint32_t nb, Dec
   for (uint32_t i = 0; i < nb; ++i) {
     const qm_kv* kv = seqs[i];
     AttnSeq sd = seq_desc(kv);
-    plan_pages(kv, kv->length, kv->length + 1, &sd.new_page_first, &sd.new_page_count, &sd.new_page_id);
-    sd.len = kv->length + 1;
+    plan_pages(kv, kv->length, kv->length + extra, &sd.new_page_first, &sd.new_page_count, &sd.new_page_id);
+    sd.len = kv->length + extra;
     at.seqs[i] = sd;
     const uint32_t pages = (sd.len + 15) / 16;
     total_pages += pages;
@@ -334,10 +321,10 @@ size_t prefill_partial_bytes(const qm_runtime* rt, uint32_t D) {
   return waves * 32 * (D + 2) * sizeof(float);
 }
 
-// Shared validation of qm_attn_decode and its no-allocation twin.
+// Shared validation of the decode calls (`cached`: no rows to append).
 qm_status check_decode_args(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, const uint16_t* q, const uint16_t* gate,
-                            const float* k, const float* v, uint32_t H, const uint16_t* o) {
-  if (!rt || !seqs || !q || !k || !v || !o) return fail(QM_ERR_NULL_POINTER, "NULL argument");
+                            const float* k, const float* v, uint32_t H, const uint16_t* o, bool cached = false) {
+  if (!rt || !seqs || !q || (!cached && (!k || !v)) || !o) return fail(QM_ERR_NULL_POINTER, "NULL argument");
   if (B == 0 || B > 64) return fail(QM_ERR_INVALID_ARGUMENT, "batch must be 1..64 sequences");
   const qm_kv* s0 = seqs[0];
   if (!s0) return fail(QM_ERR_NULL_POINTER, "sequence 0 is NULL");
@@ -350,6 +337,8 @@ qm_status check_decode_args(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, cons
     if (!seqs[b]) return fail(QM_ERR_NULL_POINTER, "sequence %u is NULL", b);
     if (seqs[b]->kv_heads != KVH || seqs[b]->head_dim != D)
       return fail(QM_ERR_INVALID_ATTENTION_SHAPE, "all sequences must share kv_heads and head_dim");
+    if (seqs[b]->bits != s0->bits)
+      return fail(QM_ERR_INVALID_ATTENTION_SHAPE, "8-bit and 4-bit caches in one call");
     if (seqs[b]->rt->device != rt->device) return fail(QM_ERR_INVALID_ARGUMENT, "sequence %u is on another device", b);
     for (uint32_t c = 0; c < b; ++c)
       if (seqs[c] == seqs[b]) return fail(QM_ERR_INVALID_ARGUMENT, "sequence %u appears twice", b);
@@ -359,14 +348,14 @@ qm_status check_decode_args(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, cons
 
 // Plans every chunk; the caller then commits and launches them.  Nothing is
 // modified here.
-qm_status plan_decode(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, uint32_t H,
+qm_status plan_decode(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, uint32_t H, uint32_t extra,
                       std::vector<DecodeChunk>* chunks, size_t* partial_bytes) {
   *partial_bytes = 0;
   chunks->clear();
   for (uint32_t b0 = 0; b0 < B; b0 += kMaxAttnSeqs) {
     DecodeChunk c;
     const uint32_t nb = std::min<uint32_t>(kMaxAttnSeqs, B - b0);
-    qm_status st = plan_decode_chunk(rt, seqs + b0, nb, &c);
+    qm_status st = plan_decode_chunk(rt, seqs + b0, nb, extra, &c);
     if (st != QM_OK) return st;
     c.at.n_seqs = nb;
     chunks->push_back(c);
@@ -394,7 +383,7 @@ qm_status launch_decode(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, const ui
     for (uint32_t i = 0; i < nb; ++i) {
       qm_kv* kv = seqs[b0 + i];
       commit_pages(kv, at.seqs[i].new_page_first, at.seqs[i].new_page_count);
-      kv->length += 1;
+      kv->length = at.seqs[i].len;
     }
     at.q = q + (size_t)b0 * H * D;
     at.gate = gate ? gate + (size_t)b0 * H * D : nullptr;
@@ -406,14 +395,15 @@ qm_status launch_decode(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, const ui
     at.head_dim = D;
     at.head_dim_pad = Dp;
     at.prefill = 0;
-    at.k_new = k + (size_t)b0 * KVH * D;  // the decode kernel appends the new rows itself
-    at.v_new = v + (size_t)b0 * KVH * D;
-    hipError_t e = launch_q8_attention(at, c.units, c.combine, rt->stream);
+    at.k_new = k ? k + (size_t)b0 * KVH * D : nullptr;  // the decode kernel appends the new rows itself
+    at.v_new = k ? v + (size_t)b0 * KVH * D : nullptr;
+    hipError_t e = seqs[0]->bits == 4 ? launch_q4kv_attention(at, c.units, c.combine, rt->stream)
+                                      : launch_q8_attention(at, c.units, c.combine, rt->stream);
     if (e != hipSuccess) {
       // Nothing of this chunk ran: put its sequences back.
       for (uint32_t i = 0; i < nb; ++i) {
         qm_kv* kv = seqs[b0 + i];
-        kv->length -= 1;
+        kv->length = at.seqs[i].len - (k ? 1 : 0);
         rollback_pages(kv, at.seqs[i].new_page_first, at.seqs[i].new_page_count);
       }
       return hip_check(e, "attention decode launch");
@@ -445,16 +435,16 @@ qm_status qm::attn_decode_prepare(qm_runtime* rt, qm_kv* const* seqs, uint32_t B
   }
   std::vector<DecodeChunk> chunks;
   size_t pb = 0;
-  qm_status st = plan_decode(rt, seqs, B, H, &chunks, &pb);
+  qm_status st = plan_decode(rt, seqs, B, H, 1, &chunks, &pb);
   if (st != QM_OK) return st;
   if (pb && (st = ensure_partials(rt, pb)) != QM_OK) return st;
   return QM_OK;
 }
 
-extern "C" {
+namespace {
 
-qm_status qm_kv_create(qm_runtime* rt, uint32_t kv_heads, uint32_t head_dim, uint32_t page_tokens,
-                       uint32_t max_tokens, qm_kv** out) {
+qm_status create_kv(qm_runtime* rt, uint32_t bits, uint32_t kv_heads, uint32_t head_dim, uint32_t page_tokens,
+                    uint32_t max_tokens, qm_kv** out) {
   if (!rt || !out) return fail(QM_ERR_NULL_POINTER, "runtime/out is NULL");
   *out = nullptr;
   qm_status st = validate_kv_shape(kv_heads, head_dim, page_tokens);
@@ -464,6 +454,7 @@ qm_status qm_kv_create(qm_runtime* rt, uint32_t kv_heads, uint32_t head_dim, uin
   kv->kv_heads = kv_heads;
   kv->head_dim = head_dim;
   kv->dp = attn_padded_dim(head_dim);
+  kv->bits = bits;
   kv->page_tokens = page_tokens;
   kv->max_tokens = max_tokens;
   // allocate_q8_kv_state(kv_heads, head_dim, 16): one page to start with.
@@ -480,6 +471,116 @@ qm_status qm_kv_create(qm_runtime* rt, uint32_t kv_heads, uint32_t head_dim, uin
   *out = kv;
   return QM_OK;
 }
+
+// fp32 rows into one cache, for a prefill.
+hipError_t append_rows(const qm_kv* kv, const AttnSeq& sd, const float* k, const float* v, uint32_t start, uint32_t M,
+                       hipStream_t st) {
+  if (kv->bits == 4) {
+    KvAppendArgs ap{};
+    KvAppendSeq& s = ap.seqs[0];
+    s.p = KvPages{(uint8_t*)sd.k, nullptr, nullptr, nullptr, sd.pt};
+    s.start = start;
+    s.rows = M;
+    s.new_page_first = sd.new_page_first;
+    s.new_page_count = sd.new_page_count;
+    s.new_page_id = sd.new_page_id;
+    ap.n_seqs = 1;
+    ap.k = k;
+    ap.v = v;
+    ap.k_stride = ap.v_stride = (uint64_t)kv->kv_heads * kv->head_dim;
+    ap.kv_heads = kv->kv_heads;
+    ap.head_dim = kv->head_dim;
+    ap.head_dim_pad = kv->dp;
+    return launch_q4kv_append_f32(ap, kv->head_dim % 4 == 0 && aligned(k, 16) && aligned(v, 16), st);
+  }
+  AppendArgs ap{};
+  ap.k = k;
+  ap.v = v;
+  ap.kv_heads = kv->kv_heads;
+  ap.head_dim = kv->head_dim;
+  ap.head_dim_pad = kv->dp;
+  ap.decode = 0;
+  ap.start = start;
+  ap.seqs[0] = sd;
+  return launch_q8_append(ap, M, st);
+}
+
+// Causal attention of the rows behind the cached tokens, which it appends (k and
+// v), or of the last M tokens.
+qm_status prefill(qm_runtime* rt, qm_kv* seq, const uint16_t* q, const uint16_t* gate, const float* k, const float* v,
+                  uint32_t H, uint32_t M, uint16_t* o) {
+  if (M == 0) return fail(QM_ERR_INVALID_ATTENTION_SHAPE, "prefill needs at least one row");
+  const uint32_t KVH = seq->kv_heads, D = seq->head_dim;
+  qm_status st = check_heads(H, KVH);
+  if (st != QM_OK) return st;
+  if ((st = check_q_alignment(q, gate, D)) != QM_OK) return st;
+  if (!aligned(k, 4) || !aligned(v, 4)) return fail(QM_ERR_MISALIGNED, "k/v must be 4-byte aligned");
+  if (seq->rt->device != rt->device) return fail(QM_ERR_INVALID_ARGUMENT, "the cache is on another device");
+  const uint64_t end = (uint64_t)seq->length + (k ? M : 0);
+  if (end > 0xFFFFFFFFull) return fail(QM_ERR_DIMENSION_OVERFLOW, "KV token capacity");
+  DeviceGuard g(rt->device);
+  if (!g.ok()) return no_device();
+  if (!k && (st = check_stream(rt, "attention over cached rows")) != QM_OK) return st;
+  if ((st = kv_grow(seq, end)) != QM_OK) return st;
+  const uint32_t before = seq->length, start = (uint32_t)end - M;
+  AttnSeq sd = seq_desc(seq);
+  plan_pages(seq, before, (uint32_t)end, &sd.new_page_first, &sd.new_page_count, &sd.new_page_id);
+  sd.len = (uint32_t)end;
+  AttnArgs at{};
+  at.q = q;
+  at.gate = gate;
+  at.o = o;
+  at.heads = H;
+  at.kv_heads = KVH;
+  at.head_dim = D;
+  at.head_dim_pad = seq->dp;
+  at.n_seqs = 1;
+  at.prefill = 1;
+  at.rows = M;
+  at.start = start;
+  at.seqs[0] = sd;
+  at.out8 = D % 8 == 0 && aligned(o, 8);
+  plan_prefill(rt, &at);
+  if (at.splits > 1) {
+    at.part_rows = M * at.splits;
+    const size_t bytes = (size_t)at.part_rows * H * (seq->dp + 2) * sizeof(float);
+    if (try_partials(rt, std::max(bytes, prefill_partial_bytes(rt, seq->dp))) || try_partials(rt, bytes))
+      at.partials = (float*)rt->partials;
+    else
+      at.splits = 1;
+  }
+  // A cache owned by another runtime: its pending work comes first.
+  if ((st = stream_after(rt, seq->rt)) != QM_OK) return st;
+  commit_pages(seq, sd.new_page_first, sd.new_page_count);
+  seq->length = (uint32_t)end;
+  hipError_t e = k ? append_rows(seq, sd, k, v, start, M, rt->stream) : hipSuccess;
+  // The prefill launcher sizes its own grid (rows per workgroup depend on the
+  // kernel's column blocks).
+  if (e == hipSuccess)
+    e = seq->bits == 4 ? launch_q4kv_attention(at, 0, false, rt->stream) : launch_q8_attention(at, 0, false, rt->stream);
+  if (e != hipSuccess) {
+    seq->length = before;
+    rollback_pages(seq, sd.new_page_first, sd.new_page_count);
+    return hip_check(e, "attention prefill launch");
+  }
+  return stream_after(seq->rt, rt);
+}
+
+}  // namespace
+
+extern "C" {
+
+qm_status qm_kv_create(qm_runtime* rt, uint32_t kv_heads, uint32_t head_dim, uint32_t page_tokens,
+                       uint32_t max_tokens, qm_kv** out) {
+  return create_kv(rt, 8, kv_heads, head_dim, page_tokens, max_tokens, out);
+}
+
+qm_status qm_kv_create_q4(qm_runtime* rt, uint32_t kv_heads, uint32_t head_dim, uint32_t page_tokens,
+                          uint32_t max_tokens, qm_kv** out) {
+  return create_kv(rt, 4, kv_heads, head_dim, page_tokens, max_tokens, out);
+}
+
+uint32_t qm_kv_bits(const qm_kv* kv) { return kv ? kv->bits : 0; }
 
 void qm_kv_destroy(qm_kv* kv) {
   if (!kv) return;
@@ -508,7 +609,7 @@ int64_t qm_kv_page_for_token(const qm_kv* kv, uint32_t token) {
 qm_status qm_kv_reserve(qm_kv* kv, uint32_t additional) {
   if (!kv) return fail(QM_ERR_NULL_POINTER, "kv is NULL");
   const uint64_t end = (uint64_t)kv->length + additional;
-  if (end > 0xFFFFFFFFull) return fail(QM_ERR_DIMENSION_OVERFLOW, "Q8 KV token capacity");
+  if (end > 0xFFFFFFFFull) return fail(QM_ERR_DIMENSION_OVERFLOW, "KV token capacity");
   qm_status st = kv_grow(kv, end);
   if (st != QM_OK) return st;
   int32_t first, count, id;
@@ -536,7 +637,7 @@ qm_status qm_kv_clone(const qm_kv* src, qm_kv** out) {
   if (!src || !out) return fail(QM_ERR_NULL_POINTER, "src/out is NULL");
   *out = nullptr;
   qm_kv* kv = nullptr;
-  qm_status st = qm_kv_create(src->rt, src->kv_heads, src->head_dim, src->page_tokens, src->max_tokens, &kv);
+  qm_status st = create_kv(src->rt, src->bits, src->kv_heads, src->head_dim, src->page_tokens, src->max_tokens, &kv);
   if (st != QM_OK) return st;
   // Same capacity as the source (clone_q8_kv_state, :7338-7379): its pages
   // may hold more tokens than max_tokens allows, so grow to what it may hold.
@@ -549,15 +650,8 @@ qm_status qm_kv_clone(const qm_kv* src, qm_kv** out) {
   kv->next_page_id = src->next_page_id;
   DeviceGuard g(src->rt->device);
   if (!g.ok()) return no_device();
-  const size_t n = (size_t)src->next_page_id;
   hipStream_t s = src->rt->stream;
-  hipError_t e = hipMemcpyAsync(kv->d_pt, src->d_pt, src->cap_pages * sizeof(int32_t), hipMemcpyDeviceToDevice, s);
-  if (e == hipSuccess && n) e = hipMemcpyAsync(kv->k, src->k, n * kv_page_bytes(src), hipMemcpyDeviceToDevice, s);
-  if (e == hipSuccess && n) e = hipMemcpyAsync(kv->v, src->v, n * kv_page_bytes(src), hipMemcpyDeviceToDevice, s);
-  if (e == hipSuccess && n)
-    e = hipMemcpyAsync(kv->ks, src->ks, n * scale_page_count(src) * 4, hipMemcpyDeviceToDevice, s);
-  if (e == hipSuccess && n)
-    e = hipMemcpyAsync(kv->vs, src->vs, n * scale_page_count(src) * 4, hipMemcpyDeviceToDevice, s);
+  hipError_t e = copy_pages(src, KvBuffers{kv->d_pt, kv->k, kv->v, kv->ks, kv->vs}, s);
   if (e == hipSuccess) e = hipStreamSynchronize(s);
   if (e != hipSuccess) {
     qm_kv_destroy(kv);
@@ -569,11 +663,12 @@ qm_status qm_kv_clone(const qm_kv* src, qm_kv** out) {
 
 qm_status qm_kv_read(const qm_kv* kv, int8_t* keys, int8_t* values, float* key_scales, float* value_scales) {
   if (!kv) return fail(QM_ERR_NULL_POINTER, "kv is NULL");
+  if (kv->bits != 8) return fail(QM_ERR_INVALID_ARGUMENT, "a 4-bit cache: qm_kv_read_q4");
   DeviceGuard g(kv->rt->device);
   if (!g.ok()) return no_device();
   const size_t n = (size_t)kv->next_page_id;
   const uint32_t KVH = kv->kv_heads, D = kv->head_dim, Dp = kv->dp, T = kv->length;
-  std::vector<int8_t> hk(n * kv_page_bytes(kv)), hv(n * kv_page_bytes(kv));
+  std::vector<int8_t> hk(n * k_page_bytes(kv)), hv(n * v_page_bytes(kv));
   std::vector<float> hks(n * scale_page_count(kv)), hvs(n * scale_page_count(kv));
   hipStream_t s = kv->rt->stream;
   hipError_t e = hipSuccess;
@@ -601,6 +696,46 @@ qm_status qm_kv_read(const qm_kv* kv, int8_t* keys, int8_t* values, float* key_s
   return QM_OK;
 }
 
+qm_status qm_kv_read_q4(const qm_kv* kv, int8_t* keys, int8_t* values, uint16_t* key_scales, uint16_t* value_scales) {
+  if (!kv) return fail(QM_ERR_NULL_POINTER, "kv is NULL");
+  if (kv->bits != 4) return fail(QM_ERR_INVALID_ARGUMENT, "an 8-bit cache: qm_kv_read");
+  DeviceGuard g(kv->rt->device);
+  if (!g.ok()) return no_device();
+  const uint32_t KVH = kv->kv_heads, D = kv->head_dim, Dp = kv->dp, G = (D + kQ4KvGroup - 1) / kQ4KvGroup;
+  std::vector<uint8_t> h((size_t)kv->next_page_id * k_page_bytes(kv));
+  hipError_t e = hipSuccess;
+  if (!h.empty()) {
+    e = hipMemcpyAsync(h.data(), kv->k, h.size(), hipMemcpyDeviceToHost, kv->rt->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(kv->rt->stream);
+  }
+  if (e != hipSuccess) return hip_check(e, "KV read");
+  for (uint32_t t = 0; t < kv->length; ++t) {
+    const uint32_t slot = t % 16;
+    for (uint32_t hh = 0; hh < KVH; ++hh) {
+      const uint8_t* block = h.data() + ((size_t)kv->pages[t / 16] * KVH + hh) * q4kv_block_bytes(Dp);
+      auto word = [&](uint32_t byte) {
+        uint32_t w;
+        memcpy(&w, block + byte, 4);
+        return w;
+      };
+      const size_t row = (size_t)t * KVH + hh;
+      for (uint32_t d = 0; d < D; ++d) {
+        if (keys) keys[row * D + d] = (int8_t)((int)(word(q4kv_k_word(Dp, slot, d)) >> q4kv_k_bit(d) & 15) - 8);
+        if (values)
+          values[row * D + d] =
+              (int8_t)((int)((word(q4kv_v_bytes(Dp) + q4kv_v_word(Dp, slot, d)) >> q4kv_v_bit(slot, d) & 15) ^ 8) - 8);
+      }
+      for (uint32_t g = 0; g < G; ++g)
+        for (uint32_t kind = 0; kind < 2; ++kind) {
+          uint16_t* out = kind ? value_scales : key_scales;
+          const uint32_t w = word(q4kv_scale_bytes(Dp) + 4 * q4kv_scale_word(Dp, kind, g, slot));
+          if (out) out[(row * G + g) * 2] = (uint16_t)w, out[(row * G + g) * 2 + 1] = (uint16_t)(w >> 16);
+        }
+    }
+  }
+  return QM_OK;
+}
+
 qm_status qm_attn_decode(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, const uint16_t* q, const uint16_t* gate,
                          const float* k, const float* v, uint32_t H, uint16_t* o) {
   qm_status st = check_decode_args(rt, seqs, B, q, gate, k, v, H, o);
@@ -612,7 +747,7 @@ qm_status qm_attn_decode(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, const u
   if ((st = attn_decode_prepare(rt, seqs, B, H)) != QM_OK) return st;
   std::vector<DecodeChunk> chunks;
   size_t pb = 0;
-  if ((st = plan_decode(rt, seqs, B, H, &chunks, &pb)) != QM_OK) return st;
+  if ((st = plan_decode(rt, seqs, B, H, 1, &chunks, &pb)) != QM_OK) return st;
   return launch_decode(rt, seqs, B, q, gate, k, v, H, o, chunks, (float*)rt->partials, rt->partial_bytes);
 }
 
@@ -632,7 +767,7 @@ qm_status qm_attn_decode_noalloc(qm_runtime* rt, qm_kv* const* seqs, uint32_t B,
   if ((st = hip_check(attn_noalloc_scratch(rt->device, &ws), "attention scratch")) != QM_OK) return st;
   std::vector<DecodeChunk> chunks;
   size_t pb = 0;
-  if ((st = plan_decode(rt, seqs, B, H, &chunks, &pb)) != QM_OK) return st;
+  if ((st = plan_decode(rt, seqs, B, H, 1, &chunks, &pb)) != QM_OK) return st;
   if (pb > ws.partial_bytes)
     return fail(QM_ERR_CAPACITY_EXCEEDED, "split partials of %zu bytes exceed the %zu-byte no-allocation scratch", pb,
                 ws.partial_bytes);
@@ -642,71 +777,34 @@ qm_status qm_attn_decode_noalloc(qm_runtime* rt, qm_kv* const* seqs, uint32_t B,
   return st != QM_OK ? st : end;
 }
 
+qm_status qm_attn_decode_cached(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, const uint16_t* q,
+                                const uint16_t* gate, uint32_t H, uint16_t* o) {
+  qm_status st = check_decode_args(rt, seqs, B, q, gate, nullptr, nullptr, H, o, true);
+  if (st != QM_OK) return st;
+  for (uint32_t b = 0; b < B; ++b)
+    if (seqs[b]->length == 0) return fail(QM_ERR_INVALID_SEQUENCE_LENGTH, "sequence %u holds no token", b);
+  DeviceGuard g(rt->device);
+  if (!g.ok()) return no_device();
+  if ((st = check_stream(rt, "attention over cached rows")) != QM_OK) return st;
+  std::vector<DecodeChunk> chunks;
+  size_t pb = 0;
+  if ((st = plan_decode(rt, seqs, B, H, 0, &chunks, &pb)) != QM_OK) return st;
+  if (pb && (st = ensure_partials(rt, pb)) != QM_OK) return st;
+  return launch_decode(rt, seqs, B, q, gate, nullptr, nullptr, H, o, chunks, (float*)rt->partials, rt->partial_bytes);
+}
+
 qm_status qm_attn_prefill(qm_runtime* rt, qm_kv* seq, const uint16_t* q, const uint16_t* gate, const float* k,
                           const float* v, uint32_t H, uint32_t M, uint16_t* o) {
   if (!rt || !seq || !q || !k || !v || !o) return fail(QM_ERR_NULL_POINTER, "NULL argument");
-  if (M == 0) return fail(QM_ERR_INVALID_ATTENTION_SHAPE, "prefill needs at least one row");
-  const uint32_t KVH = seq->kv_heads, D = seq->head_dim;
-  qm_status st = check_heads(H, KVH);
-  if (st != QM_OK) return st;
-  if ((st = check_q_alignment(q, gate, D)) != QM_OK) return st;
-  if (!aligned(k, 4) || !aligned(v, 4)) return fail(QM_ERR_MISALIGNED, "k/v must be 4-byte aligned");
-  if (seq->rt->device != rt->device) return fail(QM_ERR_INVALID_ARGUMENT, "the cache is on another device");
-  const uint64_t end = (uint64_t)seq->length + M;
-  if (end > 0xFFFFFFFFull) return fail(QM_ERR_DIMENSION_OVERFLOW, "Q8 KV token capacity");
-  DeviceGuard g(rt->device);
-  if (!g.ok()) return no_device();
-  if ((st = kv_grow(seq, end)) != QM_OK) return st;
-  const uint32_t start = seq->length;
-  AttnSeq sd = seq_desc(seq);
-  plan_pages(seq, start, start + M, &sd.new_page_first, &sd.new_page_count, &sd.new_page_id);
-  sd.len = start + M;
-  AppendArgs ap{};
-  ap.k = k;
-  ap.v = v;
-  ap.kv_heads = KVH;
-  ap.head_dim = D;
-  ap.head_dim_pad = seq->dp;
-  ap.decode = 0;
-  ap.start = start;
-  ap.seqs[0] = sd;
-  AttnArgs at{};
-  at.q = q;
-  at.gate = gate;
-  at.o = o;
-  at.heads = H;
-  at.kv_heads = KVH;
-  at.head_dim = D;
-  at.head_dim_pad = seq->dp;
-  at.n_seqs = 1;
-  at.prefill = 1;
-  at.rows = M;
-  at.start = start;
-  at.seqs[0] = sd;
-  at.out8 = D % 8 == 0 && aligned(o, 8);
-  plan_prefill(rt, &at);
-  if (at.splits > 1) {
-    at.part_rows = M * at.splits;
-    const size_t bytes = (size_t)at.part_rows * H * (seq->dp + 2) * sizeof(float);
-    if (try_partials(rt, std::max(bytes, prefill_partial_bytes(rt, seq->dp))) || try_partials(rt, bytes))
-      at.partials = (float*)rt->partials;
-    else
-      at.splits = 1;
-  }
-  // A cache owned by another runtime: its pending work comes first.
-  if ((st = stream_after(rt, seq->rt)) != QM_OK) return st;
-  commit_pages(seq, sd.new_page_first, sd.new_page_count);
-  seq->length = start + M;
-  hipError_t e = launch_q8_append(ap, M, rt->stream);
-  // The prefill launcher sizes its own grid (rows per workgroup depend on the
-  // kernel's column blocks).
-  if (e == hipSuccess) e = launch_q8_attention(at, 0, false, rt->stream);
-  if (e != hipSuccess) {
-    seq->length = start;
-    rollback_pages(seq, sd.new_page_first, sd.new_page_count);
-    return hip_check(e, "attention prefill launch");
-  }
-  return stream_after(seq->rt, rt);
+  return prefill(rt, seq, q, gate, k, v, H, M, o);
+}
+
+qm_status qm_attn_prefill_cached(qm_runtime* rt, qm_kv* seq, const uint16_t* q, const uint16_t* gate, uint32_t H,
+                                 uint32_t M, uint16_t* o) {
+  if (!rt || !seq || !q || !o) return fail(QM_ERR_NULL_POINTER, "NULL argument");
+  if (M > seq->length)
+    return fail(QM_ERR_INVALID_SEQUENCE_LENGTH, "%u rows of a sequence of %u tokens", M, seq->length);
+  return prefill(rt, seq, q, gate, nullptr, nullptr, H, M, o);
 }
 
 }  // extern "C"

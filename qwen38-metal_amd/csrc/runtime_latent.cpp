@@ -49,21 +49,7 @@ void free_weights(qm_latent_weights* w) {
 
 namespace {
 
-bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
-
 size_t row_bytes(const qm_latent_kv* kv) { return kv->rank_pad + kLatentRope; }
-
-// A call whose position is fixed when it is made, and whose workspaces belong
-// to one stream's order: neither a capture (its graph would keep the position
-// and buffers that growth frees) nor the per-thread stream (one handle, several
-// streams).
-qm_status check_stream(const qm_runtime* rt, const char* what) {
-  if (rt->device < 0) return no_device();
-  if (stream_capturing(rt->stream)) return fail(QM_ERR_INVALID_ARGUMENT, "%s: the stream is being captured", what);
-  if (rt->stream == hipStreamPerThread)
-    return fail(QM_ERR_INVALID_ARGUMENT, "%s: not on the per-thread default stream", what);
-  return QM_OK;
-}
 
 qm_status check_cache_dims(uint32_t rank, uint32_t rope) {
   if (rank == 0 || rank > kLatentMaxRank || rank % 8 != 0 || rope == 0 || rope > kLatentRope || rope % 8 != 0)
@@ -119,63 +105,6 @@ void free_cache(qm_latent_kv* kv) {
   (void)hipFree(kv->rows.codes);
   (void)hipFree(kv->rows.scales);
   delete kv;
-}
-
-// Byte ranges of M rows of `width` elements, `stride` apart.
-struct Extent {
-  uintptr_t base;
-  uint64_t stride, width, bytes;
-};
-Extent extent(const void* p, uint64_t stride, uint64_t width, uint64_t M) {
-  return Extent{(uintptr_t)p, 2 * stride, 2 * width, 2 * (stride * (M - 1) + width)};
-}
-// Whether two sets of rows share memory.  With equal strides two columns of one
-// buffer do not, though their extents overlap.
-bool overlap(const Extent& x, const Extent& y) {
-  if (x.base + x.bytes <= y.base || y.base + y.bytes <= x.base) return false;
-  if (x.stride != y.stride) return true;
-  const uint64_t d = (x.base > y.base ? x.base - y.base : y.base - x.base) % x.stride;
-  const uint64_t low = x.base > y.base ? y.width : x.width, high = x.base > y.base ? x.width : y.width;
-  return d < low || x.stride - d < high;
-}
-
-qm_status rotary_frequencies(const qm_rotary_config& c, double* freq, float* factor) {
-  if (c.rotary_dim == 0 || c.rotary_dim > kRotaryMaxDim || c.rotary_dim % 2 != 0)
-    return fail(QM_ERR_INVALID_ATTENTION_SHAPE, "rotary_dim %u must be even, 2..%u", c.rotary_dim, kRotaryMaxDim);
-  if (c.layout > QM_ROTARY_INTERLEAVED || c.scaling > QM_ROTARY_YARN)
-    return fail(QM_ERR_INVALID_ARGUMENT, "rotary layout %u or scaling %u is unknown", c.layout, c.scaling);
-  if (!(c.theta > 1.0f) || !isfinite(c.theta)) return fail(QM_ERR_INVALID_ARGUMENT, "theta must be > 1");
-  if (!(c.attention_factor >= 0.0f) || !isfinite(c.attention_factor))
-    return fail(QM_ERR_INVALID_ARGUMENT, "attention_factor must be finite and not negative");
-  if (c.scaling != QM_ROTARY_PLAIN && (!(c.factor >= 1.0f) || !isfinite(c.factor)))
-    return fail(QM_ERR_INVALID_ARGUMENT, "the scaling's factor must be >= 1");
-  double low = 0.0, high = 0.0;
-  if (c.scaling == QM_ROTARY_YARN) {
-    if (c.original_positions == 0 || !(c.beta_slow > 0.0f) || !(c.beta_fast > c.beta_slow) || !isfinite(c.beta_fast))
-      return fail(QM_ERR_INVALID_ARGUMENT, "YARN needs original_positions > 0 and beta_fast > beta_slow > 0");
-    // The (fractional) frequency index that turns `beta` times within the original positions.
-    auto index = [&](double beta) {
-      return c.rotary_dim * log(c.original_positions / (beta * 2.0 * M_PI)) / (2.0 * log((double)c.theta));
-    };
-    low = std::max(floor(index(c.beta_fast)), 0.0);
-    high = std::min(ceil(index(c.beta_slow)), (double)c.rotary_dim - 1.0);
-  }
-  const double width = std::max(high - low, 0.001);
-  for (uint32_t i = 0; i < c.rotary_dim / 2; ++i) {
-    const double f = pow((double)c.theta, -2.0 * i / c.rotary_dim);
-    if (c.scaling == QM_ROTARY_PLAIN) {
-      freq[i] = f;
-    } else if (c.scaling == QM_ROTARY_LINEAR) {
-      freq[i] = f / c.factor;
-    } else {
-      const double ramp = std::min(std::max((i - low) / width, 0.0), 1.0);
-      freq[i] = f / c.factor * ramp + f * (1.0 - ramp);
-    }
-  }
-  *factor = c.attention_factor;
-  if (c.attention_factor == 0.0f)
-    *factor = c.scaling == QM_ROTARY_YARN ? (float)(0.1 * log((double)c.factor) + 1.0) : 1.0f;
-  return QM_OK;
 }
 
 qm_status check_weights_config(const qm_latent_config& c) {
@@ -439,6 +368,57 @@ qm_status plan_expanded(qm_runtime* rt, const qm_latent_weights* w, const qm_lat
 }
 
 }  // namespace
+
+// A call whose position is fixed when it is made, and whose workspaces belong
+// to one stream's order: neither a capture (its graph would keep the position
+// and buffers that growth frees) nor the per-thread stream (one handle, several
+// streams).
+qm_status qm::check_stream(const qm_runtime* rt, const char* what) {
+  if (rt->device < 0) return no_device();
+  if (stream_capturing(rt->stream)) return fail(QM_ERR_INVALID_ARGUMENT, "%s: the stream is being captured", what);
+  if (rt->stream == hipStreamPerThread)
+    return fail(QM_ERR_INVALID_ARGUMENT, "%s: not on the per-thread default stream", what);
+  return QM_OK;
+}
+
+qm_status qm::rotary_frequencies(const qm_rotary_config& c, double* freq, float* factor) {
+  if (c.rotary_dim == 0 || c.rotary_dim > kRotaryMaxDim || c.rotary_dim % 2 != 0)
+    return fail(QM_ERR_INVALID_ATTENTION_SHAPE, "rotary_dim %u must be even, 2..%u", c.rotary_dim, kRotaryMaxDim);
+  if (c.layout > QM_ROTARY_INTERLEAVED || c.scaling > QM_ROTARY_YARN)
+    return fail(QM_ERR_INVALID_ARGUMENT, "rotary layout %u or scaling %u is unknown", c.layout, c.scaling);
+  if (!(c.theta > 1.0f) || !isfinite(c.theta)) return fail(QM_ERR_INVALID_ARGUMENT, "theta must be > 1");
+  if (!(c.attention_factor >= 0.0f) || !isfinite(c.attention_factor))
+    return fail(QM_ERR_INVALID_ARGUMENT, "attention_factor must be finite and not negative");
+  if (c.scaling != QM_ROTARY_PLAIN && (!(c.factor >= 1.0f) || !isfinite(c.factor)))
+    return fail(QM_ERR_INVALID_ARGUMENT, "the scaling's factor must be >= 1");
+  double low = 0.0, high = 0.0;
+  if (c.scaling == QM_ROTARY_YARN) {
+    if (c.original_positions == 0 || !(c.beta_slow > 0.0f) || !(c.beta_fast > c.beta_slow) || !isfinite(c.beta_fast))
+      return fail(QM_ERR_INVALID_ARGUMENT, "YARN needs original_positions > 0 and beta_fast > beta_slow > 0");
+    // The (fractional) frequency index that turns `beta` times within the original positions.
+    auto index = [&](double beta) {
+      return c.rotary_dim * log(c.original_positions / (beta * 2.0 * M_PI)) / (2.0 * log((double)c.theta));
+    };
+    low = std::max(floor(index(c.beta_fast)), 0.0);
+    high = std::min(ceil(index(c.beta_slow)), (double)c.rotary_dim - 1.0);
+  }
+  const double width = std::max(high - low, 0.001);
+  for (uint32_t i = 0; i < c.rotary_dim / 2; ++i) {
+    const double f = pow((double)c.theta, -2.0 * i / c.rotary_dim);
+    if (c.scaling == QM_ROTARY_PLAIN) {
+      freq[i] = f;
+    } else if (c.scaling == QM_ROTARY_LINEAR) {
+      freq[i] = f / c.factor;
+    } else {
+      const double ramp = std::min(std::max((i - low) / width, 0.0), 1.0);
+      freq[i] = f / c.factor * ramp + f * (1.0 - ramp);
+    }
+  }
+  *factor = c.attention_factor;
+  if (c.attention_factor == 0.0f)
+    *factor = c.scaling == QM_ROTARY_YARN ? (float)(0.1 * log((double)c.factor) + 1.0) : 1.0f;
+  return QM_OK;
+}
 
 extern "C" {
 

@@ -14,8 +14,6 @@ constexpr uint32_t kDecodeMaxRows = 16;
 // bytes) with 32-bit offsets.
 constexpr uint32_t kMaxInElems = 1u << 24;
 
-bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
-
 // validate_mapped_q4_affine_shape / MatvecShape::validate
 // (metal_runtime.rs:8854-8898, 8932-8984) for device-resident jobs.
 qm_status validate_job(const qm_q4_job* job, uint32_t in_elems, const char* name) {

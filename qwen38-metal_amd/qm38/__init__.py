@@ -39,6 +39,8 @@ EXPORTS = [
     "qm_q4_project", "qm_q4_project_set", "qm_q4_swiglu", "qm_q4_mlp", "qm_q4_argmax", "qm_q4_job_from_mapped",
     "qm_kv_create", "qm_kv_destroy", "qm_kv_length", "qm_kv_capacity", "qm_kv_allocated_pages", "qm_kv_page_for_token",
     "qm_kv_reserve", "qm_kv_truncate", "qm_kv_clone", "qm_kv_read",
+    "qm_kv_create_q4", "qm_kv_bits", "qm_kv_read_q4", "qm_kv_append", "qm_kv_load",
+    "qm_attn_decode_cached", "qm_attn_prefill_cached",
     "qm_attn_decode", "qm_attn_decode_noalloc", "qm_attn_prefill", "qm_attn_prepare",
     "qm_rotary",
     "qm_latent_kv_create", "qm_latent_kv_destroy", "qm_latent_kv_length", "qm_latent_kv_capacity",
@@ -119,6 +121,14 @@ class RotaryTensor(C.Structure):
                 ("offset", C.c_uint32), ("in_stride", C.c_uint64), ("out_stride", C.c_uint64)]
 
 
+class KvRows(C.Structure):
+    """qm_kv_rows"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_uint64), ("v_stride", C.c_uint64),
+                ("rotary", C.POINTER(RotaryConfig)), ("offset", C.c_uint32), ("positions", C.c_void_p),
+                ("q", C.c_void_p), ("q_out", C.c_void_p), ("heads", C.c_uint32), ("q_stride", C.c_uint64),
+                ("q_out_stride", C.c_uint64)]
+
+
 class LatentConfig(C.Structure):
     """qm_latent_config: the widths of latent attention and its softmax scale."""
     _fields_ = [("heads", C.c_uint32), ("rank", C.c_uint32), ("nope_dim", C.c_uint32), ("rope_dim", C.c_uint32),
@@ -196,6 +206,13 @@ def load(path: str | os.PathLike | None = None) -> C.CDLL:
         "qm_kv_truncate": ([vp, u32], i32),
         "qm_kv_clone": ([vp, C.POINTER(vp)], i32),
         "qm_kv_read": ([vp, vp, vp, vp, vp], i32),
+        "qm_kv_create_q4": ([vp, u32, u32, u32, u32, C.POINTER(vp)], i32),
+        "qm_kv_bits": ([vp], u32),
+        "qm_kv_read_q4": ([vp, vp, vp, vp, vp], i32),
+        "qm_kv_append": ([vp, C.POINTER(vp), C.POINTER(u32), u32, C.POINTER(KvRows)], i32),
+        "qm_kv_load": ([vp, vp, u32, u32, vp, vp], i32),
+        "qm_attn_decode_cached": ([vp, C.POINTER(vp), u32, vp, vp, u32, vp], i32),
+        "qm_attn_prefill_cached": ([vp, vp, vp, vp, u32, u32, vp], i32),
         "qm_attn_decode": ([vp, C.POINTER(vp), u32, vp, vp, vp, vp, u32, vp], i32),
         "qm_attn_decode_noalloc": ([vp, C.POINTER(vp), u32, vp, vp, vp, vp, u32, vp], i32),
         "qm_attn_prefill": ([vp, vp, vp, vp, vp, vp, u32, u32, vp], i32),
@@ -260,6 +277,12 @@ def _check(status: int) -> None:
     if status != 0:
         msg = load().qm_last_error_message().decode()
         raise QmError(status, msg)
+
+
+def _stride(t) -> int:
+    """Elements between the rows of a torch tensor; 0 (rows that follow one
+    another) for a raw address or None."""
+    return t.stride(0) if hasattr(t, "stride") and t.shape[0] > 1 else 0
 
 
 def _ptr(t) -> int | None:
@@ -362,6 +385,36 @@ class Runtime:
                            page_tokens: int = 16) -> "KvCache":
         """create_q8_kv_state; max_tokens = 0 grows without limit (the reference's policy)."""
         return KvCache(self, kv_heads, head_dim, page_tokens, max_tokens)
+
+    def create_q4_kv_state(self, kv_heads: int, head_dim: int, max_tokens: int = 0,
+                           page_tokens: int = 16) -> "KvCache":
+        """The same cache in 4 bits (qm_kv_create_q4); every call that takes a KvCache takes it."""
+        return KvCache(self, kv_heads, head_dim, page_tokens, max_tokens, bits=4)
+
+    def kv_append(self, seqs, counts, k, v, rotary: RotaryConfig | None = None, positions=None, q=None, q_out=None,
+                  num_heads: int = 0, offset: int = 0) -> None:
+        """qm_kv_append: counts[b] rows of k and v (bf16 [rows][kv_heads][head_dim],
+        the rows any stride apart) behind what seqs[b] cache; with `rotary`, keys
+        turned on the way and the rows of q (num_heads heads) into q_out.
+        positions: uint32/int32 per row on the device, or None for each row's
+        place in its cache."""
+        arr = (C.c_void_p * len(seqs))(*[s.handle for s in seqs])
+        n = (C.c_uint32 * len(seqs))(*counts)
+        rows = KvRows(k=_ptr(k), v=_ptr(v), k_stride=_stride(k), v_stride=_stride(v), offset=offset,
+                      positions=_ptr(positions), q=_ptr(q), q_out=_ptr(q_out), heads=num_heads,
+                      q_stride=_stride(q), q_out_stride=_stride(q_out))
+        if rotary is not None:
+            rows.rotary = C.pointer(rotary)
+        _check(self.lib.qm_kv_append(self.handle, arr, n, len(seqs), C.byref(rows)))
+
+    def gqa_attention(self, seqs, q, gate, num_heads: int, o) -> None:
+        """The query of every sequence's last cached token over all its tokens (qm_attn_decode_cached)."""
+        arr = (C.c_void_p * len(seqs))(*[s.handle for s in seqs])
+        _check(self.lib.qm_attn_decode_cached(self.handle, arr, len(seqs), _ptr(q), _ptr(gate), num_heads, _ptr(o)))
+
+    def gqa_attention_prefill(self, seq, q, gate, num_heads: int, rows: int, o) -> None:
+        """Causal attention of the last `rows` cached tokens (qm_attn_prefill_cached)."""
+        _check(self.lib.qm_attn_prefill_cached(self.handle, seq.handle, _ptr(q), _ptr(gate), num_heads, rows, _ptr(o)))
 
     def gqa_attention_q8(self, seqs, q, gate, k, v, num_heads: int, o) -> None:
         arr = (C.c_void_p * len(seqs))(*[s.handle for s in seqs])
@@ -541,16 +594,18 @@ class DecodeGraph:
 
 
 class KvCache:
-    """Paged Q8 KV cache (Q8KvState + LogicalPageTable)."""
+    """Paged KV cache in 8 bits (Q8KvState + LogicalPageTable) or 4."""
 
     def __init__(self, rt: Runtime, kv_heads: int, head_dim: int, page_tokens: int, max_tokens: int,
-                 handle=None):
+                 handle=None, bits: int = 8):
         self.rt = rt
+        self.bits = bits
         self.kv_heads = kv_heads
         self.head_dim = head_dim
         if handle is None:
             h = C.c_void_p()
-            _check(rt.lib.qm_kv_create(rt.handle, kv_heads, head_dim, page_tokens, max_tokens, C.byref(h)))
+            create = rt.lib.qm_kv_create_q4 if bits == 4 else rt.lib.qm_kv_create
+            _check(create(rt.handle, kv_heads, head_dim, page_tokens, max_tokens, C.byref(h)))
             handle = h
         self.handle = handle
         rt._children.add(self)
@@ -591,14 +646,25 @@ class KvCache:
     def clone(self) -> "KvCache":
         h = C.c_void_p()
         _check(self.rt.lib.qm_kv_clone(self.handle, C.byref(h)))
-        return KvCache(self.rt, self.kv_heads, self.head_dim, 16, 0, handle=h)
+        return KvCache(self.rt, self.kv_heads, self.head_dim, 16, 0, handle=h, bits=self.bits)
+
+    def load(self, first: int, count: int, k, v) -> None:
+        """Tokens first .. first + count - 1 as bf16 [count][kv_heads][head_dim]; k or v may be None."""
+        _check(self.rt.lib.qm_kv_load(self.rt.handle, self.handle, first, count, _ptr(k), _ptr(v)))
 
     def read(self):
-        """Returns (keys int8 [T][KVH][d], values, key_scales f32 [T][KVH], value_scales)."""
+        """Returns (keys int8 [T][KVH][d], values, key_scales f32 [T][KVH], value_scales);
+        of a 4-bit cache the scales are bf16 bits uint16 [T][KVH][groups][2]."""
         import numpy as np
         T = self.sequence_length
         keys = np.zeros((T, self.kv_heads, self.head_dim), np.int8)
         values = np.zeros_like(keys)
+        if self.bits == 4:
+            ks = np.zeros((T, self.kv_heads, -(-self.head_dim // 64), 2), np.uint16)
+            vs = np.zeros_like(ks)
+            _check(self.rt.lib.qm_kv_read_q4(self.handle, keys.ctypes.data, values.ctypes.data, ks.ctypes.data,
+                                             vs.ctypes.data))
+            return keys, values, ks, vs
         ks = np.zeros((T, self.kv_heads), np.float32)
         vs = np.zeros_like(ks)
         _check(self.rt.lib.qm_kv_read(self.handle, keys.ctypes.data, values.ctypes.data, ks.ctypes.data,
