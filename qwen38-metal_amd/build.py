@@ -39,6 +39,7 @@ COMMON = [
 # otherwise park them in AGPRs and copy them back every step).
 PER_FILE = {
     "q8_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "q4kv_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     # The score products in VGPRs; the sums then take the AGPRs without copies.
     "latent_expanded.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "latent_absorbed.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],

@@ -85,6 +85,9 @@ hipError_t attn_noalloc_scratch(int device, AttnScratch* out);
 hipError_t attn_noalloc_begin(int device, hipStream_t stream);
 hipError_t attn_noalloc_end(int device, hipStream_t stream);
 
+// Merges the split partials of a decode or prefill launch into its outputs.
+void launch_attn_combine(const AttnArgs& a, hipStream_t st);
+
 hipError_t launch_q8_append(const AppendArgs& a, uint32_t items, hipStream_t st);
 // Decode: `units` workgroups; when need_combine, q8_combine_kernel merges the
 // split partials (which must be set) in a second launch.

@@ -88,6 +88,17 @@ __device__ __forceinline__ uint32_t q4kv_group(const float (&x)[4], uint32_t d0,
   return sb | mb << 16;
 }
 
+// Eight codes of a K word as bf16 of 128 + (c + 8), in order: 0x4300 | u is the bf16
+// 128 + u.  Both constants in registers that the compiler cannot see through: it
+// then takes one AND-OR a pair (two literals would make it two operations).
+struct Q4KvUnpack {
+  uint32_t mask = 0x000F000Fu, one = 0x43004300u;
+  __device__ __forceinline__ Q4KvUnpack() { asm("" : "+s"(mask), "+v"(one)); }
+  __device__ __forceinline__ u32x4 operator()(uint32_t w) const {
+    return u32x4{(w & mask) | one, ((w >> 4) & mask) | one, ((w >> 8) & mask) | one, ((w >> 12) & mask) | one};
+  }
+};
+
 // What a code stands for (the product is exact: one rounding).
 __device__ __forceinline__ float q4kv_value(int c, uint32_t word) {
   return __builtin_fmaf((float)c, bf16_to_f32(word & 0xFFFFu), __uint_as_float(word & 0xFFFF0000u));

@@ -38,14 +38,11 @@
 
 #include <mutex>
 
-#include "attention.h"
-#include "common.h"
+#include "attention_device.h"
 #include "kv_quant.h"
 
 namespace qm {
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
 
 // A row's values 4 lane .. 4 lane + 3 (zero past dr): one 16-byte load when
 // dr is a multiple of 4.
@@ -85,23 +82,6 @@ __device__ __forceinline__ void q8_store_row(const AttnSeq& sq, const float* src
     }
   }
   if (lane == 0) (kind == 0 ? sq.ks : sq.vs)[pkv * 16 + slot] = s;
-}
-
-// Eight bf16 of a query/gate row starting at element d0, zero past the real
-// dimension dr; `full` (dr == Dp) takes one 16-byte load.
-__device__ __forceinline__ u32x4 load_bf16x8(const uint16_t* row, uint32_t d0, uint32_t dr, bool full) {
-  if (full) return *(const u32x4*)(row + d0);
-  uint32_t h[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) h[e] = d0 + e < dr ? (uint32_t)row[d0 + e] : 0u;
-  return u32x4{h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16)};
-}
-
-// Physical page of logical page p: pages materialised by this call are not
-// in the device table until this call writes them.
-__device__ __forceinline__ int32_t page_id(const AttnSeq& sq, uint32_t p) {
-  return sq.new_page_count > 0 && (int32_t)p >= sq.new_page_first ? sq.new_page_id + ((int32_t)p - sq.new_page_first)
-                                                                 : sq.pt[p];
 }
 
 // ---------------------------------------------------------------------------
@@ -183,10 +163,6 @@ __global__ __launch_bounds__(64 * kAppendWaves) void q8_append_pages_kernel(Appe
 // ---------------------------------------------------------------------------
 // Decode: pages stream through a per-wave LDS ring by buffer->LDS DMA
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, uint32_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
-}
-
 // Lane i's `size` bytes land at lds + i*size.  The builtin exists only in the
 // device pass; the host pass of single-source HIP must not see it.
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -221,15 +197,6 @@ __device__ __forceinline__ uint32_t k_chunk_slot(uint32_t tok, uint32_t j) {
   return tok * kChunks + (j ^ sw);
 }
 
-// Two fp32 values -> packed bf16 (round to nearest even, v_cvt_pk_bf16_f32).
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
-  const bf16x2_t v = {(__bf16)lo, (__bf16)hi};
-  return __builtin_bit_cast(uint32_t, v);
-}
-__device__ __forceinline__ float bf16_lo_f32(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float bf16_hi_f32(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
-
 // 4 int8 -> fp16 of 1024 + (int8 + 128), exact: (0x64 << 8 | u) is the fp16
 // 1024 + u.  Element order (b0, b2), (b1, b3): one AND-OR per pair.
 __device__ __forceinline__ u32x2 q8x4_to_f16_biased(uint32_t w) {
@@ -254,32 +221,10 @@ __device__ __forceinline__ floatx4 mfma16x16x32_f16(u32x4 a, u32x4 b, floatx4 c)
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c,
                                                 0, 0, 0);
 }
-// Maximum over the four lanes l, l^16, l^32, l^48 (the kq lanes of one MFMA
-// column) with the gfx950 row-swap permutes instead of LDS shuffles.
-__device__ __forceinline__ float max4_across_kq(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  // fmaxf is v_max_f32 (one operation; the operands are never NaN), where a
-  // compare and select would be two plus a VCC hazard wait.
-  const float m = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
 __device__ __forceinline__ floatx16 mfma32x32x16_f16(u32x4 a, u32x4 b, floatx16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0,
                                                 0, 0);
 }
-// Maximum over lanes l and l ^ 32 (the two halves of one 32-wide MFMA column).
-__device__ __forceinline__ float max2_across_halves(float v) {
-  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
-}
-
-template <bool B>
-struct BoolTag {
-  static constexpr bool value = B;
-};
-
 template <int D, int W>
 struct DecodeLds {
   static constexpr int kWaves = W;
@@ -287,8 +232,7 @@ struct DecodeLds {
   static constexpr int kK = 16 * D, kV = 16 * D, kS = 512;  // K, V, scales (K 256 B + V 256 B)
   static constexpr int kPage = kK + kV + kS;
   static constexpr int kWaveRing = kRing * kPage;
-  static constexpr int kPad = 17;  // floats per (wave, d) row of the O reduction (16 columns + 1)
-  static constexpr int kRed = W * D * kPad * 4 + (3 * W + 2) * 16 * 4;  // O, m, l, weights, max, sums
+  static constexpr int kRed = kMergeBytes<D, W>;
   static constexpr int kBytes = W * kWaveRing > kRed ? W * kWaveRing : kRed;
 };
 
@@ -545,75 +489,7 @@ __global__ __launch_bounds__(64 * W) void q8_decode_kernel(AttnArgs args) {
       }
   }
 
-  // ---- combine the waves of the workgroup ------------------------------------
-  float l_tot = l_lane + __shfl_xor(l_lane, 16);
-  l_tot += __shfl_xor(l_tot, 32);
-  __syncthreads();  // the rings are reused for the reduction
-  constexpr int kPad = L::kPad;
-  float* red_o = reinterpret_cast<float*>(lds);  // [wave][d][kPad]
-  float(*red_m)[16] = reinterpret_cast<float(*)[16]>(lds + kWaves * D * kPad * 4);
-  float(*red_l)[16] = red_m + kWaves;
-#pragma unroll
-  for (int db = 0; db < kDB; ++db)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) red_o[(wave * D + 16 * db + 4 * kq + r) * kPad + col] = o[db][r];
-  if (kq == 0) {
-    red_m[wave][col] = m_run;
-    red_l[wave][col] = l_tot;
-  }
-  __syncthreads();
-  // Per (wave, column) weights exp2(m_w - max) and the column sums, once;
-  // the element loop below is then multiply-adds only.
-  float(*red_f)[16] = red_l + kWaves;  // [wave][col]
-  float* red_mx = red_l[2 * kWaves];
-  float* red_L = red_mx + 16;
-  if (threadIdx.x < 16) {
-    const uint32_t c = threadIdx.x;
-    float mx = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, red_m[w][c]);
-    float Ls = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float f = red_m[w][c] == -INFINITY ? 0.0f : exp2f(red_m[w][c] - mx);
-      red_f[w][c] = f;
-      Ls += f * red_l[w][c];
-    }
-    red_mx[c] = mx;
-    red_L[c] = Ls;
-  }
-  __syncthreads();
-  const uint32_t nsplit = sq.nsplit;
-  // Split partials: O [split row][H][D], then (m, l) [split row][H][2];
-  // q8_combine_kernel merges them after this launch.
-  const size_t o_rows = (size_t)args.part_rows * H;
-  float* po = args.partials;
-  float* pm = args.partials + o_rows * D;
-  constexpr uint32_t kD4 = D / 4;
-  for (uint32_t e = threadIdx.x; e < gh * kD4; e += 64 * kWaves) {
-    const uint32_t c = e / kD4, d0 = 4 * (e % kD4);
-    floatx4 O = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) O[i] += red_f[w][c] * red_o[(w * D + d0 + i) * kPad + c];
-    const uint32_t hh = kvh * gh + c;
-    if (nsplit == 1) {
-      const float inv = 1.0f / fmaxf(red_L[c], FLT_MIN);
-      const size_t oi = ((size_t)b * H + hh) * dr + d0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (d0 + i >= dr) break;
-        float v = O[i] * inv;
-        if (args.gate) v *= sigmoid_f(bf16_to_f32(args.gate[oi + i]));
-        args.o[oi + i] = f32_to_bf16(v);
-      }
-    } else {
-      const size_t row = (size_t)(sq.part_begin + split) * H + hh;
-      *(floatx4*)(po + row * D + d0) = O;
-      if (d0 == 0) *(float2*)(pm + row * 2) = float2{red_mx[c], red_L[c]};
-    }
-  }
+  decode_merge<D, W>(args, sq, b, kvh, split, lds, o, m_run, l_lane);
 }
 
 // Merge the split partials of one (sequence, head, 32-wide d slice): grid
@@ -771,37 +647,6 @@ __global__ __launch_bounds__(64) void q8_combine_small_kernel(AttnArgs args) {
       args.o[oi + e] = f32_to_bf16(v);
     }
   }
-}
-
-// Sigmoid of a bf16 gate.  A bf16 (8 bits) times log2(e) cut to 16 bits is exact,
-// and what the cut takes from the exponential goes into the Newton step of the
-// reciprocal.  Over every bf16 gate from -87 up: at most 1.95 ulp, 0.250 rms,
-// where expf and an IEEE division (sigmoid_f) have 1.98 and 0.252; a sigmoid
-// below the smallest normal number is zero.  The limits, which pass NaN on,
-// keep infinities out of the products.  A wave ends with up to 128 of these in
-// a row, and a short prompt waits for that: 2 rows of 24 / 4 heads of 256 take
-// 17.2 us a call, 23.6 with sigmoid_f and the integer form of f32_to_bf16.
-__device__ __forceinline__ float gate_sigmoid(float x) {
-  constexpr float kCut = 1.44268798828125f;
-  constexpr float kRest = (float)((1.0 - 1.4426950408889634 / kCut) * 0.6931471805599453);
-  const float t = __builtin_elementwise_maximum(__builtin_elementwise_minimum(x * -kCut, 127.0f), -126.0f);
-  const float e = __builtin_amdgcn_exp2f(t), d = 1.0f + e, q = __builtin_amdgcn_rcpf(d);
-  const float n = __builtin_fmaf(e * (t * kRest), q, __builtin_fmaf(-d, q, 1.0f));
-  return __builtin_fmaf(n, q, q);
-}
-
-// Four outputs as bf16, and with the sigmoid of four bf16 gates.
-__device__ __forceinline__ u32x2 bf16x4_of(floatx4 v) {
-  return u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-}
-__device__ __forceinline__ u32x2 gated_bf16x4(floatx4 v, u32x2 gate) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t w = i < 2 ? gate.x : gate.y;
-    const float x = i & 1 ? bf16_hi_f32(w) : bf16_lo_f32(w);
-    v[i] *= gate_sigmoid(x);
-  }
-  return bf16x4_of(v);
 }
 
 // Causal prefill on 32x32x16 MFMA.  The rows of one KV head are a list of
@@ -1220,10 +1065,14 @@ __global__ __launch_bounds__(256) void q8_combine_rows_kernel(AttnArgs args) {
 
 template <int D>
 void launch_combine(const AttnArgs& a, uint32_t rows, uint32_t max_split, hipStream_t st) {
-  if (max_split <= 32)
+  if (a.prefill && max_split <= (uint32_t)kRowSplits) {
+    const size_t items = (size_t)a.rows * a.heads * (D / 4);
+    hipLaunchKernelGGL(q8_combine_rows_kernel<D>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, a);
+  } else if (max_split <= 32) {
     hipLaunchKernelGGL(q8_combine_small_kernel<D>, dim3(rows * a.heads * (D / 32)), dim3(64), 0, st, a);
-  else
+  } else {
     hipLaunchKernelGGL(q8_combine_kernel<D>, dim3(rows * a.heads * (D / 32)), dim3(256), 0, st, a);
+  }
 }
 
 template <int D, int W>
@@ -1231,12 +1080,7 @@ hipError_t launch_prefill(const AttnArgs& a, hipStream_t st) {
   const uint32_t cols = a.rows * (a.heads / a.kv_heads);
   const uint32_t units = a.kv_heads * ((cols + 32 * W - 1) / (32 * W)) * a.splits;
   hipLaunchKernelGGL((q8_prefill_kernel<D, W>), dim3(units), dim3(64 * W), 0, st, a);
-  if (a.splits > 1 && a.splits <= (uint32_t)kRowSplits) {
-    const size_t items = (size_t)a.rows * a.heads * (D / 4);
-    hipLaunchKernelGGL(q8_combine_rows_kernel<D>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, a);
-  } else if (a.splits > 1) {
-    launch_combine<D>(a, a.rows, a.splits, st);
-  }
+  if (a.splits > 1) launch_attn_combine(a, st);
   return hipGetLastError();
 }
 
@@ -1251,15 +1095,25 @@ hipError_t launch_attn_d(const AttnArgs& a, uint32_t units, bool need_combine, h
     hipLaunchKernelGGL((q8_decode_kernel<D, 8>), dim3(units), dim3(512), 0, st, a);
   else
     hipLaunchKernelGGL((q8_decode_kernel<D, 4>), dim3(units), dim3(256), 0, st, a);
-  if (need_combine) {
-    uint32_t max_split = 0;
-    for (uint32_t i = 0; i < a.n_seqs; ++i) max_split = max_split > a.seqs[i].nsplit ? max_split : a.seqs[i].nsplit;
-    launch_combine<D>(a, a.n_seqs, max_split, st);
-  }
+  if (need_combine) launch_attn_combine(a, st);
   return hipGetLastError();
 }
 
 }  // namespace
+
+void launch_attn_combine(const AttnArgs& a, hipStream_t st) {
+  uint32_t max_split = a.splits;
+  if (!a.prefill) {
+    max_split = 0;
+    for (uint32_t i = 0; i < a.n_seqs; ++i) max_split = max_split > a.seqs[i].nsplit ? max_split : a.seqs[i].nsplit;
+  }
+  const uint32_t rows = a.prefill ? a.rows : a.n_seqs;
+  switch (a.head_dim_pad) {
+    case 64: launch_combine<64>(a, rows, max_split, st); break;
+    case 128: launch_combine<128>(a, rows, max_split, st); break;
+    default: launch_combine<256>(a, rows, max_split, st); break;
+  }
+}
 
 hipError_t launch_q8_append(const AppendArgs& a, uint32_t items, hipStream_t st) {
   if (items == 0) return hipSuccess;
