@@ -92,6 +92,8 @@ hipError_t launch_q8_append(const AppendArgs& a, uint32_t items, hipStream_t st)
 // Decode: `units` workgroups; when need_combine, q8_combine_kernel merges the
 // split partials (which must be set) in a second launch.
 hipError_t launch_q8_attention(const AttnArgs& a, uint32_t units, bool need_combine, hipStream_t st);
+// Workgroups that share the query heads of a KV head in decode over 4-bit caches.
+constexpr uint32_t q4kv_head_sets(uint32_t heads_per_kv) { return (heads_per_kv + 7) / 8; }
 // The same over 4-bit caches (q4kv_attention.hip).
 hipError_t launch_q4kv_attention(const AttnArgs& a, uint32_t units, bool need_combine, hipStream_t st);
 

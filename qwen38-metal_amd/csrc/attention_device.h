@@ -99,15 +99,17 @@ constexpr int kMergeBytes = W * D * kMergePad * 4 + (3 * W + 2) * 16 * 4;
 
 // Ends a decode workgroup: its waves' sums (lane (col, kq) holds o[db][r] for d = 16
 // db + 4 kq + r of column col, m_run of it and its own share of l) meet in LDS and
-// leave as outputs, or as one split's partials.  Every wave of the workgroup calls it.
-template <int D, int W>
-__device__ __forceinline__ void decode_merge(const AttnArgs& args, const AttnSeq& sq, uint32_t b, uint32_t kvh,
-                                             uint32_t split, uint8_t* lds, const floatx4 (&o)[D / 16], float m_run,
-                                             float l_lane) {
-  constexpr int kWaves = W, kDB = D / 16, kPad = kMergePad;
+// leave as outputs, or as one split's partials.  Head head0 + c (of n_heads) has
+// columns c, c + 16 / S, ...: S sums of disjoint tokens.  Every wave of the
+// workgroup calls it.
+template <int D, int W, int S>
+__device__ __forceinline__ void decode_merge(const AttnArgs& args, const AttnSeq& sq, uint32_t b, uint32_t head0,
+                                             uint32_t n_heads, uint32_t split, uint8_t* lds,
+                                             const floatx4 (&o)[D / 16], float m_run, float l_lane) {
+  constexpr int kWaves = W, kDB = D / 16, kPad = kMergePad, kCols = 16 / S;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, kq = lane >> 4;
-  const uint32_t H = args.heads, gh = H / args.kv_heads, dr = args.head_dim;
+  const uint32_t H = args.heads, dr = args.head_dim;
   float l_tot = l_lane + __shfl_xor(l_lane, 16);
   l_tot += __shfl_xor(l_tot, 32);
   __syncthreads();  // the rings are reused for the reduction
@@ -128,18 +130,23 @@ __device__ __forceinline__ void decode_merge(const AttnArgs& args, const AttnSeq
   float(*red_f)[16] = red_l + kWaves;  // [wave][col]
   float* red_mx = red_l[2 * kWaves];
   float* red_L = red_mx + 16;
-  if (threadIdx.x < 16) {
+  if (threadIdx.x < kCols) {
     const uint32_t c = threadIdx.x;
     float mx = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, red_m[w][c]);
+    for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+      for (int s = 0; s < S; ++s) mx = fmaxf(mx, red_m[w][c + kCols * s]);
     float Ls = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float f = red_m[w][c] == -INFINITY ? 0.0f : exp2f(red_m[w][c] - mx);
-      red_f[w][c] = f;
-      Ls += f * red_l[w][c];
-    }
+    for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const uint32_t cs = c + kCols * s;
+        const float f = red_m[w][cs] == -INFINITY ? 0.0f : exp2f(red_m[w][cs] - mx);
+        red_f[w][cs] = f;
+        Ls += f * red_l[w][cs];
+      }
     red_mx[c] = mx;
     red_L[c] = Ls;
   }
@@ -151,14 +158,17 @@ __device__ __forceinline__ void decode_merge(const AttnArgs& args, const AttnSeq
   float* po = args.partials;
   float* pm = args.partials + o_rows * D;
   constexpr uint32_t kD4 = D / 4;
-  for (uint32_t e = threadIdx.x; e < gh * kD4; e += 64 * kWaves) {
+  for (uint32_t e = threadIdx.x; e < n_heads * kD4; e += 64 * kWaves) {
     const uint32_t c = e / kD4, d0 = 4 * (e % kD4);
     floatx4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < kWaves; ++w)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) O[i] += red_f[w][c] * red_o[(w * D + d0 + i) * kPad + c];
-    const uint32_t hh = kvh * gh + c;
+      for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          O[i] += red_f[w][c + kCols * s] * red_o[(w * D + d0 + i) * kPad + c + kCols * s];
+    const uint32_t hh = head0 + c;
     if (nsplit == 1) {
       const float inv = 1.0f / fmaxf(red_L[c], FLT_MIN);
       const size_t oi = ((size_t)b * H + hh) * dr + d0;

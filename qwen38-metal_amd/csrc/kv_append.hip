@@ -180,7 +180,7 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvAppendArgs a) {
       if (mine) {
         if ((lane & 1) == 0) *(uint32_t*)(k_img + q4kv_k_word(Dp, slot, d0)) = w;
         *(uint32_t*)(v_codes + slot * Dp + d0) =
-            (vc[0] & 15) | (vc[1] & 15) << 8 | (vc[2] & 15) << 16 | (vc[3] & 15) << 24;
+            (vc[0] + 8) | (vc[1] + 8) << 8 | (vc[2] + 8) << 16 | (vc[3] + 8) << 24;
         if (i16 == 0) {
           scales[q4kv_scale_word(Dp, 0, g, slot)] = kw;
           scales[q4kv_scale_word(Dp, 1, g, slot)] = vw;
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(kThreads) void kv_load_kernel(KvLoadArgs a) {
       for (int e = 0; e < 4; ++e) {
         const uint32_t vc = *(const uint32_t*)(kv + q4kv_v_bytes(Dp) + q4kv_v_word(Dp, slot, d0 + e));
         k[e] = q4kv_value((int)(kc >> q4kv_k_bit(d0 + e) & 15) - 8, kw);
-        v[e] = q4kv_value((int)((vc >> q4kv_v_bit(slot, d0 + e) & 15) ^ 8) - 8, vw);
+        v[e] = q4kv_value((int)(vc >> q4kv_v_bit(slot, d0 + e) & 15) - 8, vw);
       }
     } else {
       const float ks = a.p.ks[block * 16 + slot], vs = a.p.vs[block * 16 + slot];

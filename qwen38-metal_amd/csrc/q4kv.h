@@ -10,13 +10,12 @@
 //     of it in nibble (e >> 1) + 4 (e & 1), as c + 8: masks of one shifted word are
 //     pairs (e, e + 1) of bf16 operands.
 //   V, 8 Dp bytes: the lane of (d % 16, kq) holds tokens 4 kq .. 4 kq + 3 of its d's;
-//     word j holds d / 16 = 2 j in its low half and 2 j + 1 in its high half, a
-//     token each nibble, as c in two's complement.
+//     word j holds d / 16 = 2 j and 2 j + 1, token r of the four in nibble
+//     2 (d / 16 % 2) + (r >> 1) + 4 (r & 1), as c + 8: pairs of tokens again.
 //   Words 0..3 of a lane are 16 bytes, words 4..7 (Dp = 256) the 16 bytes 1024
 //   further; with Dp = 64 a lane has two words.
-//   Scales, 2 Dp bytes: a word per (K or V, group, token), s in its low half and m
-//     in its high one, at q4kv_scale_word: the 16 lanes that share kq load the
-//     words of tokens 4 kq .. 4 kq + 3.
+//   Scales, 2 Dp bytes: token by token a word per group of K, then of V, s in its low
+//     half and m in its high one.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -43,12 +42,11 @@ __host__ __device__ constexpr uint32_t q4kv_v_word(uint32_t dp, uint32_t token, 
   return q4kv_lane_word(dp, 16 * (token / 4) + d % 16, d / 32);
 }
 __host__ __device__ constexpr uint32_t q4kv_v_bit(uint32_t token, uint32_t d) {
-  return 16 * (d / 16 % 2) + 4 * (token % 4);
+  return 4 * (2 * (d / 16 % 2) + (token % 4 >> 1) + 4 * (token & 1));
 }
 // Index of the scale word of (kind: 0 K, 1 V; group; token).
 __host__ __device__ constexpr uint32_t q4kv_scale_word(uint32_t dp, uint32_t kind, uint32_t group, uint32_t token) {
-  const uint32_t item = 4 * group + token % 4;
-  return dp == 256 ? 64 * kind + 16 * (token / 4) + item : dp / 8 * (token / 4) + dp / 16 * kind + item;
+  return dp / 32 * token + dp / 64 * kind + group;
 }
 
 }  // namespace qm

@@ -15,12 +15,8 @@ namespace {
 
 // Exponent of values whose weights are kept low, so that sums of up to 2^22 of them stay finite.
 constexpr int kBigValue = 96;
+constexpr float kBigSize = 0x1p92f;  // of a scale or offset that may hold one
 
-// One value of each DPP row for all 16 lanes of the row.
-template <int I>
-__device__ __forceinline__ float row_bcast(float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + I, 0xF, 0xF, true));
-}
 template <int N, class F>
 __device__ __forceinline__ void static_for(F f) {
   if constexpr (N > 0) {
@@ -29,14 +25,36 @@ __device__ __forceinline__ void static_for(F f) {
   }
 }
 
-// Two words of signed nibbles (tokens 4 kq .. + 3 of d / 16 = 2 j, low half, and 2 j + 1)
-// as bf16 of 16 c, exact.
-__device__ __forceinline__ void v_operand(uint32_t w, u32x2& even, u32x2& odd) {
-  const uint32_t hi = w & 0xF0F0F0F0u, lo = (w << 4) & 0xF0F0F0F0u;
-  even = u32x2{pack_bf16x2((float)(int8_t)lo, (float)(int8_t)hi),
-               pack_bf16x2((float)(int8_t)(lo >> 8), (float)(int8_t)(hi >> 8))};
-  odd = u32x2{pack_bf16x2((float)(int8_t)(lo >> 16), (float)(int8_t)(hi >> 16)),
-              pack_bf16x2((float)(int8_t)(lo >> 24), (float)(int8_t)(hi >> 24))};
+// Products with one lane's value of every quad, x[r] (op)= (lane r's value) * y[r]: the
+// broadcast rides on the multiplication as a DPP operand.  (The compiler folds it
+// into plain products only; a multiply-add would get a copy.)  Each block begins
+// with the two wait states that a DPP read needs after a VALU write.
+#define QM_QUAD(op, x, v, y, r) op " %" #x ", %" #v ", %" #y " quad_perm:[" #r "," #r "," #r "," #r "] row_mask:0xf bank_mask:0xf\n"
+// x[r] = v_r * y
+__device__ __forceinline__ void quad_mul(float (&x)[4], float v, float y) {
+  asm("s_nop 1\n" QM_QUAD("v_mul_f32_dpp", 0, 4, 5, 0) QM_QUAD("v_mul_f32_dpp", 1, 4, 5, 1)
+      QM_QUAD("v_mul_f32_dpp", 2, 4, 5, 2) QM_QUAD("v_mul_f32_dpp", 3, 4, 5, 3)
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]) : "v"(v), "v"(y));
+}
+// x[r] += v_r * y
+__device__ __forceinline__ void quad_fma(float (&x)[4], float v, float y) {
+  asm("s_nop 1\n" QM_QUAD("v_fmac_f32_dpp", 0, 4, 5, 0) QM_QUAD("v_fmac_f32_dpp", 1, 4, 5, 1)
+      QM_QUAD("v_fmac_f32_dpp", 2, 4, 5, 2) QM_QUAD("v_fmac_f32_dpp", 3, 4, 5, 3)
+      : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]) : "v"(v), "v"(y));
+}
+// x[r] = v_r * y[r], sum += u_r * y[r]
+__device__ __forceinline__ void quad_mul_sum(float (&x)[4], float& sum, float v, float u, const float (&y)[4]) {
+  asm("s_nop 1\n" QM_QUAD("v_mul_f32_dpp", 0, 5, 7, 0) QM_QUAD("v_fmac_f32_dpp", 4, 6, 7, 0)
+      QM_QUAD("v_mul_f32_dpp", 1, 5, 8, 1) QM_QUAD("v_fmac_f32_dpp", 4, 6, 8, 1)
+      QM_QUAD("v_mul_f32_dpp", 2, 5, 9, 2) QM_QUAD("v_fmac_f32_dpp", 4, 6, 9, 2)
+      QM_QUAD("v_mul_f32_dpp", 3, 5, 10, 3) QM_QUAD("v_fmac_f32_dpp", 4, 6, 10, 3)
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "+v"(sum)
+      : "v"(v), "v"(u), "v"(y[0]), "v"(y[1]), "v"(y[2]), "v"(y[3]));
+}
+#undef QM_QUAD
+template <int R>
+__device__ __forceinline__ float quad_bcast(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), R * 0x55, 0xF, 0xF, true));
 }
 
 // Eight bf16 of a query row from element d0 on, zero past the real dimension dr.
@@ -45,11 +63,11 @@ __device__ __forceinline__ u32x4 load_q8(const uint16_t* row, uint32_t d0, uint3
   return load_bf16x8(row, d0, dr, false);
 }
 
-// What the words of a lane hold of one page (layout: q4kv.h).
+// A lane's words of a pair of pages: codes of both, and the scale words (K's groups,
+// then V's) of one token of one of them.
 template <int D>
-struct PageRegs {
-  static constexpr int kW = D / 32, kS = D == 256 ? 2 : 1;
-  uint32_t k[kW], v[kW], s[kS];
+struct PairRegs {
+  uint32_t k[2][D / 32], v[2][D / 32], s[D / 32];
 };
 template <int D>
 __device__ __forceinline__ void load_part(__amdgpu_buffer_rsrc_t r, uint32_t base, int lane, uint32_t (&w)[D / 32]) {
@@ -66,34 +84,48 @@ __device__ __forceinline__ void load_part(__amdgpu_buffer_rsrc_t r, uint32_t bas
   }
 }
 
+// Decode: a workgroup takes up to 8 query heads of one KV head and a split of the
+// pages.  Every wave walks its pages two at a time, straight from memory into
+// registers, and the 16 columns of a matrix operand are 8 heads times the two pages:
+//   S^T[token][column] = K Q^T with queries of zero in the other page's columns, so both
+//   pages' products add up in one accumulator, each in its columns;
+//   a lane's four scores are tokens 4 kq .. + 3 of its column's page, and its quad holds
+//   these tokens' scale words, a lane each;
+//   O^T[d][column] += V^T P'^T with both pages' tokens along K and P' of zero for
+//   the other page.
+// A column's softmax is its page's alone; decode_merge joins the columns of a head.
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(AttnArgs args) {
-  constexpr int G = D / 64, kDB = D / 16, kRing = D == 256 ? 4 : 8;
-  // Two waves a SIMD of D = 256 have no registers for the Q operand, which is the
-  // same for all of them: it lies in LDS.
+  constexpr int G = D / 64, kDB = D / 16, kRing = D == 256 ? 2 : 4;  // pairs of pages in flight
+  // Two waves a SIMD of D = 256 have no registers for the Q operands, which are the
+  // same for all of them: they lie in LDS.
   constexpr bool kTight = D == 256;
-  constexpr int kQBytes = kTight ? 2 * G * 1024 : 0;
+  constexpr int kQBytes = kTight ? 4 * G * 1024 : 0;
   __shared__ __attribute__((aligned(16))) uint8_t lds[kMergeBytes<D, W> + kQBytes];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, kq = lane >> 4;
+  const bool in_b = col >= 8;
+  const uint32_t mask_b = in_b ? ~0u : 0u, mask_a = ~mask_b;
   const uint32_t H = args.heads, KVH = args.kv_heads, gh = H / KVH;
 
   uint32_t b = 0;
   const uint32_t unit = blockIdx.x;
   while (b + 1 < args.n_seqs && unit >= args.seqs[b + 1].unit_begin) ++b;
   const AttnSeq& sq = args.seqs[b];
-  const uint32_t u = unit - sq.unit_begin;
-  const uint32_t kvh = u % KVH, split = u / KVH;
+  const uint32_t u = unit - sq.unit_begin, sets = q4kv_head_sets(gh);
+  const uint32_t kvh = u % KVH, set = u / KVH % sets, split = u / (KVH * sets);
+  const uint32_t per_set = (gh + sets - 1) / sets;
+  const uint32_t head0 = kvh * gh + set * per_set, n_heads = min(per_set, gh - set * per_set);
   // Tokens read from pages: all but the one that this call brings.
   const bool append = args.k_new != nullptr;
   const uint32_t visible = sq.len - (append ? 1 : 0);
   const uint32_t pages = (visible + 15) / 16;
   const uint32_t p_begin = min(pages, split * args.pages_per_split);
   const uint32_t p_end = min(pages, p_begin + args.pages_per_split);
-  const bool col_ok = (uint32_t)col < gh;
-  const uint32_t head = kvh * gh + col;
+  const uint32_t head = head0 + (col & 7);
+  const bool col_ok = (uint32_t)(col & 7) < n_heads;
   const uint32_t dr = args.head_dim;
   const float sm_scale = kLog2e / sqrtf((float)dr);
 
@@ -107,31 +139,46 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(AttnArgs args) {
     return j < n_mine ? sq.pt[first + W * j] : 0;
   };
   int32_t ids = load_ids(0), ids_next = load_ids(64);
-  const size_t block = (size_t)q4kv_block_bytes(D);
-  // A page past the wave's last reads nothing: a buffer of no bytes.
+  constexpr size_t block = q4kv_block_bytes(D);
+  const uint32_t s_at = q4kv_scale_bytes(D) + 4 * q4kv_scale_word(D, 0, 0, 4 * kq + (lane & 3));
+  // Pages j (even) and j + 1.  Codes of a page past the wave's last read nothing: a
+  // buffer of no bytes.
   auto load = [&](uint32_t j) __attribute__((always_inline)) {
     if ((j & 63) == 0 && j > 0) {
       ids = ids_next;
       ids_next = load_ids(j + 64);
     }
-    const int32_t phys = __builtin_amdgcn_readlane(ids, (int)(j & 63));
-    const __amdgpu_buffer_rsrc_t r =
-        make_rsrc((const uint8_t*)sq.k + ((size_t)phys * KVH + kvh) * block, j < n_mine ? (uint32_t)block : 0u);
-    PageRegs<D> p;
-    load_part<D>(r, 0, lane, p.k);
-    if constexpr (D == 256) {
-      p.s[0] = __builtin_amdgcn_raw_buffer_load_b32(r, q4kv_scale_bytes(D) + 4 * lane, 0, 0);
-      p.s[1] = __builtin_amdgcn_raw_buffer_load_b32(r, q4kv_scale_bytes(D) + 256 + 4 * lane, 0, 0);
-    } else {
-      const uint32_t at = D == 128 ? lane : 8 * kq + (lane & 7);
-      p.s[0] = __builtin_amdgcn_raw_buffer_load_b32(r, q4kv_scale_bytes(D) + 4 * at, 0, 0);
+    PairRegs<D> p;
+    const uint8_t* page[2];
+    __amdgpu_buffer_rsrc_t r[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int32_t phys = __builtin_amdgcn_readlane(ids, (int)((j + h) & 63));
+      page[h] = (const uint8_t*)sq.k + ((size_t)phys * KVH + kvh) * block;
+      r[h] = make_rsrc(page[h], j + h < n_mine ? (uint32_t)block : 0u);
+      load_part<D>(r[h], 0, lane, p.k[h]);
     }
-    load_part<D>(r, q4kv_v_bytes(D), lane, p.v);
+    // (A page id past the last is 0, whose memory is there.)
+    const uint8_t* sp = (in_b ? page[1] : page[0]) + s_at;
+    if constexpr (D == 64) {
+      const u32x2 x = *(const u32x2*)sp;
+      p.s[0] = x.x, p.s[1] = x.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < D / 128; ++i) {
+        const u32x4 x = *(const u32x4*)(sp + 16 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p.s[4 * i + e] = x[e];
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) load_part<D>(r[h], q4kv_v_bytes(D), lane, p.v[h]);
     return p;
   };
 
-  // Q operand (B of K Q^T): the lane's 16 elements of every group, d = 64 g + 16 kq .. + 15.
-  u32x4 qb[kTight ? 1 : 2 * G];
+  // Q operands (B of K Q^T) of both pages: the lane's 16 elements of every group, d = 64 g
+  // + 16 kq .. + 15.
+  u32x4 qb[2][kTight ? 1 : 2 * G];
   u32x4* ql = (u32x4*)(lds + kMergeBytes<D, W>) + lane;
   {
     const uint16_t* qp = args.q + ((size_t)b * H + head) * dr;
@@ -143,17 +190,25 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(AttnArgs args) {
 #pragma unroll
       for (int j = 0; j < 2 * G / W; ++j) x[j] = q_part(wave + W * j);
 #pragma unroll
-      for (int j = 0; j < 2 * G / W; ++j) ql[64 * (wave + W * j)] = x[j];
+      for (int j = 0; j < 2 * G / W; ++j) {
+        ql[64 * (wave + W * j)] = x[j] & mask_a;
+        ql[64 * (2 * G + wave + W * j)] = x[j] & mask_b;
+      }
     } else {
+      u32x4 x[2 * G];
 #pragma unroll
-      for (int j = 0; j < 2 * G; ++j) qb[j] = q_part(j);
+      for (int j = 0; j < 2 * G; ++j) x[j] = q_part(j);
+#pragma unroll
+      for (int j = 0; j < 2 * G; ++j) qb[0][j] = x[j] & mask_a, qb[1][j] = x[j] & mask_b;
     }
   }
-  auto q_of = [&](int j) __attribute__((always_inline)) { return kTight ? ql[64 * j] : qb[kTight ? 0 : j]; };
-  PageRegs<D> ring[kRing];
+  auto q_of = [&](int h, int j) __attribute__((always_inline)) {
+    return kTight ? ql[64 * (2 * G * h + j)] : qb[h][kTight ? 0 : j];
+  };
+  PairRegs<D> ring[kRing];
 #pragma unroll
   for (int r = 0; r < kRing; ++r) {
-    ring[r] = load(r);
+    ring[r] = load(2 * r);
     // In order, or the loop's first wait would be for all of them.
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -165,7 +220,7 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(AttnArgs args) {
     float x = 0.0f;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const u32x4 q = q_of(2 * g + j);
+      const u32x4 q = q_of(0, 2 * g + j) | q_of(1, 2 * g + j);
 #pragma unroll
       for (int i = 0; i < 4; ++i) x += bf16_lo_f32(q[i]) + bf16_hi_f32(q[i]);
     }
@@ -177,21 +232,24 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(AttnArgs args) {
 #pragma unroll
   for (int i = 0; i < kDB; ++i) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
   float om[G] = {};  // what the values' offsets add, a group each (this lane's tokens)
+  floatx4 ow[G];     // -136 sums of P' since they last went into o (four times the same)
+#pragma unroll
+  for (int g = 0; g < G; ++g) ow[g] = floatx4{0.f, 0.f, 0.f, 0.f};
   float m_run = -INFINITY, l_lane = 0.0f;
 
   // ---- the token that this call brings ---------------------------------------
   // A wave with the fewest pages of the last split quantises it, writes it into its
-  // page and starts its own softmax from it: no other wave waits, and nobody reads
-  // the token back.  (Waves that read the page meanwhile see its other tokens'
-  // nibbles in either version of a word, and give the new one no weight.)
+  // page (for the first heads' workgroup) and starts its own softmax from it: no
+  // other wave waits, and nobody reads the token back.  (Waves that read the page
+  // meanwhile see its other tokens' nibbles in either version of a word, and give
+  // the new one no weight.)
   if (append && split + 1 == sq.nsplit && wave == (int)((p_end - p_begin) % W)) {
     const uint32_t token = sq.len - 1, slot = token % 16;
     const bool fresh = sq.new_page_count > 0;
     const int32_t phys = fresh ? sq.new_page_id : sq.pt[token / 16];
-    if (fresh && kvh == 0 && lane == 0) sq.pt[token / 16] = phys;
     uint8_t* page = (uint8_t*)sq.k + ((size_t)phys * KVH + kvh) * block;
     float* xs = (float*)lds;               // values as the codes have them, K then V
-    uint8_t* cs = lds + 2 * D * 4;         // codes, c & 15
+    uint8_t* cs = lds + 2 * D * 4;         // codes, c + 8
     uint32_t old[D / 32];                  // the lane's V words of the page
 #pragma unroll
     for (int w = 0; w < D / 32; ++w) old[w] = *(const uint32_t*)(page + q4kv_v_bytes(D) + q4kv_lane_word(D, lane, w));
@@ -203,42 +261,50 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(AttnArgs args) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[kind][e] = d0 + e < dr ? src[d0 + e] : 0.0f;
     }
+    uint32_t word[2];
 #pragma unroll
     for (int kind = 0; kind < 2; ++kind) {
       int c[4];
-      const uint32_t w = q4kv_group(x[kind], d0, dr, c);
+      word[kind] = q4kv_group(x[kind], d0, dr, c);
       if (kq >= G) continue;  // (copies of the first groups)
       floatx4 y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = q4kv_value(c[e], w);
+      for (int e = 0; e < 4; ++e) y[e] = q4kv_value(c[e], word[kind]);
       *(floatx4*)(xs + D * kind + d0) = y;
-      *(uint32_t*)(cs + D * kind + d0) = (c[0] & 15) | (c[1] & 15) << 8 | (c[2] & 15) << 16 | (c[3] & 15) << 24;
-      if (col == 0) *(uint32_t*)(page + q4kv_scale_bytes(D) + 4 * q4kv_scale_word(D, kind, g, slot)) = w;
+      *(uint32_t*)(cs + D * kind + d0) = (c[0] + 8) | (c[1] + 8) << 8 | (c[2] + 8) << 16 | (c[3] + 8) << 24;
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    if ((uint32_t)col == slot) {
+    if (set == 0) {
+      if (fresh && kvh == 0 && lane == 0) sq.pt[token / 16] = phys;
+      if (col == 0 && kq < G) {
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        const uint8_t* c = cs + 64 * (j / 2) + 16 * kq + 8 * (j % 2);
-        uint32_t w = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w |= (uint32_t)(c[e] ^ 8) << q4kv_k_bit(e);
-        *(uint32_t*)(page + q4kv_lane_word(D, lane, j)) = w;
+        for (int kind = 0; kind < 2; ++kind)
+          *(uint32_t*)(page + q4kv_scale_bytes(D) + 4 * q4kv_scale_word(D, kind, g, slot)) = word[kind];
       }
-    }
-    if ((uint32_t)kq == slot / 4) {
+      if ((uint32_t)col == slot) {
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        const uint32_t sh = 4 * (slot % 4), c = cs[D + 32 * j + col] | cs[D + 32 * j + 16 + col] << 16;
-        *(uint32_t*)(page + q4kv_v_bytes(D) + q4kv_lane_word(D, lane, j)) = (old[j] & ~(0x000F000Fu << sh)) | c << sh;
+        for (int j = 0; j < D / 32; ++j) {
+          const uint8_t* c = cs + 64 * (j / 2) + 16 * kq + 8 * (j % 2);
+          uint32_t w = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w |= (uint32_t)c[e] << q4kv_k_bit(e);
+          *(uint32_t*)(page + q4kv_lane_word(D, lane, j)) = w;
+        }
+      }
+      if ((uint32_t)kq == slot / 4) {
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          const uint32_t sh = q4kv_v_bit(slot, 0), c = cs[D + 32 * j + col] | cs[D + 32 * j + 16 + col] << 8;
+          *(uint32_t*)(page + q4kv_v_bytes(D) + q4kv_lane_word(D, lane, j)) = (old[j] & ~(0x0F0Fu << sh)) | c << sh;
+        }
       }
     }
     float dot = 0.0f;
 #pragma unroll
     for (int j = 0; j < 2 * G; ++j) {
       const float* y = xs + 64 * (j / 2) + 16 * kq + 8 * (j % 2);
-      const u32x4 q = q_of(j);
+      const u32x4 q = q_of(0, j);
 #pragma unroll
       for (int i = 0; i < 4; ++i) dot += bf16_lo_f32(q[i]) * y[2 * i] + bf16_hi_f32(q[i]) * y[2 * i + 1];
     }
@@ -250,77 +316,61 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(AttnArgs args) {
     for (int i = 0; i < G; ++i) size = fmaxf(size, fabsf(xs[D + 64 * i + lane]));
     size = wave_allmax(size);
     const float excess = fmaxf(0.0f, (float)((int)(__float_as_uint(size) >> 23) - 127 - kBigValue));
-    const float p = exp2f(-excess);
-    m_run = dot * sm_scale + excess;
+    const float p = in_b ? 0.0f : exp2f(-excess);
+    if (!in_b) m_run = dot * sm_scale + excess;
     l_lane = kq == 0 ? p : 0.0f;
+    if (!in_b) {
 #pragma unroll
-    for (int db = 0; db < kDB; ++db) o[db] = *(const floatx4*)(xs + D + 16 * db + 4 * kq) * p;
+      for (int db = 0; db < kDB; ++db) o[db] = *(const floatx4*)(xs + D + 16 * db + 4 * kq) * p;
+    }
     if (dot != dot) l_lane = dot;  // a NaN in the query or the key
   }
 
-  const Q4KvUnpack k_operand;
-  // Scores of two pages, S^T[token][col]: codes enter as 128 + (c + 8), exactly, and the
-  // sums start 136 sums of the queries lower.
-  auto qk = [&](const PageRegs<D>& pa, const PageRegs<D>& pb, float (&sc)[8]) __attribute__((always_inline)) {
-    const float sa = bf16_lo_f32(pa.s[0]) * sm_scale, ma = bf16_hi_f32(pa.s[0]) * sm_scale;
-    const float sb = bf16_lo_f32(pb.s[0]) * sm_scale, mb = bf16_hi_f32(pb.s[0]) * sm_scale;
+  const Q4KvUnpack unpack;
+  const u32x4 minus136 = {0xC308C308u, 0xC308C308u, 0xC308C308u, 0xC308C308u};
+  auto step = [&](PairRegs<D>& pg, uint32_t j, auto may_be_last) __attribute__((always_inline)) {
+    const bool last = decltype(may_be_last)::value && j + 2 >= n_mine;
+    // This lane's page: its first token of four, and the end of what it may see.
+    const uint32_t t0 = (first + W * (j + (in_b ? 1 : 0))) * 16 + 4 * kq;
+    const uint32_t end = in_b && j + 1 >= n_mine ? 0 : visible;
+    if (last && t0 + (lane & 3) >= end) {  // tokens past the last one have neither scale nor offset
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) pg.s[i] = 0;
+    }
+    // Scores: codes enter as 128 + (c + 8), exactly, and the sums start 136 sums of the
+    // queries lower.
+    float x[4];
     static_for<G>([&](auto gi) __attribute__((always_inline)) {
       constexpr int g = gi;
       const float c0 = -136.0f * qs[g];
-      floatx4 a = {c0, c0, c0, c0}, c = a;
-      const u32x4 q0 = q_of(2 * g), q1 = q_of(2 * g + 1);
-      a = mfma16x16x32(k_operand(pa.k[2 * g]), q0, a);
-      c = mfma16x16x32(k_operand(pb.k[2 * g]), q0, c);
-      a = mfma16x16x32(k_operand(pa.k[2 * g + 1]), q1, a);
-      c = mfma16x16x32(k_operand(pb.k[2 * g + 1]), q1, c);
+      floatx4 acc = {c0, c0, c0, c0};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 2 * g; i < 2 * g + 2; ++i) acc = mfma16x16x32(unpack(pg.k[h][i]), q_of(h, i), acc);
+      const float sk = bf16_lo_f32(pg.s[g]) * sm_scale, mk = bf16_hi_f32(pg.s[g]) * sm_scale;
+      if (g == 0) quad_mul(x, mk, qs[g]);
+      else quad_fma(x, mk, qs[g]);
       static_for<4>([&](auto ri) __attribute__((always_inline)) {
-        constexpr int r = ri, i = 4 * g + r;
-        const float xa = row_bcast<i>(ma) * qs[g], xb = row_bcast<i>(mb) * qs[g];
-        sc[r] = __builtin_fmaf(row_bcast<i>(sa), a[r], g ? sc[r] + xa : xa);
-        sc[4 + r] = __builtin_fmaf(row_bcast<i>(sb), c[r], g ? sc[4 + r] + xb : xb);
+        constexpr int r = ri;
+        x[r] = __builtin_fmaf(quad_bcast<r>(sk), acc[r], x[r]);
       });
       if constexpr (kTight) __builtin_amdgcn_sched_barrier(0);
     });
-  };
-  // Two pages a step: two independent score chains, one look at the running maximum,
-  // then P'V with both pages' tokens in the K dimension.
-  auto step = [&](PageRegs<D>& pa, PageRegs<D>& pb, uint32_t ja, auto may_be_last) __attribute__((always_inline)) {
-    const bool last = decltype(may_be_last)::value && ja + 2 >= n_mine;
-    constexpr int kVi = D == 256 ? 0 : 4 * G;  // the V items of a row's scale words
-    const uint32_t ta = (first + W * ja) * 16 + 4 * kq, tb = ta + 16 * W;
-    const bool has_b = ja + 1 < n_mine;
-    if (last) {  // tokens past the last one have neither scale nor offset
-#pragma unroll
-      for (int i = 0; i < PageRegs<D>::kS; ++i) {
-        if (ta + (lane & 3) >= visible) pa.s[i] = 0;
-        if (!has_b || tb + (lane & 3) >= visible) pb.s[i] = 0;
-      }
-    }
-    float sc[8];
-    qk(pa, pb, sc);
     if (last) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (ta + r >= visible) sc[r] = -INFINITY;
-        if (!has_b || tb + r >= visible) sc[4 + r] = -INFINITY;
-      }
+      for (int r = 0; r < 4; ++r)
+        if (t0 + r >= end) x[r] = -INFINITY;
     }
-    float bmax = sc[0];
-#pragma unroll
-    for (int r = 1; r < 8; ++r) bmax = fmaxf(bmax, sc[r]);
-    bmax = max4_across_kq(bmax);
+    float bmax = max4_across_kq(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
     // Values above 2^kBigValue weigh less from the start, so that their sums stay
     // finite: the reference covers score and size.
-    const uint32_t wa = pa.s[PageRegs<D>::kS - 1], wb = pb.s[PageRegs<D>::kS - 1];
-    {
-      constexpr uint32_t kS = (127 + kBigValue - 4) << 7, kM = (127 + kBigValue) << 7;
-      const bool big = (D == 256 || (lane & 15) >= kVi) && ((wa & 0x7F80u) >= kS || (wb & 0x7F80u) >= kS ||
-                                                            (wa >> 16 & 0x7F80u) >= kM || (wb >> 16 & 0x7F80u) >= kM);
-      if (__builtin_amdgcn_ballot_w64(big)) {
-        const uint32_t e = max(max(wa >> 7 & 0xFF, wb >> 7 & 0xFF) + 4, max(wa >> 23 & 0xFF, wb >> 23 & 0xFF));
-        bmax += wave_allmax(big ? (float)e - (127 + kBigValue) : 0.0f);
-      }
-    }
+    float size = 0.0f;
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      size = fmaxf(size, fmaxf(bf16_lo_f32(pg.s[G + g]), fabsf(bf16_hi_f32(pg.s[G + g]))));
+    if (__builtin_amdgcn_ballot_w64(size > kBigSize))
+      bmax += fmaxf(0.0f, wave_allmax((float)(int)(__float_as_uint(size) >> 23)) + (4 - 127 - kBigValue));
     // Lazy rescaling: the reference only moves when a score exceeds it by more than
     // 2^8 (see the 8-bit kernel).
     const float m_new = bmax > m_run + 8.0f ? bmax : m_run;
@@ -331,66 +381,69 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(AttnArgs args) {
 #pragma unroll
       for (int db = 0; db < kDB; ++db) o[db] *= corr;
 #pragma unroll
-      for (int g = 0; g < G; ++g) om[g] *= corr;
+      for (int g = 0; g < G; ++g) om[g] *= corr, ow[g] *= corr;
     }
     m_run = m_new;
-    float p[8];
+    float p[4];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      p[r] = __builtin_amdgcn_exp2f(sc[r] - m_new);
+    for (int r = 0; r < 4; ++r) {
+      p[r] = __builtin_amdgcn_exp2f(x[r] - m_new);
+      // (a column that has seen nothing: its reference is -inf too)
+      if (decltype(may_be_last)::value && x[r] == -INFINITY) p[r] = 0.0f;
       l_lane += p[r];
     }
-    // P' = p s / 16 as bf16 hi + lo (error 2^-17), a group each; V enters as signed
-    // codes times 16: nothing accumulates into O but sum_t s c p.
-    const float sa = bf16_lo_f32(wa) * 0.0625f, ma = bf16_hi_f32(wa);
-    const float sb = bf16_lo_f32(wb) * 0.0625f, mb = bf16_hi_f32(wb);
+    // P' = p s as bf16 hi + lo (error 2^-17), a group each.  Values enter as 128 + (c + 8)
+    // too; the sum of 136 P' that they bring along is formed by the same operands
+    // against -136, so its roundings of P' are the same, and goes into O every round.
     static_for<G>([&](auto gi) __attribute__((always_inline)) {
       constexpr int g = gi;
-      float w[8];
-      static_for<4>([&](auto ri) __attribute__((always_inline)) {
-        constexpr int r = ri, i = kVi + 4 * g + r;
-        w[r] = p[r] * row_bcast<i>(sa);
-        w[4 + r] = p[4 + r] * row_bcast<i>(sb);
-        om[g] += row_bcast<i>(ma) * p[r];
-        om[g] += row_bcast<i>(mb) * p[4 + r];
-      });
-      u32x4 hi, lo;
+      float w[4];
+      quad_mul_sum(w, om[g], bf16_lo_f32(pg.s[G + g]), bf16_hi_f32(pg.s[G + g]), p);
+      const uint32_t h01 = pack_bf16x2(w[0], w[1]), h23 = pack_bf16x2(w[2], w[3]);
+      const uint32_t l01 = pack_bf16x2(w[0] - bf16_lo_f32(h01), w[1] - bf16_hi_f32(h01));
+      const uint32_t l23 = pack_bf16x2(w[2] - bf16_lo_f32(h23), w[3] - bf16_hi_f32(h23));
+      const u32x4 hi = {h01 & mask_a, h23 & mask_a, h01 & mask_b, h23 & mask_b};
+      const u32x4 lo = {l01 & mask_a, l23 & mask_a, l01 & mask_b, l23 & mask_b};
+      ow[g] = mfma16x16x32(minus136, hi, ow[g]);
+      ow[g] = mfma16x16x32(minus136, lo, ow[g]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        hi[i] = pack_bf16x2(w[2 * i], w[2 * i + 1]);
-        lo[i] = pack_bf16x2(w[2 * i] - bf16_lo_f32(hi[i]), w[2 * i + 1] - bf16_hi_f32(hi[i]));
-      }
-#pragma unroll
-      for (int j = 2 * g; j < 2 * g + 2; ++j) {
-        u32x2 ae, ao, be, bo;
-        v_operand(pa.v[j], ae, ao);
-        v_operand(pb.v[j], be, bo);
-        const u32x4 even = {ae.x, ae.y, be.x, be.y}, odd = {ao.x, ao.y, bo.x, bo.y};
-        o[2 * j] = mfma16x16x32(even, hi, o[2 * j]);
-        o[2 * j + 1] = mfma16x16x32(odd, hi, o[2 * j + 1]);
-        o[2 * j] = mfma16x16x32(even, lo, o[2 * j]);
-        o[2 * j + 1] = mfma16x16x32(odd, lo, o[2 * j + 1]);
+      for (int i = 2 * g; i < 2 * g + 2; ++i) {
+        const u32x4 va = unpack(pg.v[0][i]), vb = unpack(pg.v[1][i]);
+        const u32x4 even = {va.x, va.y, vb.x, vb.y}, odd = {va.z, va.w, vb.z, vb.w};
+        o[2 * i] = mfma16x16x32(even, hi, o[2 * i]);
+        o[2 * i + 1] = mfma16x16x32(odd, hi, o[2 * i + 1]);
+        o[2 * i] = mfma16x16x32(even, lo, o[2 * i]);
+        o[2 * i + 1] = mfma16x16x32(odd, lo, o[2 * i + 1]);
         if constexpr (kTight) __builtin_amdgcn_sched_barrier(0);
       }
     });
+  };
+  auto settle = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+#pragma unroll
+      for (int db = 4 * g; db < 4 * g + 4; ++db) o[db] += ow[g];
+      ow[g] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
   };
 
   // Whole rounds of the ring, then what is left.  (A round that could end early would
   // make every wait in it one for nearly all loads.)
   uint32_t i = 0;
-  for (; i + kRing < n_mine; i += kRing) {
+  for (; i + 2 * kRing < n_mine; i += 2 * kRing) {
 #pragma unroll
-    for (int s = 0; s < kRing; s += 2) {
-      step(ring[s], ring[s + 1], i + s, BoolTag<false>{});
-      ring[s] = load(i + s + kRing);
-      ring[s + 1] = load(i + s + 1 + kRing);
+    for (int s = 0; s < kRing; ++s) {
+      step(ring[s], i + 2 * s, BoolTag<false>{});
+      ring[s] = load(i + 2 * s + 2 * kRing);
     }
+    settle();
   }
 #pragma unroll
-  for (int s = 0; s < kRing; s += 2) {
-    if (i + s >= n_mine) break;
-    step(ring[s], ring[s + 1], i + s, BoolTag<true>{});
+  for (int s = 0; s < kRing; ++s) {
+    if (i + 2 * s >= n_mine) break;
+    step(ring[s], i + 2 * s, BoolTag<true>{});
   }
+  settle();
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     float x = om[g] + __shfl_xor(om[g], 16);
@@ -398,7 +451,7 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(AttnArgs args) {
 #pragma unroll
     for (int db = 4 * g; db < 4 * g + 4; ++db) o[db] += x;
   }
-  decode_merge<D, W>(args, sq, b, kvh, split, lds, o, m_run, l_lane);
+  decode_merge<D, W, 2>(args, sq, b, head0, n_heads, split, lds, o, m_run, l_lane);
 }
 
 template <int D>
@@ -445,7 +498,7 @@ __global__ __launch_bounds__(64) void q4kv_attention_kernel(AttnArgs args) {
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       const uint32_t d = 64 * g + lane;
-      const int c = (int)((*(const uint32_t*)(kv + q4kv_v_bytes(D) + q4kv_v_word(D, slot, d)) >> q4kv_v_bit(slot, d) & 15) ^ 8) - 8;
+      const int c = (int)(*(const uint32_t*)(kv + q4kv_v_bytes(D) + q4kv_v_word(D, slot, d)) >> q4kv_v_bit(slot, d) & 15) - 8;
       o[g] = o[g] * r + p * q4kv_value(c, scales[q4kv_scale_word(D, 1, g, slot)]);
     }
   }

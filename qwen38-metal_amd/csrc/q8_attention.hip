@@ -489,7 +489,7 @@ __global__ __launch_bounds__(64 * W) void q8_decode_kernel(AttnArgs args) {
       }
   }
 
-  decode_merge<D, W>(args, sq, b, kvh, split, lds, o, m_run, l_lane);
+  decode_merge<D, W, 1>(args, sq, b, kvh * gh, gh, split, lds, o, m_run, l_lane);
 }
 
 // Merge the split partials of one (sequence, head, 32-wide d slice): grid

@@ -216,8 +216,9 @@ struct DecodeChunk {
 // one 8-wave workgroup per CU if the splits fit that (measured faster at 32K:
 // the CU's waves share one split), else two 4-wave workgroups per CU.
 // `extra`: tokens that the call appends to each sequence (1 or 0).
-qm_status plan_decode_chunk(qm_runtime* rt, qm_kv* const* seqs, uint32_t nb, uint32_t extra, DecodeChunk* c) {
-  const uint32_t KVH = seqs[0]->kv_heads;
+qm_status plan_decode_chunk(qm_runtime* rt, qm_kv* const* seqs, uint32_t nb, uint32_t H, uint32_t extra, DecodeChunk* c) {
+  // Workgroups of a split.
+  const uint32_t KVH = seqs[0]->kv_heads * (seqs[0]->bits == 4 ? q4kv_head_sets(H / seqs[0]->kv_heads) : 1);
   AttnArgs& at = c->at;
   uint64_t total_pages = 0;
   uint32_t max_pages = 0;
@@ -355,7 +356,7 @@ qm_status plan_decode(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, uint32_t H
   for (uint32_t b0 = 0; b0 < B; b0 += kMaxAttnSeqs) {
     DecodeChunk c;
     const uint32_t nb = std::min<uint32_t>(kMaxAttnSeqs, B - b0);
-    qm_status st = plan_decode_chunk(rt, seqs + b0, nb, extra, &c);
+    qm_status st = plan_decode_chunk(rt, seqs + b0, nb, H, extra, &c);
     if (st != QM_OK) return st;
     c.at.n_seqs = nb;
     chunks->push_back(c);
@@ -723,7 +724,7 @@ qm_status qm_kv_read_q4(const qm_kv* kv, int8_t* keys, int8_t* values, uint16_t*
         if (keys) keys[row * D + d] = (int8_t)((int)(word(q4kv_k_word(Dp, slot, d)) >> q4kv_k_bit(d) & 15) - 8);
         if (values)
           values[row * D + d] =
-              (int8_t)((int)((word(q4kv_v_bytes(Dp) + q4kv_v_word(Dp, slot, d)) >> q4kv_v_bit(slot, d) & 15) ^ 8) - 8);
+              (int8_t)((int)(word(q4kv_v_bytes(Dp) + q4kv_v_word(Dp, slot, d)) >> q4kv_v_bit(slot, d) & 15) - 8);
       }
       for (uint32_t g = 0; g < G; ++g)
         for (uint32_t kind = 0; kind < 2; ++kind) {
