@@ -80,6 +80,11 @@ __device__ __forceinline__ uint32_t q4kv_group(const float (&x)[4], uint32_t d0,
   const float s = bf16_to_f32(sb);
   const uint32_t mb = f32_to_bf16(s * 8.0f - low);
   const float m = bf16_to_f32(mb);
+  if (!(fabsf(m) < INFINITY)) {  // (a middle past bf16's range)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[e] = 0;
+    return 0x7FC07FC0u;
+  }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const float t = (x[e] - m) / s;

@@ -454,70 +454,505 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(AttnArgs args) {
   decode_merge<D, W, 2>(args, sq, b, head0, n_heads, split, lds, o, m_run, l_lane);
 }
 
-template <int D>
-__global__ __launch_bounds__(64) void q4kv_attention_kernel(AttnArgs args) {
+// Causal prefill on 32x32x16 MFMA; columns, tiles, splits and the two LDS stages as in
+// the 8-bit kernel.  A tile's 32 tokens are unpacked once per workgroup:
+//   K as its codes in bf16 (16 c, exact), so a group's product is exact and its scale
+//     and offset act on the scores: x = sum_g s_g (K_g Q_g) + m_g (sum of Q_g).  The
+//     second part and the running reference come from one more matrix instruction,
+//     whose K dimension holds m_g against three bf16 terms of the sums, and ones
+//     against three of minus the reference.
+//   V as values in fp16, each token under a power of two of its own, 2^-E: the weight of
+//     P V is then w = p 2^(E - R) in fp16, one product instead of the two of a split P'
+//     (V and w round by 2^-11 at most each).  R is the largest E so far, O is in units of
+//     2^R, and a column's reference keeps its w between 2^-24 and 2^15.5: what is lost
+//     is below 2^-36 of the largest w.  Tokens whose values are over 2^80 below the
+//     largest up to their tile lose bits.
+// The tables of a tile (scales, offsets, powers) are formed a tile ahead of its
+// unpacking by one wave, from one load.
+template <int D, int W>
+struct PrefillLds {
+  static constexpr int G = D / 64;
+  static constexpr int kK = 32 * D * 2, kV = 32 * D * 2, kStage = kK + kV;
+  // A tile's tables: K scales [G][32], K offsets as matrix operand [2][32] of 16 bytes,
+  // weights 2^(E - R) [32], V scales and offsets [G][32] of 8 bytes, then 2^(R before -
+  // R), and tokens with NaN values, a word per group.
+  static constexpr int kKb = G * 128, kEv = kKb + 1024, kVs = kEv + 128, kMisc = kVs + G * 256, kTab = kMisc + 32;
+  static constexpr int kTabs = 2 * kStage;
+  static constexpr int kQ = kTabs + 3 * kTab;
+  // Steps of the Q operand that wait in LDS: half of them where D = 256 leaves two
+  // waves a SIMD no registers for all.
+  static constexpr int kQSteps = D == 256 && W == 8 ? D / 32 : 0;
+  static constexpr int kBytes = kQ + W * kQSteps * 1024;
+};
+
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t){a, b}, half2_t));
+}
+__device__ __forceinline__ floatx16 mfma32x32x16_f16(u32x4 a, u32x4 b, floatx16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0,
+                                                0, 0);
+}
+// x as three bf16 terms, 24 bits together.
+__device__ __forceinline__ void split3(float x, uint32_t (&t)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    t[i] = pack_bf16x2(x, 0.0f);
+    x -= bf16_lo_f32(t[i]);
+  }
+}
+// Eight codes of a K word as bf16 of 16 c, in order.
+__device__ __forceinline__ u32x4 k_codes16(uint32_t w) {
+  w ^= 0x88888888u;  // c in two's complement
+  const uint32_t hi = w & 0xF0F0F0F0u, lo = (w << 4) & 0xF0F0F0F0u;
+  auto f = [](uint32_t x, int b) { return (float)(int8_t)(x >> (8 * b)); };
+  // Nibbles of elements 0 .. 7: 0, 4, 1, 5, 2, 6, 3, 7.
+  return u32x4{pack_bf16x2(f(lo, 0), f(lo, 2)), pack_bf16x2(f(hi, 0), f(hi, 2)), pack_bf16x2(f(lo, 1), f(lo, 3)),
+               pack_bf16x2(f(hi, 1), f(hi, 3))};
+}
+
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill_kernel(AttnArgs args) {
+  using L = PrefillLds<D, W>;
   constexpr int G = D / 64;
-  const uint32_t H = args.heads, KVH = args.kv_heads, dr = args.head_dim;
-  const uint32_t row = blockIdx.x / H, head = blockIdx.x % H, kvh = head / (H / KVH);
-  const uint32_t lane = threadIdx.x;
-  const AttnSeq& sq = args.seqs[args.prefill ? 0 : row];
-  const uint32_t visible = args.prefill ? args.start + row + 1 : sq.len;
-  const float scale = kLog2e / sqrtf((float)dr);
-  float q[G], o[G];
+  constexpr int kDB = D / 32;  // 32-wide d blocks of O^T
+  constexpr int kKS = D / 16;  // QK k-steps
+  constexpr int kUnits = (4 * D + 64 * W - 1) / (64 * W);  // 8-byte units of a tile per thread
+  constexpr bool kTight = D == 256 && W == 8;
+  constexpr float kWMost = 46340.0f;  // 2^15.5: weights above it move the reference
+  __shared__ __attribute__((aligned(16))) uint8_t lds[L::kBytes];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lc = lane & 31, hf = lane >> 5;
+  const uint32_t H = args.heads, KVH = args.kv_heads, gh = H / KVH;  // gh <= 16
+  const AttnSeq& sq = args.seqs[0];
+
+  // Workgroups as in the 8-bit kernel: a KV head's on the same XCDs, the longest first.
+  const uint32_t cols = args.rows * gh;
+  const uint32_t blocks = (cols + 32 * W - 1) / (32 * W);
+  const uint32_t kvh = blockIdx.x % KVH, bs = blockIdx.x / KVH;
+  const uint32_t S = args.splits, split = bs % S, rb = blocks - 1 - bs / S;
+  const uint32_t c0 = rb * 32 * W + wave * 32;
+  // Columns past the last one repeat it and are not stored.
+  const uint32_t c = min(c0 + lc, cols - 1);
+  const bool col_ok = c0 + lc < cols;
+  const uint32_t row = c / gh, head = kvh * gh + (c - row * gh);
+  const uint32_t visible = min(args.start + row + 1, sq.len);
+
+  const uint32_t last_row = (min(cols, (rb + 1) * 32 * W) - 1) / gh;
+  const uint32_t n_tiles = (min(args.start + last_row + 1, sq.len) + 31) / 32;
+  const uint32_t t0 = (uint32_t)((uint64_t)n_tiles * split / S), t1 = (uint32_t)((uint64_t)n_tiles * (split + 1) / S);
+  const uint32_t last_page = (sq.len - 1) / 16;
+
+  const uint32_t dr = args.head_dim;
+  const float sm_scale = kLog2e / sqrtf((float)dr);
+  constexpr int kQReg = kKS - L::kQSteps;
+  u32x4 qb[kQReg];
+  u32x4* ql = (u32x4*)(lds + L::kQ) + wave * L::kQSteps * 64 + lane;  // read by the lane that wrote it
+  // What the bias product multiplies: three terms of every group's sum of queries (half
+  // 0 holds slots 0..7, half 1 slots 8..15), and of minus the reference in slots 12..14.
+  u32x4 qbias;
+  {
+    const uint16_t* qp = args.q + ((size_t)row * H + head) * dr;
+    float qs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const uint32_t d = 64 * g + lane;
-    q[g] = d < dr ? bf16_to_f32(args.q[((size_t)row * H + head) * dr + d]) : 0.0f;
-    o[g] = 0.0f;
-  }
-  float m = -INFINITY, l = 0.0f;
-  for (uint32_t t = 0; t < visible; ++t) {
-    const uint32_t slot = t % 16;
-    const uint8_t* kv = (const uint8_t*)sq.k + ((size_t)sq.pt[t / 16] * KVH + kvh) * q4kv_block_bytes(D);
-    const uint32_t* scales = (const uint32_t*)(kv + q4kv_scale_bytes(D));
-    float dot = 0.0f;
+    for (int s = 0; s < kKS; ++s) {
+      const u32x4 x = load_q8(qp, 16 * s + 8 * hf, dr);
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const uint32_t d = 64 * g + lane;
-      const int c = (int)(*(const uint32_t*)(kv + q4kv_k_word(D, slot, d)) >> q4kv_k_bit(d) & 15) - 8;
-      if (d < dr) dot += q[g] * q4kv_value(c, scales[q4kv_scale_word(D, 0, g, slot)]);
+      for (int i = 0; i < 4; ++i) qs[s / 4] += bf16_lo_f32(x[i]) + bf16_hi_f32(x[i]);
+      if (s < kQReg) qb[s] = x;
+      else ql[64 * (s - kQReg)] = x;
     }
-    const float s = wave_allsum(dot) * scale;
-    // Values above 2^96 weigh less from the start, so that their sums stay finite:
-    // the reference covers score and size.
+    uint32_t t[4][3];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) split3((qs[g] + __shfl_xor(qs[g], 32)) * sm_scale, t[g]);
+    qbias = hf == 0 ? u32x4{t[0][0] | t[0][1] << 16, t[0][2] | t[1][0] << 16, t[1][1] | t[1][2] << 16,
+                            t[2][0] | t[2][1] << 16}
+                    : u32x4{t[2][2] | t[3][0] << 16, t[3][1] | t[3][2] << 16, 0u, 0u};
+  }
+
+  floatx16 o[kDB];
+#pragma unroll
+  for (int i = 0; i < kDB; ++i) o[i] = floatx16{};
+  float m_run = 0.0f, l_lane = 0.0f;  // (the first tile sets the reference)
+
+  // A tile's 4 D 8-byte units: K of its two pages, then V (D units a page).  Kind and
+  // page are uniform over a wave.
+  struct Raw {
+    u32x2 u[kUnits];
+  };
+  struct Pages {
+    int32_t a, b;
+  };
+  auto page_ids = [&](uint32_t t) __attribute__((always_inline)) {
+    return Pages{sq.pt[min(2 * t, last_page)], sq.pt[min(2 * t + 1, last_page)]};
+  };
+  auto block_of = [&](int32_t phys) __attribute__((always_inline)) {
+    return (const uint8_t*)sq.k + ((size_t)phys * KVH + kvh) * q4kv_block_bytes(D);
+  };
+  auto fetch = [&](Pages ph, Raw& r) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const int u0 = i * 64 * W + wave * 64;
+      if (u0 < 4 * D)
+        r.u[i] = *(const u32x2*)(block_of((u0 / D) & 1 ? ph.b : ph.a) + (u0 < 2 * D ? 0 : q4kv_v_bytes(D)) +
+                                 8 * (u0 % D + lane));
+    }
+  };
+  // Scale words: lane (token, kind) of the last wave.
+  struct Words {
+    uint32_t w[G];
+  };
+  auto fetch_words = [&](Pages ph, Words& r) __attribute__((always_inline)) {
+    if (wave != W - 1) return;
+    const uint8_t* p = block_of(lc & 16 ? ph.b : ph.a) + q4kv_scale_bytes(D) + 4 * q4kv_scale_word(D, hf, 0, lc & 15);
+    if constexpr (G == 1) {
+      r.w[0] = *(const uint32_t*)p;
+    } else if constexpr (G == 2) {
+      const u32x2 x = *(const u32x2*)p;
+      r.w[0] = x.x, r.w[1] = x.y;
+    } else {
+      const u32x4 x = *(const u32x4*)p;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) r.w[g] = x[g];
+    }
+  };
+  auto table = [&](uint32_t t) __attribute__((always_inline)) { return lds + L::kTabs + t % 3 * L::kTab; };
+  int r_exp = -126;  // R: exponent of the unit of O (the last wave's)
+  auto write_table = [&](uint32_t t, Words r) __attribute__((always_inline)) {
+    if (wave != W - 1) return;
+    uint8_t* tab = table(t);
+    if (32 * t + lc >= sq.len) {  // slots past the last token hold whatever was there
+#pragma unroll
+      for (int g = 0; g < G; ++g) r.w[g] = 0;
+    }
+    // Sizes: 2^E <= max(8 s, |m|) of a token's groups, NaN aside.
     float size = 0.0f;
+    uint32_t nan = 0;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const uint32_t w = scales[q4kv_scale_word(D, 1, g, slot)];
-      size = fmaxf(size, fmaxf(bf16_to_f32(w & 0xFFFFu), fabsf(__uint_as_float(w & 0xFFFF0000u))));
+      const float s = bf16_lo_f32(r.w[g]);
+      if (s == s) size = fmaxf(size, fmaxf(8.0f * s, fabsf(bf16_hi_f32(r.w[g]))));
+      else nan |= 1u << g;
     }
-    const float mn = fmaxf(m, s + fmaxf(0.0f, (float)((int)(__float_as_uint(size) >> 23) - 127 - kBigValue)));
-    const float r = mn == -INFINITY ? 1.0f : exp2f(m - mn), p = exp2f(s - mn);
-    l = l * r + p;
-    m = mn;
+    const int e = min((int)(__float_as_uint(size) >> 23) - 127, 126);
+    const int before = r_exp;
+    r_exp = max(r_exp, (int)wave_allmax(hf ? (float)e : -126.0f));
+    uint32_t nan_tokens[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) nan_tokens[g] = (uint32_t)(__builtin_amdgcn_ballot_w64(nan >> g & 1) >> 32);
+    if (hf == 0) {
+      uint32_t m[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        *(float*)(tab + 128 * g + 4 * lc) = bf16_lo_f32(r.w[g]) * (sm_scale * 0.0625f);  // (codes are 16 c)
+        m[g] = r.w[g] >> 16;
+      }
+      *(u32x4*)(tab + L::kKb + 16 * lc) =
+          u32x4{m[0] | m[0] << 16, m[0] | m[1] << 16, m[1] | m[1] << 16, m[2] | m[2] << 16};
+      *(u32x4*)(tab + L::kKb + 512 + 16 * lc) =
+          u32x4{m[2] | m[3] << 16, m[3] | m[3] << 16, 0x3F803F80u, 0x00003F80u};
+    } else {
+      const int ec = max(e, r_exp - 80);
+      const float inv = __uint_as_float((uint32_t)(127 - max(ec, -126)) << 23);  // 2^-E (E <= 126)
+      *(float*)(tab + L::kEv + 4 * lc) = __uint_as_float((uint32_t)(127 + max(ec, -126) - r_exp) << 23);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const bool bad = nan >> g & 1;
+        const float s = bad ? 0.0f : bf16_lo_f32(r.w[g]) * inv, m = bad ? 0.0f : bf16_hi_f32(r.w[g]) * inv;
+        *(float2*)(tab + L::kVs + 256 * g + 8 * lc) = float2{s, m - 8.0f * s};  // (codes enter as c + 8)
+      }
+      if (lc == 0) {
+        *(float*)(tab + L::kMisc) = exp2f((float)(before - r_exp));
+        uint32_t any = 0;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          *(uint32_t*)(tab + L::kMisc + 8 + 4 * g) = nan_tokens[g];
+          any |= nan_tokens[g];
+        }
+        *(uint32_t*)(tab + L::kMisc + 4) = any;
+        *(float*)(tab + L::kMisc + 24) = (float)r_exp;
+      }
+    }
+  };
+  // LDS images: K 16-byte chunk (8 d) q of token t at unit 32 q + (t ^ swz), V^T chunk
+  // (page, half, d) at unit (2 page + half) D + d, where half 0 holds a page's tokens
+  // 0..3, 8..11 and half 1 tokens 4..7, 12..15.
+  auto k_swz = [](uint32_t pair) { return pair & 7; };
+  auto stage_in = [&](uint32_t t, const Raw& r, int st) __attribute__((always_inline)) {
+    uint8_t* kl = lds + st * L::kStage;
+    uint8_t* vl = kl + L::kK;
+    const uint8_t* tab = table(t);
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const int u0 = i * 64 * W + wave * 64;
+      if (u0 >= 4 * D) continue;
+      const u32x2 w = r.u[i];
+      const uint32_t pg = (u0 / D) & 1, u = u0 % D + lane;
+      const uint32_t l = D == 64 ? u : u % 128 / 2, g = D == 64 ? 0 : 2 * (u / 128) + u % 2;
+      const uint32_t low = l & 15, kq = l >> 4;
+      if (u0 < 2 * D) {
+        const uint32_t tok = 16 * pg + low, pair = 4 * g + kq;
+        uint8_t* dst = kl + 16 * (64 * pair + (tok ^ k_swz(pair)));
+        *(u32x4*)dst = k_codes16(w.x);
+        *(u32x4*)(dst + 512) = k_codes16(w.y);
+      } else {
+        const floatx4* sm = (const floatx4*)(tab + L::kVs + 256 * g + 8 * (16 * pg + 4 * kq));
+        const floatx4 a = sm[0], b = sm[1];  // (s, m) of four tokens
+        uint8_t* dst = vl + 16 * ((2 * pg + (kq & 1)) * D + 64 * g + low) + 8 * (kq >> 1);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t lo = w[j] & 0x0F0F0F0Fu, hi = (w[j] >> 4) & 0x0F0F0F0Fu;
+          // Token r of d / 16 = 2 j + k in nibble 2 k + (r >> 1) + 4 (r & 1).
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float x0 = (float)(lo >> (8 * k) & 0xFF), x1 = (float)(lo >> (8 * k + 16) & 0xFF);
+            const float x2 = (float)(hi >> (8 * k) & 0xFF), x3 = (float)(hi >> (8 * k + 16) & 0xFF);
+            *(u32x2*)(dst + 256 * (2 * j + k)) =
+                u32x2{pack_f16x2(__builtin_fmaf(x0, a.x, a.y), __builtin_fmaf(x1, a.z, a.w)),
+                      pack_f16x2(__builtin_fmaf(x2, b.x, b.y), __builtin_fmaf(x3, b.z, b.w))};
+          }
+        }
+      }
+    }
+  };
+
+  // Softmax and P V of tile t from LDS stage st.  MASKED is false for tiles every
+  // column of the wave sees whole.
+  auto compute = [&](uint32_t t, int st, auto masked) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(masked)::value;
+    const uint8_t* base = lds + st * L::kStage;
+    const u32x4* kl = (const u32x4*)base;
+    const u32x4* vl = (const u32x4*)(base + L::kK);
+    const uint8_t* tab = table(t);
+    // (the same in every lane)
+    const float unit = __uint_as_float(__builtin_amdgcn_readfirstlane(*(const uint32_t*)(tab + L::kMisc)));
+    const uint32_t nan_any = __builtin_amdgcn_readfirstlane(*(const uint32_t*)(tab + L::kMisc + 4));
+    floatx16 x = mfma32x32x16(*(const u32x4*)(tab + L::kKb + 16 * lane), qbias, floatx16{});
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const uint32_t d = 64 * g + lane;
-      const int c = (int)(*(const uint32_t*)(kv + q4kv_v_bytes(D) + q4kv_v_word(D, slot, d)) >> q4kv_v_bit(slot, d) & 15) - 8;
-      o[g] = o[g] * r + p * q4kv_value(c, scales[q4kv_scale_word(D, 1, g, slot)]);
-    }
-  }
+      floatx16 s = floatx16{};
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const uint32_t d = 64 * g + lane;
-    if (d >= dr) continue;
-    const size_t at = ((size_t)row * H + head) * dr + d;
-    float v = o[g] / l;
-    if (args.gate) v *= sigmoid_f(bf16_to_f32(args.gate[at]));
-    args.o[at] = f32_to_bf16(v);
+      for (int j = 4 * g; j < 4 * g + 4; ++j) {
+        const u32x4 ka = kl[32 * (2 * j + hf) + (lc ^ k_swz(j))];
+        s = mfma32x32x16(ka, j < kQReg ? qb[j < kQReg ? j : 0] : ql[64 * (j - kQReg)], s);
+        if constexpr (kTight) __builtin_amdgcn_sched_barrier(0);
+      }
+      const floatx4* sl = (const floatx4*)(tab + 128 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const floatx4 k = sl[2 * i + hf];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * i + e] = __builtin_fmaf(s[4 * i + e], k[e], x[4 * i + e]);
+      }
+    }
+    const floatx4* evl = (const floatx4*)(tab + L::kEv);
+    floatx4 ev[kTight ? 1 : 4];
+    if constexpr (!kTight) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ev[i] = evl[2 * i + hf];
+    }
+    auto ev_of = [&](int i) __attribute__((always_inline)) { return kTight ? evl[2 * i + hf] : ev[kTight ? 0 : i]; };
+    // Element e is token 32 t + 8 (e >> 2) + 4 hf + (e & 3).
+    float p[16];
+    float wmax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const floatx4 v = ev_of(i);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int e = 4 * i + k;
+        if (MASKED && 32 * t + 8 * i + 4 * hf + k >= visible) x[e] = -INFINITY;
+        p[e] = __builtin_amdgcn_exp2f(x[e]);
+        wmax = fmaxf(wmax, p[e] * v[k]);
+      }
+    }
+    // (unit: below 1 where the tile has a token of larger values than any before)
+    const bool move = t == t0 || unit != 1.0f || __builtin_amdgcn_ballot_w64(wmax > kWMost);
+    float shift = 0.0f;
+    if (move) {
+      float y = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const floatx4 v = ev_of(i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y = fmaxf(y, x[4 * i + k] + (float)((int)(__float_as_uint(v[k]) >> 23) - 127));
+      }
+      y = max2_across_halves(y);
+      // Whole numbers: the largest weight becomes 2^11 .. 2^12.
+      if ((t == t0 || y > 15.5f) && y > -INFINITY) shift = ceilf(y - 12.0f);
+      m_run += shift;
+      const float corr = __builtin_amdgcn_exp2f(-shift);
+      if (t != t0) {  // (nothing is there yet in the first tile, and corr may be infinite)
+        l_lane *= corr;
+#pragma unroll
+        for (int db = 0; db < kDB; ++db) o[db] *= corr * unit;
+      }
+      uint32_t r[3];
+      split3(-m_run, r);
+      if (hf) qbias.z = r[0] | r[1] << 16, qbias.w = r[2];
+    }
+    // Two waves of D = 256 have no registers for scores beside probabilities: they
+    // form them again.
+    if (move || kTight) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(x[e] - shift);
+    }
+    float psum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      u32x4 ph;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const floatx4 v = ev_of(2 * j + i);
+        const int e = 8 * j + 4 * i;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          psum[0] += p[e + 2 * k];
+          psum[1] += p[e + 2 * k + 1];
+          ph[2 * i + k] = pack_f16x2(p[e + 2 * k] * v[2 * k], p[e + 2 * k + 1] * v[2 * k + 1]);
+        }
+      }
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) {
+        o[db] = mfma32x32x16_f16(vl[(2 * j + hf) * D + 32 * db + lc], ph, o[db]);
+        if constexpr (kTight) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    l_lane += psum[0] + psum[1];
+    if (nan_any) {  // values that are NaN: of the columns that see them, and their group
+      const uint32_t n = visible > 32 * t ? visible - 32 * t : 0, seen = n >= 32 ? ~0u : (1u << n) - 1;
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+        if (*(const uint32_t*)(tab + L::kMisc + 8 + 4 * g) & seen) {
+#pragma unroll
+          for (int db = 2 * g; db < 2 * g + 2; ++db) o[db][0] = NAN;
+#pragma unroll
+          for (int db = 2 * g; db < 2 * g + 2; ++db)
+#pragma unroll
+            for (int e = 1; e < 16; ++e) o[db][e] = NAN;
+        }
+    }
+  };
+
+  // Pipeline, one barrier per tile: tile t + 1 (fetched a tile earlier) is unpacked
+  // into the other stage, the tables of tile t + 2 are written, tile t + 2 and the scale
+  // words of t + 3 are fetched, then tile t is reduced from its stage.
+  Raw raw{};
+  Words words{};
+  Pages next{}, after{};
+  if (t0 < t1) {
+    Words w1{};
+    const Pages ids = page_ids(t0);
+    fetch_words(ids, words);
+    fetch(ids, raw);
+    if (t0 + 1 < t1) {
+      next = page_ids(t0 + 1);
+      fetch_words(next, w1);
+    }
+    write_table(t0, words);
+    if (t0 + 1 < t1) write_table(t0 + 1, w1);
+    lds_barrier();
+    stage_in(t0, raw, 0);
+    if (t0 + 1 < t1) fetch(next, raw);
+    if (t0 + 2 < t1) {
+      next = page_ids(t0 + 2);
+      fetch_words(next, words);
+    }
+    if (t0 + 3 < t1) after = page_ids(t0 + 3);
   }
+  lds_barrier();
+  auto step = [&](uint32_t t, auto masked) __attribute__((always_inline)) {
+    const int st = (t - t0) & 1;
+    if (t + 1 < t1) stage_in(t + 1, raw, st ^ 1);
+    if (t + 2 < t1) {
+      write_table(t + 2, words);
+      fetch(next, raw);
+      if (t + 3 < t1) {
+        fetch_words(after, words);
+        next = after;
+        if (t + 4 < t1) after = page_ids(t + 4);
+      }
+    }
+    if (D == 128 || W == 8 || c0 < cols) compute(t, st, masked);
+    lds_barrier();
+  };
+  // Tiles below full_end are visible to every column of the wave.
+  const uint32_t first_row = min(c0, cols - 1) / gh;
+  const uint32_t full_end = min(max(min(args.start + first_row + 1, sq.len) / 32, t0), t1);
+  for (uint32_t t = t0; t < full_end; ++t) step(t, BoolTag<false>{});
+  for (uint32_t t = full_end; t < t1; ++t) step(t, BoolTag<true>{});
+
+  const float l_tot = l_lane + __shfl_xor(l_lane, 32);
+  const float unit = t0 < t1 ? __builtin_amdgcn_exp2f(*(const float*)(table(t1 - 1) + L::kMisc + 24)) : 1.0f;
+  if (!col_ok) return;
+  if (S > 1) {
+    // Partials as in decode, row by row: O [row][split][H][D], then (m, l): here O over
+    // its own sum, whose logarithm goes into m, so that it stays finite.
+    const size_t pr = ((size_t)row * S + split) * H + head;
+    float* po = args.partials + pr * D;
+    const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
+#pragma unroll
+    for (int db = 0; db < kDB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *(floatx4*)(po + 32 * db + 8 * g + 4 * hf) =
+            floatx4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]} * inv * unit;
+    if (hf == 0)
+      *(float2*)(args.partials + (size_t)args.part_rows * H * D + pr * 2) =
+          l_tot == 0.0f ? float2{-FLT_MAX, 0.0f} : float2{m_run + log2f(l_tot), 1.0f};
+    return;
+  }
+  const float inv = 1.0f / l_tot;
+  const size_t obase = ((size_t)row * H + head) * dr;
+  if (args.out8) {  // 8-byte accesses: dr % 8 == 0, o and gate aligned
+    u32x2 gt[kDB][4];
+    if (args.gate) {
+#pragma unroll
+      for (int i = 0; i < kDB * 4; ++i) {
+        const uint32_t d0 = 8 * i + 4 * hf;
+        if (d0 < dr) gt[i >> 2][i & 3] = *(const u32x2*)(args.gate + obase + d0);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kDB * 4; ++i) {
+      const uint32_t d0 = 8 * i + 4 * hf;
+      if (d0 >= dr) continue;
+      const int db = i >> 2, g = i & 3;
+      const floatx4 v = floatx4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]} * inv * unit;
+      *(u32x2*)(args.o + obase + d0) = args.gate ? gated_bf16x4(v, gt[db][g]) : bf16x4_of(v);
+    }
+  } else {
+#pragma unroll 1
+    for (int e = 0; e < 16; ++e)
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) {
+        const uint32_t d = 32 * db + 8 * (e >> 2) + 4 * hf + (e & 3);
+        if (d >= dr) continue;
+        float v = o[db][e] * inv * unit;
+        if (args.gate) v *= gate_sigmoid(bf16_to_f32(args.gate[obase + d]));
+        args.o[obase + d] = f32_to_bf16(v);
+      }
+  }
+}
+
+template <int D, int W>
+hipError_t launch_prefill(const AttnArgs& a, hipStream_t st) {
+  const uint32_t cols = a.rows * (a.heads / a.kv_heads);
+  const uint32_t units = a.kv_heads * ((cols + 32 * W - 1) / (32 * W)) * a.splits;
+  hipLaunchKernelGGL((q4kv_prefill_kernel<D, W>), dim3(units), dim3(64 * W), 0, st, a);
+  if (a.splits > 1) launch_attn_combine(a, st);
+  return hipGetLastError();
 }
 
 template <int D>
 hipError_t launch_d(const AttnArgs& a, uint32_t units, bool need_combine, hipStream_t st) {
   if (a.prefill) {
-    hipLaunchKernelGGL(q4kv_attention_kernel<D>, dim3(a.rows * a.heads), dim3(64), 0, st, a);
-    return hipGetLastError();
+    if (a.splits == 0 || (a.splits > 1 && !a.partials)) return hipErrorInvalidValue;
+    return a.wg_waves == 8 ? launch_prefill<D, 8>(a, st) : launch_prefill<D, 4>(a, st);
   }
   if (need_combine && !a.partials) return hipErrorInvalidValue;
   if (a.wg_waves == 8)
