@@ -461,33 +461,39 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(AttnArgs args) {
 //     second part and the running reference come from one more matrix instruction,
 //     whose K dimension holds m_g against three bf16 terms of the sums, and ones
 //     against three of minus the reference.
-//   V as values in fp16, each token under a power of two of its own, 2^-E: the weight of
-//     P V is then w = p 2^(E - R) in fp16, one product instead of the two of a split P'
-//     (V and w round by 2^-11 at most each).  R is the largest E so far, O is in units of
-//     2^R, and a column's reference keeps its w between 2^-24 and 2^15.5: what is lost
-//     is below 2^-36 of the largest w.  Tokens whose values are over 2^80 below the
-//     largest up to their tile lose bits.
+//   V as values in fp16 under a power of two of its tile, 2^-E: the weight of P V is
+//     w = p 2^(E - R) in fp16, one product instead of the two of a split P' (V and w
+//     round by 2^-11 at most each).  O is in units of 2^R, R the first tile's E until one
+//     is over 2^64 above it; E - R is part of the exponent, by the same bias product.  A
+//     column's reference keeps its w between 2^-24 and 2^15.5: what is lost is below
+//     2^-36 of the largest w.  Values of a token more than 2^24 below the largest of its
+//     32 lose bits, as do those of tiles more than 2^80 below an earlier one.
 // The tables of a tile (scales, offsets, powers) are formed a tile ahead of its
-// unpacking by one wave, from one load.
+// unpacking by two waves.
 template <int D, int W>
 struct PrefillLds {
   static constexpr int G = D / 64;
-  static constexpr int kK = 32 * D * 2, kV = 32 * D * 2, kStage = kK + kV;
+  // Two waves a SIMD of D = 256: half of the Q operand waits in LDS, and a tile's scores
+  // are formed, a group at a time, in the step that uses them.
+  static constexpr bool kTight = D == 256 && W == 8;
+  // One barrier a tile: K of a tile and the next, V of the last one too.
+  static constexpr int kNK = 2, kNV = kTight ? 2 : 3, kNTabs = 3;
+  static constexpr int kK = 32 * D * 2, kV = 32 * D * 2;
   // A tile's tables: K scales [G][32], K offsets as matrix operand [2][32] of 16 bytes,
-  // weights 2^(E - R) [32], V scales and offsets [G][32] of 8 bytes, then 2^(R before -
-  // R), and tokens with NaN values, a word per group.
-  static constexpr int kKb = G * 128, kEv = kKb + 1024, kVs = kEv + 128, kMisc = kVs + G * 256, kTab = kMisc + 32;
-  static constexpr int kTabs = 2 * kStage;
-  static constexpr int kQ = kTabs + 3 * kTab;
-  // Steps of the Q operand that wait in LDS: half of them where D = 256 leaves two
-  // waves a SIMD no registers for all.
-  static constexpr int kQSteps = D == 256 && W == 8 ? D / 32 : 0;
+  // V scales and offsets in fp16 [G][8 token quads] of 16 bytes, then 2^(R before - R),
+  // whether a value is NaN, such tokens, a word per group, 2^(R - E) and 2^R.
+  static constexpr int kKb = G * 128, kVs = kKb + 1024, kMisc = kVs + G * 128, kTab = kMisc + 32;
+  static constexpr int kVAt = kNK * kK, kTabs = kVAt + kNV * kV;
+  static constexpr int kIds = kTabs + kNTabs * kTab;
+  static constexpr int kQ = kIds + 512, kQSteps = kTight ? D / 32 : 0;
   static constexpr int kBytes = kQ + W * kQSteps * 1024;
 };
 
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float2_t __attribute__((ext_vector_type(2)));
+// (By value: a bit cast of a vector's element takes its first.)
+__device__ __forceinline__ half2_t as_half2(uint32_t x) { return __builtin_bit_cast(half2_t, x); }
 __device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t){a, b}, half2_t));
 }
@@ -495,6 +501,17 @@ __device__ __forceinline__ floatx16 mfma32x32x16_f16(u32x4 a, u32x4 b, floatx16 
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0,
                                                 0, 0);
 }
+// The eight codes of a V word in fp16: 0x6400 | u is the fp16 1024 + u, of which 1032
+// leaves c, exactly.
+struct Q4KvUnpackF16 {
+  uint32_t mask = 0x000F000Fu, one = 0x64006400u;
+  __device__ __forceinline__ Q4KvUnpackF16() { asm("" : "+s"(mask), "+v"(one)); }
+  __device__ __forceinline__ void operator()(uint32_t w, half2_t (&c)[4]) const {
+    const half2_t bias = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = as_half2((w >> (4 * i) & mask) | one) + bias;
+  }
+};
 // x as three bf16 terms, 24 bits together.
 __device__ __forceinline__ void split3(float x, uint32_t (&t)[3]) {
 #pragma unroll
@@ -519,9 +536,8 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
   constexpr int G = D / 64;
   constexpr int kDB = D / 32;  // 32-wide d blocks of O^T
   constexpr int kKS = D / 16;  // QK k-steps
-  constexpr int kUnits = (4 * D + 64 * W - 1) / (64 * W);  // 8-byte units of a tile per thread
-  constexpr bool kTight = D == 256 && W == 8;
-  constexpr float kWMost = 46340.0f;  // 2^15.5: weights above it move the reference
+  constexpr int kWords = 4 * D >= 64 * W ? 4 * D / (64 * W) : 1;  // words of a tile's K, and of its V, per thread
+  constexpr float kMost = 15.5f;  // exponents above it move the reference
   __shared__ __attribute__((aligned(16))) uint8_t lds[L::kBytes];
 
   const int lane = threadIdx.x & 63;
@@ -549,11 +565,13 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
 
   const uint32_t dr = args.head_dim;
   const float sm_scale = kLog2e / sqrtf((float)dr);
+  constexpr bool kTight = L::kTight;
   constexpr int kQReg = kKS - L::kQSteps;
   u32x4 qb[kQReg];
-  u32x4* ql = (u32x4*)(lds + L::kQ) + wave * L::kQSteps * 64 + lane;  // read by the lane that wrote it
+  u32x4* ql = (u32x4*)(lds + L::kQ + wave * L::kQSteps * 1024) + lane;
   // What the bias product multiplies: three terms of every group's sum of queries (half
-  // 0 holds slots 0..7, half 1 slots 8..15), and of minus the reference in slots 12..14.
+  // 0 holds slots 0..7, half 1 slots 8..15), of minus the reference in slots 12..14,
+  // and one.
   u32x4 qbias;
   {
     const uint16_t* qp = args.q + ((size_t)row * H + head) * dr;
@@ -563,7 +581,7 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
       const u32x4 x = load_q8(qp, 16 * s + 8 * hf, dr);
 #pragma unroll
       for (int i = 0; i < 4; ++i) qs[s / 4] += bf16_lo_f32(x[i]) + bf16_hi_f32(x[i]);
-      if (s < kQReg) qb[s] = x;
+      if (s < kQReg) qb[s < kQReg ? s : 0] = x;
       else ql[64 * (s - kQReg)] = x;
     }
     uint32_t t[4][3];
@@ -571,7 +589,7 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
     for (int g = 0; g < 4; ++g) split3((qs[g] + __shfl_xor(qs[g], 32)) * sm_scale, t[g]);
     qbias = hf == 0 ? u32x4{t[0][0] | t[0][1] << 16, t[0][2] | t[1][0] << 16, t[1][1] | t[1][2] << 16,
                             t[2][0] | t[2][1] << 16}
-                    : u32x4{t[2][2] | t[3][0] << 16, t[3][1] | t[3][2] << 16, 0u, 0u};
+                    : u32x4{t[2][2] | t[3][0] << 16, t[3][1] | t[3][2] << 16, 0u, 0x3F800000u};
   }
 
   floatx16 o[kDB];
@@ -579,36 +597,58 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
   for (int i = 0; i < kDB; ++i) o[i] = floatx16{};
   float m_run = 0.0f, l_lane = 0.0f;  // (the first tile sets the reference)
 
-  // A tile's 4 D 8-byte units: K of its two pages, then V (D units a page).  Kind and
-  // page are uniform over a wave.
+  // Without registers to spare, what depends on the lane alone is formed anew each step.
+  auto anew = [](int x) __attribute__((always_inline)) {
+    if (kTight) asm volatile("" : "+v"(x));
+    return x;
+  };
+  // A thread's words of a tile: kWords in a row of its 4 D words of K, and the same of V
+  // (2 D a page; the page is uniform over a wave).
   struct Raw {
-    u32x2 u[kUnits];
+    uint32_t k[kWords], v[kWords];
   };
   struct Pages {
-    int32_t a, b;
+    u32x2 id;
+  };
+  constexpr bool kAll = 4 * D >= 64 * W;  // every wave has words
+  const int page_half = wave * 64 * kWords / (2 * D);
+  const uint32_t word0 = (wave * 64 + lane) * kWords % (2 * D);
+  // Ids of the pages of 64 tiles wait in LDS, 32 tiles ahead.  (Held in registers over
+  // the loop they would be copied at its end, with a wait for every load in flight.)
+  auto load_ids = [&](uint32_t t) __attribute__((always_inline)) {  // of tiles t .. t + 31
+    ((int32_t*)(lds + L::kIds))[2 * ((t - t0) & 63) + lane] = sq.pt[min(2 * t + lane, last_page)];
   };
   auto page_ids = [&](uint32_t t) __attribute__((always_inline)) {
-    return Pages{sq.pt[min(2 * t, last_page)], sq.pt[min(2 * t + 1, last_page)]};
+    return Pages{*(const u32x2*)(lds + L::kIds + 8 * ((t - t0) & 63))};
   };
-  auto block_of = [&](int32_t phys) __attribute__((always_inline)) {
-    return (const uint8_t*)sq.k + ((size_t)phys * KVH + kvh) * q4kv_block_bytes(D);
+  auto block_of = [&](uint32_t phys) __attribute__((always_inline)) {
+    return (const uint8_t*)sq.k + ((size_t)(int32_t)phys * KVH + kvh) * q4kv_block_bytes(D);
   };
-  auto fetch = [&](Pages ph, Raw& r) __attribute__((always_inline)) {
+  auto load_words = [&](const uint8_t* p, uint32_t (&w)[kWords]) __attribute__((always_inline)) {
+    if constexpr (kWords == 1) {
+      w[0] = *(const uint32_t*)p;
+    } else if constexpr (kWords == 2) {
+      const u32x2 x = *(const u32x2*)p;
+      w[0] = x.x, w[1] = x.y;
+    } else {
+      const u32x4 x = *(const u32x4*)p;
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-      const int u0 = i * 64 * W + wave * 64;
-      if (u0 < 4 * D)
-        r.u[i] = *(const u32x2*)(block_of((u0 / D) & 1 ? ph.b : ph.a) + (u0 < 2 * D ? 0 : q4kv_v_bytes(D)) +
-                                 8 * (u0 % D + lane));
+      for (int i = 0; i < 4; ++i) w[i] = x[i];
     }
   };
-  // Scale words: lane (token, kind) of the last wave.
+  auto fetch = [&](const Pages& ph, Raw& r) __attribute__((always_inline)) {
+    if (!kAll && wave >= 4 * D / 64) return;
+    const uint8_t* p = block_of(__builtin_amdgcn_readfirstlane(page_half ? ph.id.y : ph.id.x)) + 4 * word0;
+    load_words(p, r.k);
+    load_words(p + q4kv_v_bytes(D), r.v);
+  };
+  // Scale words of K (wave 0) and V (wave 1): a token a lane, twice.
   struct Words {
     uint32_t w[G];
   };
-  auto fetch_words = [&](Pages ph, Words& r) __attribute__((always_inline)) {
-    if (wave != W - 1) return;
-    const uint8_t* p = block_of(lc & 16 ? ph.b : ph.a) + q4kv_scale_bytes(D) + 4 * q4kv_scale_word(D, hf, 0, lc & 15);
+  auto fetch_words = [&](const Pages& ph, Words& r) __attribute__((always_inline)) {
+    if (wave >= 2) return;
+    const uint8_t* p = block_of(lc & 16 ? ph.id.y : ph.id.x) + q4kv_scale_bytes(D) + 4 * q4kv_scale_word(D, wave, 0, lc & 15);
     if constexpr (G == 1) {
       r.w[0] = *(const uint32_t*)p;
     } else if constexpr (G == 2) {
@@ -620,31 +660,16 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
       for (int g = 0; g < 4; ++g) r.w[g] = x[g];
     }
   };
-  auto table = [&](uint32_t t) __attribute__((always_inline)) { return lds + L::kTabs + t % 3 * L::kTab; };
-  int r_exp = -126;  // R: exponent of the unit of O (the last wave's)
+  auto table = [&](uint32_t t) __attribute__((always_inline)) { return lds + L::kTabs + t % L::kNTabs * L::kTab; };
+  int r_exp = 0;  // R: exponent of the unit of O (wave 1's)
   auto write_table = [&](uint32_t t, Words r) __attribute__((always_inline)) {
-    if (wave != W - 1) return;
+    if (wave >= 2) return;
     uint8_t* tab = table(t);
     if (32 * t + lc >= sq.len) {  // slots past the last token hold whatever was there
 #pragma unroll
       for (int g = 0; g < G; ++g) r.w[g] = 0;
     }
-    // Sizes: 2^E <= max(8 s, |m|) of a token's groups, NaN aside.
-    float size = 0.0f;
-    uint32_t nan = 0;
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const float s = bf16_lo_f32(r.w[g]);
-      if (s == s) size = fmaxf(size, fmaxf(8.0f * s, fabsf(bf16_hi_f32(r.w[g]))));
-      else nan |= 1u << g;
-    }
-    const int e = min((int)(__float_as_uint(size) >> 23) - 127, 126);
-    const int before = r_exp;
-    r_exp = max(r_exp, (int)wave_allmax(hf ? (float)e : -126.0f));
-    uint32_t nan_tokens[G];
-#pragma unroll
-    for (int g = 0; g < G; ++g) nan_tokens[g] = (uint32_t)(__builtin_amdgcn_ballot_w64(nan >> g & 1) >> 32);
-    if (hf == 0) {
+    if (wave == 0) {
       uint32_t m[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
       for (int g = 0; g < G; ++g) {
@@ -653,137 +678,153 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
       }
       *(u32x4*)(tab + L::kKb + 16 * lc) =
           u32x4{m[0] | m[0] << 16, m[0] | m[1] << 16, m[1] | m[1] << 16, m[2] | m[2] << 16};
-      *(u32x4*)(tab + L::kKb + 512 + 16 * lc) =
-          u32x4{m[2] | m[3] << 16, m[3] | m[3] << 16, 0x3F803F80u, 0x00003F80u};
-    } else {
-      const int ec = max(e, r_exp - 80);
-      const float inv = __uint_as_float((uint32_t)(127 - max(ec, -126)) << 23);  // 2^-E (E <= 126)
-      *(float*)(tab + L::kEv + 4 * lc) = __uint_as_float((uint32_t)(127 + max(ec, -126) - r_exp) << 23);
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const bool bad = nan >> g & 1;
-        const float s = bad ? 0.0f : bf16_lo_f32(r.w[g]) * inv, m = bad ? 0.0f : bf16_hi_f32(r.w[g]) * inv;
-        *(float2*)(tab + L::kVs + 256 * g + 8 * lc) = float2{s, m - 8.0f * s};  // (codes enter as c + 8)
-      }
-      if (lc == 0) {
-        *(float*)(tab + L::kMisc) = exp2f((float)(before - r_exp));
-        uint32_t any = 0;
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          *(uint32_t*)(tab + L::kMisc + 8 + 4 * g) = nan_tokens[g];
-          any |= nan_tokens[g];
-        }
-        *(uint32_t*)(tab + L::kMisc + 4) = any;
-        *(float*)(tab + L::kMisc + 24) = (float)r_exp;
-      }
+      // Slots 12..14: ones for the reference; 15: E - R, by wave 1.
+      *(u32x2*)(tab + L::kKb + 512 + 16 * lc) = u32x2{m[2] | m[3] << 16, m[3] | m[3] << 16};
+      *(uint32_t*)(tab + L::kKb + 520 + 16 * lc) = 0x3F803F80u;
+      return;
     }
+    // Size of the tile's values, NaN aside: 2^13 to 2^14 of the unit 2^E.
+    float sv[G], mv[G], size = 0.0f;
+    bool nan = false;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      sv[g] = bf16_lo_f32(r.w[g]), mv[g] = bf16_hi_f32(r.w[g]);
+      size = fmaxf(size, fmaxf(8.0f * sv[g], fabsf(mv[g])));
+      nan |= sv[g] != sv[g];
+    }
+    size = row_allmax(size);
+    const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(size), __float_as_uint(size), false, false);
+    const uint32_t top = __builtin_amdgcn_readfirstlane(max(sw[0], sw[1]));  // (not negative)
+    int e = max(min((int)(top >> 23), 253) - (127 + 13), -113);
+    const int before = r_exp;
+    if (t == t0 || e > r_exp + 64) r_exp = e;
+    e = max(e, r_exp - 80);
+    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+    *(uint32_t*)(tab + L::kKb + 524 + 16 * lc) = 0x3F80u | (__float_as_uint((float)(e - r_exp)) & 0xFFFF0000u);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const bool bad = sv[g] != sv[g];
+      _Float16* at = (_Float16*)(tab + L::kVs + 16 * (8 * g + (lc >> 2)) + 2 * (lc & 3));
+      at[0] = (_Float16)(bad ? 0.0f : sv[g] * inv);
+      at[4] = (_Float16)(bad ? 0.0f : mv[g] * inv);
+    }
+    const uint32_t any = (uint32_t)__builtin_amdgcn_ballot_w64(nan);
+    if (any) {
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+        *(uint32_t*)(tab + L::kMisc + 8 + 4 * g) = (uint32_t)__builtin_amdgcn_ballot_w64(sv[g] != sv[g]);
+    }
+    *(float2*)(tab + L::kMisc) =
+        float2{t == t0 ? 1.0f : __builtin_amdgcn_exp2f((float)(before - r_exp)), __uint_as_float(any)};
+    *(float2*)(tab + L::kMisc + 24) =
+        float2{__uint_as_float((uint32_t)(127 + r_exp - e) << 23), __uint_as_float((uint32_t)(127 + r_exp) << 23)};
   };
   // LDS images: K 16-byte chunk (8 d) q of token t at unit 32 q + (t ^ swz), V^T chunk
-  // (page, half, d) at unit (2 page + half) D + d, where half 0 holds a page's tokens
-  // 0..3, 8..11 and half 1 tokens 4..7, 12..15.
-  auto k_swz = [](uint32_t pair) { return pair & 7; };
-  auto stage_in = [&](uint32_t t, const Raw& r, int st) __attribute__((always_inline)) {
-    uint8_t* kl = lds + st * L::kStage;
-    uint8_t* vl = kl + L::kK;
+  // (page, half, d) at unit (2 page + half) D + (d ^ swz), where half 0 holds a page's
+  // tokens 0..3, 8..11 and half 1 tokens 4..7, 12..15.  The swizzles spread what
+  // neighbouring threads write over the banks.
+  auto k_unit = [](uint32_t q, uint32_t tok) { return 32 * q + (tok ^ ((q >> 1 & 7) ^ (q & 1) << 1)); };
+  auto v_unit = [](uint32_t half, uint32_t d) { return half * D + (d ^ (d >> 3 & 12)); };
+  auto k_tile = [&](uint32_t t) __attribute__((always_inline)) { return lds + t % L::kNK * L::kK; };
+  auto v_tile = [&](uint32_t t) __attribute__((always_inline)) { return lds + L::kVAt + t % L::kNV * L::kV; };
+  const Q4KvUnpackF16 unpack;
+  auto stage_in = [&](uint32_t t, const Raw& r) __attribute__((always_inline)) {
+    if (!kAll && wave >= 4 * D / 64) return;
+    uint8_t *kl = k_tile(t), *vl = v_tile(t);
     const uint8_t* tab = table(t);
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-      const int u0 = i * 64 * W + wave * 64;
-      if (u0 >= 4 * D) continue;
-      const u32x2 w = r.u[i];
-      const uint32_t pg = (u0 / D) & 1, u = u0 % D + lane;
-      const uint32_t l = D == 64 ? u : u % 128 / 2, g = D == 64 ? 0 : 2 * (u / 128) + u % 2;
+    for (int n = 0; n < kWords; ++n) {
+      const uint32_t wi = (wave * 64 + anew(lane)) * kWords % (2 * D) + n;
+      const uint32_t l = D == 64 ? wi / 2 : wi % 256 / 4, j = D == 64 ? wi % 2 : 4 * (wi / 256) + wi % 4;
       const uint32_t low = l & 15, kq = l >> 4;
-      if (u0 < 2 * D) {
-        const uint32_t tok = 16 * pg + low, pair = 4 * g + kq;
-        uint8_t* dst = kl + 16 * (64 * pair + (tok ^ k_swz(pair)));
-        *(u32x4*)dst = k_codes16(w.x);
-        *(u32x4*)(dst + 512) = k_codes16(w.y);
-      } else {
-        const floatx4* sm = (const floatx4*)(tab + L::kVs + 256 * g + 8 * (16 * pg + 4 * kq));
-        const floatx4 a = sm[0], b = sm[1];  // (s, m) of four tokens
-        uint8_t* dst = vl + 16 * ((2 * pg + (kq & 1)) * D + 64 * g + low) + 8 * (kq >> 1);
+      // d = 64 (j / 2) + 16 kq + 8 (j % 2) .. + 7
+      *(u32x4*)(kl + 16 * k_unit(8 * (j / 2) + 2 * kq + j % 2, 16 * page_half + low)) = k_codes16(r.k[n]);
+      const u32x4 sm = *(const u32x4*)(tab + L::kVs + 16 * (8 * (j / 2) + 4 * page_half + kq));
+      const half2_t s01 = as_half2(sm.x), s23 = as_half2(sm.y), m01 = as_half2(sm.z), m23 = as_half2(sm.w);
+      half2_t c[4];  // tokens 0, 1 and 2, 3 of d / 16 = 2 j, then of 2 j + 1
+      unpack(r.v[n], c);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t lo = w[j] & 0x0F0F0F0Fu, hi = (w[j] >> 4) & 0x0F0F0F0Fu;
-          // Token r of d / 16 = 2 j + k in nibble 2 k + (r >> 1) + 4 (r & 1).
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float x0 = (float)(lo >> (8 * k) & 0xFF), x1 = (float)(lo >> (8 * k + 16) & 0xFF);
-            const float x2 = (float)(hi >> (8 * k) & 0xFF), x3 = (float)(hi >> (8 * k + 16) & 0xFF);
-            *(u32x2*)(dst + 256 * (2 * j + k)) =
-                u32x2{pack_f16x2(__builtin_fmaf(x0, a.x, a.y), __builtin_fmaf(x1, a.z, a.w)),
-                      pack_f16x2(__builtin_fmaf(x2, b.x, b.y), __builtin_fmaf(x3, b.z, b.w))};
-          }
-        }
+      for (int i = 0; i < 2; ++i) {
+        const half2_t a = __builtin_elementwise_fma(c[2 * i], s01, m01), b = __builtin_elementwise_fma(c[2 * i + 1], s23, m23);
+        *(u32x2*)(vl + 16 * v_unit(2 * page_half + (kq & 1), 32 * j + 16 * i + low) + 8 * (kq >> 1)) =
+            u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
       }
     }
   };
 
-  // Softmax and P V of tile t from LDS stage st.  MASKED is false for tiles every
-  // column of the wave sees whole.
-  auto compute = [&](uint32_t t, int st, auto masked) __attribute__((always_inline)) {
+  u32x4 ph[2];  // the weights of a tile, two k-steps
+  floatx16 x, sc[kTight ? 1 : G];
+  auto scaled = [&](uint32_t t, const floatx16& s, int g) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const floatx4 k = ((const floatx4*)(table(t) + 128 * g))[2 * i + hf];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * i + e] = __builtin_fmaf(s[4 * i + e], k[e], x[4 * i + e]);
+    }
+  };
+  // Scores of tile t: their offsets and reference in x, the groups' products in sc.
+  auto products = [&](uint32_t t) __attribute__((always_inline)) {
+    const int lc = anew(lane) & 31, hf = anew(lane) >> 5;
+    const u32x4* kl = (const u32x4*)k_tile(t);
+    x = mfma32x32x16(*(const u32x4*)(table(t) + L::kKb + 16 * lane), qbias, floatx16{});
+    if constexpr (kTight) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        sc[0] = floatx16{};
+#pragma unroll
+        for (int j = 4 * g; j < 4 * g + 4; ++j) {
+          sc[0] = mfma32x32x16(kl[k_unit(2 * j + hf, lc)], j < kQReg ? qb[j < kQReg ? j : 0] : ql[64 * (j - kQReg)], sc[0]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        scaled(t, sc[0], g);
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < G; ++g) sc[g] = floatx16{};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const int j = 4 * g + i;
+          sc[g] = mfma32x32x16(kl[k_unit(2 * j + hf, lc)], qb[j], sc[g]);
+        }
+    }
+  };
+  auto add_values = [&](uint32_t t) __attribute__((always_inline)) {
+    const int lc = anew(lane) & 31, hf = anew(lane) >> 5;
+    const u32x4* vl = (const u32x4*)v_tile(t);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) {
+        o[db] = mfma32x32x16_f16(vl[v_unit(2 * j + hf, 32 * db + lc)], ph[j], o[db]);
+        if (kTight) __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+
+  // Weights of tile t.  MASKED is false for tiles every column of the wave sees whole.
+  auto weights = [&](uint32_t t, auto masked) __attribute__((always_inline)) {
     constexpr bool MASKED = decltype(masked)::value;
-    const uint8_t* base = lds + st * L::kStage;
-    const u32x4* kl = (const u32x4*)base;
-    const u32x4* vl = (const u32x4*)(base + L::kK);
     const uint8_t* tab = table(t);
     // (the same in every lane)
     const float unit = __uint_as_float(__builtin_amdgcn_readfirstlane(*(const uint32_t*)(tab + L::kMisc)));
     const uint32_t nan_any = __builtin_amdgcn_readfirstlane(*(const uint32_t*)(tab + L::kMisc + 4));
-    floatx16 x = mfma32x32x16(*(const u32x4*)(tab + L::kKb + 16 * lane), qbias, floatx16{});
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      floatx16 s = floatx16{};
-#pragma unroll
-      for (int j = 4 * g; j < 4 * g + 4; ++j) {
-        const u32x4 ka = kl[32 * (2 * j + hf) + (lc ^ k_swz(j))];
-        s = mfma32x32x16(ka, j < kQReg ? qb[j < kQReg ? j : 0] : ql[64 * (j - kQReg)], s);
-        if constexpr (kTight) __builtin_amdgcn_sched_barrier(0);
-      }
-      const floatx4* sl = (const floatx4*)(tab + 128 * g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const floatx4 k = sl[2 * i + hf];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 * i + e] = __builtin_fmaf(s[4 * i + e], k[e], x[4 * i + e]);
-      }
-    }
-    const floatx4* evl = (const floatx4*)(tab + L::kEv);
-    floatx4 ev[kTight ? 1 : 4];
     if constexpr (!kTight) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) ev[i] = evl[2 * i + hf];
+      for (int g = 0; g < G; ++g) scaled(t, sc[g], g);
     }
-    auto ev_of = [&](int i) __attribute__((always_inline)) { return kTight ? evl[2 * i + hf] : ev[kTight ? 0 : i]; };
     // Element e is token 32 t + 8 (e >> 2) + 4 hf + (e & 3).
-    float p[16];
-    float wmax = 0.0f;
+    float xmax = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const floatx4 v = ev_of(i);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int e = 4 * i + k;
-        if (MASKED && 32 * t + 8 * i + 4 * hf + k >= visible) x[e] = -INFINITY;
-        p[e] = __builtin_amdgcn_exp2f(x[e]);
-        wmax = fmaxf(wmax, p[e] * v[k]);
-      }
+    for (int e = 0; e < 16; ++e) {
+      if (MASKED && 32 * t + 8 * (e >> 2) + 4 * hf + (e & 3) >= visible) x[e] = -INFINITY;
+      xmax = fmaxf(xmax, x[e]);
     }
-    // (unit: below 1 where the tile has a token of larger values than any before)
-    const bool move = t == t0 || unit != 1.0f || __builtin_amdgcn_ballot_w64(wmax > kWMost);
-    float shift = 0.0f;
-    if (move) {
-      float y = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const floatx4 v = ev_of(i);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) y = fmaxf(y, x[4 * i + k] + (float)((int)(__float_as_uint(v[k]) >> 23) - 127));
-      }
-      y = max2_across_halves(y);
+    // (unit: not 1 where the tile has changed R)
+    if (t == t0 || unit != 1.0f || __builtin_amdgcn_ballot_w64(xmax > kMost)) {
+      xmax = max2_across_halves(xmax);
       // Whole numbers: the largest weight becomes 2^11 .. 2^12.
-      if ((t == t0 || y > 15.5f) && y > -INFINITY) shift = ceilf(y - 12.0f);
+      const float shift = (t == t0 || xmax > kMost) && xmax > -INFINITY ? ceilf(xmax - 12.0f) : 0.0f;
       m_run += shift;
       const float corr = __builtin_amdgcn_exp2f(-shift);
       if (t != t0) {  // (nothing is there yet in the first tile, and corr may be infinite)
@@ -793,93 +834,78 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
       }
       uint32_t r[3];
       split3(-m_run, r);
-      if (hf) qbias.z = r[0] | r[1] << 16, qbias.w = r[2];
+      if (hf) qbias.z = r[0] | r[1] << 16, qbias.w = r[2] | 0x3F800000u;
+      x -= shift;
     }
-    // Two waves of D = 256 have no registers for scores beside probabilities: they
-    // form them again.
-    if (move || kTight) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(x[e] - shift);
-    }
+    // The sum takes the weights as they are rounded.
     float psum[2] = {0.0f, 0.0f};
+    const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      u32x4 ph;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const floatx4 v = ev_of(2 * j + i);
-        const int e = 8 * j + 4 * i;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          psum[0] += p[e + 2 * k];
-          psum[1] += p[e + 2 * k + 1];
-          ph[2 * i + k] = pack_f16x2(p[e + 2 * k] * v[2 * k], p[e + 2 * k + 1] * v[2 * k + 1]);
-        }
-      }
-#pragma unroll
-      for (int db = 0; db < kDB; ++db) {
-        o[db] = mfma32x32x16_f16(vl[(2 * j + hf) * D + 32 * db + lc], ph, o[db]);
-        if constexpr (kTight) __builtin_amdgcn_sched_barrier(0);
-      }
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t w = pack_f16x2(__builtin_amdgcn_exp2f(x[2 * i]), __builtin_amdgcn_exp2f(x[2 * i + 1]));
+      ph[i >> 2][i & 3] = w;
+      psum[i & 1] = __builtin_amdgcn_fdot2(as_half2(w), ones, psum[i & 1], false);
     }
-    l_lane += psum[0] + psum[1];
+    l_lane = __builtin_fmaf(psum[0] + psum[1], *(const float*)(tab + L::kMisc + 24), l_lane);
     if (nan_any) {  // values that are NaN: of the columns that see them, and their group
       const uint32_t n = visible > 32 * t ? visible - 32 * t : 0, seen = n >= 32 ? ~0u : (1u << n) - 1;
 #pragma unroll
       for (int g = 0; g < G; ++g)
         if (*(const uint32_t*)(tab + L::kMisc + 8 + 4 * g) & seen) {
 #pragma unroll
-          for (int db = 2 * g; db < 2 * g + 2; ++db) o[db][0] = NAN;
-#pragma unroll
           for (int db = 2 * g; db < 2 * g + 2; ++db)
 #pragma unroll
-            for (int e = 1; e < 16; ++e) o[db][e] = NAN;
+            for (int e = 0; e < 16; ++e) o[db][e] = NAN;
         }
     }
   };
 
-  // Pipeline, one barrier per tile: tile t + 1 (fetched a tile earlier) is unpacked
-  // into the other stage, the tables of tile t + 2 are written, tile t + 2 and the scale
-  // words of t + 3 are fetched, then tile t is reduced from its stage.
   Raw raw{};
   Words words{};
-  Pages next{}, after{};
   if (t0 < t1) {
-    Words w1{};
-    const Pages ids = page_ids(t0);
-    fetch_words(ids, words);
-    fetch(ids, raw);
-    if (t0 + 1 < t1) {
-      next = page_ids(t0 + 1);
-      fetch_words(next, w1);
-    }
-    write_table(t0, words);
-    if (t0 + 1 < t1) write_table(t0 + 1, w1);
+    if (wave == 0) load_ids(t0);
     lds_barrier();
-    stage_in(t0, raw, 0);
-    if (t0 + 1 < t1) fetch(next, raw);
-    if (t0 + 2 < t1) {
-      next = page_ids(t0 + 2);
-      fetch_words(next, words);
-    }
-    if (t0 + 3 < t1) after = page_ids(t0 + 3);
+    Words w0{}, w1{};
+    Raw r0{};
+    const Pages p0 = page_ids(t0), p1 = page_ids(t0 + 1), p2 = page_ids(t0 + 2);
+    fetch_words(p0, w0);
+    fetch_words(p1, w1);
+    fetch(p0, r0);
+    fetch(p1, raw);
+    fetch_words(p2, words);
+    write_table(t0, w0);
+    write_table(t0 + 1, w1);
+    lds_barrier();
+    stage_in(t0, r0);
   }
   lds_barrier();
+  // A wave without columns only unpacks (not for D = 128, where the branch keeps the
+  // products out of a common schedule).
+  const bool busy = D == 128 || W == 8 || c0 < cols;
+  // A step: the weights of tile t, with which tile t + 1 (fetched a step earlier) is
+  // unpacked, the tables of t + 2 are written, and tile t + 2 and the scale words of t + 3
+  // are fetched; then the matrix products of the scores of t + 1 and of the values of t.
+  // (Tiles from t1 on too, pages past the last as the last: nothing uses them, and the
+  // loop has no conditions.)
   auto step = [&](uint32_t t, auto masked) __attribute__((always_inline)) {
-    const int st = (t - t0) & 1;
-    if (t + 1 < t1) stage_in(t + 1, raw, st ^ 1);
-    if (t + 2 < t1) {
-      write_table(t + 2, words);
-      fetch(next, raw);
-      if (t + 3 < t1) {
-        fetch_words(after, words);
-        next = after;
-        if (t + 4 < t1) after = page_ids(t + 4);
-      }
+    const Pages p2 = page_ids(t + 2), p3 = page_ids(t + 3);
+    stage_in(t + 1, raw);
+    fetch(p2, raw);
+    if (busy) {
+      if constexpr (kTight) products(t);
+      weights(t, masked);
     }
-    if (D == 128 || W == 8 || c0 < cols) compute(t, st, masked);
+    write_table(t + 2, words);
+    fetch_words(p3, words);
+    if (((t - t0) & 31) == 16 && wave == W - 1) load_ids(t + 16);  // (in use from 13 steps on)
+    if (busy && kTight) add_values(t);
     lds_barrier();
+    if (busy && !kTight) {
+      products(t + 1);
+      add_values(t);
+    }
   };
+  if (busy && !kTight) products(t0);
   // Tiles below full_end are visible to every column of the wave.
   const uint32_t first_row = min(c0, cols - 1) / gh;
   const uint32_t full_end = min(max(min(args.start + first_row + 1, sq.len) / 32, t0), t1);
@@ -887,7 +913,7 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
   for (uint32_t t = full_end; t < t1; ++t) step(t, BoolTag<true>{});
 
   const float l_tot = l_lane + __shfl_xor(l_lane, 32);
-  const float unit = t0 < t1 ? __builtin_amdgcn_exp2f(*(const float*)(table(t1 - 1) + L::kMisc + 24)) : 1.0f;
+  const float unit = t0 < t1 ? *(const float*)(table(t1 - 1) + L::kMisc + 28) : 1.0f;
   if (!col_ok) return;
   if (S > 1) {
     // Partials as in decode, row by row: O [row][split][H][D], then (m, l): here O over
