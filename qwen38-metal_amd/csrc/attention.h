@@ -6,6 +6,7 @@
 namespace qm {
 
 constexpr int kMaxAttnSeqs = 16;  // sequences per launch (kernel-argument table)
+constexpr int kMaxQ4KvSeqs = 64;  // the same of decode over 4-bit caches
 constexpr int kMaxSplits = 2048;         // page splits per sequence
 constexpr int kMaxPagesPerSplit = 1024;  // pages per decode workgroup
 
@@ -44,7 +45,7 @@ struct AppendArgs {
   AttnSeq seqs[kMaxAttnSeqs];
 };
 
-struct AttnArgs {
+struct AttnCommon {
   const uint16_t* q;     // bf16 [rows][H][D]
   const uint16_t* gate;  // bf16 [rows][H][D] or null
   uint16_t* o;           // bf16 [rows][H][D]
@@ -64,8 +65,55 @@ struct AttnArgs {
   uint32_t out8;             // prefill: o and gate rows take 8-byte accesses
   uint32_t rows;   // prefill: query rows
   uint32_t start;  // prefill: cache position of row 0
+};
+
+struct AttnArgs : AttnCommon {
   AttnSeq seqs[kMaxAttnSeqs];
 };
+
+// Decode over 4-bit caches: what its kernel needs of an AttnSeq.
+struct Q4KvSeq {
+  uint8_t* k;
+  int32_t* pt;
+  uint32_t len, unit_begin, nsplit, part_begin;
+  int32_t new_page_count, new_page_id;
+};
+struct Q4KvArgs : AttnCommon {
+  Q4KvSeq seqs[kMaxQ4KvSeqs];
+};
+
+// What merges the split partials of a decode or prefill launch.
+struct AttnCombineArgs {
+  const uint16_t* gate;
+  uint16_t* o;
+  const float* partials;
+  uint32_t heads, head_dim, head_dim_pad, part_rows;
+  uint32_t prefill, splits, out8;
+  uint32_t rows;  // query rows (prefill) or sequences
+  struct {
+    uint32_t nsplit, part_begin;
+  } seqs[kMaxQ4KvSeqs];  // decode
+};
+template <class Args>
+AttnCombineArgs combine_args(const Args& a) {
+  AttnCombineArgs c{};
+  c.gate = a.gate;
+  c.o = a.o;
+  c.partials = a.partials;
+  c.heads = a.heads;
+  c.head_dim = a.head_dim;
+  c.head_dim_pad = a.head_dim_pad;
+  c.part_rows = a.part_rows;
+  c.prefill = a.prefill;
+  c.splits = a.splits;
+  c.out8 = a.out8;
+  c.rows = a.prefill ? a.rows : a.n_seqs;
+  for (uint32_t i = 0; !a.prefill && i < a.n_seqs; ++i) {
+    c.seqs[i].nsplit = a.seqs[i].nsplit;
+    c.seqs[i].part_begin = a.seqs[i].part_begin;
+  }
+  return c;
+}
 
 // Split partials of qm_attn_decode_noalloc: a file-scope device array of the
 // attention source (one copy per GPU, held until the process ends) whose
@@ -86,7 +134,7 @@ hipError_t attn_noalloc_begin(int device, hipStream_t stream);
 hipError_t attn_noalloc_end(int device, hipStream_t stream);
 
 // Merges the split partials of a decode or prefill launch into its outputs.
-void launch_attn_combine(const AttnArgs& a, hipStream_t st);
+void launch_attn_combine(const AttnCombineArgs& a, hipStream_t st);
 
 hipError_t launch_q8_append(const AppendArgs& a, uint32_t items, hipStream_t st);
 // Decode: `units` workgroups; when need_combine, q8_combine_kernel merges the
@@ -94,7 +142,8 @@ hipError_t launch_q8_append(const AppendArgs& a, uint32_t items, hipStream_t st)
 hipError_t launch_q8_attention(const AttnArgs& a, uint32_t units, bool need_combine, hipStream_t st);
 // Workgroups that share the query heads of a KV head in decode over 4-bit caches.
 constexpr uint32_t q4kv_head_sets(uint32_t heads_per_kv) { return (heads_per_kv + 7) / 8; }
-// The same over 4-bit caches (q4kv_attention.hip).
-hipError_t launch_q4kv_attention(const AttnArgs& a, uint32_t units, bool need_combine, hipStream_t st);
+// The same over 4-bit caches (q4kv_attention.hip), and prefill over one.
+hipError_t launch_q4kv_decode(const Q4KvArgs& a, uint32_t units, bool need_combine, hipStream_t st);
+hipError_t launch_q4kv_prefill(const AttnArgs& a, hipStream_t st);
 
 }  // namespace qm

@@ -102,8 +102,8 @@ constexpr int kMergeBytes = W * D * kMergePad * 4 + (3 * W + 2) * 16 * 4;
 // leave as outputs, or as one split's partials.  Head head0 + c (of n_heads) has
 // columns c, c + 16 / S, ...: S sums of disjoint tokens.  Every wave of the
 // workgroup calls it.
-template <int D, int W, int S>
-__device__ __forceinline__ void decode_merge(const AttnArgs& args, const AttnSeq& sq, uint32_t b, uint32_t head0,
+template <int D, int W, int S, class Seq>
+__device__ __forceinline__ void decode_merge(const AttnCommon& args, const Seq& sq, uint32_t b, uint32_t head0,
                                              uint32_t n_heads, uint32_t split, uint8_t* lds,
                                              const floatx4 (&o)[D / 16], float m_run, float l_lane) {
   constexpr int kWaves = W, kDB = D / 16, kPad = kMergePad, kCols = 16 / S;

@@ -95,7 +95,7 @@ __device__ __forceinline__ void load_part(__amdgpu_buffer_rsrc_t r, uint32_t bas
 //   the other page.
 // A column's softmax is its page's alone; decode_merge joins the columns of a head.
 template <int D, int W>
-__global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(AttnArgs args) {
+__global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(Q4KvArgs args) {
   constexpr int G = D / 64, kDB = D / 16, kRing = D == 256 ? 2 : 4;  // pairs of pages in flight
   // Two waves a SIMD of D = 256 have no registers for the Q operands, which are the
   // same for all of them: they lie in LDS.
@@ -110,10 +110,12 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(AttnArgs args) {
   const uint32_t mask_b = in_b ? ~0u : 0u, mask_a = ~mask_b;
   const uint32_t H = args.heads, KVH = args.kv_heads, gh = H / KVH;
 
-  uint32_t b = 0;
+  // Its sequence: a lane looks at each (one load, where a search would wait for several).
   const uint32_t unit = blockIdx.x;
-  while (b + 1 < args.n_seqs && unit >= args.seqs[b + 1].unit_begin) ++b;
-  const AttnSeq& sq = args.seqs[b];
+  uint32_t b = 0;
+  if (args.n_seqs > 1)
+    b = __builtin_popcountll(__builtin_amdgcn_ballot_w64((uint32_t)lane < args.n_seqs && unit >= args.seqs[lane].unit_begin)) - 1;
+  const Q4KvSeq& sq = args.seqs[b];
   const uint32_t u = unit - sq.unit_begin, sets = q4kv_head_sets(gh);
   const uint32_t kvh = u % KVH, set = u / KVH % sets, split = u / (KVH * sets);
   const uint32_t per_set = (gh + sets - 1) / sets;
@@ -154,7 +156,7 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(AttnArgs args) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int32_t phys = __builtin_amdgcn_readlane(ids, (int)((j + h) & 63));
-      page[h] = (const uint8_t*)sq.k + ((size_t)phys * KVH + kvh) * block;
+      page[h] = sq.k + ((size_t)phys * KVH + kvh) * block;
       r[h] = make_rsrc(page[h], j + h < n_mine ? (uint32_t)block : 0u);
       load_part<D>(r[h], 0, lane, p.k[h]);
     }
@@ -247,7 +249,7 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(AttnArgs args) {
     const uint32_t token = sq.len - 1, slot = token % 16;
     const bool fresh = sq.new_page_count > 0;
     const int32_t phys = fresh ? sq.new_page_id : sq.pt[token / 16];
-    uint8_t* page = (uint8_t*)sq.k + ((size_t)phys * KVH + kvh) * block;
+    uint8_t* page = sq.k + ((size_t)phys * KVH + kvh) * block;
     float* xs = (float*)lds;               // values as the codes have them, K then V
     uint8_t* cs = lds + 2 * D * 4;         // codes, c + 8
     uint32_t old[D / 32];                  // the lane's V words of the page
@@ -970,32 +972,43 @@ hipError_t launch_prefill(const AttnArgs& a, hipStream_t st) {
   const uint32_t cols = a.rows * (a.heads / a.kv_heads);
   const uint32_t units = a.kv_heads * ((cols + 32 * W - 1) / (32 * W)) * a.splits;
   hipLaunchKernelGGL((q4kv_prefill_kernel<D, W>), dim3(units), dim3(64 * W), 0, st, a);
-  if (a.splits > 1) launch_attn_combine(a, st);
+  if (a.splits > 1) launch_attn_combine(combine_args(a), st);
   return hipGetLastError();
 }
 
 template <int D>
-hipError_t launch_d(const AttnArgs& a, uint32_t units, bool need_combine, hipStream_t st) {
-  if (a.prefill) {
-    if (a.splits == 0 || (a.splits > 1 && !a.partials)) return hipErrorInvalidValue;
-    return a.wg_waves == 8 ? launch_prefill<D, 8>(a, st) : launch_prefill<D, 4>(a, st);
-  }
-  if (need_combine && !a.partials) return hipErrorInvalidValue;
+hipError_t launch_prefill_d(const AttnArgs& a, hipStream_t st) {
+  return a.wg_waves == 8 ? launch_prefill<D, 8>(a, st) : launch_prefill<D, 4>(a, st);
+}
+
+template <int D>
+hipError_t launch_decode_d(const Q4KvArgs& a, uint32_t units, bool need_combine, hipStream_t st) {
   if (a.wg_waves == 8)
     hipLaunchKernelGGL((q4kv_decode_kernel<D, 8>), dim3(units), dim3(512), 0, st, a);
   else
     hipLaunchKernelGGL((q4kv_decode_kernel<D, 4>), dim3(units), dim3(256), 0, st, a);
-  if (need_combine) launch_attn_combine(a, st);
+  if (need_combine) launch_attn_combine(combine_args(a), st);
   return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_q4kv_attention(const AttnArgs& a, uint32_t units, bool need_combine, hipStream_t st) {
+hipError_t launch_q4kv_prefill(const AttnArgs& a, hipStream_t st) {
+  if (a.splits == 0 || (a.splits > 1 && !a.partials)) return hipErrorInvalidValue;
   switch (a.head_dim_pad) {
-    case 64: return launch_d<64>(a, units, need_combine, st);
-    case 128: return launch_d<128>(a, units, need_combine, st);
-    case 256: return launch_d<256>(a, units, need_combine, st);
+    case 64: return launch_prefill_d<64>(a, st);
+    case 128: return launch_prefill_d<128>(a, st);
+    case 256: return launch_prefill_d<256>(a, st);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+hipError_t launch_q4kv_decode(const Q4KvArgs& a, uint32_t units, bool need_combine, hipStream_t st) {
+  if (need_combine && !a.partials) return hipErrorInvalidValue;
+  switch (a.head_dim_pad) {
+    case 64: return launch_decode_d<64>(a, units, need_combine, st);
+    case 128: return launch_decode_d<128>(a, units, need_combine, st);
+    case 256: return launch_decode_d<256>(a, units, need_combine, st);
     default: return hipErrorInvalidValue;
   }
 }

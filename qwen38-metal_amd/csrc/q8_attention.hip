@@ -499,7 +499,7 @@ __global__ __launch_bounds__(64 * W) void q8_decode_kernel(AttnArgs args) {
 // trip spread over many workgroups; the per-head maximum and the sums over
 // splits then meet in LDS.
 template <int D>
-__global__ __launch_bounds__(256) void q8_combine_kernel(AttnArgs args) {
+__global__ __launch_bounds__(256) void q8_combine_kernel(AttnCombineArgs args) {
   constexpr int kWgPerHead = D / 32;  // workgroups per (sequence, head)
   constexpr int kGroups = 32;         // split groups (threads per slice)
   constexpr int kMaxPer = 4;          // splits a thread holds in registers per pass
@@ -587,7 +587,7 @@ __global__ __launch_bounds__(256) void q8_combine_kernel(AttnArgs args) {
 // the maximum and the sums over g meet through lane swaps (xor 8, 16, 32),
 // so the merge needs no LDS and no barrier.
 template <int D>
-__global__ __launch_bounds__(64) void q8_combine_small_kernel(AttnArgs args) {
+__global__ __launch_bounds__(64) void q8_combine_small_kernel(AttnCombineArgs args) {
   constexpr int kWgPerHead = D / 32;
   constexpr int kPer = 4;  // splits per lane
   const uint32_t H = args.heads, dr = args.head_dim;
@@ -1021,7 +1021,7 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q8_prefill_k
 // rows of 24 heads of 256: the dispatch alone took longer than the product.)
 constexpr int kRowSplits = 8;
 template <int D>
-__global__ __launch_bounds__(256) void q8_combine_rows_kernel(AttnArgs args) {
+__global__ __launch_bounds__(256) void q8_combine_rows_kernel(AttnCombineArgs args) {
   const uint32_t H = args.heads, dr = args.head_dim, ns = args.splits;
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
   const size_t pair = i / (D / 4);
@@ -1064,14 +1064,14 @@ __global__ __launch_bounds__(256) void q8_combine_rows_kernel(AttnArgs args) {
 }
 
 template <int D>
-void launch_combine(const AttnArgs& a, uint32_t rows, uint32_t max_split, hipStream_t st) {
+void launch_combine(const AttnCombineArgs& a, uint32_t max_split, hipStream_t st) {
   if (a.prefill && max_split <= (uint32_t)kRowSplits) {
     const size_t items = (size_t)a.rows * a.heads * (D / 4);
     hipLaunchKernelGGL(q8_combine_rows_kernel<D>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, a);
   } else if (max_split <= 32) {
-    hipLaunchKernelGGL(q8_combine_small_kernel<D>, dim3(rows * a.heads * (D / 32)), dim3(64), 0, st, a);
+    hipLaunchKernelGGL(q8_combine_small_kernel<D>, dim3(a.rows * a.heads * (D / 32)), dim3(64), 0, st, a);
   } else {
-    hipLaunchKernelGGL(q8_combine_kernel<D>, dim3(rows * a.heads * (D / 32)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(q8_combine_kernel<D>, dim3(a.rows * a.heads * (D / 32)), dim3(256), 0, st, a);
   }
 }
 
@@ -1080,7 +1080,7 @@ hipError_t launch_prefill(const AttnArgs& a, hipStream_t st) {
   const uint32_t cols = a.rows * (a.heads / a.kv_heads);
   const uint32_t units = a.kv_heads * ((cols + 32 * W - 1) / (32 * W)) * a.splits;
   hipLaunchKernelGGL((q8_prefill_kernel<D, W>), dim3(units), dim3(64 * W), 0, st, a);
-  if (a.splits > 1) launch_attn_combine(a, st);
+  if (a.splits > 1) launch_attn_combine(combine_args(a), st);
   return hipGetLastError();
 }
 
@@ -1095,23 +1095,19 @@ hipError_t launch_attn_d(const AttnArgs& a, uint32_t units, bool need_combine, h
     hipLaunchKernelGGL((q8_decode_kernel<D, 8>), dim3(units), dim3(512), 0, st, a);
   else
     hipLaunchKernelGGL((q8_decode_kernel<D, 4>), dim3(units), dim3(256), 0, st, a);
-  if (need_combine) launch_attn_combine(a, st);
+  if (need_combine) launch_attn_combine(combine_args(a), st);
   return hipGetLastError();
 }
 
 }  // namespace
 
-void launch_attn_combine(const AttnArgs& a, hipStream_t st) {
-  uint32_t max_split = a.splits;
-  if (!a.prefill) {
-    max_split = 0;
-    for (uint32_t i = 0; i < a.n_seqs; ++i) max_split = max_split > a.seqs[i].nsplit ? max_split : a.seqs[i].nsplit;
-  }
-  const uint32_t rows = a.prefill ? a.rows : a.n_seqs;
+void launch_attn_combine(const AttnCombineArgs& a, hipStream_t st) {
+  uint32_t max_split = a.prefill ? a.splits : 0;
+  for (uint32_t i = 0; !a.prefill && i < a.rows; ++i) max_split = max_split > a.seqs[i].nsplit ? max_split : a.seqs[i].nsplit;
   switch (a.head_dim_pad) {
-    case 64: launch_combine<64>(a, rows, max_split, st); break;
-    case 128: launch_combine<128>(a, rows, max_split, st); break;
-    default: launch_combine<256>(a, rows, max_split, st); break;
+    case 64: launch_combine<64>(a, max_split, st); break;
+    case 128: launch_combine<128>(a, max_split, st); break;
+    default: launch_combine<256>(a, max_split, st); break;
   }
 }
 

@@ -203,9 +203,10 @@ qm_status check_q_alignment(const uint16_t* q, const uint16_t* gate, uint32_t D)
   return QM_OK;
 }
 
-// One launch's worth of decode work (at most kMaxAttnSeqs sequences).
+// One launch's worth of decode work (at most kMaxAttnSeqs sequences, or kMaxQ4KvSeqs).
 struct DecodeChunk {
-  AttnArgs at{};
+  AttnCommon at{};
+  AttnSeq seqs[kMaxQ4KvSeqs] = {};
   uint32_t units = 0;
   uint32_t parts = 0;
   bool combine = false;
@@ -215,20 +216,28 @@ struct DecodeChunk {
 // kernel's page limits, and all splits should run in one residency round:
 // one 8-wave workgroup per CU if the splits fit that (measured faster at 32K:
 // the CU's waves share one split), else two 4-wave workgroups per CU.
+//
+// Over 4-bit caches, whose pages are half as long to read, one 4-wave workgroup per CU
+// where a split has at most 96 pages: its waves' sums meet sooner (64 / 8 heads of 128 on
+// 32768 tokens: 16.1 us against 17.9 with eight; on 131071 tokens of 24 / 4 heads of
+// 256, 132 pages a split, 43.3 against 42.4).  With heads of 256 two workgroups do not
+// share a CU.  Sequences of at most 16 pages are not split at all: a second launch costs
+// more than the four pages a wave (250 tokens: 9.1 us against 10.8).
 // `extra`: tokens that the call appends to each sequence (1 or 0).
 qm_status plan_decode_chunk(qm_runtime* rt, qm_kv* const* seqs, uint32_t nb, uint32_t H, uint32_t extra, DecodeChunk* c) {
   // Workgroups of a split.
   const uint32_t KVH = seqs[0]->kv_heads * (seqs[0]->bits == 4 ? q4kv_head_sets(H / seqs[0]->kv_heads) : 1);
-  AttnArgs& at = c->at;
+  AttnCommon& at = c->at;
+  AttnSeq* const sd = c->seqs;
   uint64_t total_pages = 0;
   uint32_t max_pages = 0;
   for (uint32_t i = 0; i < nb; ++i) {
     const qm_kv* kv = seqs[i];
-    AttnSeq sd = seq_desc(kv);
-    plan_pages(kv, kv->length, kv->length + extra, &sd.new_page_first, &sd.new_page_count, &sd.new_page_id);
-    sd.len = kv->length + extra;
-    at.seqs[i] = sd;
-    const uint32_t pages = (sd.len + 15) / 16;
+    AttnSeq& s = sd[i];
+    s = seq_desc(kv);
+    plan_pages(kv, kv->length, kv->length + extra, &s.new_page_first, &s.new_page_count, &s.new_page_id);
+    s.len = kv->length + extra;
+    const uint32_t pages = (s.len + 15) / 16;
     total_pages += pages;
     max_pages = std::max(max_pages, pages);
   }
@@ -236,7 +245,7 @@ qm_status plan_decode_chunk(qm_runtime* rt, qm_kv* const* seqs, uint32_t nb, uin
     return fail(QM_ERR_CAPACITY_EXCEEDED, "sequence of %u pages exceeds the decode kernel's limit", max_pages);
   auto units_for = [&](uint64_t q) {
     uint64_t u = 0;
-    for (uint32_t i = 0; i < nb; ++i) u += ((at.seqs[i].len + 15) / 16 + q - 1) / q * KVH;
+    for (uint32_t i = 0; i < nb; ++i) u += ((sd[i].len + 15) / 16 + q - 1) / q * KVH;
     return u;
   };
   const int forced = rt->tune.attn_pps;
@@ -257,17 +266,21 @@ qm_status plan_decode_chunk(qm_runtime* rt, qm_kv* const* seqs, uint32_t nb, uin
   const int target_env = rt->tune.attn_target_wgs;
   uint32_t waves = 8;
   uint64_t pps = pps_for(target_env > 0 ? (uint32_t)target_env : rt->cu_count);
-  if (waves_env == 4 || (waves_env != 8 && units_for(pps) > (uint64_t)rt->cu_count)) {
+  const bool q4 = seqs[0]->bits == 4, one = q4 && seqs[0]->dp == 256;
+  if (q4 && forced <= 0 && max_pages <= 16) pps = 16;
+  if (waves_env == 0 && q4 && pps <= 96 && (one || units_for(pps) <= (uint64_t)rt->cu_count))
+    waves = 4;
+  else if (waves_env == 4 || (waves_env != 8 && !one && units_for(pps) > (uint64_t)rt->cu_count)) {
     waves = 4;
     pps = pps_for(target_env > 0 ? (uint32_t)target_env : 2 * rt->cu_count);
   }
   uint32_t units = 0, parts = 0;
   for (uint32_t i = 0; i < nb; ++i) {
-    const uint32_t pages = (at.seqs[i].len + 15) / 16;
+    const uint32_t pages = (sd[i].len + 15) / 16;
     const uint32_t ns = (uint32_t)((pages + pps - 1) / pps);
-    at.seqs[i].unit_begin = units;
-    at.seqs[i].nsplit = ns;
-    at.seqs[i].part_begin = parts;
+    sd[i].unit_begin = units;
+    sd[i].nsplit = ns;
+    sd[i].part_begin = parts;
     units += ns * KVH;
     if (ns > 1) {
       parts += ns;
@@ -353,13 +366,14 @@ qm_status plan_decode(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, uint32_t H
                       std::vector<DecodeChunk>* chunks, size_t* partial_bytes) {
   *partial_bytes = 0;
   chunks->clear();
-  for (uint32_t b0 = 0; b0 < B; b0 += kMaxAttnSeqs) {
-    DecodeChunk c;
-    const uint32_t nb = std::min<uint32_t>(kMaxAttnSeqs, B - b0);
+  const uint32_t most = seqs[0]->bits == 4 ? kMaxQ4KvSeqs : kMaxAttnSeqs;
+  for (uint32_t b0 = 0; b0 < B; b0 += most) {
+    chunks->emplace_back();
+    DecodeChunk& c = chunks->back();
+    const uint32_t nb = std::min(most, B - b0);
     qm_status st = plan_decode_chunk(rt, seqs + b0, nb, H, extra, &c);
     if (st != QM_OK) return st;
     c.at.n_seqs = nb;
-    chunks->push_back(c);
     *partial_bytes = std::max(*partial_bytes, (size_t)c.parts * H * (seqs[0]->dp + 2) * sizeof(float));
   }
   return QM_OK;
@@ -375,16 +389,17 @@ qm_status launch_decode(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, const ui
     qm_status st = stream_after(rt, seqs[b]->rt);
     if (st != QM_OK) return st;
   }
-  for (size_t ci = 0; ci < chunks.size(); ++ci) {
-    DecodeChunk& c = chunks[ci];
-    const uint32_t b0 = (uint32_t)ci * kMaxAttnSeqs, nb = c.at.n_seqs;
-    AttnArgs& at = c.at;
+  uint32_t b0 = 0, nb = 0;
+  for (DecodeChunk& c : chunks) {
+    b0 += nb;
+    nb = c.at.n_seqs;
+    AttnCommon& at = c.at;
     if (c.combine && (size_t)c.parts * H * (Dp + 2) * sizeof(float) > partial_bytes)
       return fail(QM_ERR_INVALID_ARGUMENT, "attention decode: split partials exceed the workspace");
     for (uint32_t i = 0; i < nb; ++i) {
       qm_kv* kv = seqs[b0 + i];
-      commit_pages(kv, at.seqs[i].new_page_first, at.seqs[i].new_page_count);
-      kv->length = at.seqs[i].len;
+      commit_pages(kv, c.seqs[i].new_page_first, c.seqs[i].new_page_count);
+      kv->length = c.seqs[i].len;
     }
     at.q = q + (size_t)b0 * H * D;
     at.gate = gate ? gate + (size_t)b0 * H * D : nullptr;
@@ -398,14 +413,27 @@ qm_status launch_decode(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, const ui
     at.prefill = 0;
     at.k_new = k ? k + (size_t)b0 * KVH * D : nullptr;  // the decode kernel appends the new rows itself
     at.v_new = k ? v + (size_t)b0 * KVH * D : nullptr;
-    hipError_t e = seqs[0]->bits == 4 ? launch_q4kv_attention(at, c.units, c.combine, rt->stream)
-                                      : launch_q8_attention(at, c.units, c.combine, rt->stream);
+    hipError_t e;
+    if (seqs[0]->bits == 4) {
+      Q4KvArgs a{};
+      (AttnCommon&)a = at;
+      for (uint32_t i = 0; i < nb; ++i) {
+        const AttnSeq& s = c.seqs[i];
+        a.seqs[i] = Q4KvSeq{(uint8_t*)s.k, s.pt, s.len, s.unit_begin, s.nsplit, s.part_begin, s.new_page_count, s.new_page_id};
+      }
+      e = launch_q4kv_decode(a, c.units, c.combine, rt->stream);
+    } else {
+      AttnArgs a{};
+      (AttnCommon&)a = at;
+      std::copy(c.seqs, c.seqs + nb, a.seqs);
+      e = launch_q8_attention(a, c.units, c.combine, rt->stream);
+    }
     if (e != hipSuccess) {
       // Nothing of this chunk ran: put its sequences back.
       for (uint32_t i = 0; i < nb; ++i) {
         qm_kv* kv = seqs[b0 + i];
-        kv->length = at.seqs[i].len - (k ? 1 : 0);
-        rollback_pages(kv, at.seqs[i].new_page_first, at.seqs[i].new_page_count);
+        kv->length = c.seqs[i].len - (k ? 1 : 0);
+        rollback_pages(kv, c.seqs[i].new_page_first, c.seqs[i].new_page_count);
       }
       return hip_check(e, "attention decode launch");
     }
@@ -558,7 +586,7 @@ qm_status prefill(qm_runtime* rt, qm_kv* seq, const uint16_t* q, const uint16_t*
   // The prefill launcher sizes its own grid (rows per workgroup depend on the
   // kernel's column blocks).
   if (e == hipSuccess)
-    e = seq->bits == 4 ? launch_q4kv_attention(at, 0, false, rt->stream) : launch_q8_attention(at, 0, false, rt->stream);
+    e = seq->bits == 4 ? launch_q4kv_prefill(at, rt->stream) : launch_q8_attention(at, 0, false, rt->stream);
   if (e != hipSuccess) {
     seq->length = before;
     rollback_pages(seq, sd.new_page_first, sd.new_page_count);
