@@ -46,8 +46,10 @@ struct KvAppendArgs {
   uint32_t head_dim_pad;
   uint32_t rotary_dim;  // 0: keys as given
   uint32_t offset;      // first rotated element of a key
+  uint32_t half_log;    // least with 2^half_log >= rotary_dim / 2; filled by the launcher
   uint32_t row0, rows;  // the launch's rows of the call; filled by the launcher
   uint32_t units;       // workgroups that append; filled by the launcher
+  uint32_t share;       // KV heads of one such workgroup; filled by the launcher
   uint32_t q_items;     // filled by the launcher
   uint32_t q_groups;
 };

@@ -54,43 +54,80 @@ __device__ __forceinline__ float q8_rows_quant(const float (&vals)[4], uint32_t 
   return q8_quant_with(amax, vals, qv);
 }
 
-// A group of the 4-bit cache held 4 values per lane of a DPP row (elements d0 ..
-// d0 + 3, those from D on not its own): returns its scale word (s in the low, m in
-// the high half), and the codes, -8..7.
-__device__ __forceinline__ uint32_t q4kv_group(const float (&x)[4], uint32_t d0, uint32_t D, int (&c)[4]) {
-  float top = -INFINITY, low = -INFINITY;  // of x, and of -x
-  bool bad = false;
+// The same of four values at once; all 64 lanes take part.  (A DPP operand is read two
+// wait states after its register was written at the earliest.)
+__device__ __forceinline__ void row_allmax4(float (&v)[4]) {
+#define QM_STEP(how) QM_MAX(0, how) QM_MAX(1, how) QM_MAX(2, how) QM_MAX(3, how)
+#define QM_MAX(r, how) "v_max_f32_dpp %" #r ", %" #r ", %" #r " " how " row_mask:0xf bank_mask:0xf\n"
+  asm("s_nop 1\n" QM_STEP("quad_perm:[1,0,3,2]") QM_STEP("quad_perm:[2,3,0,1]") QM_STEP("row_ror:4") QM_STEP("row_ror:8")
+      : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
+#undef QM_MAX
+#undef QM_STEP
+}
+
+// The groups of a key (x[0]) and of a value (x[1]) in the 4-bit cache, held 4 elements
+// per lane of a DPP row: d0 .. d0 + 3, those from D on not the group's own (WHOLE: all
+// or none are).  Gives the scale words (s in the low, m in the high half) and the
+// codes + 8.  All 64 lanes take part.
+//
+// Quotients round as divisions do: by a reciprocal and one step on the remainder, both
+// exact but for their last rounding.
+template <bool WHOLE>
+__device__ __forceinline__ void q4kv_groups(const float (&x)[2][4], uint32_t d0, uint32_t D, uint32_t (&word)[2],
+                                            uint32_t (&u)[2][4]) {
+  float stat[4];  // maxima of x[0], -x[0], x[1], -x[1]
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if (d0 + e >= D) continue;
-    top = fmaxf(top, x[e]);
-    low = fmaxf(low, -x[e]);
-    bad |= !(fabsf(x[e]) < INFINITY);
-  }
-  if (bad) top = INFINITY;  // (a maximum passes NaN over)
-  top = row_allmax(top);
-  low = row_allmax(low);
-  if (!(fabsf(top) < INFINITY)) {  // NaN; and zeros in a group past D
+  for (int k = 0; k < 2; ++k) {
+    float top, low, z = x[k][0] * 0.0f;
+    if constexpr (WHOLE) {
+      asm("v_max_f32 %0, %4, %5\nv_max_f32 %1, -%4, -%5\nv_max3_f32 %0, %2, %3, %0\nv_max3_f32 %1, -%2, -%3, %1"
+          : "=&v"(top), "=&v"(low)
+          : "v"(x[k][0]), "v"(x[k][1]), "v"(x[k][2]), "v"(x[k][3]));
+      if (d0 >= D) top = low = -INFINITY;
+    } else {
+      top = low = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) c[e] = 0;
-    return top > 0.0f ? 0x7FC07FC0u : 0u;
-  }
-  // Halves: the difference of any two finite values is finite.
-  const uint32_t sb = f32_to_bf16(fmaxf((top * 0.5f + low * 0.5f) / 7.5f, FLT_MIN));
-  const float s = bf16_to_f32(sb);
-  const uint32_t mb = f32_to_bf16(s * 8.0f - low);
-  const float m = bf16_to_f32(mb);
-  if (!(fabsf(m) < INFINITY)) {  // (a middle past bf16's range)
+      for (int e = 0; e < 4; ++e) {
+        top = fmaxf(top, d0 + e < D ? x[k][e] : -INFINITY);
+        low = fmaxf(low, d0 + e < D ? -x[k][e] : -INFINITY);
+      }
+    }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) c[e] = 0;
-    return 0x7FC07FC0u;
+    for (int e = 1; e < 4; ++e) z = __builtin_fmaf(x[k][e], 0.0f, z);
+    stat[2 * k] = z == 0.0f ? top : INFINITY;  // (a maximum passes NaN over)
+    stat[2 * k + 1] = low;
   }
+  row_allmax4(stat);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float t = (x[e] - m) / s;
-    c[e] = d0 + e < D ? (int)rintf(fminf(fmaxf(t, -8.0f), 7.0f)) : 0;
+  for (int k = 0; k < 2; ++k) {
+    const float top = stat[2 * k], low = stat[2 * k + 1];
+    // Halves: the difference of any two finite values is finite.  Small ones are scaled
+    // up, so that no remainder is lost.
+    const float h0 = top * 0.5f + low * 0.5f;
+    const bool tiny = h0 < 0x1p-60f;
+    const float h = tiny ? h0 * 0x1p64f : h0, r75 = 1.0f / 7.5f;
+    float q = h * r75;
+    q = __builtin_fmaf(__builtin_fmaf(-q, 7.5f, h), r75, q);
+    const uint32_t sb = f32_to_bf16(fmaxf(tiny ? q * 0x1p-64f : q, FLT_MIN));
+    const uint32_t mb = f32_to_bf16(__builtin_fmaf(bf16_to_f32(sb), 8.0f, -low));
+    const float m = bf16_to_f32(mb);
+    // Not fine: a value that is not finite, a middle past bf16's range, or no element.
+    const bool fine = fabsf(top) < INFINITY && fabsf(m) < INFINITY;
+    word[k] = fine ? sb | mb << 16 : top == -INFINITY ? 0u : 0x7FC07FC0u;
+    // (x - m) / s with s = sn 2^e, sn in [1, 2) (of 8 bits: no reciprocal lies near a
+    // border); its codes by the rounding of a sum with 1.5 2^23.
+    const int e2 = 127 - (int)(sb >> 7);
+    const float sn = __uint_as_float((sb & 0x7Fu) << 16 | 0x3F800000u);
+    float r = __builtin_amdgcn_rcpf(sn);
+    r = __builtin_fmaf(__builtin_fmaf(-sn, r, 1.0f), r, r);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float a = __builtin_amdgcn_ldexpf(x[k][e] - m, e2), t0 = a * r;
+      const float t = __builtin_fmaf(__builtin_fmaf(-t0, sn, a), r, t0);
+      const uint32_t c = __float_as_uint(__builtin_amdgcn_fmed3f(t, -8.0f, 7.0f) + 12582920.0f) & 15;
+      u[k][e] = fine && d0 + (WHOLE ? 0 : e) < D ? c : 8u;
+    }
   }
-  return sb | mb << 16;
 }
 
 // Eight codes of a K word as bf16 of 128 + (c + 8), in order: 0x4300 | u is the bf16

@@ -263,17 +263,16 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(Q4KvArgs args) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[kind][e] = d0 + e < dr ? src[d0 + e] : 0.0f;
     }
-    uint32_t word[2];
+    uint32_t word[2], u[2][4];
+    q4kv_groups<false>(x, d0, dr, word, u);
 #pragma unroll
     for (int kind = 0; kind < 2; ++kind) {
-      int c[4];
-      word[kind] = q4kv_group(x[kind], d0, dr, c);
       if (kq >= G) continue;  // (copies of the first groups)
       floatx4 y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = q4kv_value(c[e], word[kind]);
+      for (int e = 0; e < 4; ++e) y[e] = q4kv_value((int)u[kind][e] - 8, word[kind]);
       *(floatx4*)(xs + D * kind + d0) = y;
-      *(uint32_t*)(cs + D * kind + d0) = (c[0] + 8) | (c[1] + 8) << 8 | (c[2] + 8) << 16 | (c[3] + 8) << 24;
+      *(uint32_t*)(cs + D * kind + d0) = u[kind][0] | u[kind][1] << 8 | u[kind][2] << 16 | u[kind][3] << 24;
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();

@@ -36,43 +36,65 @@ __device__ __forceinline__ void rotary_table(const double* freq, uint32_t half, 
   }
 }
 
+// 8 elements of a head, as a work item takes them, and its pairs' other elements.
+// (Which product of a sum is rounded first is written out below, so that every kernel
+// that rotates gives the same bits.)
+struct RotaryPiece {
+  u32x4 x, z;
+};
+template <bool INTERLEAVED>
+__device__ __forceinline__ RotaryPiece rotary_load(const RotaryTensor& t, const uint16_t* in, uint32_t local, uint32_t rd) {
+  const uint32_t per = t.head_dim / 8, head = local / per, e = (local - head * per) * 8;
+  const uint16_t* at = in + (size_t)head * t.head_dim + e;
+  const uint32_t c = e - t.offset;  // element of the rotated part (wraps below it)
+  const bool turned = e >= t.offset && c < rd;
+  RotaryPiece p;
+  p.x = *(const u32x4*)at;
+  p.z = !INTERLEAVED && turned && c < rd / 2 ? *(const u32x4*)(at + rd / 2) : p.x;
+  return p;
+}
+template <bool INTERLEAVED>
+__device__ __forceinline__ void rotary_finish(const RotaryTensor& t, const RotaryPiece& p, bool copy, uint16_t* out,
+                                              uint32_t local, uint32_t rd, const float* cos_s, const float* sin_s) {
+  const uint32_t half = rd / 2;
+  const uint32_t per = t.head_dim / 8, head = local / per, e = (local - head * per) * 8;
+  const size_t at = (size_t)head * t.head_dim + e;
+  const uint32_t c = e - t.offset;
+  if (e < t.offset || c >= rd) {
+    if (copy) *(u32x4*)(out + at) = p.x;
+    return;
+  }
+  float x[8], y[8];
+  unpack8(p.x, x);
+  if constexpr (INTERLEAVED) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float cs = cos_s[c / 2 + j], sn = sin_s[c / 2 + j];
+      y[2 * j] = __builtin_fmaf(x[2 * j], cs, -(x[2 * j + 1] * sn));
+      y[2 * j + 1] = __builtin_fmaf(x[2 * j + 1], cs, x[2 * j] * sn);
+    }
+    *(u32x4*)(out + at) = pack8(y);
+  } else {
+    if (c >= half) return;  // its partner's item takes it
+    float z[8], w[8];
+    unpack8(p.z, z);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float cs = cos_s[c + j], sn = sin_s[c + j];
+      y[j] = __builtin_fmaf(x[j], cs, -(z[j] * sn));
+      w[j] = j == 0 ? __builtin_fmaf(z[j], cs, x[j] * sn) : __builtin_fmaf(x[j], sn, z[j] * cs);
+    }
+    *(u32x4*)(out + at) = pack8(y);
+    *(u32x4*)(out + at + half) = pack8(w);
+  }
+}
+
 // Work item `local` of one row of a tensor: 8 elements of a head (VEC) or one.
 template <bool INTERLEAVED, bool VEC>
 __device__ __forceinline__ void rotary_item(const RotaryTensor& t, const uint16_t* in, uint16_t* out, uint32_t local,
                                             uint32_t rd, const float* cos_s, const float* sin_s) {
-  const uint32_t half = rd / 2;
   if constexpr (VEC) {
-    const uint32_t per = t.head_dim / 8, head = local / per, e = (local - head * per) * 8;
-    const size_t at = (size_t)head * t.head_dim + e;
-    const uint32_t c = e - t.offset;  // element of the rotated part (wraps below it)
-    if (e < t.offset || c >= rd) {
-      if (out != in) *(u32x4*)(out + at) = *(const u32x4*)(in + at);
-      return;
-    }
-    float x[8], y[8];
-    if constexpr (INTERLEAVED) {
-      unpack8(*(const u32x4*)(in + at), x);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float cs = cos_s[c / 2 + j], sn = sin_s[c / 2 + j];
-        y[2 * j] = x[2 * j] * cs - x[2 * j + 1] * sn;
-        y[2 * j + 1] = x[2 * j + 1] * cs + x[2 * j] * sn;
-      }
-      *(u32x4*)(out + at) = pack8(y);
-    } else {
-      if (c >= half) return;  // its partner's item takes it
-      float z[8], w[8];
-      unpack8(*(const u32x4*)(in + at), x);
-      unpack8(*(const u32x4*)(in + at + half), z);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float cs = cos_s[c + j], sn = sin_s[c + j];
-        y[j] = x[j] * cs - z[j] * sn;
-        w[j] = z[j] * cs + x[j] * sn;
-      }
-      *(u32x4*)(out + at) = pack8(y);
-      *(u32x4*)(out + at + half) = pack8(w);
-    }
+    rotary_finish<INTERLEAVED>(t, rotary_load<INTERLEAVED>(t, in, local, rd), out != in, out, local, rd, cos_s, sin_s);
   } else {
     const uint32_t head = local / t.head_dim, e = local - head * t.head_dim;
     const size_t at = (size_t)head * t.head_dim + e;
@@ -82,11 +104,11 @@ __device__ __forceinline__ void rotary_item(const RotaryTensor& t, const uint16_
       return;
     }
     // The first element of a pair takes its second along.
-    if (INTERLEAVED ? c % 2 != 0 : c >= half) return;
-    const uint32_t f = INTERLEAVED ? c / 2 : c, step = INTERLEAVED ? 1 : half;
+    if (INTERLEAVED ? c % 2 != 0 : c >= rd / 2) return;
+    const uint32_t f = INTERLEAVED ? c / 2 : c, step = INTERLEAVED ? 1 : rd / 2;
     const float x = bf16_to_f32(in[at]), z = bf16_to_f32(in[at + step]);
-    out[at] = f32_to_bf16(x * cos_s[f] - z * sin_s[f]);
-    out[at + step] = f32_to_bf16(z * cos_s[f] + x * sin_s[f]);
+    out[at] = f32_to_bf16(__builtin_fmaf(x, cos_s[f], -(z * sin_s[f])));
+    out[at + step] = f32_to_bf16(__builtin_fmaf(x, sin_s[f], z * cos_s[f]));
   }
 }
 
