@@ -62,7 +62,7 @@ struct AttnCommon {
   uint32_t wg_waves;         // waves per workgroup, 4 or 8 (decode: two workgroups per CU, or one)
   uint32_t prefill;
   uint32_t splits;           // prefill: workgroups sharing the tiles of a column block
-  uint32_t out8;             // prefill: o and gate rows take 8-byte accesses
+  uint32_t out8;             // o and gate rows take 8-byte accesses
   uint32_t rows;   // prefill: query rows
   uint32_t start;  // prefill: cache position of row 0
 };

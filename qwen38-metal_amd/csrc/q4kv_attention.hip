@@ -84,6 +84,70 @@ __device__ __forceinline__ void load_part(__amdgpu_buffer_rsrc_t r, uint32_t bas
   }
 }
 
+// Ends a decode workgroup.  Lane (col, kq) of a wave holds o[db][r] for d = 16 db + 4 kq
+// + r of column col, its reference m and its own share of the sum of weights l.  Head
+// head0 + c has columns c and c + 8 of every wave: all meet in LDS, in 16-byte pieces
+// (rows of D + 4 floats spread 16 columns over the banks), and every thread weighs
+// them by itself.  They leave as outputs, or as one split's partials.
+constexpr int kMergeRow(int D) { return D + 4; }
+template <int D, int W>
+constexpr int kMergeBytes = W * 16 * (kMergeRow(D) * 4 + 8);
+template <int D, int W>
+__device__ __forceinline__ void merge_columns(const AttnCommon& args, const Q4KvSeq& sq, uint32_t b, uint32_t head0,
+                                              uint32_t n_heads, uint32_t split, uint8_t* lds,
+                                              const floatx4 (&o)[D / 16], float m, float l_lane) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, kq = lane >> 4;
+  const uint32_t H = args.heads, dr = args.head_dim;
+  const float l = sum4_across_kq(l_lane);
+  float* sums = (float*)lds;                               // [wave][column][kMergeRow(D)]
+  float4* ml = (float4*)(sums + W * 16 * kMergeRow(D));  // [head][wave]: m, l of both columns
+#pragma unroll
+  for (int db = 0; db < D / 16; ++db)
+    *(floatx4*)(sums + (16 * wave + col) * kMergeRow(D) + 16 * db + 4 * kq) = o[db];
+  if (kq == 0) ((float2*)ml)[((col & 7) * W + wave) * 2 + (col >> 3)] = float2{m, l};
+  lds_barrier();
+  for (uint32_t e = threadIdx.x; e < n_heads * (D / 4); e += 64 * W) {
+    const uint32_t c = e / (D / 4), d0 = 4 * (e % (D / 4)), head = head0 + c;
+    float4 x[W];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      x[w] = ml[c * W + w];
+      mx = fmaxf(mx, fmaxf(x[w].x, x[w].z));
+    }
+    floatx4 O = {0.f, 0.f, 0.f, 0.f};
+    float L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // (a column that saw nothing holds zeros)
+        const float mw = h ? x[w].z : x[w].x, f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - mx);
+        O += *(const floatx4*)(sums + (16 * w + 8 * h + c) * kMergeRow(D) + d0) * f;
+        L += (h ? x[w].w : x[w].y) * f;
+      }
+    if (sq.nsplit > 1) {
+      // Partials: O [split row][H][D], then (m, l) [split row][H][2].
+      const size_t row = (size_t)(sq.part_begin + split) * H + head;
+      *(floatx4*)(args.partials + row * D + d0) = O;
+      if (d0 == 0) *(float2*)(args.partials + (size_t)args.part_rows * H * D + row * 2) = float2{mx, L};
+      continue;
+    }
+    if (d0 >= dr) continue;
+    O *= 1.0f / fmaxf(L, FLT_MIN);
+    const size_t at = ((size_t)b * H + head) * dr + d0;
+    if (args.out8) {
+      *(u32x2*)(args.o + at) = args.gate ? gated_bf16x4(O, *(const u32x2*)(args.gate + at)) : bf16x4_of(O);
+    } else {
+      for (int i = 0; i < 4 && d0 + i < dr; ++i) {
+        float v = O[i];
+        if (args.gate) v *= gate_sigmoid(bf16_to_f32(args.gate[at + i]));
+        args.o[at + i] = f32_to_bf16(v);
+      }
+    }
+  }
+}
+
 // Decode: a workgroup takes up to 8 query heads of one KV head and a split of the
 // pages.  Every wave walks its pages two at a time, straight from memory into
 // registers, and the 16 columns of a matrix operand are 8 heads times the two pages:
@@ -93,14 +157,15 @@ __device__ __forceinline__ void load_part(__amdgpu_buffer_rsrc_t r, uint32_t bas
 //   these tokens' scale words, a lane each;
 //   O^T[d][column] += V^T P'^T with both pages' tokens along K and P' of zero for
 //   the other page.
-// A column's softmax is its page's alone; decode_merge joins the columns of a head.
+// A column's softmax is its page's alone; merge_columns joins the columns of a head.
 template <int D, int W>
-__global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(Q4KvArgs args) {
+__global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void q4kv_decode_kernel(Q4KvArgs args) {
   constexpr int G = D / 64, kDB = D / 16, kRing = D == 256 ? 2 : 4;  // pairs of pages in flight
   // Two waves a SIMD of D = 256 have no registers for the Q operands, which are the
-  // same for all of them: they lie in LDS.
-  constexpr bool kTight = D == 256;
-  constexpr int kQBytes = kTight ? 4 * G * 1024 : 0;
+  // same for all of them: they lie in LDS, and the columns' sums of their 8-element
+  // pieces behind them.
+  constexpr bool kTight = D == 256 && W == 8;
+  constexpr int kQBytes = kTight ? 4 * G * 1024 + 16 * 2 * G * 4 : 0;
   __shared__ __attribute__((aligned(16))) uint8_t lds[kMergeBytes<D, W> + kQBytes];
 
   const int lane = threadIdx.x & 63;
@@ -140,8 +205,36 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(Q4KvArgs args) {
     const uint32_t j = j0 + lane;
     return j < n_mine ? sq.pt[first + W * j] : 0;
   };
-  int32_t ids = load_ids(0), ids_next = load_ids(64);
   constexpr size_t block = q4kv_block_bytes(D);
+  // The wave that takes the token that this call brings (below) has its loads under way
+  // first.
+  const bool takes_new = append && split + 1 == sq.nsplit && wave == (int)((p_end - p_begin) % W);
+  const bool fresh = sq.new_page_count > 0;
+  int32_t new_phys = sq.new_page_id;
+  float xn[2][4];  // elements 4 col .. + 3 of group kq % G, of the key and of the value
+  if (takes_new) {
+    if (!fresh) new_phys = sq.pt[(sq.len - 1) / 16];
+#pragma unroll
+    for (int kind = 0; kind < 2; ++kind) {
+      const float* src = (kind ? args.v_new : args.k_new) + ((size_t)b * KVH + kvh) * dr;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t d = 64 * (kq % G) + 4 * col + e;
+        xn[kind][e] = d < dr ? src[d] : 0.0f;
+      }
+    }
+  }
+  int32_t ids = load_ids(0), ids_next = load_ids(64);
+  // The lane's pieces of the queries, 8 elements: piece j holds d = 64 (j / 2) + 16 kq + 8
+  // (j % 2) .. + 7.
+  constexpr int kMine = kTight ? 2 * G / W : 2 * G;
+  u32x4 qx[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int j = kTight ? wave + W * i : i;
+    qx[i] = col_ok ? load_q8(args.q + ((size_t)b * H + head) * dr, 64 * (j / 2) + 16 * kq + 8 * (j % 2), dr)
+                   : u32x4{0u, 0u, 0u, 0u};
+  }
   const uint32_t s_at = q4kv_scale_bytes(D) + 4 * q4kv_scale_word(D, 0, 0, 4 * kq + (lane & 3));
   // Pages j (even) and j + 1.  Codes of a page past the wave's last read nothing: a
   // buffer of no bytes.
@@ -178,35 +271,6 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(Q4KvArgs args) {
     return p;
   };
 
-  // Q operands (B of K Q^T) of both pages: the lane's 16 elements of every group, d = 64 g
-  // + 16 kq .. + 15.
-  u32x4 qb[2][kTight ? 1 : 2 * G];
-  u32x4* ql = (u32x4*)(lds + kMergeBytes<D, W>) + lane;
-  {
-    const uint16_t* qp = args.q + ((size_t)b * H + head) * dr;
-    auto q_part = [&](int j) __attribute__((always_inline)) {
-      return col_ok ? load_q8(qp, 64 * (j / 2) + 16 * kq + 8 * (j % 2), dr) : u32x4{0u, 0u, 0u, 0u};
-    };
-    if constexpr (kTight) {
-      u32x4 x[2 * G / W];
-#pragma unroll
-      for (int j = 0; j < 2 * G / W; ++j) x[j] = q_part(wave + W * j);
-#pragma unroll
-      for (int j = 0; j < 2 * G / W; ++j) {
-        ql[64 * (wave + W * j)] = x[j] & mask_a;
-        ql[64 * (2 * G + wave + W * j)] = x[j] & mask_b;
-      }
-    } else {
-      u32x4 x[2 * G];
-#pragma unroll
-      for (int j = 0; j < 2 * G; ++j) x[j] = q_part(j);
-#pragma unroll
-      for (int j = 0; j < 2 * G; ++j) qb[0][j] = x[j] & mask_a, qb[1][j] = x[j] & mask_b;
-    }
-  }
-  auto q_of = [&](int h, int j) __attribute__((always_inline)) {
-    return kTight ? ql[64 * (2 * G * h + j)] : qb[h][kTight ? 0 : j];
-  };
   PairRegs<D> ring[kRing];
 #pragma unroll
   for (int r = 0; r < kRing; ++r) {
@@ -214,21 +278,51 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(Q4KvArgs args) {
     // In order, or the loop's first wait would be for all of them.
     __builtin_amdgcn_sched_barrier(0);
   }
-  if constexpr (kTight) lds_barrier();
-  // Sums of the queries' groups, for the keys' offsets.
-  float qs[G];
+  // The word that the new token shares with others of its page, in every piece.
+  uint8_t* const new_page = sq.k + ((size_t)new_phys * KVH + kvh) * block;
+  uint32_t old[D / 32];
+  if (takes_new) {
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    float x = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const u32x4 q = q_of(0, 2 * g + j) | q_of(1, 2 * g + j);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x += bf16_lo_f32(q[i]) + bf16_hi_f32(q[i]);
-    }
-    x += __shfl_xor(x, 16);
-    qs[g] = x + __shfl_xor(x, 32);
+    for (int w = 0; w < D / 32; ++w)
+      old[w] = *(const uint32_t*)(new_page + q4kv_v_bytes(D) + q4kv_lane_word(D, lane, w));
   }
+  // Q operands (B of K Q^T) of both pages, and the sums of the queries' groups for the
+  // keys' offsets.
+  u32x4 qb[2][kTight ? 1 : 2 * G];
+  u32x4* ql = (u32x4*)(lds + kMergeBytes<D, W>) + lane;
+  float qs[G];
+  {
+    float piece[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      float x = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x += bf16_lo_f32(qx[i][e]) + bf16_hi_f32(qx[i][e]);
+      piece[i] = x;
+    }
+    if constexpr (kTight) {
+      float* sums = (float*)(lds + kMergeBytes<D, W> + 4 * G * 1024);  // [column][piece]
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int j = wave + W * i;
+        ql[64 * j] = qx[i] & mask_a;
+        ql[64 * (2 * G + j)] = qx[i] & mask_b;
+        piece[i] = sum4_across_kq(piece[i]);
+        if (kq == 0) sums[2 * G * col + j] = piece[i];
+      }
+      lds_barrier();
+#pragma unroll
+      for (int g = 0; g < G; ++g) qs[g] = sums[2 * G * col + 2 * g] + sums[2 * G * col + 2 * g + 1];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2 * G; ++j) qb[0][j] = qx[j] & mask_a, qb[1][j] = qx[j] & mask_b;
+#pragma unroll
+      for (int g = 0; g < G; ++g) qs[g] = sum4_across_kq(piece[kTight ? 0 : 2 * g] + piece[kTight ? 0 : 2 * g + 1]);
+    }
+  }
+  auto q_of = [&](int h, int j) __attribute__((always_inline)) {
+    return kTight ? ql[64 * (2 * G * h + j)] : qb[h][kTight ? 0 : j];
+  };
 
   floatx4 o[kDB];
 #pragma unroll
@@ -245,26 +339,14 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(Q4KvArgs args) {
   // other wave waits, and nobody reads the token back.  (Waves that read the page
   // meanwhile see its other tokens' nibbles in either version of a word, and give
   // the new one no weight.)
-  if (append && split + 1 == sq.nsplit && wave == (int)((p_end - p_begin) % W)) {
+  if (takes_new) {
     const uint32_t token = sq.len - 1, slot = token % 16;
-    const bool fresh = sq.new_page_count > 0;
-    const int32_t phys = fresh ? sq.new_page_id : sq.pt[token / 16];
-    uint8_t* page = sq.k + ((size_t)phys * KVH + kvh) * block;
-    float* xs = (float*)lds;               // values as the codes have them, K then V
-    uint8_t* cs = lds + 2 * D * 4;         // codes, c + 8
-    uint32_t old[D / 32];                  // the lane's V words of the page
-#pragma unroll
-    for (int w = 0; w < D / 32; ++w) old[w] = *(const uint32_t*)(page + q4kv_v_bytes(D) + q4kv_lane_word(D, lane, w));
+    // In the wave's own part of LDS (others may be about to leave their sums in theirs).
+    float* xs = (float*)lds + 16 * wave * kMergeRow(D);  // values as the codes have them, K then V
+    uint8_t* cs = (uint8_t*)(xs + 2 * D);                  // codes, c + 8
     const uint32_t g = kq % G, d0 = 64 * g + 4 * col;
-    float x[2][4];
-#pragma unroll
-    for (int kind = 0; kind < 2; ++kind) {
-      const float* src = (kind ? args.v_new : args.k_new) + ((size_t)b * KVH + kvh) * dr;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[kind][e] = d0 + e < dr ? src[d0 + e] : 0.0f;
-    }
     uint32_t word[2], u[2][4];
-    q4kv_groups<false>(x, d0, dr, word, u);
+    q4kv_groups<false>(xn, d0, dr, word, u);
 #pragma unroll
     for (int kind = 0; kind < 2; ++kind) {
       if (kq >= G) continue;  // (copies of the first groups)
@@ -277,11 +359,11 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(Q4KvArgs args) {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     if (set == 0) {
-      if (fresh && kvh == 0 && lane == 0) sq.pt[token / 16] = phys;
+      if (fresh && kvh == 0 && lane == 0) sq.pt[token / 16] = new_phys;
       if (col == 0 && kq < G) {
 #pragma unroll
         for (int kind = 0; kind < 2; ++kind)
-          *(uint32_t*)(page + q4kv_scale_bytes(D) + 4 * q4kv_scale_word(D, kind, g, slot)) = word[kind];
+          *(uint32_t*)(new_page + q4kv_scale_bytes(D) + 4 * q4kv_scale_word(D, kind, g, slot)) = word[kind];
       }
       if ((uint32_t)col == slot) {
 #pragma unroll
@@ -290,14 +372,14 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(Q4KvArgs args) {
           uint32_t w = 0;
 #pragma unroll
           for (int e = 0; e < 8; ++e) w |= (uint32_t)c[e] << q4kv_k_bit(e);
-          *(uint32_t*)(page + q4kv_lane_word(D, lane, j)) = w;
+          *(uint32_t*)(new_page + q4kv_lane_word(D, lane, j)) = w;
         }
       }
       if ((uint32_t)kq == slot / 4) {
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
           const uint32_t sh = q4kv_v_bit(slot, 0), c = cs[D + 32 * j + col] | cs[D + 32 * j + 16 + col] << 8;
-          *(uint32_t*)(page + q4kv_v_bytes(D) + q4kv_lane_word(D, lane, j)) = (old[j] & ~(0x0F0Fu << sh)) | c << sh;
+          *(uint32_t*)(new_page + q4kv_v_bytes(D) + q4kv_lane_word(D, lane, j)) = (old[j] & ~(0x0F0Fu << sh)) | c << sh;
         }
       }
     }
@@ -309,8 +391,7 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(Q4KvArgs args) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) dot += bf16_lo_f32(q[i]) * y[2 * i] + bf16_hi_f32(q[i]) * y[2 * i + 1];
     }
-    dot += __shfl_xor(dot, 16);
-    dot += __shfl_xor(dot, 32);
+    dot = sum4_across_kq(dot);
     // Weight 1 against its own score, or less where the value is large (as below).
     float size = 0.0f;
 #pragma unroll
@@ -447,12 +528,11 @@ __global__ __launch_bounds__(64 * W, 2) void q4kv_decode_kernel(Q4KvArgs args) {
   settle();
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    float x = om[g] + __shfl_xor(om[g], 16);
-    x += __shfl_xor(x, 32);
+    const float x = sum4_across_kq(om[g]);
 #pragma unroll
     for (int db = 4 * g; db < 4 * g + 4; ++db) o[db] += x;
   }
-  decode_merge<D, W, 2>(args, sq, b, head0, n_heads, split, lds, o, m_run, l_lane);
+  merge_columns<D, W>(args, sq, b, head0, n_heads, split, lds, o, m_run, l_lane);
 }
 
 // Causal prefill on 32x32x16 MFMA; columns, tiles, splits and the two LDS stages as in

@@ -84,6 +84,92 @@ __device__ __forceinline__ void q8_store_row(const AttnSeq& sq, const float* src
   if (lane == 0) (kind == 0 ? sq.ks : sq.vs)[pkv * 16 + slot] = s;
 }
 
+// LDS of decode_merge: the waves' O, then m, l, weights, maximum and sums.
+constexpr int kMergePad = 17;  // floats per (wave, d) row of the O reduction (16 columns + 1)
+template <int D, int W>
+constexpr int kMergeBytes = W * D * kMergePad * 4 + (3 * W + 2) * 16 * 4;
+
+// Ends a decode workgroup: its waves' sums (lane (col, kq) holds o[db][r] for d = 16
+// db + 4 kq + r of column col, m_run of it and its own share of l) meet in LDS and
+// leave as outputs, or as one split's partials.  Head head0 + c (of n_heads) has
+// column c.  Every wave of the workgroup calls it.
+template <int D, int W>
+__device__ __forceinline__ void decode_merge(const AttnCommon& args, const AttnSeq& sq, uint32_t b, uint32_t head0,
+                                             uint32_t n_heads, uint32_t split, uint8_t* lds,
+                                             const floatx4 (&o)[D / 16], float m_run, float l_lane) {
+  constexpr int kWaves = W, kDB = D / 16, kPad = kMergePad;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, kq = lane >> 4;
+  const uint32_t H = args.heads, dr = args.head_dim;
+  float l_tot = l_lane + __shfl_xor(l_lane, 16);
+  l_tot += __shfl_xor(l_tot, 32);
+  __syncthreads();  // the rings are reused for the reduction
+  float* red_o = reinterpret_cast<float*>(lds);  // [wave][d][kPad]
+  float(*red_m)[16] = reinterpret_cast<float(*)[16]>(lds + kWaves * D * kPad * 4);
+  float(*red_l)[16] = red_m + kWaves;
+#pragma unroll
+  for (int db = 0; db < kDB; ++db)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) red_o[(wave * D + 16 * db + 4 * kq + r) * kPad + col] = o[db][r];
+  if (kq == 0) {
+    red_m[wave][col] = m_run;
+    red_l[wave][col] = l_tot;
+  }
+  __syncthreads();
+  // Per (wave, column) weights exp2(m_w - max) and the column sums, once;
+  // the element loop below is then multiply-adds only.
+  float(*red_f)[16] = red_l + kWaves;  // [wave][col]
+  float* red_mx = red_l[2 * kWaves];
+  float* red_L = red_mx + 16;
+  if (threadIdx.x < 16) {
+    const uint32_t c = threadIdx.x;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, red_m[w][c]);
+    float Ls = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = red_m[w][c] == -INFINITY ? 0.0f : exp2f(red_m[w][c] - mx);
+      red_f[w][c] = f;
+      Ls += f * red_l[w][c];
+    }
+    red_mx[c] = mx;
+    red_L[c] = Ls;
+  }
+  __syncthreads();
+  const uint32_t nsplit = sq.nsplit;
+  // Split partials: O [split row][H][D], then (m, l) [split row][H][2];
+  // q8_combine_kernel merges them after this launch.
+  const size_t o_rows = (size_t)args.part_rows * H;
+  float* po = args.partials;
+  float* pm = args.partials + o_rows * D;
+  constexpr uint32_t kD4 = D / 4;
+  for (uint32_t e = threadIdx.x; e < n_heads * kD4; e += 64 * kWaves) {
+    const uint32_t c = e / kD4, d0 = 4 * (e % kD4);
+    floatx4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) O[i] += red_f[w][c] * red_o[(w * D + d0 + i) * kPad + c];
+    const uint32_t hh = head0 + c;
+    if (nsplit == 1) {
+      const float inv = 1.0f / fmaxf(red_L[c], FLT_MIN);
+      const size_t oi = ((size_t)b * H + hh) * dr + d0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (d0 + i >= dr) break;
+        float v = O[i] * inv;
+        if (args.gate) v *= sigmoid_f(bf16_to_f32(args.gate[oi + i]));
+        args.o[oi + i] = f32_to_bf16(v);
+      }
+    } else {
+      const size_t row = (size_t)(sq.part_begin + split) * H + hh;
+      *(floatx4*)(po + row * D + d0) = O;
+      if (d0 == 0) *(float2*)(pm + row * 2) = float2{red_mx[c], red_L[c]};
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Append
 // ---------------------------------------------------------------------------
@@ -489,7 +575,7 @@ __global__ __launch_bounds__(64 * W) void q8_decode_kernel(AttnArgs args) {
       }
   }
 
-  decode_merge<D, W, 1>(args, sq, b, kvh * gh, gh, split, lds, o, m_run, l_lane);
+  decode_merge<D, W>(args, sq, b, kvh * gh, gh, split, lds, o, m_run, l_lane);
 }
 
 // Merge the split partials of one (sequence, head, 32-wide d slice): grid

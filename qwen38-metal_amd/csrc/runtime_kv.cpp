@@ -411,6 +411,7 @@ qm_status launch_decode(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, const ui
     at.head_dim = D;
     at.head_dim_pad = Dp;
     at.prefill = 0;
+    at.out8 = D % 4 == 0 && aligned(at.o, 8) && aligned(at.gate, 8);
     at.k_new = k ? k + (size_t)b0 * KVH * D : nullptr;  // the decode kernel appends the new rows itself
     at.v_new = k ? v + (size_t)b0 * KVH * D : nullptr;
     hipError_t e;
