@@ -222,10 +222,10 @@ struct DecodeChunk {
 // 32768 tokens: 16.1 us against 17.9 with eight; on 131071 tokens of 24 / 4 heads of
 // 256, 132 pages a split, 43.3 against 42.4).  With heads of 256 two workgroups do not
 // share a CU.
-// Sequences of at most 32 pages are not split at all, with eight waves from nine pages on:
-// a second launch costs more than the four pages a wave (500 tokens of 24 / 4 heads of
-// 256: 11.2 us against 12.3; of 64 / 8 of 128: 8.7 against 9.3; 1000 tokens: 17.5 against
-// 10.9).
+// Sequences of at most 32 pages are not split at all, with eight waves from 17 pages on (9
+// with heads of 256): a second launch costs more than the four pages a wave (500 tokens of
+// 24 / 4 heads of 256: 11.2 us against 12.3; of 64 / 8 of 128: 8.7 against 9.3; 1000
+// tokens of the former: 17.5 against 10.9).
 // `extra`: tokens that the call appends to each sequence (1 or 0).
 qm_status plan_decode_chunk(qm_runtime* rt, qm_kv* const* seqs, uint32_t nb, uint32_t H, uint32_t extra, DecodeChunk* c) {
   // Workgroups of a split.
@@ -273,7 +273,7 @@ qm_status plan_decode_chunk(qm_runtime* rt, qm_kv* const* seqs, uint32_t nb, uin
   const bool whole = q4 && forced <= 0 && max_pages <= 32;
   if (whole) pps = 32;
   if (waves_env == 0 && whole)
-    waves = max_pages > 8 ? 8 : 4;
+    waves = max_pages > (one ? 8 : 16) ? 8 : 4;
   else if (waves_env == 0 && q4 && pps <= 96 && (one || units_for(pps) <= (uint64_t)rt->cu_count))
     waves = 4;
   else if (waves_env == 4 || (waves_env != 8 && !one && units_for(pps) > (uint64_t)rt->cu_count)) {
