@@ -226,21 +226,17 @@ struct DecodeChunk {
 // with heads of 256): a second launch costs more than the four pages a wave (500 tokens of
 // 24 / 4 heads of 256: 11.2 us against 12.3; of 64 / 8 of 128: 8.7 against 9.3; 1000
 // tokens of the former: 17.5 against 10.9).
-// `extra`: tokens that the call appends to each sequence (1 or 0).
-qm_status plan_decode_chunk(qm_runtime* rt, qm_kv* const* seqs, uint32_t nb, uint32_t H, uint32_t extra, DecodeChunk* c) {
+// The chunk's sequences are there, caches like kv; their splits are filled in.
+qm_status plan_decode_splits(const qm_runtime* rt, const qm_kv* kv, uint32_t nb, uint32_t H, DecodeChunk* c) {
   // Workgroups of a split.
-  const uint32_t KVH = seqs[0]->kv_heads * (seqs[0]->bits == 4 ? q4kv_head_sets(H / seqs[0]->kv_heads) : 1);
+  const uint32_t KVH = kv->kv_heads * (kv->bits == 4 ? q4kv_head_sets(H / kv->kv_heads) : 1);
   AttnCommon& at = c->at;
+  at.n_seqs = nb;
   AttnSeq* const sd = c->seqs;
   uint64_t total_pages = 0;
   uint32_t max_pages = 0;
   for (uint32_t i = 0; i < nb; ++i) {
-    const qm_kv* kv = seqs[i];
-    AttnSeq& s = sd[i];
-    s = seq_desc(kv);
-    plan_pages(kv, kv->length, kv->length + extra, &s.new_page_first, &s.new_page_count, &s.new_page_id);
-    s.len = kv->length + extra;
-    const uint32_t pages = (s.len + 15) / 16;
+    const uint32_t pages = (sd[i].len + 15) / 16;
     total_pages += pages;
     max_pages = std::max(max_pages, pages);
   }
@@ -262,14 +258,14 @@ qm_status plan_decode_chunk(qm_runtime* rt, qm_kv* const* seqs, uint32_t nb, uin
     if (forced > 0) pps = (uint64_t)forced;
     pps = std::max<uint64_t>(pps, (max_pages + kMaxSplits - 1) / kMaxSplits);
     if (forced <= 0)
-      while (pps < kMaxPagesPerSplit && units_for(pps) > target) pps += 4;
+      while (pps < std::min<uint64_t>(kMaxPagesPerSplit, max_pages) && units_for(pps) > target) pps += 4;
     return std::min<uint64_t>(pps, kMaxPagesPerSplit);
   };
   const int waves_env = rt->tune.attn_waves;
   const int target_env = rt->tune.attn_target_wgs;
   uint32_t waves = 8;
   uint64_t pps = pps_for(target_env > 0 ? (uint32_t)target_env : rt->cu_count);
-  const bool q4 = seqs[0]->bits == 4, one = q4 && seqs[0]->dp == 256;
+  const bool q4 = kv->bits == 4, one = q4 && kv->dp == 256;
   const bool whole = q4 && forced <= 0 && max_pages <= 32;
   if (whole) pps = 32;
   if (waves_env == 0 && whole)
@@ -298,6 +294,30 @@ qm_status plan_decode_chunk(qm_runtime* rt, qm_kv* const* seqs, uint32_t nb, uin
   c->units = units;
   c->parts = parts;
   return QM_OK;
+}
+
+// One chunk of a decode call, which appends `extra` tokens (1 or 0) to each sequence.
+qm_status plan_decode_chunk(const qm_runtime* rt, qm_kv* const* seqs, uint32_t nb, uint32_t H, uint32_t extra,
+                            DecodeChunk* c) {
+  for (uint32_t i = 0; i < nb; ++i) {
+    const qm_kv* kv = seqs[i];
+    AttnSeq& s = c->seqs[i];
+    s = seq_desc(kv);
+    plan_pages(kv, kv->length, kv->length + extra, &s.new_page_first, &s.new_page_count, &s.new_page_id);
+    s.len = kv->length + extra;
+  }
+  return plan_decode_splits(rt, seqs[0], nb, H, c);
+}
+
+// Kernel arguments of a chunk over 4-bit caches.
+Q4KvArgs q4kv_args(const DecodeChunk& c) {
+  Q4KvArgs a{};
+  (AttnCommon&)a = c.at;
+  for (uint32_t i = 0; i < c.at.n_seqs; ++i) {
+    const AttnSeq& s = c.seqs[i];
+    a.seqs[i] = Q4KvSeq{(uint8_t*)s.k, s.pt, s.len, s.unit_begin, s.nsplit, s.part_begin, s.new_page_count, s.new_page_id};
+  }
+  return a;
 }
 
 // The prefill kernel's launch shape: waves per workgroup (32 columns each; a
@@ -379,7 +399,6 @@ qm_status plan_decode(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, uint32_t H
     const uint32_t nb = std::min(most, B - b0);
     qm_status st = plan_decode_chunk(rt, seqs + b0, nb, H, extra, &c);
     if (st != QM_OK) return st;
-    c.at.n_seqs = nb;
     *partial_bytes = std::max(*partial_bytes, (size_t)c.parts * H * (seqs[0]->dp + 2) * sizeof(float));
   }
   return QM_OK;
@@ -422,13 +441,7 @@ qm_status launch_decode(qm_runtime* rt, qm_kv* const* seqs, uint32_t B, const ui
     at.v_new = k ? v + (size_t)b0 * KVH * D : nullptr;
     hipError_t e;
     if (seqs[0]->bits == 4) {
-      Q4KvArgs a{};
-      (AttnCommon&)a = at;
-      for (uint32_t i = 0; i < nb; ++i) {
-        const AttnSeq& s = c.seqs[i];
-        a.seqs[i] = Q4KvSeq{(uint8_t*)s.k, s.pt, s.len, s.unit_begin, s.nsplit, s.part_begin, s.new_page_count, s.new_page_id};
-      }
-      e = launch_q4kv_decode(a, c.units, c.combine, rt->stream);
+      e = launch_q4kv_decode(q4kv_args(c), c.units, c.combine, rt->stream);
     } else {
       AttnArgs a{};
       (AttnCommon&)a = at;
@@ -541,6 +554,15 @@ hipError_t append_rows(const qm_kv* kv, const AttnSeq& sd, const float* k, const
   return launch_q8_append(ap, M, st);
 }
 
+// Rows over a 4-bit cache that go as a decode step of as many sequences that share it:
+// those of one launch, as long as the prefill kernel's unpacking, which serves all of
+// them, does not win (64 / 8 heads of 128, 20000 tokens: 8 rows 37.6 us against 39.7, 12
+// rows 60.8 against 44.1; 4000 tokens: 32 rows 29.5 against 35.9; 24 / 4 of 256, 20000
+// tokens: 5 rows 32.5 against 44.3).
+bool few_rows(const qm_kv* kv, uint32_t H, uint32_t M, uint64_t tokens) {
+  return kv->bits == 4 && M <= kMaxQ4KvSeqs && M * q4kv_head_sets(H / kv->kv_heads) * tokens <= 160 * 1024;
+}
+
 // Causal attention of the rows behind the cached tokens, which it appends (k and
 // v), or of the last M tokens.
 qm_status prefill(qm_runtime* rt, qm_kv* seq, const uint16_t* q, const uint16_t* gate, const float* k, const float* v,
@@ -576,7 +598,23 @@ qm_status prefill(qm_runtime* rt, qm_kv* seq, const uint16_t* q, const uint16_t*
   at.start = start;
   at.seqs[0] = sd;
   at.out8 = D % 8 == 0 && aligned(o, 8);
-  plan_prefill(rt, &at);
+  bool few = few_rows(seq, H, M, end);
+  DecodeChunk c;
+  if (few) {
+    c.at = at;
+    c.at.prefill = 0;
+    c.at.out8 = D % 4 == 0 && aligned(o, 8) && aligned(gate, 8);
+    for (uint32_t i = 0; i < M; ++i) {
+      c.seqs[i] = sd;
+      c.seqs[i].len = start + i + 1;
+    }
+    if ((st = plan_decode_splits(rt, seq, M, H, &c)) != QM_OK) return st;
+    const size_t bytes = (size_t)c.parts * H * (seq->dp + 2) * sizeof(float);
+    few = bytes == 0 || try_partials(rt, bytes);  // (no room, as under capture: without)
+    c.at.part_rows = c.parts;
+    c.at.partials = (float*)rt->partials;
+  }
+  if (!few) plan_prefill(rt, &at);
   if (at.splits > 1) {
     at.part_rows = M * at.splits;
     const size_t bytes = (size_t)at.part_rows * H * (seq->dp + 2) * sizeof(float);
@@ -593,7 +631,9 @@ qm_status prefill(qm_runtime* rt, qm_kv* seq, const uint16_t* q, const uint16_t*
   // The prefill launcher sizes its own grid (rows per workgroup depend on the
   // kernel's column blocks).
   if (e == hipSuccess)
-    e = seq->bits == 4 ? launch_q4kv_prefill(at, rt->stream) : launch_q8_attention(at, 0, false, rt->stream);
+    e = few ? launch_q4kv_decode(q4kv_args(c), c.units, c.combine, rt->stream)
+        : seq->bits == 4 ? launch_q4kv_prefill(at, rt->stream)
+                         : launch_q8_attention(at, 0, false, rt->stream);
   if (e != hipSuccess) {
     seq->length = before;
     rollback_pages(seq, sd.new_page_first, sd.new_page_count);
