@@ -918,14 +918,14 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
       if (hf) qbias.z = r[0] | r[1] << 16, qbias.w = r[2] | 0x3F800000u;
       x -= shift;
     }
-    // The sum takes the weights as they are rounded.
+    // The sum takes the weights before they round: those of a tile whose values are far
+    // smaller than others' may round to nothing, but count.
     float psum[2] = {0.0f, 0.0f};
-    const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t w = pack_f16x2(__builtin_amdgcn_exp2f(x[2 * i]), __builtin_amdgcn_exp2f(x[2 * i + 1]));
-      ph[i >> 2][i & 3] = w;
-      psum[i & 1] = __builtin_amdgcn_fdot2(as_half2(w), ones, psum[i & 1], false);
+      const float w0 = __builtin_amdgcn_exp2f(x[2 * i]), w1 = __builtin_amdgcn_exp2f(x[2 * i + 1]);
+      ph[i >> 2][i & 3] = pack_f16x2(w0, w1);
+      psum[0] += w0, psum[1] += w1;
     }
     l_lane = __builtin_fmaf(psum[0] + psum[1], *(const float*)(tab + L::kMisc + 24), l_lane);
     if (nan_any) {  // values that are NaN: of the columns that see them, and their group
