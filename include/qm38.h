@@ -280,7 +280,12 @@ qm_status qm_kv_read(const qm_kv* kv, int8_t* keys, int8_t* values,
  * infinity stands for NaN.  4.5 bits an element where head_dim is its storage
  * width (Dp as above), kept as one block per (page, KV head).  Every call below
  * that takes a qm_kv takes either kind, and so does a decode layer; one call takes
- * caches of one kind. */
+ * caches of one kind.
+ *
+ * Attention over these caches takes weights and values in 16 bits at least, sums in
+ * fp32.  A prefill of many rows has its values in fp16 under a power of two for every 32
+ * tokens: what lies more than 2^24 below the largest of the 32, or 2^80 apart from the
+ * first tokens' size, may be lost beside it. */
 qm_status qm_kv_create_q4(qm_runtime* rt, uint32_t kv_heads, uint32_t head_dim,
                           uint32_t page_tokens, uint32_t max_tokens, qm_kv** out);
 uint32_t qm_kv_bits(const qm_kv* kv); /* 8 or 4; 0 for NULL */

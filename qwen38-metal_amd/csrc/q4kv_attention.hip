@@ -1,7 +1,13 @@
 // GQA attention over the paged 4-bit KV cache (layout and codes: q4kv.h).
 //
-// A wave takes a (row, query head) and walks the row's tokens with a running
-// maximum and sum; a lane holds the head's elements lane, lane + 64, ...
+// With x = s c + m for every element of a group g, what attention needs splits into
+// products of codes, which matrix instructions form exactly, and a few products a token:
+//   q . k = sum_g s_g (q_g . c_g) + m_g (sum of q_g),
+//   sum_t p_t v_t = sum_t (p_t s_t) c_t + (sum_t p_t m_t)      (decode).
+// Decode reads every page once, straight into registers, and is bound by that stream and
+// by its vector instructions; prefill unpacks a tile once for up to 256 columns and is
+// bound by the issue of its vector and matrix instructions.  Softmax with a running
+// reference and sum in fp32.
 #include <float.h>
 
 #include <type_traits>
@@ -158,6 +164,12 @@ __device__ __forceinline__ void merge_columns(const AttnCommon& args, const Q4Kv
 //   O^T[d][column] += V^T P'^T with both pages' tokens along K and P' of zero for
 //   the other page.
 // A column's softmax is its page's alone; merge_columns joins the columns of a head.
+//
+// Weights P' = p s are bf16 hi + lo (error 2^-17), codes exact.  131072 tokens of 24 / 4
+// heads of 256: 36.7 us, 151 MB at 4.1 TB/s (a copy reaches 4.7), vector instructions
+// busy for 40 % of the cycles, matrix ones for 14 %; 16 sequences of 32768 tokens of 64 / 8
+// heads of 128: 117 us, 604 MB at 5.2 TB/s (the loads alone 109).  With one page a round,
+// its 8 heads in 8 of the 16 columns, a ragged batch of 8 took 71.8 us against 66.1.
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void q4kv_decode_kernel(Q4KvArgs args) {
   constexpr int G = D / 64, kDB = D / 16, kRing = D == 256 ? 2 : 4;  // pairs of pages in flight
@@ -551,6 +563,12 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void q4kv_decod
 //     32 lose bits, as do those of tiles more than 2^80 below an earlier one.
 // The tables of a tile (scales, offsets, powers) are formed a tile ahead of its
 // unpacking by two waves.
+//
+// 2048 rows on 4096 tokens of 64 / 8 heads of 128: 457 us, 750 TFLOP/s (a large matrix
+// product reaches 1230), matrix instructions busy for 32 % of the cycles, vector ones
+// for 44 %, half of those for the unpacking and the softmax's exponentials.  The same
+// without scores a tile ahead took 618 us, with a tile's tables and V on the last waves
+// alone 564.  1000 rows of 24 / 4 heads of 256: 69 us.
 template <int D, int W>
 struct PrefillLds {
   static constexpr int G = D / 64;
