@@ -36,17 +36,81 @@ __device__ __forceinline__ void rotary_table(const double* freq, uint32_t half, 
   }
 }
 
-// 8 elements of a head, as a work item takes them, and its pairs' other elements.
-// (Which product of a sum is rounded first is written out below, so that every kernel
-// that rotates gives the same bits.)
+// Eight pairs' or four interleaved pairs' rotation, c their place in the table.  (Which
+// product of a sum is rounded first is written out, so that every kernel that rotates
+// gives the same bits.)
+__device__ __forceinline__ void turn_interleaved(const float (&x)[8], float (&y)[8], const float* cos_s, const float* sin_s,
+                                                 uint32_t c) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float cs = cos_s[c + j], sn = sin_s[c + j];
+    y[2 * j] = __builtin_fmaf(x[2 * j], cs, -(x[2 * j + 1] * sn));
+    y[2 * j + 1] = __builtin_fmaf(x[2 * j + 1], cs, x[2 * j] * sn);
+  }
+}
+__device__ __forceinline__ void turn_halves(const float (&x)[8], const float (&z)[8], float (&y)[8], float (&w)[8],
+                                            const float* cos_s, const float* sin_s, uint32_t c) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float cs = cos_s[c + j], sn = sin_s[c + j];
+    y[j] = __builtin_fmaf(x[j], cs, -(z[j] * sn));
+    w[j] = j == 0 ? __builtin_fmaf(z[j], cs, x[j] * sn) : __builtin_fmaf(x[j], sn, z[j] * cs);
+  }
+}
+
+// Work item `local` of one row of a tensor: 8 elements of a head (VEC) or one.
+template <bool INTERLEAVED, bool VEC>
+__device__ __forceinline__ void rotary_item(const RotaryTensor& t, const uint16_t* in, uint16_t* out, uint32_t local,
+                                            uint32_t rd, const float* cos_s, const float* sin_s) {
+  const uint32_t half = rd / 2;
+  if constexpr (VEC) {
+    const uint32_t per = t.head_dim / 8, head = local / per, e = (local - head * per) * 8;
+    const size_t at = (size_t)head * t.head_dim + e;
+    const uint32_t c = e - t.offset;  // element of the rotated part (wraps below it)
+    if (e < t.offset || c >= rd) {
+      if (out != in) *(u32x4*)(out + at) = *(const u32x4*)(in + at);
+      return;
+    }
+    float x[8], y[8];
+    if constexpr (INTERLEAVED) {
+      unpack8(*(const u32x4*)(in + at), x);
+      turn_interleaved(x, y, cos_s, sin_s, c / 2);
+      *(u32x4*)(out + at) = pack8(y);
+    } else {
+      if (c >= half) return;  // its partner's item takes it
+      float z[8], w[8];
+      unpack8(*(const u32x4*)(in + at), x);
+      unpack8(*(const u32x4*)(in + at + half), z);
+      turn_halves(x, z, y, w, cos_s, sin_s, c);
+      *(u32x4*)(out + at) = pack8(y);
+      *(u32x4*)(out + at + half) = pack8(w);
+    }
+  } else {
+    const uint32_t head = local / t.head_dim, e = local - head * t.head_dim;
+    const size_t at = (size_t)head * t.head_dim + e;
+    const uint32_t c = e - t.offset;
+    if (e < t.offset || c >= rd) {
+      if (out != in) out[at] = in[at];
+      return;
+    }
+    // The first element of a pair takes its second along.
+    if (INTERLEAVED ? c % 2 != 0 : c >= half) return;
+    const uint32_t f = INTERLEAVED ? c / 2 : c, step = INTERLEAVED ? 1 : half;
+    const float x = bf16_to_f32(in[at]), z = bf16_to_f32(in[at + step]);
+    out[at] = f32_to_bf16(__builtin_fmaf(x, cos_s[f], -(z * sin_s[f])));
+    out[at + step] = f32_to_bf16(__builtin_fmaf(x, sin_s[f], z * cos_s[f]));
+  }
+}
+
+// The same item (VEC) in two steps, for a caller that forms its table meanwhile.
 struct RotaryPiece {
-  u32x4 x, z;
+  u32x4 x, z;  // z: the pairs' other elements
 };
 template <bool INTERLEAVED>
 __device__ __forceinline__ RotaryPiece rotary_load(const RotaryTensor& t, const uint16_t* in, uint32_t local, uint32_t rd) {
   const uint32_t per = t.head_dim / 8, head = local / per, e = (local - head * per) * 8;
   const uint16_t* at = in + (size_t)head * t.head_dim + e;
-  const uint32_t c = e - t.offset;  // element of the rotated part (wraps below it)
+  const uint32_t c = e - t.offset;
   const bool turned = e >= t.offset && c < rd;
   RotaryPiece p;
   p.x = *(const u32x4*)at;
@@ -67,48 +131,15 @@ __device__ __forceinline__ void rotary_finish(const RotaryTensor& t, const Rotar
   float x[8], y[8];
   unpack8(p.x, x);
   if constexpr (INTERLEAVED) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float cs = cos_s[c / 2 + j], sn = sin_s[c / 2 + j];
-      y[2 * j] = __builtin_fmaf(x[2 * j], cs, -(x[2 * j + 1] * sn));
-      y[2 * j + 1] = __builtin_fmaf(x[2 * j + 1], cs, x[2 * j] * sn);
-    }
+    turn_interleaved(x, y, cos_s, sin_s, c / 2);
     *(u32x4*)(out + at) = pack8(y);
   } else {
-    if (c >= half) return;  // its partner's item takes it
+    if (c >= half) return;
     float z[8], w[8];
     unpack8(p.z, z);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float cs = cos_s[c + j], sn = sin_s[c + j];
-      y[j] = __builtin_fmaf(x[j], cs, -(z[j] * sn));
-      w[j] = j == 0 ? __builtin_fmaf(z[j], cs, x[j] * sn) : __builtin_fmaf(x[j], sn, z[j] * cs);
-    }
+    turn_halves(x, z, y, w, cos_s, sin_s, c);
     *(u32x4*)(out + at) = pack8(y);
     *(u32x4*)(out + at + half) = pack8(w);
-  }
-}
-
-// Work item `local` of one row of a tensor: 8 elements of a head (VEC) or one.
-template <bool INTERLEAVED, bool VEC>
-__device__ __forceinline__ void rotary_item(const RotaryTensor& t, const uint16_t* in, uint16_t* out, uint32_t local,
-                                            uint32_t rd, const float* cos_s, const float* sin_s) {
-  if constexpr (VEC) {
-    rotary_finish<INTERLEAVED>(t, rotary_load<INTERLEAVED>(t, in, local, rd), out != in, out, local, rd, cos_s, sin_s);
-  } else {
-    const uint32_t head = local / t.head_dim, e = local - head * t.head_dim;
-    const size_t at = (size_t)head * t.head_dim + e;
-    const uint32_t c = e - t.offset;
-    if (e < t.offset || c >= rd) {
-      if (out != in) out[at] = in[at];
-      return;
-    }
-    // The first element of a pair takes its second along.
-    if (INTERLEAVED ? c % 2 != 0 : c >= rd / 2) return;
-    const uint32_t f = INTERLEAVED ? c / 2 : c, step = INTERLEAVED ? 1 : rd / 2;
-    const float x = bf16_to_f32(in[at]), z = bf16_to_f32(in[at + step]);
-    out[at] = f32_to_bf16(__builtin_fmaf(x, cos_s[f], -(z * sin_s[f])));
-    out[at + step] = f32_to_bf16(__builtin_fmaf(x, sin_s[f], z * cos_s[f]));
   }
 }
 
