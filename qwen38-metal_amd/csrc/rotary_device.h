@@ -54,7 +54,7 @@ __device__ __forceinline__ void turn_halves(const float (&x)[8], const float (&z
   for (int j = 0; j < 8; ++j) {
     const float cs = cos_s[c + j], sn = sin_s[c + j];
     y[j] = __builtin_fmaf(x[j], cs, -(z[j] * sn));
-    w[j] = j == 0 ? __builtin_fmaf(z[j], cs, x[j] * sn) : __builtin_fmaf(x[j], sn, z[j] * cs);
+    w[j] = __builtin_fmaf(z[j], cs, x[j] * sn);
   }
 }
 
