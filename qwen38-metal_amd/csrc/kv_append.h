@@ -54,6 +54,12 @@ struct KvAppendArgs {
   uint32_t q_groups;
 };
 
+// Workgroups that a launch takes: its threads are counted in 32 bits.
+constexpr uint64_t kv_append_most(uint32_t head_dim_pad) { return 0xFFFFFFFFull / (4 * head_dim_pad); }
+constexpr uint64_t kv_load_most(uint32_t head_dim_pad) { return 0xFFFFFFFFull / (5 * head_dim_pad / 2); }
+// Workgroups that rotate queries share a row where rows are few, up to this many in all.
+constexpr uint32_t kQueryGroups = 1024;
+
 // `vec`: keys and values take 8-byte loads (4 elements) and a key's pairs lie 4
 // elements at a time; `qvec`: queries as launch_rotary's vec.
 hipError_t launch_kv_append(const KvAppendArgs& a, uint32_t bits, bool interleaved, bool vec, bool qvec,

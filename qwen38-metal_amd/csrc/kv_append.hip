@@ -382,10 +382,10 @@ hipError_t launch_kv_append(const KvAppendArgs& args, uint32_t bits, bool interl
   if (a.q.in) {
     a.q_items = a.q.heads * a.q.head_dim / (qvec ? 8 : 1);
     const uint32_t most = (a.q_items + 4 * a.head_dim_pad - 1) / (4 * a.head_dim_pad);
-    a.q_groups = std::max(1u, std::min(most, (1024u + a.rows - 1) / a.rows));
+    a.q_groups = std::max(1u, std::min(most, (kQueryGroups + a.rows - 1) / a.rows));
     grid += (uint64_t)a.rows * a.q_groups;
   }
-  if (grid > 0xFFFFFFFFull / 1024) return hipErrorInvalidValue;
+  if (grid > kv_append_most(a.head_dim_pad)) return hipErrorInvalidValue;
   if (bits == 4)
     interleaved ? launch_append<4, true>(a, vec, qvec, (uint32_t)grid, st)
                 : launch_append<4, false>(a, vec, qvec, (uint32_t)grid, st);
@@ -399,7 +399,7 @@ hipError_t launch_q4kv_append_f32(const KvAppendArgs& args, bool vec, hipStream_
   KvAppendArgs a = args;
   const uint64_t grid = plan_units(&a);
   if (a.rows == 0) return hipSuccess;
-  if (grid > 0xFFFFFFFFull / 1024) return hipErrorInvalidValue;
+  if (grid > kv_append_most(a.head_dim_pad)) return hipErrorInvalidValue;
   auto kernel = vec ? kv_append_kernel<4, float, false, true, false> : kv_append_kernel<4, float, false, false, false>;
   hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(4 * a.head_dim_pad), 0, st, a);
   return hipGetLastError();
@@ -407,7 +407,7 @@ hipError_t launch_q4kv_append_f32(const KvAppendArgs& args, bool vec, hipStream_
 
 hipError_t launch_kv_load(const KvLoadArgs& a, uint32_t bits, hipStream_t st) {
   const uint64_t units = (uint64_t)((a.first + (uint64_t)a.count - 1) / 16 - a.first / 16 + 1) * a.kv_heads;
-  if (a.count == 0 || units > 0xFFFFFFFFull / 640) return hipErrorInvalidValue;
+  if (a.count == 0 || units > kv_load_most(a.head_dim_pad)) return hipErrorInvalidValue;
   const bool vec = a.head_dim % 8 == 0 && (uintptr_t)a.k % 16 == 0 && (uintptr_t)a.v % 16 == 0;
   auto kernel = bits == 4 ? (vec ? kv_load_kernel<4, true> : kv_load_kernel<4, false>)
                           : (vec ? kv_load_kernel<8, true> : kv_load_kernel<8, false>);

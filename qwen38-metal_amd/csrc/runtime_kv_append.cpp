@@ -96,9 +96,9 @@ qm_status qm_kv_append(qm_runtime* rt, qm_kv* const* seqs, const uint32_t* count
     if (overlap(out, extent(a.k, a.k_stride, width, total)) || overlap(out, extent(a.v, a.v_stride, width, total)) ||
         (!(t.in == t.out && t.in_stride == t.out_stride) && overlap(out, extent(t.in, t.in_stride, qwidth, total))))
       return fail(QM_ERR_INVALID_ARGUMENT, "q_out overlaps an input");
-    units += total * ((qwidth / (qvec ? 8 : 1) + 255) / 256);
+    units += total + kQueryGroups;
   }
-  if (units > (1u << 24) - 1) return fail(QM_ERR_DIMENSION_OVERFLOW, "rows * heads pass one launch");
+  if (units > kv_append_most(s0->dp)) return fail(QM_ERR_DIMENSION_OVERFLOW, "rows * heads pass one launch");
   DeviceGuard g(rt->device);
   if (!g.ok()) return no_device();
   qm_status st = check_stream(rt, "append");
@@ -150,7 +150,7 @@ qm_status qm_kv_load(qm_runtime* rt, const qm_kv* kv, uint32_t first, uint32_t c
     return fail(QM_ERR_INVALID_SEQUENCE_LENGTH, "tokens %u .. of a sequence of %u", first, kv->length);
   if (!aligned(k, 2) || !aligned(v, 2)) return fail(QM_ERR_MISALIGNED, "k and v need 2-byte alignment");
   if (kv->rt->device != rt->device) return fail(QM_ERR_INVALID_ARGUMENT, "the cache is on another device");
-  if (((uint64_t)count / 16 + 2) * kv->kv_heads > (1u << 24) - 1)
+  if (((uint64_t)count / 16 + 2) * kv->kv_heads > kv_load_most(kv->dp))
     return fail(QM_ERR_DIMENSION_OVERFLOW, "tokens * kv_heads pass one launch");
   DeviceGuard g(rt->device);
   if (!g.ok()) return no_device();

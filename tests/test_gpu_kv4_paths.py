@@ -441,6 +441,12 @@ def test_refused_appends(rt):
     assert status(rt.kv_append, [a], [8], k.data_ptr() + 1, v) == "QM_ERR_MISALIGNED"
     narrow = torch.as_strided(k, (8, KVH, D), (64, D, 1))
     assert status(rt.kv_append, [a], [8], narrow, v) == bad
+    # More workgroups than a launch takes (refused before anything grows or is read).
+    for heads, dim in ((512, 1), (80, 256)):
+        many = make(rt, 4, heads, dim)
+        assert status(rt.kv_append, [many], [1 << 20], k.data_ptr(), v.data_ptr()) == "QM_ERR_DIMENSION_OVERFLOW"
+        assert many.capacity_tokens < 1 << 20
+        many.close()
     torch.cuda.synchronize()
     assert (out == 2).all()
     for c, old in zip((a, b, full), was):
