@@ -19,6 +19,20 @@ inline uint32_t attn_padded_dim(uint32_t d) { return d <= 64 ? 64 : d <= 128 ? 1
 // Q operand D / 4.
 constexpr int attn_prefill_waves(uint32_t D, int W) { return D == 64 ? 3 : D == 256 && W == 4 ? 1 : 2; }
 
+// Prefill: 32-token tiles that a block of columns walks (its last row's), and the
+// workgroups that share them.
+__host__ __device__ inline uint32_t prefill_tiles(uint32_t block, uint32_t block_cols, uint32_t cols, uint32_t gh,
+                                                  uint32_t start, uint32_t len) {
+  const uint32_t end = (block + 1) * block_cols, last = ((end < cols ? end : cols) - 1) / gh;
+  const uint32_t seen = start + last + 1;
+  return ((seen < len ? seen : len) + 31) / 32;
+}
+__host__ __device__ inline uint32_t prefill_block_splits(uint32_t tiles, uint32_t split_tiles, uint32_t splits) {
+  if (split_tiles == 0) return splits;
+  const uint32_t n = (tiles + split_tiles - 1) / split_tiles;
+  return n < splits ? n : splits;
+}
+
 struct AttnSeq {
   int8_t* k;          // K pages   [page][kv_head][16][D]; 4-bit caches: [page][kv_head] blocks, v, ks and vs unused
   int8_t* v;          // V pages   [page][kv_head][D][16]
@@ -61,7 +75,8 @@ struct AttnCommon {
   uint32_t pages_per_split;  // decode
   uint32_t wg_waves;         // waves per workgroup, 4 or 8 (decode: two workgroups per CU, or one)
   uint32_t prefill;
-  uint32_t splits;           // prefill: workgroups sharing the tiles of a column block
+  uint32_t splits;           // prefill: workgroups sharing the tiles of a column block (at most, where the next is set)
+  uint32_t split_tiles;      // prefill over 4-bit caches: tiles of a workgroup at most; 0: splits for every block
   uint32_t out8;             // o and gate rows take 8-byte accesses
   uint32_t rows;   // prefill: query rows
   uint32_t start;  // prefill: cache position of row 0
@@ -90,6 +105,7 @@ struct AttnCombineArgs {
   uint32_t heads, head_dim, head_dim_pad, part_rows;
   uint32_t prefill, splits, out8;
   uint32_t rows;  // query rows (prefill) or sequences
+  uint32_t kv_heads, block_cols, split_tiles, start, len;  // prefill: which splits a block of columns has
   struct {
     uint32_t nsplit, part_begin;
   } seqs[kMaxQ4KvSeqs];  // decode
@@ -108,12 +124,25 @@ AttnCombineArgs combine_args(const Args& a) {
   c.splits = a.splits;
   c.out8 = a.out8;
   c.rows = a.prefill ? a.rows : a.n_seqs;
+  c.kv_heads = a.kv_heads;
+  c.block_cols = 32 * a.wg_waves;
+  c.split_tiles = a.prefill ? a.split_tiles : 0;
+  c.start = a.start;
+  c.len = a.seqs[0].len;
   for (uint32_t i = 0; !a.prefill && i < a.n_seqs; ++i) {
     c.seqs[i].nsplit = a.seqs[i].nsplit;
     c.seqs[i].part_begin = a.seqs[i].part_begin;
   }
   return c;
 }
+
+// Prefill over 4-bit caches.  With split_tiles set, the workgroups of a KV head are those
+// of split 0 of every block, then of split 1 of the blocks that have one, ...: blocks
+// from the last one on, their tiles never grow.
+constexpr int kMaxBlockSplits = 16;
+struct Q4KvPrefillArgs : AttnArgs {
+  uint32_t split_begin[kMaxBlockSplits];  // first workgroup of each split
+};
 
 // Split partials of qm_attn_decode_noalloc: a file-scope device array of the
 // attention source (one copy per GPU, held until the process ends) whose

@@ -630,7 +630,7 @@ __device__ __forceinline__ u32x4 k_codes16(uint32_t w) {
 }
 
 template <int D, int W>
-__global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill_kernel(AttnArgs args) {
+__global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill_kernel(Q4KvPrefillArgs args) {
   using L = PrefillLds<D, W>;
   constexpr int G = D / 64;
   constexpr int kDB = D / 32;  // 32-wide d blocks of O^T
@@ -649,7 +649,17 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
   const uint32_t cols = args.rows * gh;
   const uint32_t blocks = (cols + 32 * W - 1) / (32 * W);
   const uint32_t kvh = blockIdx.x % KVH, bs = blockIdx.x / KVH;
-  const uint32_t S = args.splits, split = bs % S, rb = blocks - 1 - bs / S;
+  uint32_t split = bs % args.splits, rb = blocks - 1 - bs / args.splits;
+  if (args.split_tiles) {
+    uint32_t first = 0;
+    split = 0;
+#pragma unroll
+    for (int s = 1; s < kMaxBlockSplits; ++s)
+      if (bs >= args.split_begin[s]) split = s, first = args.split_begin[s];
+    rb = blocks - 1 - (bs - first);
+  }
+  split = __builtin_amdgcn_readfirstlane(split);
+  rb = __builtin_amdgcn_readfirstlane(rb);
   const uint32_t c0 = rb * 32 * W + wave * 32;
   // Columns past the last one repeat it and are not stored.
   const uint32_t c = min(c0 + lc, cols - 1);
@@ -657,8 +667,10 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
   const uint32_t row = c / gh, head = kvh * gh + (c - row * gh);
   const uint32_t visible = min(args.start + row + 1, sq.len);
 
-  const uint32_t last_row = (min(cols, (rb + 1) * 32 * W) - 1) / gh;
-  const uint32_t n_tiles = (min(args.start + last_row + 1, sq.len) + 31) / 32;
+  // A block of one split needs no partials; with gates it leaves them all the same, as the
+  // merge applies those with the whole chip.
+  const uint32_t n_tiles = prefill_tiles(rb, 32 * W, cols, gh, args.start, sq.len);
+  const uint32_t S = prefill_block_splits(n_tiles, args.split_tiles, args.splits);
   const uint32_t t0 = (uint32_t)((uint64_t)n_tiles * split / S), t1 = (uint32_t)((uint64_t)n_tiles * (split + 1) / S);
   const uint32_t last_page = (sq.len - 1) / 16;
 
@@ -1014,10 +1026,10 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
   const float l_tot = l_lane + __shfl_xor(l_lane, 32);
   const float unit = t0 < t1 ? *(const float*)(table(t1 - 1) + L::kMisc + 28) : 1.0f;
   if (!col_ok) return;
-  if (S > 1) {
+  if (S > 1 || (args.split_tiles && args.gate)) {
     // Partials as in decode, row by row: O [row][split][H][D], then (m, l): here O over
     // its own sum, whose logarithm goes into m, so that it stays finite.
-    const size_t pr = ((size_t)row * S + split) * H + head;
+    const size_t pr = ((size_t)row * args.splits + split) * H + head;
     float* po = args.partials + pr * D;
     const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
 #pragma unroll
@@ -1067,8 +1079,24 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
 template <int D, int W>
 hipError_t launch_prefill(const AttnArgs& a, hipStream_t st) {
   const uint32_t cols = a.rows * (a.heads / a.kv_heads);
-  const uint32_t units = a.kv_heads * ((cols + 32 * W - 1) / (32 * W)) * a.splits;
-  hipLaunchKernelGGL((q4kv_prefill_kernel<D, W>), dim3(units), dim3(64 * W), 0, st, a);
+  const uint32_t blocks = (cols + 32 * W - 1) / (32 * W);
+  uint32_t units = blocks * a.splits;
+  Q4KvPrefillArgs args{};
+  (AttnArgs&)args = a;
+  if (a.split_tiles) {
+    // (A workgroup that only ends would not do: they are dealt to the shader engines in
+    // turn, and some of those would get few others.)
+    units = 0;
+    for (uint32_t s = 0, first = 0; s < (uint32_t)kMaxBlockSplits; ++s) {
+      while (first < blocks && s > 0 &&
+             prefill_block_splits(prefill_tiles(first, 32 * W, cols, a.heads / a.kv_heads, a.start, a.seqs[0].len),
+                                  a.split_tiles, a.splits) <= s)
+        ++first;
+      args.split_begin[s] = s < a.splits ? units : ~0u;
+      units += blocks - first;
+    }
+  }
+  hipLaunchKernelGGL((q4kv_prefill_kernel<D, W>), dim3(units * a.kv_heads), dim3(64 * W), 0, st, args);
   if (a.splits > 1) launch_attn_combine(combine_args(a), st);
   return hipGetLastError();
 }

@@ -578,6 +578,16 @@ __global__ __launch_bounds__(64 * W) void q8_decode_kernel(AttnArgs args) {
   decode_merge<D, W>(args, sq, b, kvh * gh, gh, split, lds, o, m_run, l_lane);
 }
 
+// Splits of a (prefill row, head), or of a sequence.
+__device__ __forceinline__ uint32_t combine_splits(const AttnCombineArgs& a, uint32_t b, uint32_t hh) {
+  if (!a.prefill) return a.seqs[b].nsplit;
+  if (a.split_tiles == 0) return a.splits;
+  const uint32_t gh = a.heads / a.kv_heads;
+  const uint32_t tiles =
+      prefill_tiles((b * gh + hh % gh) / a.block_cols, a.block_cols, a.rows * gh, gh, a.start, a.len);
+  return prefill_block_splits(tiles, a.split_tiles, a.splits);
+}
+
 // Merge the split partials of one (sequence, head, 32-wide d slice): grid
 // (n_seqs * H * D/32), 256 threads.  Thread t owns float4 slice c = t % 8 of
 // the workgroup's 32 d and the splits s = t / 8 + 32 k, and loads every
@@ -597,9 +607,9 @@ __global__ __launch_bounds__(256) void q8_combine_kernel(AttnCombineArgs args) {
   const uint32_t bh = blockIdx.x / kWgPerHead;
   const uint32_t b = bh / H, hh = bh % H;
   // b is a sequence (decode) or a query row (prefill: the same splits for all).
-  const uint32_t ns = args.prefill ? args.splits : args.seqs[b].nsplit;
-  if (ns <= 1 || 32 * wq >= dr) return;
-  const size_t part_begin = args.prefill ? (size_t)b * ns : args.seqs[b].part_begin;
+  const uint32_t ns = combine_splits(args, b, hh);
+  if ((ns <= 1 && !(args.split_tiles && args.gate)) || 32 * wq >= dr) return;
+  const size_t part_begin = args.prefill ? (size_t)b * args.splits : args.seqs[b].part_begin;
   const size_t o_rows = (size_t)args.part_rows * H;
   const float* obase = args.partials + (part_begin * H + hh) * D;
   const float* mbase = args.partials + o_rows * D + (part_begin * H + hh) * 2;
@@ -681,9 +691,9 @@ __global__ __launch_bounds__(64) void q8_combine_small_kernel(AttnCombineArgs ar
   const uint32_t bh = blockIdx.x / kWgPerHead;
   const uint32_t b = bh / H, hh = bh % H;
   // b is a sequence (decode) or a query row (prefill: the same splits for all).
-  const uint32_t ns = args.prefill ? args.splits : args.seqs[b].nsplit;
-  if (ns <= 1 || 32 * wq >= dr) return;
-  const size_t part_begin = args.prefill ? (size_t)b * ns : args.seqs[b].part_begin;
+  const uint32_t ns = combine_splits(args, b, hh);
+  if ((ns <= 1 && !(args.split_tiles && args.gate)) || 32 * wq >= dr) return;
+  const size_t part_begin = args.prefill ? (size_t)b * args.splits : args.seqs[b].part_begin;
   const size_t o_rows = (size_t)args.part_rows * H;
   const float* obase = args.partials + (part_begin * H + hh) * D;
   const float* mbase = args.partials + o_rows * D + (part_begin * H + hh) * 2;
@@ -1108,18 +1118,20 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q8_prefill_k
 constexpr int kRowSplits = 8;
 template <int D>
 __global__ __launch_bounds__(256) void q8_combine_rows_kernel(AttnCombineArgs args) {
-  const uint32_t H = args.heads, dr = args.head_dim, ns = args.splits;
+  const uint32_t H = args.heads, dr = args.head_dim;
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
   const size_t pair = i / (D / 4);
   const uint32_t d0 = 4 * (uint32_t)(i % (D / 4));
   if (pair >= (size_t)args.rows * H || d0 >= dr) return;
   const size_t row = pair / H, hh = pair % H;
+  const uint32_t ns = combine_splits(args, (uint32_t)row, (uint32_t)hh);
+  if (ns <= 1 && !args.gate) return;
   floatx4 ov[kRowSplits];
   float2 ml[kRowSplits];
 #pragma unroll
   for (int s = 0; s < kRowSplits; ++s) {
     if ((uint32_t)s >= ns) break;
-    const size_t pr = (row * ns + s) * H + hh;
+    const size_t pr = (row * args.splits + s) * H + hh;
     ov[s] = *(const floatx4*)(args.partials + pr * D + d0);
     ml[s] = *(const float2*)(args.partials + (size_t)args.part_rows * H * D + pr * 2);
   }

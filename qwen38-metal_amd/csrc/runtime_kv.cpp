@@ -336,7 +336,7 @@ Q4KvArgs q4kv_args(const DecodeChunk& c) {
 // many; otherwise as many as run in one residency round, each with at least
 // four tiles, and none below 16 tiles, where the merge costs more than the
 // walk (512 rows of an empty cache: 37 us in two splits, 35 in one).
-void plan_prefill(const qm_runtime* rt, AttnArgs* at) {
+void plan_prefill(const qm_runtime* rt, bool q4, AttnArgs* at) {
   const uint32_t D = at->head_dim_pad;
   const uint64_t tiles = ((uint64_t)at->seqs[0].len + 31) / 32, cus = rt->cu_count;
   const uint64_t cols = (uint64_t)at->rows * (at->heads / at->kv_heads);
@@ -350,6 +350,30 @@ void plan_prefill(const qm_runtime* rt, AttnArgs* at) {
   const uint64_t u = units(at->wg_waves);
   const uint64_t room = cus * attn_prefill_waves(D, at->wg_waves) * 4 / at->wg_waves;
   at->splits = tiles <= 16 || 2 * u > room ? 1 : (uint32_t)std::max<uint64_t>(1, std::min(room / u, tiles / 4));
+  if (!q4) return;
+  // Over 4-bit caches: where a prompt's blocks see very different numbers of tiles, each
+  // has workgroups for its own, of at least four tiles, as many as run in one round (24 / 4
+  // heads of 256 on an empty cache: 512 rows 68 -> 46 us, 1000 rows 82 -> 67, 1500 rows
+  // 162 -> 103; 64 / 8 of 128, 1000 rows, whose blocks nearly fill a round: not split,
+  // 63 against 70).
+  const uint32_t gh = at->heads / at->kv_heads, block = 32 * at->wg_waves, blocks = (uint32_t)(u / at->kv_heads);
+  auto tiles_of = [&](uint32_t b) { return prefill_tiles(b, block, (uint32_t)cols, gh, at->start, at->seqs[0].len); };
+  const uint32_t longest = tiles_of(blocks - 1);
+  if (u > room || longest < 8 || 2 * tiles_of(0) > longest) return;
+  auto fits = [&](uint32_t t) {
+    uint64_t n = 0;
+    for (uint32_t b = 0; b < blocks; ++b) n += (tiles_of(b) + t - 1) / t;
+    return n * at->kv_heads <= room;
+  };
+  uint32_t lo = std::max<uint32_t>(4, (longest + kMaxBlockSplits - 1) / kMaxBlockSplits), hi = std::max(lo, longest);
+  while (lo < hi) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (fits(mid)) hi = mid;
+    else lo = mid + 1;
+  }
+  if (4 * hi > 3 * longest) return;
+  at->splits = (longest + hi - 1) / hi;
+  at->split_tiles = hi;
 }
 
 // Partials of any split prefill with this head storage: its workgroups fit one
@@ -614,11 +638,13 @@ qm_status prefill(qm_runtime* rt, qm_kv* seq, const uint16_t* q, const uint16_t*
     c.at.part_rows = c.parts;
     c.at.partials = (float*)rt->partials;
   }
-  if (!few) plan_prefill(rt, &at);
+  if (!few) plan_prefill(rt, seq->bits == 4, &at);
   if (at.splits > 1) {
     at.part_rows = M * at.splits;
     const size_t bytes = (size_t)at.part_rows * H * (seq->dp + 2) * sizeof(float);
-    if (try_partials(rt, std::max(bytes, prefill_partial_bytes(rt, seq->dp))) || try_partials(rt, bytes))
+    // (By blocks, rows of few splits leave gaps: up to twice as much.)
+    const size_t usual = prefill_partial_bytes(rt, seq->dp) * (seq->bits == 4 ? 2 : 1);
+    if (try_partials(rt, std::max(bytes, usual)) || try_partials(rt, bytes))
       at.partials = (float*)rt->partials;
     else
       at.splits = 1;

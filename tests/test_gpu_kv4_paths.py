@@ -52,6 +52,19 @@ def test_prefill_of_many_rows(rt, shape, rows, cached):
     cache.close()
 
 
+@pytest.mark.parametrize("rows,cached", [(513, 0), (700, 13), (1101, 0)])
+@pytest.mark.parametrize("shape", [(64, 8, 128), (20, 5, 80), (24, 4, 256), (32, 8, 64), (16, 1, 128), (6, 2, 37)])
+def test_prompts_split_by_blocks(rt, shape, rows, cached):
+    """Blocks of columns with different numbers of workgroups, gated (odd rows) and not."""
+    test_prefill_of_many_rows(rt, shape, rows, cached)
+
+
+@pytest.mark.parametrize("rows", [2100, 2101])
+@pytest.mark.parametrize("shape", [(2, 1, 64), (3, 1, 256)])
+def test_prompts_in_many_splits(rt, shape, rows):
+    test_prefill_of_many_rows(rt, shape, rows, 0)
+
+
 @pytest.mark.parametrize("shape", [(8, 2, 64), (8, 2, 128), (12, 2, 256), (40, 2, 256)])
 @pytest.mark.parametrize("kind", [0, 1])
 def test_nan_reaches_many_rows(rt, kind, shape):
