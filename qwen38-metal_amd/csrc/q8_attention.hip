@@ -578,10 +578,11 @@ __global__ __launch_bounds__(64 * W) void q8_decode_kernel(AttnArgs args) {
   decode_merge<D, W>(args, sq, b, kvh * gh, gh, split, lds, o, m_run, l_lane);
 }
 
-// Splits of a (prefill row, head), or of a sequence.
+// Splits of a (prefill row, head), or of a sequence.  BLOCKS: a prefill's blocks of columns
+// have numbers of their own (split_tiles).
+template <bool BLOCKS>
 __device__ __forceinline__ uint32_t combine_splits(const AttnCombineArgs& a, uint32_t b, uint32_t hh) {
-  if (!a.prefill) return a.seqs[b].nsplit;
-  if (a.split_tiles == 0) return a.splits;
+  if (!BLOCKS) return a.prefill ? a.splits : a.seqs[b].nsplit;
   const uint32_t gh = a.heads / a.kv_heads;
   const uint32_t tiles =
       prefill_tiles((b * gh + hh % gh) / a.block_cols, a.block_cols, a.rows * gh, gh, a.start, a.len);
@@ -607,8 +608,8 @@ __global__ __launch_bounds__(256) void q8_combine_kernel(AttnCombineArgs args) {
   const uint32_t bh = blockIdx.x / kWgPerHead;
   const uint32_t b = bh / H, hh = bh % H;
   // b is a sequence (decode) or a query row (prefill: the same splits for all).
-  const uint32_t ns = combine_splits(args, b, hh);
-  if ((ns <= 1 && !(args.split_tiles && args.gate)) || 32 * wq >= dr) return;
+  const uint32_t ns = combine_splits<false>(args, b, hh);
+  if (ns <= 1 || 32 * wq >= dr) return;
   const size_t part_begin = args.prefill ? (size_t)b * args.splits : args.seqs[b].part_begin;
   const size_t o_rows = (size_t)args.part_rows * H;
   const float* obase = args.partials + (part_begin * H + hh) * D;
@@ -682,7 +683,7 @@ __global__ __launch_bounds__(256) void q8_combine_kernel(AttnCombineArgs args) {
 // float4 slice c and splits g, g + 8, g + 16, g + 24, all loaded at once;
 // the maximum and the sums over g meet through lane swaps (xor 8, 16, 32),
 // so the merge needs no LDS and no barrier.
-template <int D>
+template <int D, bool BLOCKS>
 __global__ __launch_bounds__(64) void q8_combine_small_kernel(AttnCombineArgs args) {
   constexpr int kWgPerHead = D / 32;
   constexpr int kPer = 4;  // splits per lane
@@ -691,8 +692,8 @@ __global__ __launch_bounds__(64) void q8_combine_small_kernel(AttnCombineArgs ar
   const uint32_t bh = blockIdx.x / kWgPerHead;
   const uint32_t b = bh / H, hh = bh % H;
   // b is a sequence (decode) or a query row (prefill: the same splits for all).
-  const uint32_t ns = combine_splits(args, b, hh);
-  if ((ns <= 1 && !(args.split_tiles && args.gate)) || 32 * wq >= dr) return;
+  const uint32_t ns = combine_splits<BLOCKS>(args, b, hh);
+  if ((ns <= 1 && !(BLOCKS && args.gate)) || 32 * wq >= dr) return;
   const size_t part_begin = args.prefill ? (size_t)b * args.splits : args.seqs[b].part_begin;
   const size_t o_rows = (size_t)args.part_rows * H;
   const float* obase = args.partials + (part_begin * H + hh) * D;
@@ -1116,7 +1117,7 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q8_prefill_k
 // (A workgroup per (row, head, 32 d), as above, is 192000 of them for 1000
 // rows of 24 heads of 256: the dispatch alone took longer than the product.)
 constexpr int kRowSplits = 8;
-template <int D>
+template <int D, bool BLOCKS>
 __global__ __launch_bounds__(256) void q8_combine_rows_kernel(AttnCombineArgs args) {
   const uint32_t H = args.heads, dr = args.head_dim;
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
@@ -1124,8 +1125,8 @@ __global__ __launch_bounds__(256) void q8_combine_rows_kernel(AttnCombineArgs ar
   const uint32_t d0 = 4 * (uint32_t)(i % (D / 4));
   if (pair >= (size_t)args.rows * H || d0 >= dr) return;
   const size_t row = pair / H, hh = pair % H;
-  const uint32_t ns = combine_splits(args, (uint32_t)row, (uint32_t)hh);
-  if (ns <= 1 && !args.gate) return;
+  const uint32_t ns = combine_splits<BLOCKS>(args, (uint32_t)row, (uint32_t)hh);
+  if (BLOCKS && ns <= 1 && !args.gate) return;
   floatx4 ov[kRowSplits];
   float2 ml[kRowSplits];
 #pragma unroll
@@ -1161,16 +1162,20 @@ __global__ __launch_bounds__(256) void q8_combine_rows_kernel(AttnCombineArgs ar
   }
 }
 
-template <int D>
-void launch_combine(const AttnCombineArgs& a, uint32_t max_split, hipStream_t st) {
+template <int D, bool BLOCKS>
+void launch_combine_as(const AttnCombineArgs& a, uint32_t max_split, hipStream_t st) {
   if (a.prefill && max_split <= (uint32_t)kRowSplits) {
     const size_t items = (size_t)a.rows * a.heads * (D / 4);
-    hipLaunchKernelGGL(q8_combine_rows_kernel<D>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((q8_combine_rows_kernel<D, BLOCKS>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, a);
   } else if (max_split <= 32) {
-    hipLaunchKernelGGL(q8_combine_small_kernel<D>, dim3(a.rows * a.heads * (D / 32)), dim3(64), 0, st, a);
-  } else {
+    hipLaunchKernelGGL((q8_combine_small_kernel<D, BLOCKS>), dim3(a.rows * a.heads * (D / 32)), dim3(64), 0, st, a);
+  } else {  // (blocks have at most kMaxBlockSplits)
     hipLaunchKernelGGL(q8_combine_kernel<D>, dim3(a.rows * a.heads * (D / 32)), dim3(256), 0, st, a);
   }
+}
+template <int D>
+void launch_combine(const AttnCombineArgs& a, uint32_t max_split, hipStream_t st) {
+  a.split_tiles ? launch_combine_as<D, true>(a, max_split, st) : launch_combine_as<D, false>(a, max_split, st);
 }
 
 template <int D, int W>
