@@ -547,8 +547,8 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void q4kv_decod
   merge_columns<D, W>(args, sq, b, head0, n_heads, split, lds, o, m_run, l_lane);
 }
 
-// Causal prefill on 32x32x16 MFMA; columns, tiles, splits and the two LDS stages as in
-// the 8-bit kernel.  A tile's 32 tokens are unpacked once per workgroup:
+// Causal prefill on 32x32x16 MFMA; columns and tiles as in the 8-bit kernel, splits too
+// or by block (Q4KvPrefillArgs).  A tile's 32 tokens are unpacked once per workgroup:
 //   K as its codes in bf16 (16 c, exact), so a group's product is exact and its scale
 //     and offset act on the scores: x = sum_g s_g (K_g Q_g) + m_g (sum of Q_g).  The
 //     second part and the running reference come from one more matrix instruction,
@@ -568,7 +568,8 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void q4kv_decod
 // product reaches 1230), matrix instructions busy for 32 % of the cycles, vector ones
 // for 44 %, half of those for the unpacking and the softmax's exponentials.  The same
 // without scores a tile ahead took 618 us, with a tile's tables and V on the last waves
-// alone 564.  1000 rows of 24 / 4 heads of 256: 69 us.
+// alone 564.  1000 rows of 24 / 4 heads of 256: 52 us (69 with the same number of
+// workgroups for every block of columns).
 template <int D, int W>
 struct PrefillLds {
   static constexpr int G = D / 64;
