@@ -241,11 +241,23 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void q4kv_decod
   // (j % 2) .. + 7.
   constexpr int kMine = kTight ? 2 * G / W : 2 * G;
   u32x4 qx[kMine];
+  auto piece_of = [&](int i) { return kTight ? wave + W * i : i; };
+  if (dr % 8 == 0) {
+    // One buffer for the sequence's queries: what is not there reads as zero, with no
+    // branch whose end would wait for the loads.
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(args.q + (size_t)b * H * dr, H * dr * 2);
 #pragma unroll
-  for (int i = 0; i < kMine; ++i) {
-    const int j = kTight ? wave + W * i : i;
-    qx[i] = col_ok ? load_q8(args.q + ((size_t)b * H + head) * dr, 64 * (j / 2) + 16 * kq + 8 * (j % 2), dr)
-                   : u32x4{0u, 0u, 0u, 0u};
+    for (int i = 0; i < kMine; ++i) {
+      const uint32_t d0 = 64 * (piece_of(i) / 2) + 16 * kq + 8 * (piece_of(i) % 2);
+      const auto x = __builtin_amdgcn_raw_buffer_load_b128(r, col_ok && d0 < dr ? 2 * (head * dr + d0) : ~0u, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) qx[i][e] = x[e];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+      qx[i] = col_ok ? load_q8(args.q + ((size_t)b * H + head) * dr, 64 * (piece_of(i) / 2) + 16 * kq + 8 * (piece_of(i) % 2), dr)
+                     : u32x4{0u, 0u, 0u, 0u};
   }
   const uint32_t s_at = q4kv_scale_bytes(D) + 4 * q4kv_scale_word(D, 0, 0, 4 * kq + (lane & 3));
   // Pages j (even) and j + 1.  Codes of a page past the wave's last read nothing: a
