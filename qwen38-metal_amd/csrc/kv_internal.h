@@ -40,5 +40,9 @@ void plan_pages(const qm_kv* kv, uint32_t start, uint32_t end, int32_t* first_ne
 // Records a planned append in the host table, and takes it back.
 void commit_pages(qm_kv* kv, int32_t first_new, int32_t count);
 void rollback_pages(qm_kv* kv, int32_t first_new, int32_t count);
+// Fills in a prefill's waves, splits and split_tiles (q4: over a 4-bit cache), and takes
+// the splits back where there is no room for their partials.
+void plan_prefill(const qm_runtime* rt, bool q4, AttnArgs* at);
+void unsplit_prefill(AttnArgs* at);
 
 }  // namespace qm

@@ -1132,7 +1132,8 @@ hipError_t launch_decode_d(const Q4KvArgs& a, uint32_t units, bool need_combine,
 }  // namespace
 
 hipError_t launch_q4kv_prefill(const AttnArgs& a, hipStream_t st) {
-  if (a.splits == 0 || (a.splits > 1 && !a.partials)) return hipErrorInvalidValue;
+  // (Blocks of one split leave partials too where there is a gate.)
+  if (a.splits == 0 || ((a.splits > 1 || a.split_tiles) && !a.partials)) return hipErrorInvalidValue;
   switch (a.head_dim_pad) {
     case 64: return launch_prefill_d<64>(a, st);
     case 128: return launch_prefill_d<128>(a, st);

@@ -320,6 +320,8 @@ Q4KvArgs q4kv_args(const DecodeChunk& c) {
   return a;
 }
 
+}  // namespace
+
 // The prefill kernel's launch shape: waves per workgroup (32 columns each; a
 // column is a query head of a row) and the workgroups that share the tiles (32
 // tokens) of a column block.
@@ -336,7 +338,7 @@ Q4KvArgs q4kv_args(const DecodeChunk& c) {
 // many; otherwise as many as run in one residency round, each with at least
 // four tiles, and none below 16 tiles, where the merge costs more than the
 // walk (512 rows of an empty cache: 37 us in two splits, 35 in one).
-void plan_prefill(const qm_runtime* rt, bool q4, AttnArgs* at) {
+void qm::plan_prefill(const qm_runtime* rt, bool q4, AttnArgs* at) {
   const uint32_t D = at->head_dim_pad;
   const uint64_t tiles = ((uint64_t)at->seqs[0].len + 31) / 32, cus = rt->cu_count;
   const uint64_t cols = (uint64_t)at->rows * (at->heads / at->kv_heads);
@@ -375,6 +377,13 @@ void plan_prefill(const qm_runtime* rt, bool q4, AttnArgs* at) {
   at->splits = (longest + hi - 1) / hi;
   at->split_tiles = hi;
 }
+
+void qm::unsplit_prefill(AttnArgs* at) {
+  at->splits = 1;
+  at->split_tiles = 0;
+}
+
+namespace {
 
 // Partials of any split prefill with this head storage: its workgroups fit one
 // residency round, so their columns are bounded whatever the rows and the
@@ -647,7 +656,7 @@ qm_status prefill(qm_runtime* rt, qm_kv* seq, const uint16_t* q, const uint16_t*
     if (try_partials(rt, std::max(bytes, usual)) || try_partials(rt, bytes))
       at.partials = (float*)rt->partials;
     else
-      at.splits = 1;
+      unsplit_prefill(&at);
   }
   // A cache owned by another runtime: its pending work comes first.
   if ((st = stream_after(rt, seq->rt)) != QM_OK) return st;
