@@ -282,10 +282,13 @@ qm_status qm_kv_read(const qm_kv* kv, int8_t* keys, int8_t* values,
  * that takes a qm_kv takes either kind, and so does a decode layer; one call takes
  * caches of one kind.
  *
- * Attention over these caches takes weights and values in 16 bits at least, sums in
- * fp32.  A prefill of many rows has its values in fp16 under a power of two for every 32
- * tokens: what lies more than 2^24 below the largest of the 32, or 2^80 apart from the
- * first tokens' size, may be lost beside it. */
+ * Attention over these caches has its sums in fp32.  A decode step takes weights to 17
+ * bits and values as the codes give them.  A prefill may take both in fp16, rounded
+ * once each to 11 bits; then a weight more than 2^35 below its row's largest may count
+ * in the sum of weights alone.  (One of few rows goes as a decode step where that is
+ * faster and its workspace is there.)  Values may have any size, but where the largest of
+ * the groups of tokens are more than 2^7 above or 2^14 below those of the first tokens,
+ * a prefill of many rows is some ten times slower. */
 qm_status qm_kv_create_q4(qm_runtime* rt, uint32_t kv_heads, uint32_t head_dim,
                           uint32_t page_tokens, uint32_t max_tokens, qm_kv** out);
 uint32_t qm_kv_bits(const qm_kv* kv); /* 8 or 4; 0 for NULL */

@@ -566,13 +566,13 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void q4kv_decod
 //     second part and the running reference come from one more matrix instruction,
 //     whose K dimension holds m_g against three bf16 terms of the sums, and ones
 //     against three of minus the reference.
-//   V as values in fp16 under a power of two of its tile, 2^-E: the weight of P V is
-//     w = p 2^(E - R) in fp16, one product instead of the two of a split P' (V and w
-//     round by 2^-11 at most each).  O is in units of 2^R, R the first tile's E until one
-//     is over 2^64 above it; E - R is part of the exponent, by the same bias product.  A
-//     column's reference keeps its w between 2^-24 and 2^15.5: what is lost is below
-//     2^-36 of the largest w.  Values of a token more than 2^24 below the largest of its
-//     32 lose bits, as do those of tiles more than 2^80 below an earlier one.
+//   V as values in fp16 in units of 2^R, where the largest of the first tile are 2^6 .. 2^7.
+//     The weight of P V is p in fp16 with a reference that keeps it between 2^-24 and
+//     2^15.5: one product instead of the two of a split P' (V and p round by 2^-11 at most
+//     each), and what is lost is weights below 2^-36 of the row's largest.
+//   That holds while the sizes of all tokens' groups (8 s or |m|: no value passes twice that)
+//     lie between 2^-8 and 2^14 of the unit: above, fp16 ends; below, its steps of 2^-24 begin
+//     to count.  A workgroup that meets another size starts again (prefill_far).
 // The tables of a tile (scales, offsets, powers) are formed a tile ahead of its
 // unpacking by two waves.
 //
@@ -582,6 +582,9 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void q4kv_decod
 // without scores a tile ahead took 618 us, with a tile's tables and V on the last waves
 // alone 564.  1000 rows of 24 / 4 heads of 256: 52 us (69 with the same number of
 // workgroups for every block of columns).
+constexpr uint32_t kHasNan = 1, kHasWide = 2;
+// Sizes below it (values of the least scale) count as none.
+constexpr float kNoSize = 0x1p-121f;
 template <int D, int W>
 struct PrefillLds {
   static constexpr int G = D / 64;
@@ -592,9 +595,9 @@ struct PrefillLds {
   static constexpr int kNK = 2, kNV = kTight ? 2 : 3, kNTabs = 3;
   static constexpr int kK = 32 * D * 2, kV = 32 * D * 2;
   // A tile's tables: K scales [G][32], K offsets as matrix operand [2][32] of 16 bytes,
-  // V scales and offsets in fp16 [G][8 token quads] of 16 bytes, then 2^(R before - R),
-  // whether a value is NaN, such tokens, a word per group, 2^(R - E) and 2^R.
-  static constexpr int kKb = G * 128, kVs = kKb + 1024, kMisc = kVs + G * 128, kTab = kMisc + 32;
+  // V scales and offsets in fp16 [G][8 token quads] of 16 bytes, then 2^R, what the tile has
+  // of kHas.., and a word per group: tokens whose values are NaN.
+  static constexpr int kKb = G * 128, kVs = kKb + 1024, kMisc = kVs + G * 128, kNan = kMisc + 16, kTab = kMisc + 32;
   static constexpr int kVAt = kNK * kK, kTabs = kVAt + kNV * kV;
   static constexpr int kIds = kTabs + kNTabs * kTab;
   static constexpr int kQ = kIds + 512, kQSteps = kTight ? D / 32 : 0;
@@ -642,26 +645,22 @@ __device__ __forceinline__ u32x4 k_codes16(uint32_t w) {
                pack_bf16x2(f(hi, 1), f(hi, 3))};
 }
 
-template <int D, int W>
-__global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill_kernel(Q4KvPrefillArgs args) {
-  using L = PrefillLds<D, W>;
-  constexpr int G = D / 64;
-  constexpr int kDB = D / 32;  // 32-wide d blocks of O^T
-  constexpr int kKS = D / 16;  // QK k-steps
-  constexpr int kWords = 4 * D >= 64 * W ? 4 * D / (64 * W) : 1;  // words of a tile's K, and of its V, per thread
-  constexpr float kMost = 15.5f;  // exponents above it move the reference
-  __shared__ __attribute__((aligned(16))) uint8_t lds[L::kBytes];
-
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lc = lane & 31, hf = lane >> 5;
-  const uint32_t H = args.heads, KVH = args.kv_heads, gh = H / KVH;  // gh <= 16
-  const AttnSeq& sq = args.seqs[0];
-
+// What a wave of the prompts' kernel does: tiles t0 .. t1 - 1 for columns c0 .. c0 + 31, of
+// which a lane has column c, a query head of a row.
+struct PrefillPlace {
+  uint32_t kvh, split, splits, t0, t1, c0, cols, c, row, head, visible;
+  bool col_ok;
+};
+template <int W>
+__device__ __forceinline__ PrefillPlace prefill_place(const Q4KvPrefillArgs& args, uint32_t workgroup, uint32_t wave,
+                                                      uint32_t lane) {
+  const uint32_t lc = lane & 31;
+  const uint32_t KVH = args.kv_heads, gh = args.heads / KVH, len = args.seqs[0].len;  // gh <= 16
+  PrefillPlace p;
   // Workgroups as in the 8-bit kernel: a KV head's on the same XCDs, the longest first.
-  const uint32_t cols = args.rows * gh;
-  const uint32_t blocks = (cols + 32 * W - 1) / (32 * W);
-  const uint32_t kvh = blockIdx.x % KVH, bs = blockIdx.x / KVH;
+  p.cols = args.rows * gh;
+  const uint32_t blocks = (p.cols + 32 * W - 1) / (32 * W);
+  const uint32_t bs = workgroup / KVH;
   uint32_t split = bs % args.splits, rb = blocks - 1 - bs / args.splits;
   if (args.split_tiles) {
     uint32_t first = 0;
@@ -671,20 +670,223 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
       if (bs >= args.split_begin[s]) split = s, first = args.split_begin[s];
     rb = blocks - 1 - (bs - first);
   }
-  split = __builtin_amdgcn_readfirstlane(split);
+  p.kvh = workgroup % KVH;
+  p.split = __builtin_amdgcn_readfirstlane(split);
   rb = __builtin_amdgcn_readfirstlane(rb);
-  const uint32_t c0 = rb * 32 * W + wave * 32;
+  p.c0 = rb * 32 * W + wave * 32;
   // Columns past the last one repeat it and are not stored.
-  const uint32_t c = min(c0 + lc, cols - 1);
-  const bool col_ok = c0 + lc < cols;
-  const uint32_t row = c / gh, head = kvh * gh + (c - row * gh);
-  const uint32_t visible = min(args.start + row + 1, sq.len);
+  p.c = min(p.c0 + lc, p.cols - 1);
+  p.col_ok = p.c0 + lc < p.cols;
+  p.row = p.c / gh, p.head = p.kvh * gh + (p.c - p.row * gh);
+  p.visible = min(args.start + p.row + 1, len);
+  const uint32_t tiles = prefill_tiles(rb, 32 * W, p.cols, gh, args.start, len);
+  p.splits = prefill_block_splits(tiles, args.split_tiles, args.splits);
+  p.t0 = (uint32_t)((uint64_t)tiles * p.split / p.splits), p.t1 = (uint32_t)((uint64_t)tiles * (p.split + 1) / p.splits);
+  return p;
+}
+// Whether a block leaves partials.  One split needs none; with gates, blocks that have
+// workgroups of their own leave them all the same, as the merge applies those with the
+// whole chip.
+__device__ __forceinline__ bool leaves_partials(const Q4KvPrefillArgs& args, const PrefillPlace& p) {
+  return p.splits > 1 || (args.split_tiles && args.gate);
+}
 
-  // A block of one split needs no partials; with gates it leaves them all the same, as the
-  // merge applies those with the whole chip.
-  const uint32_t n_tiles = prefill_tiles(rb, 32 * W, cols, gh, args.start, sq.len);
-  const uint32_t S = prefill_block_splits(n_tiles, args.split_tiles, args.splits);
-  const uint32_t t0 = (uint32_t)((uint64_t)n_tiles * split / S), t1 = (uint32_t)((uint64_t)n_tiles * (split + 1) / S);
+// A wave's columns where sizes are far apart, a group of 64 dimensions at a time: no LDS,
+// few registers, K, V and Q straight from memory (2048 rows on 4096 tokens of 64 / 8
+// heads of 128: 4.6 ms against 0.46; 333 rows of 20 / 5 heads of 80: 65 us against 18).  The
+// other form's loop with groups and bands of its own was faster here, but the compiler then
+// spilled in both (0.51 to 0.71 ms for ordinary values).  The values of a token are in units of their own power of two, 2^e, O
+// in those of the group's largest so far, 2^R, and the weights are p 2^(e - R), taken to the
+// products in bands of 2^24 with a power of two for every column that makes a band's
+// largest 2^11 .. 2^12.  Nothing but parts below 2^-96 of the group's largest value is lost.
+template <int D, int W>
+__device__ __forceinline__ void prefill_far(const Q4KvPrefillArgs& args, uint32_t wave) {
+  constexpr int G = D / 64;
+  // (Formed anew: what both forms need would be held in registers over the other's loop.)
+  uint32_t workgroup = blockIdx.x, none = 0;
+  asm volatile("" : "+s"(workgroup), "+s"(wave), "+s"(none));
+  int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none));
+  const PrefillPlace p = prefill_place<W>(args, workgroup, wave, lane);
+  if (p.c0 >= p.cols) return;
+  int lc = lane & 31, hf = lane >> 5;
+  const AttnSeq& sq = args.seqs[0];
+  const uint32_t H = args.heads, KVH = args.kv_heads, dr = args.head_dim, last_page = (sq.len - 1) / 16;
+  const float sm_scale = kLog2e / sqrtf((float)dr);
+  const uint16_t* qp = args.q + ((size_t)p.row * H + p.head) * dr;
+  auto token_of = [&](int e) __attribute__((always_inline)) { return 8 * (e >> 2) + 4 * hf + (e & 3); };
+  auto power = [](float size) { return max((int)(__float_as_uint(size) >> 23) - 140, -113); };  // (up to 114)
+#pragma unroll 1
+  for (uint32_t g = 0; g < G; ++g) {
+    floatx16 o[2] = {floatx16{}, floatx16{}};
+    float m_run = 0.0f, l_lane = 0.0f;
+    int r_exp = -113;
+#pragma unroll 1
+    for (uint32_t t = p.t0; t < p.t1; ++t) {
+      asm volatile("" : "+v"(lane));
+      lc = lane & 31, hf = lane >> 5;
+      const uint8_t* block[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        block[h] = (const uint8_t*)sq.k + ((size_t)sq.pt[min(2 * t + h, last_page)] * KVH + p.kvh) * q4kv_block_bytes(D);
+      const uint8_t* own = lc & 16 ? block[1] : block[0];  // the page of token 32 t + lc
+      const uint32_t* scales = (const uint32_t*)(own + q4kv_scale_bytes(D));
+      const uint32_t slot = lc & 15;
+      const bool there = 32 * t + lc < sq.len;
+      floatx16 x{};
+#pragma unroll 1
+      for (uint32_t i = 0; i < G; ++i) {
+        floatx16 sc{};
+        float qs = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t d0 = 64 * i + 16 * j + 8 * hf;
+          const u32x4 q = load_q8(qp, d0, dr);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qs += bf16_lo_f32(q[e]) + bf16_hi_f32(q[e]);
+          sc = mfma32x32x16(k_codes16(*(const uint32_t*)(own + q4kv_k_word(D, slot, d0))), q, sc);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        qs += __shfl_xor(qs, 32);
+        const uint32_t w = there ? scales[q4kv_scale_word(D, 0, i, slot)] : 0;
+        const float sk = bf16_lo_f32(w) * (sm_scale * 0.0625f), mk = bf16_hi_f32(w) * sm_scale;  // (codes are 16 c)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          x[e] = __builtin_fmaf(__shfl(sk, token_of(e)), sc[e], __builtin_fmaf(__shfl(mk, token_of(e)), qs, x[e]));
+          if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (32 * t + token_of(e) >= p.visible) x[e] = -INFINITY;
+        top = fmaxf(top, x[e]);
+      }
+      top = max2_across_halves(top);
+      if (top > -INFINITY && (t == p.t0 || top > m_run + 12.0f)) {
+        const float corr = t == p.t0 ? 0.0f : __builtin_amdgcn_exp2f(m_run - top);
+        m_run = top;
+        l_lane *= corr;
+        o[0] *= corr, o[1] *= corr;
+      }
+      // The values' sizes, as in the other form.
+      const uint32_t w = there ? scales[q4kv_scale_word(D, 1, g, slot)] : 0;
+      const float sv = bf16_lo_f32(w), mv = bf16_hi_f32(w), size = fmaxf(8.0f * sv, fabsf(mv));
+      const bool any = size >= kNoSize, bad = sv != sv;
+      const float row_top = row_allmax(any ? size : 0.0f);
+      const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(row_top), __float_as_uint(row_top), false, false);
+      const uint32_t most = __builtin_amdgcn_readfirstlane(max(sw[0], sw[1]));  // (not negative)
+      if (most != 0 && power(__uint_as_float(most)) > r_exp + 1) {
+        const float unit = __builtin_amdgcn_exp2f((float)(r_exp - power(__uint_as_float(most))));
+        r_exp = power(__uint_as_float(most));
+        o[0] *= unit, o[1] *= unit;
+      }
+      const int e_own = any ? power(size) : r_exp;
+      const float inv = __uint_as_float((uint32_t)(127 - e_own) << 23);
+      const uint32_t sm = bad ? 0u : pack_f16x2(sv * inv, mv * inv);
+      const float part = any ? (float)(e_own - r_exp) : -INFINITY;  // (a token without a size takes no part)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        l_lane += __builtin_amdgcn_exp2f(x[e] - m_run);
+        x[e] += __shfl(part, token_of(e)) - m_run;
+        if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+      // V^T operands: tokens 4 hf .. + 3 and 8 + 4 hf .. + 3 of either page.
+      u32x4 v[2][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          half2_t s_m[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s_m[r] = as_half2(__shfl(sm, 16 * h + 8 * n + 4 * hf + r));
+#pragma unroll
+          for (int db = 0; db < 2; ++db) {
+            const uint32_t d = 64 * g + 32 * db + lc;
+            const uint32_t codes = *(const uint32_t*)(block[h] + q4kv_v_bytes(D) + q4kv_v_word(D, 8 * n + 4 * hf, d));
+            float y[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              y[r] = __builtin_fmaf((float)((int)(codes >> q4kv_v_bit(r, d) & 15) - 8), (float)s_m[r][0], (float)s_m[r][1]);
+            v[h][db][2 * n] = pack_f16x2(y[0], y[1]), v[h][db][2 * n + 1] = pack_f16x2(y[2], y[3]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      float below = INFINITY;
+      for (;;) {
+        float high = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (x[e] < below) high = fmaxf(high, x[e]);
+        high = max2_across_halves(high);
+        if (!__builtin_amdgcn_ballot_w64(high > -110.0f)) break;
+        const float low = high - 24.0f, unit = fmaxf(ceilf(high - 12.0f), -122.0f), back = __builtin_amdgcn_exp2f(unit);
+        floatx16 band[2] = {floatx16{}, floatx16{}};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            y[e] = x[8 * h + e] < below && x[8 * h + e] >= low ? __builtin_amdgcn_exp2f(x[8 * h + e] - unit) : 0.0f;
+          const u32x4 b = {pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3]), pack_f16x2(y[4], y[5]), pack_f16x2(y[6], y[7])};
+          band[0] = mfma32x32x16_f16(v[h][0], b, band[0]);
+          band[1] = mfma32x32x16_f16(v[h][1], b, band[1]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          o[0][e] = __builtin_fmaf(band[0][e], back, o[0][e]), o[1][e] = __builtin_fmaf(band[1][e], back, o[1][e]);
+        below = low;
+      }
+      // Values that are NaN: of the columns that see them.  (A NaN in a weight is in l.)
+      const uint32_t n = p.visible > 32 * t ? p.visible - 32 * t : 0, seen = n >= 32 ? ~0u : (1u << n) - 1;
+      if ((uint32_t)__builtin_amdgcn_ballot_w64(bad) & seen) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[0][e] = o[1][e] = NAN;
+      }
+    }
+    const float l_tot = l_lane + __shfl_xor(l_lane, 32);
+    const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot, unit = __uint_as_float((uint32_t)(127 + r_exp) << 23);
+    if (!p.col_ok) continue;
+    const bool partials = leaves_partials(args, p);
+    const size_t pr = ((size_t)p.row * args.splits + p.split) * H + p.head, at = ((size_t)p.row * H + p.head) * dr;
+#pragma unroll
+    for (int db = 0; db < 2; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t d = 64 * g + 32 * db + token_of(e);
+        float y = o[db][e] * inv * unit;
+        if (partials) {
+          args.partials[pr * D + d] = y;
+        } else if (d < dr) {
+          if (args.gate) y *= gate_sigmoid(bf16_to_f32(args.gate[at + d]));
+          args.o[at + d] = f32_to_bf16(y);
+        }
+      }
+    if (partials && g == 0 && hf == 0)
+      *(float2*)(args.partials + (size_t)args.part_rows * H * D + pr * 2) =
+          l_tot == 0.0f ? float2{-FLT_MAX, 0.0f} : float2{m_run + log2f(l_tot), 1.0f};
+  }
+}
+
+// A workgroup's tiles; false, and no output, where sizes are far apart.  (What is rare is
+// marked so: the compiler gives registers to the loops that it takes for frequent, and
+// those of prefill_far are nested.)
+template <int D, int W>
+__device__ __forceinline__ bool prefill_block(const Q4KvPrefillArgs& args, uint8_t* lds, const int wave) {
+  using L = PrefillLds<D, W>;
+  constexpr int G = D / 64;
+  constexpr int kDB = D / 32;  // 32-wide d blocks of O^T
+  constexpr int kKS = D / 16;  // QK k-steps
+  constexpr int kWords = 4 * D >= 64 * W ? 4 * D / (64 * W) : 1;  // words of a tile's K, and of its V, per thread
+  constexpr float kMost = 15.5f;  // exponents above it move the reference
+  constexpr int kNoUnit = 127;    // R where no tile has had a size
+  const int lane = threadIdx.x & 63;
+  const int lc = lane & 31, hf = lane >> 5;
+  const uint32_t H = args.heads, KVH = args.kv_heads, gh = H / KVH;
+  const AttnSeq& sq = args.seqs[0];
+  const PrefillPlace place = prefill_place<W>(args, blockIdx.x, wave, lane);
+  const uint32_t kvh = place.kvh, t0 = place.t0, t1 = place.t1, c0 = place.c0, cols = place.cols;
+  const uint32_t row = place.row, head = place.head, visible = place.visible;
   const uint32_t last_page = (sq.len - 1) / 16;
 
   const uint32_t dr = args.head_dim;
@@ -694,8 +896,7 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
   u32x4 qb[kQReg];
   u32x4* ql = (u32x4*)(lds + L::kQ + wave * L::kQSteps * 1024) + lane;
   // What the bias product multiplies: three terms of every group's sum of queries (half
-  // 0 holds slots 0..7, half 1 slots 8..15), of minus the reference in slots 12..14,
-  // and one.
+  // 0 holds slots 0..7, half 1 slots 8..15), and of minus the reference in slots 12..14.
   u32x4 qbias;
   {
     const uint16_t* qp = args.q + ((size_t)row * H + head) * dr;
@@ -713,7 +914,7 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
     for (int g = 0; g < 4; ++g) split3((qs[g] + __shfl_xor(qs[g], 32)) * sm_scale, t[g]);
     qbias = hf == 0 ? u32x4{t[0][0] | t[0][1] << 16, t[0][2] | t[1][0] << 16, t[1][1] | t[1][2] << 16,
                             t[2][0] | t[2][1] << 16}
-                    : u32x4{t[2][2] | t[3][0] << 16, t[3][1] | t[3][2] << 16, 0u, 0x3F800000u};
+                    : u32x4{t[2][2] | t[3][0] << 16, t[3][1] | t[3][2] << 16, 0u, 0u};
   }
 
   floatx16 o[kDB];
@@ -785,7 +986,7 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
     }
   };
   auto table = [&](uint32_t t) __attribute__((always_inline)) { return lds + L::kTabs + t % L::kNTabs * L::kTab; };
-  int r_exp = 0;  // R: exponent of the unit of O (wave 1's)
+  int r_exp = kNoUnit;  // R (wave 1's)
   auto write_table = [&](uint32_t t, Words r) __attribute__((always_inline)) {
     if (wave >= 2) return;
     uint8_t* tab = table(t);
@@ -802,46 +1003,45 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
       }
       *(u32x4*)(tab + L::kKb + 16 * lc) =
           u32x4{m[0] | m[0] << 16, m[0] | m[1] << 16, m[1] | m[1] << 16, m[2] | m[2] << 16};
-      // Slots 12..14: ones for the reference; 15: E - R, by wave 1.
-      *(u32x2*)(tab + L::kKb + 512 + 16 * lc) = u32x2{m[2] | m[3] << 16, m[3] | m[3] << 16};
-      *(uint32_t*)(tab + L::kKb + 520 + 16 * lc) = 0x3F803F80u;
+      // Slots 12..14: ones for the reference.
+      *(u32x4*)(tab + L::kKb + 512 + 16 * lc) = u32x4{m[2] | m[3] << 16, m[3] | m[3] << 16, 0x3F803F80u, 0x3F80u};
       return;
     }
-    // Size of the tile's values, NaN aside: 2^13 to 2^14 of the unit 2^E.
-    float sv[G], mv[G], size = 0.0f;
+    // Sizes of the tokens' values, NaN aside.
+    float most = 0.0f, least = INFINITY;
     bool nan = false;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      sv[g] = bf16_lo_f32(r.w[g]), mv[g] = bf16_hi_f32(r.w[g]);
-      size = fmaxf(size, fmaxf(8.0f * sv[g], fabsf(mv[g])));
-      nan |= sv[g] != sv[g];
+      const float sv = bf16_lo_f32(r.w[g]), size = fmaxf(8.0f * sv, fabsf(bf16_hi_f32(r.w[g])));
+      most = fmaxf(most, size);
+      least = fminf(least, size >= kNoSize ? size : INFINITY);
+      nan |= sv != sv;
     }
-    size = row_allmax(size);
-    const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(size), __float_as_uint(size), false, false);
-    const uint32_t top = __builtin_amdgcn_readfirstlane(max(sw[0], sw[1]));  // (not negative)
-    int e = max(min((int)(top >> 23), 253) - (127 + 13), -113);
-    const int before = r_exp;
-    if (t == t0 || e > r_exp + 64) r_exp = e;
-    e = max(e, r_exp - 80);
-    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-    *(uint32_t*)(tab + L::kKb + 524 + 16 * lc) = 0x3F80u | (__float_as_uint((float)(e - r_exp)) & 0xFFFF0000u);
+    if (r_exp == kNoUnit) {
+      const float x = row_allmax(most);
+      const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+      const uint32_t top = __builtin_amdgcn_readfirstlane(max(sw[0], sw[1]));
+      if (__uint_as_float(top) >= kNoSize) r_exp = max((int)(top >> 23) - (127 + 6), -126);
+    }
+    // (Before there is a unit, values of the least scale alone: zeros.)
+    const int e = r_exp == kNoUnit ? 0 : r_exp;
+    const float unit = __uint_as_float((uint32_t)(127 + e) << 23), inv = __uint_as_float((uint32_t)(127 - e) << 23);
+    uint32_t has = __builtin_amdgcn_ballot_w64(most >= unit * 0x1p14f || least < unit * 0x1p-8f) ? kHasWide : 0;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const bool bad = sv[g] != sv[g];
+      const float sv = bf16_lo_f32(r.w[g]);
+      const bool bad = sv != sv;
       _Float16* at = (_Float16*)(tab + L::kVs + 16 * (8 * g + (lc >> 2)) + 2 * (lc & 3));
-      at[0] = (_Float16)(bad ? 0.0f : sv[g] * inv);
-      at[4] = (_Float16)(bad ? 0.0f : mv[g] * inv);
+      at[0] = (_Float16)(bad ? 0.0f : sv * inv);
+      at[4] = (_Float16)(bad ? 0.0f : bf16_hi_f32(r.w[g]) * inv);
     }
-    const uint32_t any = (uint32_t)__builtin_amdgcn_ballot_w64(nan);
-    if (any) {
+    if (__builtin_amdgcn_ballot_w64(nan)) {
+      has |= kHasNan;
 #pragma unroll
       for (int g = 0; g < G; ++g)
-        *(uint32_t*)(tab + L::kMisc + 8 + 4 * g) = (uint32_t)__builtin_amdgcn_ballot_w64(sv[g] != sv[g]);
+        *(uint32_t*)(tab + L::kNan + 4 * g) = (uint32_t)__builtin_amdgcn_ballot_w64((r.w[g] & 0x7FFFu) > 0x7F80u);
     }
-    *(float2*)(tab + L::kMisc) =
-        float2{t == t0 ? 1.0f : __builtin_amdgcn_exp2f((float)(before - r_exp)), __uint_as_float(any)};
-    *(float2*)(tab + L::kMisc + 24) =
-        float2{__uint_as_float((uint32_t)(127 + r_exp - e) << 23), __uint_as_float((uint32_t)(127 + r_exp) << 23)};
+    *(float2*)(tab + L::kMisc) = float2{unit, __uint_as_float(has)};
   };
   // LDS images: K 16-byte chunk (8 d) q of token t at unit 32 q + (t ^ swz), V^T chunk
   // (page, half, d) at unit (2 page + half) D + (d ^ swz), where half 0 holds a page's
@@ -927,12 +1127,13 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
   };
 
   // Weights of tile t.  MASKED is false for tiles every column of the wave sees whole.
+  bool near = true;
   auto weights = [&](uint32_t t, auto masked) __attribute__((always_inline)) {
     constexpr bool MASKED = decltype(masked)::value;
     const uint8_t* tab = table(t);
     // (the same in every lane)
-    const float unit = __uint_as_float(__builtin_amdgcn_readfirstlane(*(const uint32_t*)(tab + L::kMisc)));
-    const uint32_t nan_any = __builtin_amdgcn_readfirstlane(*(const uint32_t*)(tab + L::kMisc + 4));
+    const uint32_t has = __builtin_amdgcn_readfirstlane(*(const uint32_t*)(tab + L::kMisc + 4));
+    if (__builtin_expect_with_probability((has & kHasWide) != 0, false, 1.0)) near = false;
     if constexpr (!kTight) {
 #pragma unroll
       for (int g = 0; g < G; ++g) scaled(t, sc[g], g);
@@ -944,8 +1145,7 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
       if (MASKED && 32 * t + 8 * (e >> 2) + 4 * hf + (e & 3) >= visible) x[e] = -INFINITY;
       xmax = fmaxf(xmax, x[e]);
     }
-    // (unit: not 1 where the tile has changed R)
-    if (t == t0 || unit != 1.0f || __builtin_amdgcn_ballot_w64(xmax > kMost)) {
+    if (__builtin_expect(t == t0 || __builtin_amdgcn_ballot_w64(xmax > kMost), 0)) {
       xmax = max2_across_halves(xmax);
       // Whole numbers: the largest weight becomes 2^11 .. 2^12.
       const float shift = (t == t0 || xmax > kMost) && xmax > -INFINITY ? ceilf(xmax - 12.0f) : 0.0f;
@@ -954,15 +1154,14 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
       if (t != t0) {  // (nothing is there yet in the first tile, and corr may be infinite)
         l_lane *= corr;
 #pragma unroll
-        for (int db = 0; db < kDB; ++db) o[db] *= corr * unit;
+        for (int db = 0; db < kDB; ++db) o[db] *= corr;
       }
       uint32_t r[3];
       split3(-m_run, r);
-      if (hf) qbias.z = r[0] | r[1] << 16, qbias.w = r[2] | 0x3F800000u;
+      if (hf) qbias.z = r[0] | r[1] << 16, qbias.w = r[2];
       x -= shift;
     }
-    // The sum takes the weights before they round: those of a tile whose values are far
-    // smaller than others' may round to nothing, but count.
+    // The sum takes the weights before they round.
     float psum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -970,12 +1169,12 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
       ph[i >> 2][i & 3] = pack_f16x2(w0, w1);
       psum[0] += w0, psum[1] += w1;
     }
-    l_lane = __builtin_fmaf(psum[0] + psum[1], *(const float*)(tab + L::kMisc + 24), l_lane);
-    if (nan_any) {  // values that are NaN: of the columns that see them, and their group
+    l_lane += psum[0] + psum[1];
+    if (__builtin_expect(has & kHasNan, 0)) {  // values that are NaN: of the columns that see them, and their group
       const uint32_t n = visible > 32 * t ? visible - 32 * t : 0, seen = n >= 32 ? ~0u : (1u << n) - 1;
 #pragma unroll
       for (int g = 0; g < G; ++g)
-        if (*(const uint32_t*)(tab + L::kMisc + 8 + 4 * g) & seen) {
+        if (*(const uint32_t*)(tab + L::kNan + 4 * g) & seen) {
 #pragma unroll
           for (int db = 2 * g; db < 2 * g + 2; ++db)
 #pragma unroll
@@ -1018,6 +1217,8 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
     if (busy) {
       if constexpr (kTight) products(t);
       weights(t, masked);
+    } else if (__builtin_amdgcn_readfirstlane(*(const uint32_t*)(table(t) + L::kMisc + 4)) & kHasWide) {
+      near = false;
     }
     write_table(t + 2, words);
     fetch_words(p3, words);
@@ -1033,16 +1234,18 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
   // Tiles below full_end are visible to every column of the wave.
   const uint32_t first_row = min(c0, cols - 1) / gh;
   const uint32_t full_end = min(max(min(args.start + first_row + 1, sq.len) / 32, t0), t1);
-  for (uint32_t t = t0; t < full_end; ++t) step(t, BoolTag<false>{});
-  for (uint32_t t = full_end; t < t1; ++t) step(t, BoolTag<true>{});
+  uint32_t t = t0;
+  for (; t < full_end && __builtin_expect_with_probability(near, true, 1.0); ++t) step(t, BoolTag<false>{});
+  for (; t < t1 && __builtin_expect_with_probability(near, true, 1.0); ++t) step(t, BoolTag<true>{});
+  if (__builtin_expect_with_probability(!near, false, 1.0)) return false;
 
   const float l_tot = l_lane + __shfl_xor(l_lane, 32);
-  const float unit = t0 < t1 ? *(const float*)(table(t1 - 1) + L::kMisc + 28) : 1.0f;
-  if (!col_ok) return;
-  if (S > 1 || (args.split_tiles && args.gate)) {
+  const float unit = t0 < t1 ? *(const float*)(table(t1 - 1) + L::kMisc) : 1.0f;
+  if (!place.col_ok) return true;
+  if (leaves_partials(args, place)) {
     // Partials as in decode, row by row: O [row][split][H][D], then (m, l): here O over
     // its own sum, whose logarithm goes into m, so that it stays finite.
-    const size_t pr = ((size_t)row * args.splits + split) * H + head;
+    const size_t pr = ((size_t)row * args.splits + place.split) * H + head;
     float* po = args.partials + pr * D;
     const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
 #pragma unroll
@@ -1054,7 +1257,7 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
     if (hf == 0)
       *(float2*)(args.partials + (size_t)args.part_rows * H * D + pr * 2) =
           l_tot == 0.0f ? float2{-FLT_MAX, 0.0f} : float2{m_run + log2f(l_tot), 1.0f};
-    return;
+    return true;
   }
   const float inv = 1.0f / l_tot;
   const size_t obase = ((size_t)row * H + head) * dr;
@@ -1087,6 +1290,15 @@ __global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill
         args.o[obase + d] = f32_to_bf16(v);
       }
   }
+  return true;
+}
+
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, attn_prefill_waves(D, W)) void q4kv_prefill_kernel(Q4KvPrefillArgs args) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[PrefillLds<D, W>::kBytes];
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (__builtin_expect_with_probability(prefill_block<D, W>(args, lds, wave), true, 1.0)) return;
+  prefill_far<D, W>(args, wave);
 }
 
 template <int D, int W>
