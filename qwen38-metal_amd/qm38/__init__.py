@@ -279,10 +279,48 @@ def _check(status: int) -> None:
         raise QmError(status, msg)
 
 
-def _stride(t) -> int:
-    """Elements between the rows of a torch tensor; 0 (rows that follow one
-    another) for a raw address or None."""
-    return t.stride(0) if hasattr(t, "stride") and t.shape[0] > 1 else 0
+_ROW_TYPES: set = set()  # types seen that are bf16 or its bits
+_POSITION_TYPES: set = set()
+
+
+def _take(name: str, dtype, seen: set, names: tuple) -> None:
+    if str(dtype).rpartition(".")[2] not in names:
+        raise ValueError(f"{name}: {dtype} where {names[0]} is taken")
+    seen.add(dtype)
+
+
+def _row_stride(name: str, t) -> int:
+    """Elements between the rows of a torch tensor; 0 (rows that follow one another) for one
+    row, a raw address or None.  ValueError where a tensor is no rows of bf16: another type,
+    elements that do not follow one another within a row, one row for all."""
+    dtype = getattr(t, "dtype", None)
+    if dtype is None:
+        return 0
+    if dtype not in _ROW_TYPES:
+        _take(name, dtype, _ROW_TYPES, ("bfloat16", "int16", "uint16"))
+    if t.is_contiguous():
+        return t.stride(0) if t.shape[0] > 1 else 0
+    strides, row = t.stride(), 1
+    for size, step in zip(reversed(t.shape[1:]), reversed(strides[1:])):
+        if size > 1 and step != row:
+            raise ValueError(f"{name}: the elements of a row do not follow one another (strides {strides})")
+        row *= size
+    if strides[0] == 0:
+        raise ValueError(f"{name}: one row expanded to {t.shape[0]}")
+    return strides[0] if t.shape[0] > 1 else 0
+
+
+def _check_packed(name: str, t, seen: set = _ROW_TYPES, names: tuple = ("bfloat16", "int16", "uint16")) -> bool:
+    """Whether it is a torch tensor (else a raw address or None); ValueError for one of
+    another type, or whose elements do not all follow one another."""
+    dtype = getattr(t, "dtype", None)
+    if dtype is None:
+        return False
+    if dtype not in seen:
+        _take(name, dtype, seen, names)
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: the elements do not follow one another (strides {t.stride()})")
+    return True
 
 
 def _ptr(t) -> int | None:
@@ -397,23 +435,30 @@ class Runtime:
         the rows any stride apart) behind what seqs[b] cache; with `rotary`, keys
         turned on the way and the rows of q (num_heads heads) into q_out.
         positions: uint32/int32 per row on the device, or None for each row's
-        place in its cache."""
+        place in its cache.  Tensors that are no such rows: ValueError."""
+        if len(counts) != len(seqs):
+            raise ValueError(f"counts: {len(counts)} for {len(seqs)} sequences")
+        _check_packed("positions", positions, _POSITION_TYPES, ("int32", "uint32"))
         arr = (C.c_void_p * len(seqs))(*[s.handle for s in seqs])
         n = (C.c_uint32 * len(seqs))(*counts)
-        rows = KvRows(k=_ptr(k), v=_ptr(v), k_stride=_stride(k), v_stride=_stride(v), offset=offset,
-                      positions=_ptr(positions), q=_ptr(q), q_out=_ptr(q_out), heads=num_heads,
-                      q_stride=_stride(q), q_out_stride=_stride(q_out))
-        if rotary is not None:
-            rows.rotary = C.pointer(rotary)
+        rows = KvRows(_ptr(k), _ptr(v), _row_stride("k", k), _row_stride("v", v),
+                      None if rotary is None else C.pointer(rotary), offset, _ptr(positions), _ptr(q), _ptr(q_out),
+                      num_heads, _row_stride("q", q), _row_stride("q_out", q_out))
         _check(self.lib.qm_kv_append(self.handle, arr, n, len(seqs), C.byref(rows)))
 
     def gqa_attention(self, seqs, q, gate, num_heads: int, o) -> None:
         """The query of every sequence's last cached token over all its tokens (qm_attn_decode_cached)."""
+        _check_packed("q", q)
+        _check_packed("gate", gate)
+        _check_packed("o", o)
         arr = (C.c_void_p * len(seqs))(*[s.handle for s in seqs])
         _check(self.lib.qm_attn_decode_cached(self.handle, arr, len(seqs), _ptr(q), _ptr(gate), num_heads, _ptr(o)))
 
     def gqa_attention_prefill(self, seq, q, gate, num_heads: int, rows: int, o) -> None:
         """Causal attention of the last `rows` cached tokens (qm_attn_prefill_cached)."""
+        _check_packed("q", q)
+        _check_packed("gate", gate)
+        _check_packed("o", o)
         _check(self.lib.qm_attn_prefill_cached(self.handle, seq.handle, _ptr(q), _ptr(gate), num_heads, rows, _ptr(o)))
 
     def gqa_attention_q8(self, seqs, q, gate, k, v, num_heads: int, o) -> None:
@@ -649,7 +694,13 @@ class KvCache:
         return KvCache(self.rt, self.kv_heads, self.head_dim, 16, 0, handle=h, bits=self.bits)
 
     def load(self, first: int, count: int, k, v) -> None:
-        """Tokens first .. first + count - 1 as bf16 [count][kv_heads][head_dim]; k or v may be None."""
+        """Tokens first .. first + count - 1 as bf16 [count][kv_heads][head_dim]; k or v may be None.
+        Tensors that are not packed, or too small: ValueError."""
+        least = count * self.kv_heads * self.head_dim
+        if _check_packed("k", k) and k.numel() < least:
+            raise ValueError(f"k: {k.numel()} elements for {count} tokens")
+        if _check_packed("v", v) and v.numel() < least:
+            raise ValueError(f"v: {v.numel()} elements for {count} tokens")
         _check(self.rt.lib.qm_kv_load(self.rt.handle, self.handle, first, count, _ptr(k), _ptr(v)))
 
     def read(self):
