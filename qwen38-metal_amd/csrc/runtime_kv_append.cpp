@@ -94,7 +94,8 @@ qm_status qm_kv_append(qm_runtime* rt, qm_kv* const* seqs, const uint32_t* count
            aligned(t.out, 16) && (total == 1 || (t.in_stride % 8 == 0 && t.out_stride % 8 == 0));
     const Extent out = extent(t.out, t.out_stride, qwidth, total);
     if (overlap(out, extent(a.k, a.k_stride, width, total)) || overlap(out, extent(a.v, a.v_stride, width, total)) ||
-        (!(t.in == t.out && t.in_stride == t.out_stride) && overlap(out, extent(t.in, t.in_stride, qwidth, total))))
+        (!(t.in == t.out && t.in_stride == t.out_stride) && overlap(out, extent(t.in, t.in_stride, qwidth, total))) ||
+        (a.positions && overlap(out, extent(a.positions, 2 * total, 2 * total, 1))))
       return fail(QM_ERR_INVALID_ARGUMENT, "q_out overlaps an input");
     units += total + kQueryGroups;
   }
