@@ -5,7 +5,7 @@
 // fp64, rounded once to fp32: its code is decided by what lies on either side of a
 // border, and what 4 or 8 bits make of a key then depends on the key alone.  Sine
 // and cosine are their Taylor series on [-pi/4, pi/4] (error below 1e-13).  Queries
-// take rotary.hip's own arithmetic, and so its bits.
+// take rotary.hip's own arithmetic, and so the bits that it gives for the same rows.
 //
 // 4 bits, per group of 64 elements of a (token, KV head):
 //   s = bf16(max((max - min) / 15, FLT_MIN)),  m = bf16(min + 8 s),

@@ -37,8 +37,9 @@ __device__ __forceinline__ void rotary_table(const double* freq, uint32_t half, 
 }
 
 // Eight pairs' or four interleaved pairs' rotation, c their place in the table.  (Which
-// product of a sum is rounded first is written out, so that every kernel that rotates
-// gives the same bits.)
+// product of a sum is rounded first is written out, so that the same form of rows gives
+// the same bits in every kernel.  The form of single elements rounds the other product of a
+// pair's second element first, as it always has.)
 __device__ __forceinline__ void turn_interleaved(const float (&x)[8], float (&y)[8], const float* cos_s, const float* sin_s,
                                                  uint32_t c) {
 #pragma unroll

@@ -1,6 +1,8 @@
-"""GPU tests of qm_kv_append: memory that queries must not be written over."""
+"""GPU tests of qm_kv_append: memory that queries must not be written over, and the bits
+of their rotation whatever the rows' alignment."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
@@ -38,4 +40,24 @@ def test_queries_over_the_positions(rt):
     want = torch.empty_like(q)
     rt.rotary(turn, [(q, want, H, D, 0)], n, position_base=7)
     assert torch.equal(out, want) and torch.equal(positions.cpu(), torch.arange(n, dtype=torch.int32) + 7)
+    cache.close()
+
+
+@pytest.mark.parametrize("shift,extra", [(0, 0), (0, 24), (1, 0), (4, 8), (0, 3), (1, 5), (8, 1)])
+@pytest.mark.parametrize("D,rd,interleaved", [(128, 128, False), (128, 64, True), (256, 256, False), (80, 48, True)])
+def test_query_bits_of_any_alignment(rt, D, rd, interleaved, shift, extra):
+    """Queries have the bits that qm_rotary gives for the same rows at the same place."""
+    g = generator(91)
+    H, KVH, n = 5, 1, 37
+    cache = make(rt, 4, KVH, D)
+    width = H * D + extra
+    rows = bf16(g, n * width + shift)[shift:].view(n, width)
+    q, k = rows[:, :H * D], bf16(g, n, KVH, D)
+    turn = qm38.RotaryConfig(rd, interleaved, 1e4)
+    buffer = torch.zeros(n * width + shift, dtype=torch.bfloat16, device=DEV)
+    got, want = (buffer.clone()[shift:].view(n, width) for _ in range(2))
+    rt.kv_append([cache], [n], k, k, rotary=turn, q=q, q_out=got[:, :H * D], num_heads=H)
+    rt.rotary(turn, [(q, want[:, :H * D], H, D, 0, width, width)], n)
+    assert torch.equal(got, want)
+    assert np.isfinite(got.float().cpu().numpy()).all() and not (got[:, H * D:] != 0).any()
     cache.close()
