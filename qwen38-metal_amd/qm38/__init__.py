@@ -279,48 +279,51 @@ def _check(status: int) -> None:
         raise QmError(status, msg)
 
 
-_ROW_TYPES: set = set()  # types seen that are bf16 or its bits
+# Types seen that are bf16 or its bits, and that are positions.  (A step of a batch asks
+# these few questions of every tensor: about as long as its address and strides take.)
+_ROW_TYPES: set = set()
 _POSITION_TYPES: set = set()
 
 
-def _take(name: str, dtype, seen: set, names: tuple) -> None:
-    if str(dtype).rpartition(".")[2] not in names:
-        raise ValueError(f"{name}: {dtype} where {names[0]} is taken")
-    seen.add(dtype)
+def _take(name: str, t, seen: set, names: tuple) -> None:
+    if str(t.dtype).rpartition(".")[2] not in names:
+        raise ValueError(f"{name}: {t.dtype} where {names[0]} is taken")
+    seen.add(t.dtype)
 
 
-def _row_stride(name: str, t) -> int:
-    """Elements between the rows of a torch tensor; 0 (rows that follow one another) for one
-    row, a raw address or None.  ValueError where a tensor is no rows of bf16: another type,
-    elements that do not follow one another within a row, one row for all."""
-    dtype = getattr(t, "dtype", None)
-    if dtype is None:
-        return 0
-    if dtype not in _ROW_TYPES:
-        _take(name, dtype, _ROW_TYPES, ("bfloat16", "int16", "uint16"))
+def _rows(name: str, t):
+    """Address of rows of bf16, a torch tensor, raw int or None, and the elements between
+    them (0: they follow one another).  ValueError for a tensor that is no such rows: of
+    another type, with elements that do not follow one another within a row, one row for all."""
+    if t is None or t.__class__ is int:
+        return t, 0
+    if t.dtype not in _ROW_TYPES:
+        _take(name, t, _ROW_TYPES, ("bfloat16", "int16", "uint16"))
     if t.is_contiguous():
-        return t.stride(0) if t.shape[0] > 1 else 0
+        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0
     strides, row = t.stride(), 1
-    for size, step in zip(reversed(t.shape[1:]), reversed(strides[1:])):
-        if size > 1 and step != row:
-            raise ValueError(f"{name}: the elements of a row do not follow one another (strides {strides})")
-        row *= size
+    if len(strides) != 2 or strides[1] != 1:
+        for size, step in zip(reversed(t.shape[1:]), reversed(strides[1:])):
+            if size > 1 and step != row:
+                raise ValueError(f"{name}: the elements of a row do not follow one another (strides {strides})")
+            row *= size
     if strides[0] == 0:
         raise ValueError(f"{name}: one row expanded to {t.shape[0]}")
-    return strides[0] if t.shape[0] > 1 else 0
+    return t.data_ptr(), strides[0]
 
 
-def _check_packed(name: str, t, seen: set = _ROW_TYPES, names: tuple = ("bfloat16", "int16", "uint16")) -> bool:
-    """Whether it is a torch tensor (else a raw address or None); ValueError for one of
-    another type, or whose elements do not all follow one another."""
-    dtype = getattr(t, "dtype", None)
-    if dtype is None:
-        return False
-    if dtype not in seen:
-        _take(name, dtype, seen, names)
+def _packed(name: str, t, least: int = 0, seen: set = _ROW_TYPES, names: tuple = ("bfloat16", "int16", "uint16")):
+    """Address of a torch tensor, raw int or None.  ValueError for a tensor of another type,
+    one whose elements do not all follow one another, or of fewer than `least`."""
+    if t is None or t.__class__ is int:
+        return t
+    if t.dtype not in seen:
+        _take(name, t, seen, names)
     if not t.is_contiguous():
         raise ValueError(f"{name}: the elements do not follow one another (strides {t.stride()})")
-    return True
+    if least and t.numel() < least:
+        raise ValueError(f"{name}: {t.numel()} elements, {least} are needed")
+    return t.data_ptr()
 
 
 def _ptr(t) -> int | None:
@@ -438,28 +441,25 @@ class Runtime:
         place in its cache.  Tensors that are no such rows: ValueError."""
         if len(counts) != len(seqs):
             raise ValueError(f"counts: {len(counts)} for {len(seqs)} sequences")
-        _check_packed("positions", positions, _POSITION_TYPES, ("int32", "uint32"))
         arr = (C.c_void_p * len(seqs))(*[s.handle for s in seqs])
         n = (C.c_uint32 * len(seqs))(*counts)
-        rows = KvRows(_ptr(k), _ptr(v), _row_stride("k", k), _row_stride("v", v),
-                      None if rotary is None else C.pointer(rotary), offset, _ptr(positions), _ptr(q), _ptr(q_out),
-                      num_heads, _row_stride("q", q), _row_stride("q_out", q_out))
+        (k, k_stride), (v, v_stride) = _rows("k", k), _rows("v", v)
+        (q, q_stride), (q_out, q_out_stride) = _rows("q", q), _rows("q_out", q_out)
+        rows = KvRows(k, v, k_stride, v_stride, None if rotary is None else C.pointer(rotary), offset,
+                      _packed("positions", positions, 0, _POSITION_TYPES, ("int32", "uint32")), q, q_out, num_heads,
+                      q_stride, q_out_stride)
         _check(self.lib.qm_kv_append(self.handle, arr, n, len(seqs), C.byref(rows)))
 
     def gqa_attention(self, seqs, q, gate, num_heads: int, o) -> None:
         """The query of every sequence's last cached token over all its tokens (qm_attn_decode_cached)."""
-        _check_packed("q", q)
-        _check_packed("gate", gate)
-        _check_packed("o", o)
         arr = (C.c_void_p * len(seqs))(*[s.handle for s in seqs])
-        _check(self.lib.qm_attn_decode_cached(self.handle, arr, len(seqs), _ptr(q), _ptr(gate), num_heads, _ptr(o)))
+        _check(self.lib.qm_attn_decode_cached(self.handle, arr, len(seqs), _packed("q", q), _packed("gate", gate),
+                                              num_heads, _packed("o", o)))
 
     def gqa_attention_prefill(self, seq, q, gate, num_heads: int, rows: int, o) -> None:
         """Causal attention of the last `rows` cached tokens (qm_attn_prefill_cached)."""
-        _check_packed("q", q)
-        _check_packed("gate", gate)
-        _check_packed("o", o)
-        _check(self.lib.qm_attn_prefill_cached(self.handle, seq.handle, _ptr(q), _ptr(gate), num_heads, rows, _ptr(o)))
+        _check(self.lib.qm_attn_prefill_cached(self.handle, seq.handle, _packed("q", q), _packed("gate", gate),
+                                               num_heads, rows, _packed("o", o)))
 
     def gqa_attention_q8(self, seqs, q, gate, k, v, num_heads: int, o) -> None:
         arr = (C.c_void_p * len(seqs))(*[s.handle for s in seqs])
@@ -697,11 +697,8 @@ class KvCache:
         """Tokens first .. first + count - 1 as bf16 [count][kv_heads][head_dim]; k or v may be None.
         Tensors that are not packed, or too small: ValueError."""
         least = count * self.kv_heads * self.head_dim
-        if _check_packed("k", k) and k.numel() < least:
-            raise ValueError(f"k: {k.numel()} elements for {count} tokens")
-        if _check_packed("v", v) and v.numel() < least:
-            raise ValueError(f"v: {v.numel()} elements for {count} tokens")
-        _check(self.rt.lib.qm_kv_load(self.rt.handle, self.handle, first, count, _ptr(k), _ptr(v)))
+        _check(self.rt.lib.qm_kv_load(self.rt.handle, self.handle, first, count, _packed("k", k, least),
+                                      _packed("v", v, least)))
 
     def read(self):
         """Returns (keys int8 [T][KVH][d], values, key_scales f32 [T][KVH], value_scales);
