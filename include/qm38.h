@@ -300,10 +300,10 @@ qm_status qm_kv_read_q4(const qm_kv* kv, int8_t* keys, int8_t* values,
 /* Rows of a fused or separate projection for qm_kv_append, bf16 device pointers;
  * strides are the elements between rows (0: heads * head_dim).  With `rotary`
  * set, elements offset .. offset + rotary_dim - 1 of every key are rotated on the
- * way, in fp64 and rounded once to fp32, and of every query, into q_out (bf16, with
- * the bits that qm_rotary of these rows alone, same addresses and strides, gives; rows of
- * other alignment may differ in the last bit, there as here).  positions: device uint32 per row, or NULL for the
- * row's place in its cache; read with `rotary` only. */
+ * way, in fp64 and rounded once to fp32, and of every query, into q_out (bf16, with the
+ * bits that qm_rotary gives for these rows alone at the same addresses and strides; rows
+ * of another alignment may differ in the last bit, there as here).  positions: device
+ * uint32 per row, or NULL for the row's place in its cache; read with `rotary` only. */
 typedef struct qm_rotary_config qm_rotary_config; /* Rotary positions, below */
 typedef struct qm_kv_rows {
   const uint16_t* k; /* [rows][kv_heads][head_dim] */

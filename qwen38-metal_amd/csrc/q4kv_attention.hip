@@ -576,12 +576,12 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void q4kv_decod
 // The tables of a tile (scales, offsets, powers) are formed a tile ahead of its
 // unpacking by two waves.
 //
-// 2048 rows on 4096 tokens of 64 / 8 heads of 128: 457 us, 750 TFLOP/s (a large matrix
-// product reaches 1230), matrix instructions busy for 32 % of the cycles, vector ones
-// for 44 %, half of those for the unpacking and the softmax's exponentials.  The same
-// without scores a tile ahead took 618 us, with a tile's tables and V on the last waves
-// alone 564.  1000 rows of 24 / 4 heads of 256: 52 us (69 with the same number of
-// workgroups for every block of columns).
+// 2048 rows on 4096 tokens of 64 / 8 heads of 128: 472 us, 727 TFLOP/s (a large matrix
+// product reaches 1230), matrix instructions busy for 30 % of the cycles, vector ones
+// for 42 %, half of those for the unpacking and the softmax's exponentials.  Before the
+// values had one unit (457 us) the same took 618 without scores a tile ahead, and 564 with a
+// tile's tables and V on the last waves alone.  1000 rows of 24 / 4 heads of 256, the kernel
+// alone: 50 us (about 70 with the same number of workgroups for every block of columns).
 constexpr uint32_t kHasNan = 1, kHasWide = 2;
 // Sizes below it (values of the least scale) count as none.
 constexpr float kNoSize = 0x1p-121f;

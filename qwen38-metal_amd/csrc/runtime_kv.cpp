@@ -224,8 +224,8 @@ struct DecodeChunk {
 // share a CU.
 // Sequences of at most 32 pages are not split at all, with eight waves from 17 pages on (9
 // with heads of 256): a second launch costs more than the four pages a wave (500 tokens of
-// 24 / 4 heads of 256: 11.2 us against 12.3; of 64 / 8 of 128: 8.7 against 9.3; 1000
-// tokens of the former: 17.5 against 10.9).
+// 24 / 4 heads of 256: 11.3 us unsplit, 12.5 split; of 64 / 8 of 128: 9.4 and 10.7).  Of more
+// it costs less (1000 tokens of the former: 17.3 us unsplit, 11.3 split).
 // The chunk's sequences are there, caches like kv; their splits are filled in.
 qm_status plan_decode_splits(const qm_runtime* rt, const qm_kv* kv, uint32_t nb, uint32_t H, DecodeChunk* c) {
   // Workgroups of a split.
@@ -355,9 +355,9 @@ void qm::plan_prefill(const qm_runtime* rt, bool q4, AttnArgs* at) {
   if (!q4) return;
   // Over 4-bit caches: where a prompt's blocks see very different numbers of tiles, each
   // has workgroups for its own, of at least four tiles, as many as run in one round (24 / 4
-  // heads of 256 on an empty cache: 512 rows 68 -> 46 us, 1000 rows 82 -> 67, 1500 rows
-  // 162 -> 103; 64 / 8 of 128, 1000 rows, whose blocks nearly fill a round: not split,
-  // 63 against 70).
+  // heads of 256 on an empty cache, attention of cached rows, its launches together: 512 rows
+  // 68 -> 46 us, 1000 rows 82 -> 67, 1500 rows 162 -> 103; 64 / 8 of 128, 1000 rows, whose
+  // blocks nearly fill a round: not split, 63 against 70).
   const uint32_t gh = at->heads / at->kv_heads, block = 32 * at->wg_waves, blocks = (uint32_t)(u / at->kv_heads);
   auto tiles_of = [&](uint32_t b) { return prefill_tiles(b, block, (uint32_t)cols, gh, at->start, at->seqs[0].len); };
   const uint32_t longest = tiles_of(blocks - 1);
