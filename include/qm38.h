@@ -286,9 +286,10 @@ qm_status qm_kv_read(const qm_kv* kv, int8_t* keys, int8_t* values,
  * bits and values as the codes give them.  A prefill may take both in fp16, rounded
  * once each to 11 bits; then a weight more than 2^35 below its row's largest may count
  * in the sum of weights alone.  (One of few rows goes as a decode step where that is
- * faster and its workspace is there.)  Values may have any size, but where the largest of
- * the groups of tokens are more than 2^7 above or 2^14 below those of the first tokens,
- * a prefill of many rows is some ten times slower. */
+ * faster and its workspace is there.)  Values may have any size, though a prefill may
+ * take what is below 2^-121 for zero; where a token's group is more than 2^7 above or
+ * 2^14 below the largest of the first tokens', a prefill of many rows is some ten times
+ * slower. */
 qm_status qm_kv_create_q4(qm_runtime* rt, uint32_t kv_heads, uint32_t head_dim,
                           uint32_t page_tokens, uint32_t max_tokens, qm_kv** out);
 uint32_t qm_kv_bits(const qm_kv* kv); /* 8 or 4; 0 for NULL */
@@ -332,7 +333,8 @@ qm_status qm_kv_append(qm_runtime* rt, qm_kv* const* seqs, const uint32_t* count
                        const qm_kv_rows* rows);
 /* Reads tokens first .. first + count - 1 back, what their codes stand for rounded
  * to bf16: k and v [count][kv_heads][head_dim], either may be NULL.  Past the
- * length: QM_ERR_INVALID_SEQUENCE_LENGTH. */
+ * length: QM_ERR_INVALID_SEQUENCE_LENGTH; more than one launch takes (13 million tokens of
+ * 8 heads of 256): QM_ERR_DIMENSION_OVERFLOW. */
 qm_status qm_kv_load(qm_runtime* rt, const qm_kv* kv, uint32_t first, uint32_t count,
                      uint16_t* k, uint16_t* v);
 /* qm_attn_decode of tokens that are in their caches already (qm_kv_append): the

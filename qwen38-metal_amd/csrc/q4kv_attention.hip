@@ -812,7 +812,7 @@ __device__ __forceinline__ void prefill_far(const Q4KvPrefillArgs& args, uint32_
           }
         }
       float below = INFINITY;
-      for (;;) {
+      for (int pass = 0; pass < 6; ++pass) {  // (weights are 2^12 at most: six reach below 2^-110)
         float high = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 16; ++e)
